@@ -321,6 +321,107 @@ int mkv_gdn_decode_gather(const void* state_pool, int64_t state_bytes, void* sta
                           const void* weight, int32_t kernel_size, void* conv_out,
                           int32_t* err, void* stream);
 
+/*
+ * The same conv over packed prompts (the prefill branch of _gdn_conv1d_apply,
+ * muserve/model/qwen35_layer_v2.py:163-201): sequence b is rows
+ * [cu_seqlens[b], cu_seqlens[b+1]) of x [num_tokens, channels] bf16, x_stride
+ * bytes apart;
+ *   out[t][c] = silu(sum_k weight[c][k] x[t - 3 + k][c])  (fp32, rounded to bf16)
+ * with the rows before the sequence taken from slot slots[b], which is left
+ * with the sequence's last `width` inputs (and the newest of its old ones
+ * where the sequence is shorter). A sequence without rows leaves its slot.
+ * Rows of out [num_tokens, channels] outside the sequences are left as they
+ * were. Requirements as mkv_gdn_conv_decode's, x_stride a multiple of 16.
+ * Offsets below 0, falling or above num_tokens set MKV_DEVERR_TABLE, and the
+ * call writes nothing; a slot outside [0, pool_slots) gives zeros and sets
+ * MKV_DEVERR_STATE_SLOT.
+ */
+int mkv_gdn_conv_prefill(void* conv_pool, int64_t pool_slots, int32_t channels, int32_t width,
+                         const int32_t* slots, const int32_t* cu_seqlens, int32_t batch,
+                         int64_t num_tokens, const void* x, int64_t x_stride, const void* weight,
+                         int32_t kernel_size, void* out, int32_t* err, void* stream);
+
+/* ---- linear attention over the state pool -------------------------------- */
+
+/*
+ * The recurrent form of linear attention with a decay for each head, one token
+ * per request, in place on the recurrent-state pool of one layer (the math of
+ * gated_delta_rule_decode, muserve/model/qwen35_layer_v2.py:286-295, without
+ * the gather and scatter of the states). state is [pool_slots, num_v_heads,
+ * 128, 128] fp32, values x keys. For request b and value head h, S its state
+ * in slot slots[b], q and k row b of key head h / (num_v_heads / num_k_heads):
+ *   S <- e^g S;  u = beta (v - S k)  (u = v without beta);  S <- S + u k^T
+ *   out[b][h] = scale S q  (fp32, rounded to bf16 once)
+ *   - q, k [batch, num_k_heads, 128], v [batch, num_v_heads, 128] bf16, rows
+ *     *_stride bytes apart (the heads of a row follow each other), so that the
+ *     three may be views of one buffer; out is contiguous;
+ *   - qk_norm: q and k are divided by sqrt(sum of squares + 1e-6) first;
+ *   - g, beta [batch, num_v_heads], fp32, or bf16 with gates_bf16; beta may be
+ *     NULL (a decay without the delta rule). With a_log and dt_bias
+ *     [num_v_heads] fp32 they are projections:
+ *       g = -e^a_log softplus(g + dt_bias),  beta = sigmoid(beta);
+ *   - with z [batch, num_v_heads, 128] bf16 and norm_weight [128] (fp32, or
+ *     bf16 with weight_bf16) the output is
+ *       o / sqrt(mean(o^2) + norm_eps) * norm_weight * silu(z), still rounded once.
+ * Requirements: head_dim 128, num_v_heads a multiple of num_k_heads and at
+ * most 1024, batch <= 65535 (MKV_E_UNSUPPORTED); rows, strides and the state
+ * 16-byte aligned (MKV_E_ALIGN); slots unique. A slot outside [0, pool_slots)
+ * gives zeros and sets MKV_DEVERR_STATE_SLOT.
+ */
+int mkv_linear_attn_decode(void* state, int64_t pool_slots, int32_t num_k_heads,
+                           int32_t num_v_heads, int32_t head_dim, const int32_t* slots,
+                           int32_t batch, const void* q, int64_t q_stride, const void* k,
+                           int64_t k_stride, const void* v, int64_t v_stride, const void* g,
+                           int64_t g_stride, const void* beta, int64_t beta_stride,
+                           int32_t gates_bf16, const float* a_log, const float* dt_bias,
+                           int32_t qk_norm, float scale, const void* z, int64_t z_stride,
+                           const void* norm_weight, int32_t weight_bf16, float norm_eps,
+                           void* out, int32_t* err, void* stream);
+
+/*
+ * The same recurrence over packed prompts (chunk_gated_delta_rule,
+ * muserve/model/qwen35_layer_v2.py:351-358): sequence b is rows
+ * [cu_seqlens[b], cu_seqlens[b+1]) of q, k, v, g, beta, z and out, starts from
+ * slot slots[b] (zeros after mkv_zero_blocks; a chunked prompt's later chunks
+ * from where the last one ended) and leaves its final state there. A sequence
+ * without rows leaves its slot; rows of out outside the sequences are left as
+ * they were. max_seqlen is a hint of the longest sequence (0: not known) that
+ * chooses between forms of the computation; any value is right. With z the
+ * output is rounded to bf16 before the norm as well. Arguments and
+ * requirements otherwise as above, batch <= 65535, num_tokens < 2^31.
+ * Offsets below 0, falling or above num_tokens set MKV_DEVERR_TABLE, and the
+ * call writes neither rows nor states. The workspace must be 16-byte aligned
+ * and hold mkv_linear_attn_prefill_workspace_bytes (-1: bad sizes) for the
+ * same arguments, delta: beta is given.
+ */
+int mkv_linear_attn_prefill(void* state, int64_t pool_slots, int32_t num_k_heads,
+                            int32_t num_v_heads, int32_t head_dim, const int32_t* slots,
+                            const int32_t* cu_seqlens, int32_t batch, int64_t num_tokens,
+                            int32_t max_seqlen, const void* q, int64_t q_stride, const void* k,
+                            int64_t k_stride, const void* v, int64_t v_stride, const void* g,
+                            int64_t g_stride, const void* beta, int64_t beta_stride,
+                            int32_t gates_bf16, const float* a_log, const float* dt_bias,
+                            int32_t qk_norm, float scale, const void* z, int64_t z_stride,
+                            const void* norm_weight, int32_t weight_bf16, float norm_eps,
+                            void* out, void* workspace, int64_t workspace_bytes, int32_t* err,
+                            void* stream);
+int64_t mkv_linear_attn_prefill_workspace_bytes(int64_t num_tokens, int32_t batch,
+                                                int32_t max_seqlen, int32_t num_k_heads,
+                                                int32_t num_v_heads, int32_t delta);
+
+/*
+ * out = x / sqrt(mean(x^2) + eps) * weight * silu(z), for every row of `dim`
+ * values of x, z and out [tokens, heads, dim] bf16 (fp32 arithmetic, rounded
+ * once): the norm behind a linear-attention layer. x and z rows are x_stride
+ * and z_stride bytes apart, a token's heads follow each other; out is
+ * contiguous and may be x. weight is [dim] fp32, or bf16 with weight_bf16.
+ * dim is a multiple of 8 up to 4096, tokens * heads at most 2^32
+ * (MKV_E_UNSUPPORTED); rows and strides 16-byte aligned (MKV_E_ALIGN).
+ */
+int mkv_gated_rms_norm(const void* x, int64_t x_stride, const void* z, int64_t z_stride,
+                       int64_t tokens, int32_t heads, int32_t dim, const void* weight,
+                       int32_t weight_bf16, float eps, void* out, void* stream);
+
 /* ---- host tier: layered block pack / unpack ------------------------------ */
 
 /*

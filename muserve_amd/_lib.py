@@ -69,6 +69,16 @@ SIGNATURES: dict[str, list] = {
     "mkv_gdn_conv_decode": [_P, _I64, _I32, _I32, _P, _I32, _P, _P, _I32, _P, _P, _P],
     "mkv_gdn_decode_gather": [_P, _I64, _P, _P, _I32, _I32, _I64, _P, _I32, _P, _P, _I32, _P,
                               _P, _P],
+    "mkv_gdn_conv_prefill": [_P, _I64, _I32, _I32, _P, _P, _I32, _I64, _P, _I64, _P, _I32, _P, _P,
+                             _P],
+    "mkv_linear_attn_decode": [_P, _I64, _I32, _I32, _I32, _P, _I32, _P, _I64, _P, _I64, _P, _I64,
+                               _P, _I64, _P, _I64, _I32, _P, _P, _I32, _F32, _P, _I64, _P, _I32,
+                               _F32, _P, _P, _P],
+    "mkv_linear_attn_prefill": [_P, _I64, _I32, _I32, _I32, _P, _P, _I32, _I64, _I32, _P, _I64, _P,
+                                _I64, _P, _I64, _P, _I64, _P, _I64, _I32, _P, _P, _I32, _F32, _P,
+                                _I64, _P, _I32, _F32, _P, _P, _I64, _P, _P],
+    "mkv_linear_attn_prefill_workspace_bytes": [_I64, _I32, _I32, _I32, _I32, _I32],
+    "mkv_gated_rms_norm": [_P, _I64, _P, _I64, _I64, _I32, _I32, _P, _I32, _F32, _P, _P],
     "mkv_pack_blocks": [_P, _I64, _I32, _I64, _I64, _P, _I32, _P, _P, _P],
     "mkv_unpack_blocks": [_P, _I64, _I32, _I64, _I64, _P, _I32, _P, _P, _P],
     "mkv_zero_blocks": [_P, _I64, _I32, _I64, _I64, _P, _I32, _P, _P],
@@ -108,7 +118,8 @@ SIGNATURES: dict[str, list] = {
     "mkv_probe_fill": [_P, _I64, _P],
 }
 _INT64_RESULT = {"mkv_bm_state_bytes", "mkv_decode_attention_workspace_bytes",
-                 "mkv_prefill_attention_workspace_bytes", "mkv_prefill_attention_plan_bytes"}
+                 "mkv_prefill_attention_workspace_bytes", "mkv_prefill_attention_plan_bytes",
+                 "mkv_linear_attn_prefill_workspace_bytes"}
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None

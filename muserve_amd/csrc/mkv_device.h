@@ -46,6 +46,38 @@ __device__ __forceinline__ T ld_const(const T* p) {
 // Device error bits go through a vector-memory atomic on the caller's word.
 __device__ __forceinline__ void raise_err(int32_t* err, int32_t bit) { atomicOr(err, bit); }
 
+// Whether the offsets cu[0 .. n] of packed sequences hold together: from 0 or
+// more, never falling, at most `rows`. Every thread of the workgroup calls.
+__device__ __forceinline__ bool offsets_ok(const int32_t* cu, int32_t n, int64_t rows) {
+  bool bad = false;
+  for (int32_t i = threadIdx.x; i <= n; i += blockDim.x) {
+    const int32_t x = cu[i];
+    bad |= x < 0 || x > rows || (i > 0 && cu[i - 1] > x);
+  }
+  return !__syncthreads_or(bad);
+}
+
+// Tiles of 64 rows of packed sequences without a list of them: tile c of
+// sequence b has the id cu[b] / 64 + b + c. Ids never meet (a sequence of m
+// rows from cu[b] has at most (cu[b] + m) / 64 - cu[b] / 64 + 1 tiles), and
+// rows / 64 + n ids cover all of them; ids in between belong to no tile.
+__device__ __forceinline__ int64_t first_tile(const int32_t* cu, int32_t b) {
+  return (int64_t)(cu[b] >> 6) + b;
+}
+inline int64_t tile_ids(int64_t rows, int32_t n) { return rows / 64 + n; }
+// The sequence that a tile id would belong to.
+__device__ __forceinline__ int32_t tile_sequence(const int32_t* cu, int32_t n, int64_t id) {
+  int32_t lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int32_t mid = (lo + hi + 1) >> 1;
+    if (first_tile(cu, mid) <= id)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+
 // Arguments of a block-table gather (see mkv_gather_bf16 in mkv.h). Row
 // geometry is a template parameter of each kernel, not an argument.
 struct GatherArgs {

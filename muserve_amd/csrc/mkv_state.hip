@@ -285,6 +285,111 @@ __device__ __forceinline__ void conv_row(const ConvArgs& a, uint32_t bx, int64_t
     st16(st + 16 * j, u32x4{nsw[4 * j], nsw[4 * j + 1], nsw[4 * j + 2], nsw[4 * j + 3]});
 }
 
+// ---------------------------------------------------------------------------
+// The same conv over packed prompts (qwen35_layer_v2.py:163-201, prefill
+// branch): row t of sequence b takes its taps from the rows before it, and
+// from the slot's last inputs where those lie before the sequence; the slot is
+// left with the sequence's last W inputs. Bound by HBM: every row is read and
+// written once, 16 bytes per thread and row. A workgroup takes a tile of 64
+// rows (tile ids of mkv_device.h, grid.x) and 512 channels (grid.y); a thread
+// slides over 16 rows, all loaded before the first is used, the 3 rows before
+// them again. Only the thread that reads a slot's old inputs (the first rows
+// of a sequence) writes its new ones, so no other can see them early.
+// ---------------------------------------------------------------------------
+struct ConvPrefillArgs {
+  ConvArgs c;            // x: [tokens, channels], stride x_stride; batch: sequences
+  int64_t x_stride;      // bytes between tokens
+  int64_t tokens;
+  const int32_t* cu;     // [batch + 1]
+};
+constexpr int kConvRows = 16;
+
+template <int W>
+__global__ __launch_bounds__(kThreads) void conv_prefill_kernel(ConvPrefillArgs p) {
+  const ConvArgs& a = p.c;
+  const bool ok = offsets_ok(p.cu, a.batch, p.tokens);
+  if (!ok) {  // uniform
+    if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0) raise_err(a.err, MKV_DEVERR_TABLE);
+    return;
+  }
+  const int32_t b = tile_sequence(p.cu, a.batch, blockIdx.x);
+  const int64_t end = p.cu[b + 1], seq0 = p.cu[b];
+  const int64_t tile = (int64_t)blockIdx.x - first_tile(p.cu, b);
+  const int64_t t0 = seq0 + tile * 64 + (threadIdx.x >> 6) * kConvRows;
+  const int64_t g = (int64_t)blockIdx.y * 64 + (threadIdx.x & 63);  // group of 8 channels
+  if (t0 >= end || g * 8 >= a.channels) return;
+  const int32_t slot = a.slots[b];
+  const int64_t row = (int64_t)a.channels * 2;
+  const int32_t rows = (int32_t)(end - t0 < kConvRows ? end - t0 : kConvRows);
+  uint8_t* outp = a.out + t0 * row + g * 16;
+  if (slot < 0 || slot >= a.pool_slots) {
+    if (g == 0 && t0 == seq0) raise_err(a.err, MKV_DEVERR_STATE_SLOT);
+    for (int32_t i = 0; i < rows; ++i) st16(outp + i * row, u32x4{0u, 0u, 0u, 0u});
+    return;
+  }
+  const uint8_t* xp = a.x + t0 * p.x_stride + g * 16;
+  u32x4 xv[3 + kConvRows], wv[kConvK], sv[W];
+#pragma unroll
+  for (int i = 0; i < 3 + kConvRows; ++i) {
+    xv[i] = u32x4{0u, 0u, 0u, 0u};
+    if (t0 + i - 3 >= seq0 && i - 3 < rows) xv[i] = ld16(xp + (i - 3) * p.x_stride);
+  }
+#pragma unroll
+  for (int j = 0; j < kConvK; ++j) wv[j] = ld16(a.w + (g * 8 * kConvK) * 2 + 16 * j);
+  if (t0 == seq0) {
+    uint8_t* st = a.pool + ((int64_t)slot * a.channels + g * 8) * (W * 2);
+#pragma unroll
+    for (int j = 0; j < W; ++j) sv[j] = ld16(st + 16 * j);
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; e += 2)
+        xv[i][e >> 1] = half16(sv, e * W + W - 3 + i) | (half16(sv, (e + 1) * W + W - 3 + i) << 16);
+    // the last W inputs: old ones move up where the sequence is shorter
+    const int64_t len = end - seq0;
+    u32x4 last[W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      last[j] = u32x4{0u, 0u, 0u, 0u};
+      const int64_t t = len - W + j;  // row of the sequence, or before it
+      if (t >= 0) {
+        last[j] = ld16(a.x + (seq0 + t) * p.x_stride + g * 16);
+      } else {
+        const int from = (int)(W + t);
+#pragma unroll
+        for (int k = 0; k < W; ++k)
+          if (k == from)
+#pragma unroll
+            for (int e = 0; e < 8; e += 2)
+              last[j][e >> 1] = half16(sv, e * W + k) | (half16(sv, (e + 1) * W + k) << 16);
+      }
+    }
+    uint32_t ns[4 * W];
+#pragma unroll
+    for (int e = 0; e < 4 * W; ++e) {
+      const int lo = 2 * e, hi = 2 * e + 1;
+      ns[e] = half16(&last[lo % W], lo / W) | (half16(&last[hi % W], hi / W) << 16);
+    }
+#pragma unroll
+    for (int j = 0; j < W; ++j)
+      st16(st + 16 * j, u32x4{ns[4 * j], ns[4 * j + 1], ns[4 * j + 2], ns[4 * j + 3]});
+  }
+#pragma unroll
+  for (int i = 0; i < kConvRows; ++i) {
+    u32x4 y = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float acc = 0.f;
+#pragma unroll
+      for (int k = 0; k < kConvK; ++k)
+        acc = fmaf(bits_f32(half16(wv, e * kConvK + k) << 16),
+                   bits_f32(half16(&xv[i + k], e) << 16), acc);
+      y[e >> 1] |= (uint32_t)f32_to_bf16_rne(acc / (1.0f + expf(-acc))) << (16 * (e & 1));
+    }
+    if (i < rows) st16(outp + i * row, y);
+  }
+}
+
 template <int W>
 __global__ __launch_bounds__(kThreads) void conv_decode_kernel(ConvArgs a) {
   conv_row<W>(a, blockIdx.x, blockIdx.y);
@@ -441,5 +546,34 @@ extern "C" int mkv_gdn_decode_gather(const void* state_pool, int64_t state_bytes
   else
     hipLaunchKernelGGL(gdn_decode_gather_kernel<4>, grid, dim3(kThreads), 0, as_stream(stream), s,
                        c);
+  return check_launch(fn);
+}
+
+extern "C" int mkv_gdn_conv_prefill(void* conv_pool, int64_t pool_slots, int32_t channels,
+                                    int32_t width, const int32_t* slots,
+                                    const int32_t* cu_seqlens, int32_t batch, int64_t num_tokens,
+                                    const void* x, int64_t x_stride, const void* weight,
+                                    int32_t kernel_size, void* out, int32_t* err, void* stream) {
+  clear_error();
+  const char* fn = "mkv_gdn_conv_prefill";
+  MKV_REQUIRE(num_tokens >= 0 && num_tokens < (1ll << 31), MKV_E_INVALID, "%s: bad sizes", fn);
+  ConvPrefillArgs p{};
+  const int rc = conv_args(fn, conv_pool, pool_slots, channels, width, slots,
+                           num_tokens == 0 ? 0 : batch, x, weight, kernel_size, out, err, p.c);
+  if (rc != MKV_OK) return rc == kEmpty ? MKV_OK : rc;
+  MKV_REQUIRE(cu_seqlens && aligned4(cu_seqlens), MKV_E_INVALID, "%s: null pointer", fn);
+  MKV_REQUIRE(x_stride >= (int64_t)channels * 2, MKV_E_INVALID,
+              "%s: a stride is shorter than its row", fn);
+  MKV_REQUIRE(x_stride % 16 == 0, MKV_E_ALIGN, "%s: rows must be 16-byte aligned", fn);
+  const int64_t groups = (channels / 8 + 63) / 64;
+  MKV_REQUIRE(groups <= 65535, MKV_E_UNSUPPORTED, "%s: too many channels", fn);
+  p.x_stride = x_stride;
+  p.tokens = num_tokens;
+  p.cu = cu_seqlens;
+  const dim3 grid((unsigned)tile_ids(num_tokens, batch), (unsigned)groups);
+  if (width == 3)
+    hipLaunchKernelGGL(conv_prefill_kernel<3>, grid, dim3(kThreads), 0, as_stream(stream), p);
+  else
+    hipLaunchKernelGGL(conv_prefill_kernel<4>, grid, dim3(kThreads), 0, as_stream(stream), p);
   return check_launch(fn);
 }

@@ -12,8 +12,11 @@ this module keeps them resident in two pools indexed by a request slot:
 
 ``gather(layer, slots)`` copies a batch's entries into contiguous buffers and
 ``scatter`` writes updated entries back, both layer's pools in one launch.
-Slot ids within a ``scatter`` (and ``reset``, ``conv_decode``,
-``decode_gather``) must be unique; with ``check_unique`` set a repeat is
+``conv_decode`` and ``conv_prefill`` run the layer's conv in place on the conv
+slots, ``linear_attn_decode`` and ``linear_attn_prefill`` its linear attention
+in place on the recurrent ones, so that neither is gathered or scattered.
+Slot ids within a ``scatter`` (and ``reset`` and the in-place calls) must be
+unique; with ``check_unique`` set a repeat is
 reported as MkvDeviceError at the next ``check_errors``.
 """
 from __future__ import annotations
@@ -22,6 +25,7 @@ import torch
 
 from muserve_amd import _lib
 from muserve_amd.config import GDN_CONV_KERNEL, GDN_KEY_DIM, GDN_VALUE_DIM
+from muserve_amd.kernels import linear_attention
 
 GDN_V_HEADS_PER_RANK = 8   # 64 value heads / TP 8 (muserve/model/qwen35_layer_v2.py:46-47)
 CONV_CHANNELS_PER_RANK = 2048
@@ -202,6 +206,44 @@ class StatePool:
                   slots.data_ptr(), B, x.data_ptr(), w.data_ptr(), w.shape[1], out.data_ptr(),
                   self._errors.ptr(), _lib.stream_of(self.device))
         return out
+
+    def conv_prefill(self, layer: int, slots: torch.Tensor, x: torch.Tensor,
+                     weight: torch.Tensor, cu_seqlens: torch.Tensor,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+        """``conv_decode`` for packed prompts: x [total_tokens, C] bf16 (rows may
+        be strided), sequence b rows cu_seqlens[b]..cu_seqlens[b+1], from and to
+        conv slot slots[b] (``kernels.linear_attention.causal_conv_prefill``)."""
+        if self.conv is None:
+            raise RuntimeError("this pool keeps no conv states")
+        slots = self._in_place(layer, slots)
+        return linear_attention.causal_conv_prefill(x, weight, self.conv[layer], slots, cu_seqlens,
+                                                    out=out, errors=self._errors)
+
+    def linear_attn_decode(self, layer: int, slots: torch.Tensor, q: torch.Tensor,
+                           k: torch.Tensor, v: torch.Tensor, g: torch.Tensor,
+                           beta: torch.Tensor | None = None, **how) -> torch.Tensor:
+        """The layer's linear attention for one token per request, in place on
+        the recurrent slots; arguments and keywords as
+        ``kernels.linear_attention.linear_attn_decode``."""
+        slots = self._in_place(layer, slots)
+        return linear_attention.linear_attn_decode(q, k, v, g, beta, self.state[layer], slots,
+                                                   errors=self._errors, **how)
+
+    def linear_attn_prefill(self, layer: int, slots: torch.Tensor, q: torch.Tensor,
+                            k: torch.Tensor, v: torch.Tensor, g: torch.Tensor,
+                            beta: torch.Tensor | None, cu_seqlens: torch.Tensor,
+                            **how) -> torch.Tensor:
+        """The layer's linear attention over packed prompts, from and to the
+        recurrent slots; arguments and keywords as
+        ``kernels.linear_attention.linear_attn_prefill``."""
+        slots = self._in_place(layer, slots)
+        return linear_attention.linear_attn_prefill(q, k, v, g, beta, self.state[layer], slots,
+                                                    cu_seqlens, errors=self._errors, **how)
+
+    def _in_place(self, layer: int, slots: torch.Tensor) -> torch.Tensor:
+        if not 0 <= layer < self.num_layers:
+            raise IndexError(f"GDN layer {layer} out of range (pool has {self.num_layers})")
+        return self._check(slots, unique=True)
 
     def check_errors(self) -> None:
         if self._errors is not None:
