@@ -41,6 +41,11 @@ HIP_FLAGS = [
     f"-I{CSRC}",
 ]
 
+# mkv_linear: results of matrix instructions in ordinary registers (its loops do
+# vector arithmetic on all of them; through the accumulator file each value
+# costs two moves).
+EXTRA_FLAGS = {"mkv_linear": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+
 
 def hipcc() -> str:
     for cand in (os.environ.get("HIPCC"), "/opt/rocm/bin/hipcc", shutil.which("hipcc")):
@@ -69,7 +74,8 @@ def build(verbose: bool = False, jobs: int | None = None) -> Path:
     if not sources:
         raise RuntimeError(f"no HIP sources under {CSRC}")
     objs = [BUILD / (s.stem + ".o") for s in sources]
-    cmds = [[cc, *HIP_FLAGS, "-c", str(s), "-o", str(o)] for s, o in zip(sources, objs)]
+    cmds = [[cc, *HIP_FLAGS, *EXTRA_FLAGS.get(s.stem, []), "-c", str(s), "-o", str(o)]
+            for s, o in zip(sources, objs)]
     jobs = jobs or min(len(cmds), os.cpu_count() or 4, 8)
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
         for cmd, fut in [(c, ex.submit(_run, c)) for c in cmds]:

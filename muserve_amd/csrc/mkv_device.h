@@ -57,25 +57,38 @@ __device__ __forceinline__ bool offsets_ok(const int32_t* cu, int32_t n, int64_t
   return !__syncthreads_or(bad);
 }
 
-// Tiles of 64 rows of packed sequences without a list of them: tile c of
-// sequence b has the id cu[b] / 64 + b + c. Ids never meet (a sequence of m
-// rows from cu[b] has at most (cu[b] + m) / 64 - cu[b] / 64 + 1 tiles), and
-// rows / 64 + n ids cover all of them; ids in between belong to no tile.
-__device__ __forceinline__ int64_t first_tile(const int32_t* cu, int32_t b) {
-  return (int64_t)(cu[b] >> 6) + b;
+// Tiles of R rows of packed sequences without a list of them: tile c of
+// sequence b has the id cu[b] / R + b + c. Ids never meet (a sequence of m rows
+// from cu[b] has at most (cu[b] + m) / R - cu[b] / R + 1 tiles), and rows / R + n
+// ids cover all of them; ids in between belong to no tile.
+__device__ __forceinline__ int32_t first_tile(int32_t row, int32_t b, int32_t r = 64) {
+  return row / r + b;
 }
-inline int64_t tile_ids(int64_t rows, int32_t n) { return rows / 64 + n; }
+inline int64_t tile_ids(int64_t rows, int32_t n, int32_t r = 64) { return rows / r + n; }
 // The sequence that a tile id would belong to.
-__device__ __forceinline__ int32_t tile_sequence(const int32_t* cu, int32_t n, int64_t id) {
+__device__ __forceinline__ int32_t tile_sequence(const int32_t* cu, int32_t n, int64_t id,
+                                                 int32_t r = 64) {
   int32_t lo = 0, hi = n - 1;
   while (lo < hi) {
     const int32_t mid = (lo + hi + 1) >> 1;
-    if (first_tile(cu, mid) <= id)
+    if (first_tile(cu[mid], mid, r) <= id)
       lo = mid;
     else
       hi = mid - 1;
   }
   return lo;
+}
+
+// x / (1 + e^-x) by the hardware's 2^x and reciprocal, both within an fp32 step
+// (with the exponent's rounding |x| 2^-24 of the result): for outputs in bf16.
+__device__ __forceinline__ float silu_bf16(float x) {
+  return x * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * x));
+}
+// Two floats to bf16, to nearest even, by one instruction.
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){lo, hi}, bf16x2));
 }
 
 // Arguments of a block-table gather (see mkv_gather_bf16 in mkv.h). Row

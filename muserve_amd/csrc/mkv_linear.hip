@@ -147,8 +147,6 @@ struct Rows {
   }
 };
 
-__device__ __forceinline__ float silu(float x) { return x / (1.f + expf(-x)); }
-
 __device__ __forceinline__ float weight_at(const uint8_t* w, int32_t bf16, int64_t i) {
   return bf16 ? bf16_at(w + 2 * i) : *(const float*)(w + 4 * i);
 }
@@ -175,7 +173,7 @@ __global__ __launch_bounds__(THREADS) void linear_decode_kernel(LinArgs a) {
   for (int i = 0; i < kRows; ++i)
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const u32x4 x = ld16((const uint8_t*)(st + (r0 + kGroups * i) * kDim + 32 * c + 4 * l));
+      const u32x4 x = ld_nt((const uint8_t*)(st + (r0 + kGroups * i) * kDim + 32 * c + 4 * l));
 #pragma unroll
       for (int j = 0; j < 4; ++j) m.s[i][4 * c + j] = bits_f32(x[j]);
     }
@@ -194,7 +192,7 @@ __global__ __launch_bounds__(THREADS) void linear_decode_kernel(LinArgs a) {
       u32x4 x;
 #pragma unroll
       for (int j = 0; j < 4; ++j) x[j] = f32_bits(m.s[i][4 * c + j]);
-      st16((uint8_t*)(st + (r0 + kGroups * i) * kDim + 32 * c + 4 * l), x);
+      st_stream((uint8_t*)st, (uint32_t)((r0 + kGroups * i) * kDim + 32 * c + 4 * l) * 4, x);
     }
   if (a.z) {  // uniform: o / sqrt(mean(o^2) + eps) w silu(z)
     __shared__ float part[THREADS / 64];
@@ -214,7 +212,7 @@ __global__ __launch_bounds__(THREADS) void linear_decode_kernel(LinArgs a) {
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
       const int d = r0 + kGroups * i;
-      o[i] = o[i] * r * weight_at(a.w, a.w_bf16, d) * silu(bf16_at(zp + 2 * d));
+      o[i] = o[i] * r * weight_at(a.w, a.w_bf16, d) * silu_bf16(bf16_at(zp + 2 * d));
     }
   }
   if (l == 0) {
@@ -288,6 +286,1102 @@ __global__ __launch_bounds__(256) void linear_scan_kernel(LinArgs a, int32_t* ok
 }
 
 // ---------------------------------------------------------------------------
+// Prompts in chunks of 64 tokens, on the matrix cores. With G_i the sum of a
+// chunk's log decays up to token i, k and q normalised, S0 the state before it:
+//     A_ij = beta_i e^(G_i - G_j) k_i . k_j   (j < i),   T = (I + A)^-1
+//     U = T diag(beta) (V - diag(e^G) K S0^T) (U = V without the delta rule)
+//     O = scale (diag(e^G) Q S0^T + P U),     P_ij = e^(G_i - G_j) q_i . k_j  (j <= i)
+//     S = e^G_63 S0 + sum_j e^(G_63 - G_j) u_j k_j^T
+// linear_prep_kernel makes what does not depend on the state (T, P and the
+// factors of each token), for all chunks at once; linear_chunk_kernel walks a
+// sequence's chunks with the state in registers.
+//
+// Precision: the matrix instructions of a chunk take fp16. Rows of k and q are
+// brought near 1 by a power of two, which the factors of their tokens undo: a
+// bf16 row is exact in fp16 then, but for elements below 2^-17 of its largest,
+// rounded to 2^-25 of that. An fp32 operand that the state depends on (the
+// state itself, the right-hand side, T, u) is two fp16 parts, 22 bits; the
+// product of two such drops the lower parts' (2^-22). What only the bf16 output
+// sees (the state under Q, P, u under P) is one part, 2^-12. Sums run in fp32
+// in the matrix cores. A wave keeps its state times a power of two f that holds
+// its largest element in [2^-2, 2^9], and the values go in times f too: fp16's
+// smallest step is then 2^-22 of the state or less. Against float64 a state is
+// 3e-7 off (1e-7 for fp32 arithmetic), an output 2.7e-4 before its rounding to
+// bf16 (1.66e-3). Three bf16 parts were as exact as fp32, but took 182 matrix
+// and 630 vector instructions a chunk where this takes 104 and 440.
+//
+// A column of a matrix operand (one value dim) never mixes with another, but
+// the rows (tokens) of a chunk do, also through zeros. So that what is out of
+// the ordinary in one token (infinities, NaN, a value far past f's scale) reaches
+// only the tokens after it, such a chunk is walked token by token instead: inputs
+// past 2^60 in size, a chunk whose decays grow by more than e^2 (where products
+// could overflow and the recurrence not), operands past the limits below.
+// ---------------------------------------------------------------------------
+typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 bf16x8;
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((__vector_size__(4 * sizeof(float)))) float f32x4;
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) u32x2 lds_u32x2;
+typedef __attribute__((address_space(3))) float lds_f32;
+typedef __attribute__((address_space(3))) double lds_f64;
+typedef __attribute__((address_space(3))) uint16_t lds_u16;
+
+constexpr int kChunk = 64;
+// Operand images: blocks of 1 KiB, 16 bytes per lane, one v_mfma_f32_16x16x32
+// A operand each. Lane (m = lane % 16, d = lane / 16) has row m, columns
+// 32 s + 16 (j / 4) + 4 d + j % 4, j = 0 .. 7: the order in which a lane holds
+// the rows of two 16 x 16 results, so that results are B operands as they lie.
+constexpr int kFrag = 1024;
+constexpr int kKeyImage = 48 * kFrag;  // of a chunk's key head: K, Q (4 row blocks x 4), K^T (8 x 2)
+constexpr int kLower = 6;              // operands of a 64 x 64 lower triangle
+constexpr int kTParts = 2, kPParts = 1;
+// The factors of a chunk's tokens, [64] each: of K S0^T in the right-hand side,
+// of u in the state, e^G, of the output, of v; then e^G_63, whether to walk, and
+// the largest factor of v.
+constexpr int kFactors = 2048, kFacX = 0, kFacU = 64, kFacG = 128, kFacO = 192, kFacV = 256;
+constexpr int kFacAll = 320, kFacWalk = 321, kFacMax = 322;
+constexpr int head_image(bool delta) {
+  return (delta ? kTParts * kLower * kFrag : 0) + kPParts * kLower * kFrag + kFactors;
+}
+__device__ __forceinline__ constexpr int lower(int mt, int s) {  // operand of rows 16 mt, step s
+  return mt < 2 ? mt : mt < 3 ? 2 + s : 4 + s;
+}
+constexpr uint32_t kHugeBf16 = (127 + 60) << 7;  // k, q: |x| >= 2^60, infinities and NaN
+constexpr double kLeastDecay = -1e5;             // e^g is 0 far above it; -inf would make NaN sums
+constexpr float kMostPart = 0x1p15f;    // of operands of fp16 parts (fp16 ends at 2^16)
+constexpr float kMostValue = 0x1p13f;   // of right-hand sides and u, in units of the state's scale
+constexpr float kMostState = 0x1p12f, kHighState = 0x1p9f, kLowState = 0x1p-2f;
+
+struct ChunkArgs {
+  uint8_t* keys;   // [ids][khs] key images
+  uint8_t* heads;  // [ids][khs * group] head images
+  int32_t kh0, khs;  // key heads of this launch
+  int32_t parts;     // workgroups per head
+  int32_t seg;       // tokens of a segment (a multiple of 64)
+  float* ends;       // [segment ids][heads of the launch][128][128]: B, then the first states
+  float* steps;      // as ends: M transposed; without the delta rule one factor each
+};
+
+__device__ __forceinline__ uint32_t lds_addr(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)p;
+}
+__device__ __forceinline__ u32x4 lds_ld16(uint32_t at) { return *(lds_u32x4*)(uintptr_t)at; }
+__device__ __forceinline__ void lds_st16(uint32_t at, u32x4 v) { *(lds_u32x4*)(uintptr_t)at = v; }
+__device__ __forceinline__ f32x4 lds_ldf4(uint32_t at) {
+  return __builtin_bit_cast(f32x4, lds_ld16(at));
+}
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+__device__ __forceinline__ f32x4 mfma(u32x4 x, u32x4 y, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x),
+                                                 __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ f32x4 mfma16(u32x4 x, u32x4 y, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x),
+                                                __builtin_bit_cast(f16x8, y), c, 0, 0, 0);
+}
+__device__ __forceinline__ uint32_t f16_pack(float lo, float hi) {  // to nearest even
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){lo, hi}, f16x2));
+}
+// 8 floats in fp16; cut: and what that leaves of them (exact)
+__device__ __forceinline__ u32x4 upper(const float (&x)[8]) {
+  u32x4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = f16_pack(x[2 * i], x[2 * i + 1]);
+  return w;
+}
+__device__ __forceinline__ u32x4 cut(float (&x)[8]) {
+  const u32x4 w = upper(x);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {  // x - half: one mixed fma each (the compiler converts and subtracts)
+    const uint32_t h = w[i];
+    float lo, hi;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(lo) : "v"(h), "v"(x[2 * i]));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+        : "=v"(hi)
+        : "v"(h), "v"(x[2 * i + 1]));
+    x[2 * i] = lo;
+    x[2 * i + 1] = hi;
+  }
+  return w;
+}
+// max(m, |x|, |y|): a NaN among them is passed over, or (any_of) is the result
+__device__ __forceinline__ float any_of(float m, float x, float y) {
+  asm("v_maximum3_f32 %0, %0, |%1|, |%2|" : "+v"(m) : "v"(x), "v"(y));
+  return m;
+}
+__device__ __forceinline__ float most_of(float m, float x, float y) {
+  asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(m) : "v"(x), "v"(y));
+  return m;
+}
+
+// e^x of a difference of running sums. They are float64: sums far from 0 have
+// small differences. The result's error is |x| e^x 2^-24, at most 0.4 steps of 1.
+__device__ __forceinline__ float exp_of(double x) {
+  return __builtin_amdgcn_exp2f((float)(x * 1.4426950408889634074));
+}
+
+__device__ __forceinline__ bool huge(u32x4 w) {  // any of 8 bf16
+  bool h = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    h |= (w[i] & 0x7f80u) >= kHugeBf16 || ((w[i] >> 16) & 0x7f80u) >= kHugeBf16;
+  return h;
+}
+
+// One workgroup per (chunk, key head): K and Q rows through LDS, their images;
+// then each wave takes value heads of the group in turn. A wave keeps A as 10
+// 16 x 16 blocks in LDS (row-major, 16-byte chunks XORed by row / 4). The
+// inverse runs by blocks: the diagonal ones by forward substitution, a lane per
+// column, and the rest in fp32 matrix instructions (16x16x4).
+constexpr int kRowB = 272;  // bytes of a staged row: 256 and a pad against bank conflicts
+constexpr int kBlocks = 10;
+
+template <bool DELTA>
+__global__ __launch_bounds__(256) void linear_prep_kernel(LinArgs a, ChunkArgs c) {
+  __shared__ __attribute__((aligned(16))) uint8_t stage[2 * kChunk * kRowB];
+  __shared__ __attribute__((aligned(16))) uint8_t blocks[4][DELTA ? kBlocks * kFrag : kFrag];
+  __shared__ double run[4][kChunk];
+  __shared__ float strength[4][kChunk];
+  __shared__ float inv[2][kChunk];  // 1 / norms of k, q
+  __shared__ float unit[2][kChunk];  // the powers of two that bring rows of k, q near 1
+  const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, d = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t id = blockIdx.x;
+  const int32_t kh = c.kh0 + blockIdx.y;
+  const int32_t b = tile_sequence(a.cu, a.n, id);
+  const int64_t s0 = a.cu[b], s1 = a.cu[b + 1];
+  const int64_t t0 = s0 + (id - first_tile((int32_t)s0, b)) * kChunk;
+  if (s0 < 0 || s1 > a.tokens || t0 < s0 || t0 >= s1) return;  // uniform; no tile, or bad offsets
+  const int32_t len = (int32_t)(s1 - t0 < kChunk ? s1 - t0 : kChunk);
+
+  bool odd = false;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {  // 16 chunks of 16 bytes per row
+    const int r = (tid >> 4) + 16 * u, ch = tid & 15;
+    u32x4 kv = u32x4{0u, 0u, 0u, 0u}, qv = kv;
+    if (r < len) {
+      kv = ld16(a.k + (t0 + r) * a.k_stride + kh * (kDim * 2) + ch * 16);
+      qv = ld16(a.q + (t0 + r) * a.q_stride + kh * (kDim * 2) + ch * 16);
+    }
+    odd |= huge(kv) || huge(qv);
+    *(u32x4*)(stage + r * kRowB + ch * 16) = kv;
+    *(u32x4*)(stage + (kChunk + r) * kRowB + ch * 16) = qv;
+    float kk = 0.f, qq = 0.f;
+    uint32_t ke = 37u << 7, qe = ke;  // largest exponents (as bf16), from 2^-90 up
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      ke = max(ke, max(kv[i] & 0x7f80u, (kv[i] >> 16) & 0x7f80u));
+      qe = max(qe, max(qv[i] & 0x7f80u, (qv[i] >> 16) & 0x7f80u));
+      const float k0 = bits_f32(kv[i] << 16), k1 = bits_f32(kv[i] & 0xffff0000u);
+      const float q0 = bits_f32(qv[i] << 16), q1 = bits_f32(qv[i] & 0xffff0000u);
+      kk = fmaf(k0, k0, fmaf(k1, k1, kk));
+      qq = fmaf(q0, q0, fmaf(q1, q1, qq));
+    }
+#pragma unroll
+    for (int o = 1; o < 16; o *= 2) {
+      kk += __shfl_xor(kk, o);
+      qq += __shfl_xor(qq, o);
+      ke = max(ke, (uint32_t)__shfl_xor((int)ke, o));
+      qe = max(qe, (uint32_t)__shfl_xor((int)qe, o));
+    }
+    if (ch == 0) {
+      unit[0][r] = bits_f32(0x7f000000u - (ke << 16));  // 2^(127 - e) of exponent field e
+      unit[1][r] = bits_f32(0x7f000000u - (qe << 16));
+      inv[0][r] = a.qk_norm ? 1.f / sqrtf(kk + kL2Eps) : 1.f;
+      inv[1][r] = a.qk_norm ? 1.f / sqrtf(qq + kL2Eps) : 1.f;
+    }
+  }
+  odd = __syncthreads_or(odd);
+
+  const uint32_t sk = lds_addr(stage), sq = sk + kChunk * kRowB;
+  {
+    uint8_t* img = c.keys + (id * c.khs + blockIdx.y) * kKeyImage + lane * 16;
+    auto two = [](uint32_t w, float u) __attribute__((always_inline)) {  // bf16 pair times u
+      return f16_pack(bits_f32(w << 16) * u, bits_f32(w & 0xffff0000u) * u);
+    };
+#pragma unroll
+    for (int f = 0; f < 4; ++f) {  // row block `wave`, step f
+      const uint32_t at = (16 * wave + m) * kRowB + (32 * f + 4 * d) * 2;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const uint32_t from = (x ? sq : sk) + at;
+        const float u = unit[x][16 * wave + m];
+        const u32x2 lo = *(lds_u32x2*)(uintptr_t)from, hi = *(lds_u32x2*)(uintptr_t)(from + 32);
+        st16(img + (x * 16 + 4 * wave + f) * kFrag,
+             u32x4{two(lo.x, u), two(lo.y, u), two(hi.x, u), two(hi.y, u)});
+      }
+    }
+#pragma unroll
+    for (int f = 0; f < 4; ++f) {  // K^T: keys 16 (2 wave + f / 2) + m, tokens of step f % 2
+      u32x4 w;
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        const int t = 32 * (f & 1) + 16 * (j >> 2) + 4 * d + (j & 3);
+        const uint32_t at = sk + t * kRowB + (16 * (2 * wave + (f >> 1)) + m) * 2;
+        w[j >> 1] = f16_pack(
+            bits_f32((uint32_t) * (lds_u16*)(uintptr_t)at << 16) * unit[0][t],
+            bits_f32((uint32_t) * (lds_u16*)(uintptr_t)(at + kRowB) << 16) * unit[0][t + 1]);
+      }
+      st16(img + (32 + 4 * wave + f) * kFrag, w);
+    }
+  }
+  // without norms, keys far from 1 would put u far from the state's scale: u
+  // goes in times the largest row's power of two
+  float size = 1.f;
+  if (!a.qk_norm) {
+    float x = unit[0][lane];  // (the reciprocals of the rows' sizes)
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) x = fminf(x, __shfl_xor(x, o));
+    size = fmaxf(1.f / x, 0x1p-30f);
+  }
+
+  const uint32_t blk = lds_addr(blocks[wave]);
+  // element (row i, 4 columns from 4 x) of block n
+  auto block4 = [&](int n, int i, int x) __attribute__((always_inline)) {
+    return blk + (uint32_t)(n * kFrag + i * 64 + ((x ^ ((i >> 2) & 3)) << 4));
+  };
+  // e^(G_16 mt - G_j) for j < 16 mt, mt from 1 on: in the last block's place, which is written last
+  const uint32_t since = blk + (DELTA ? (kBlocks - 1) * kFrag : 0);
+  for (int32_t o = wave; o < a.group; o += 4) {
+    const int32_t h = kh * a.group + o;
+    uint8_t* img = c.heads + ((id * c.khs + blockIdx.y) * a.group + o) * head_image(DELTA);
+    // lane i has token i's gates
+    float g = 0.f, beta = 0.f;
+    if (lane < len) load_gates(a, t0 + lane, h, g, beta);
+    float grow = fmaxf(g, 0.f);
+#pragma unroll
+    for (int s = 1; s < 64; s *= 2) grow += __shfl_xor(grow, s);
+    bool walk = odd || !(grow <= 2.f) ||
+                __builtin_amdgcn_ballot_w64(!(g <= 2.f) || !(fabsf(beta) < 0x1p20f)) != 0;
+    double gsum = g < (float)kLeastDecay ? kLeastDecay : (double)g;
+#pragma unroll
+    for (int s = 1; s < 64; s *= 2) {
+      const double x = __shfl_up(gsum, s);
+      if (lane >= s) gsum += x;
+    }
+    const double all = __shfl(gsum, 63);
+    const float rk = inv[0][lane] / unit[0][lane], rq = inv[1][lane] / unit[1][lane];
+    const float head = exp_of(gsum), strong = DELTA ? beta * size : size;
+    wave_sync();  // the last head's readers are done
+    run[wave][lane] = gsum;
+    strength[wave][lane] = beta;
+    wave_sync();
+#pragma unroll
+    for (int mt = 1; mt < 4; ++mt) {
+      const double x = run[wave][16 * mt] - gsum;
+      *(lds_f32*)(uintptr_t)(since + ((mt - 1) * kChunk + lane) * 4) = lane < 16 * mt ? exp_of(x) : 0.f;
+    }
+    wave_sync();
+    float* fac = (float*)(img + head_image(DELTA) - kFactors);
+    fac[kFacX + lane] = head * rk * strong;
+    fac[kFacU + lane] = exp_of(all - gsum) * rk / size;
+    fac[kFacG + lane] = head;
+    fac[kFacO + lane] = a.scale * rq;
+    fac[kFacV + lane] = strong;
+    float most = fabsf(strong), largest = 0.f;  // largest: of the operands written below
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) most = fmaxf(most, __shfl_xor(most, o));
+    uint8_t* pimg = img + (DELTA ? kTParts * kLower * kFrag : 0) + lane * 16;
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      u32x4 km[4], qm[4];  // rows 16 mt + m of K and Q as B operands
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        km[s] = lds_ld16(sk + (16 * mt + m) * kRowB + (32 * s + 8 * d) * 2);
+        qm[s] = lds_ld16(sq + (16 * mt + m) * kRowB + (32 * s + 8 * d) * 2);
+      }
+      const int i = 16 * mt + m;
+      // e^(G_i - G_j) below the diagonal block: by way of the block's first token
+      const double gi = run[wave][i];
+      const float from = exp_of(gi - run[wave][16 * mt]);
+      const float ki = inv[0][i] * strength[wave][i], qi = unit[1][i] / size;
+      float p[8];
+#pragma unroll
+      for (int nt = 0; nt <= mt; ++nt) {
+        // k_i . k_j and q_i . k_j for j = 16 nt + 4 d + r
+        f32x4 kk = {0.f, 0.f, 0.f, 0.f}, qk = kk;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const u32x4 kn = lds_ld16(sk + (16 * nt + m) * kRowB + (32 * s + 8 * d) * 2);
+          if (DELTA) kk = mfma(kn, km[s], kk);
+          qk = mfma(kn, qm[s], qk);
+        }
+        f32x4 av, decay;
+        if (nt < mt) {
+          decay = lds_ldf4(since + ((mt - 1) * kChunk + 16 * nt + 4 * d) * 4);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) decay[r] *= from;
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int j = 16 * nt + 4 * d + r;
+            decay[r] = exp_of(j <= i ? gi - run[wave][j] : 0.);
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int j = 16 * nt + 4 * d + r;
+          const float w = inv[0][j] * decay[r];
+          av[r] = j < i ? ki * w * kk[r] : 0.f;
+          p[4 * (nt & 1) + r] = j <= i ? qi * w * qk[r] : 0.f;
+          if (!(nt & 1)) p[4 + r] = 0.f;
+        }
+        if (DELTA) lds_st16(block4(mt * (mt + 1) / 2 + nt, m, d), __builtin_bit_cast(u32x4, av));
+        if ((nt & 1) || nt == mt) {
+#pragma unroll
+          for (int r = 0; r < 8; ++r) largest = fmaxf(largest, fabsf(p[r]));
+          st16(pimg + lower(mt, nt >> 1) * kFrag, upper(p));
+        }
+      }
+    }
+    if (DELTA) {
+      wave_sync();
+      {  // the diagonal blocks' inverses: lane (m, d) has column m of block d's
+        float t[16];
+        const int n = d * (d + 1) / 2 + d;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float acc = i == m ? 1.f : 0.f;
+#pragma unroll
+          for (int x = 0; x < (i + 3) / 4; ++x) {
+            const f32x4 av = lds_ldf4(block4(n, i, x));
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (4 * x + r < i) acc = fmaf(-av[r], t[4 * x + r], acc);
+          }
+          t[i] = acc;
+        }
+        wave_sync();
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          *(lds_f32*)(uintptr_t)(block4(n, i, m >> 2) + (m & 3) * 4) = t[i];
+        wave_sync();
+      }
+      f32x4 tb[kBlocks];  // T's blocks as results: lane has rows 4 d + r, column m
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        const int diag = mt * (mt + 1) / 2 + mt;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          tb[diag][r] = *(lds_f32*)(uintptr_t)(block4(diag, 4 * d + r, m >> 2) + (m & 3) * 4);
+        const f32x4 left = lds_ldf4(block4(diag, m, d));
+#pragma unroll
+        for (int nt = 0; nt < mt; ++nt) {  // -T_mm sum_x A_mx T_xn
+          f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int x = nt; x < mt; ++x) {
+            const f32x4 av = lds_ldf4(block4(mt * (mt + 1) / 2 + x, m, d));
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+              acc = __builtin_amdgcn_mfma_f32_16x16x4f32(av[s], tb[x * (x + 1) / 2 + nt][s], acc, 0,
+                                                         0, 0);
+          }
+          f32x4 res = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+            res = __builtin_amdgcn_mfma_f32_16x16x4f32(-left[s], acc[s], res, 0, 0, 0);
+          tb[mt * (mt + 1) / 2 + nt] = res;
+        }
+      }
+      wave_sync();
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int nt = 0; nt <= mt; ++nt) {
+          const int n = mt * (mt + 1) / 2 + nt;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            largest = fmaxf(largest, fabsf(tb[n][r]));
+            *(lds_f32*)(uintptr_t)(block4(n, 4 * d + r, m >> 2) + (m & 3) * 4) = tb[n][r];
+          }
+        }
+      wave_sync();
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int s = 0; s <= mt >> 1; ++s) {
+          float x[8];
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const int nt = 2 * s + y;
+            f32x4 v = {0.f, 0.f, 0.f, 0.f};
+            if (nt <= mt) v = lds_ldf4(block4(mt * (mt + 1) / 2 + nt, m, d));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[4 * y + r] = v[r];
+          }
+#pragma unroll
+          for (int part = 0; part < kTParts; ++part) {
+            const u32x4 w = part + 1 < kTParts ? cut(x) : upper(x);
+            st16(img + lane * 16 + (part * kLower + lower(mt, s)) * kFrag, w);
+          }
+        }
+    }
+    walk |= __builtin_amdgcn_ballot_w64(!(largest < kMostPart)) != 0;
+    if (lane == 0) {
+      fac[kFacAll] = exp_of(all);
+      ((int32_t*)fac)[kFacWalk] = walk;
+      fac[kFacMax] = most;
+    }
+  }
+}
+
+// Instruction classes of __builtin_amdgcn_sched_group_barrier.
+constexpr int kSchedValu = 0x002, kSchedMfma = 0x008, kSchedDsRead = 0x100;
+
+// 16 bytes per lane from base + voff into LDS at lds + 16 * lane, issued from
+// inline assembly so that the compiler neither waits for it nor moves LDS
+// accesses across it; the waits are explicit. M0 holds the destination.
+__device__ __forceinline__ void dma16(const uint8_t* base, uint32_t voff, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(base)
+               : "memory");
+}
+// every load and store of this wave is done, and every wave of the workgroup
+// has come here
+__device__ __forceinline__ void arrive_all() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// What a workgroup of linear_chunk_kernel walks: whole sequences (from slot to
+// slot), or segments of them in two passes. A segment's final state is affine in
+// its first one, S -> S M + B: kEnds computes B (a walk from zeros, or from the
+// slot for a sequence's first segment) and M (a walk of 128 more rows from the
+// identity with v = 0; without the delta rule M is a factor),
+// linear_join_kernel the segments' first states from them, and kRows walks
+// again from those and writes the outputs.
+enum { kWhole = 0, kEnds = 1, kRows = 2 };
+
+// One workgroup of WAVES waves per 16 WAVES value dims of a (head, sequence or
+// segment); wave w holds the state of 16 of them in registers, as results of
+// 16x16x32 (lane (n, d): value dim n, keys 16 x + 4 d + r), which are also the B
+// operands of K S0^T and Q S0^T. The images of a chunk go straight into LDS,
+// shared by the waves, while the chunk before it is computed: two buffers, one
+// barrier a chunk.
+template <int WAVES, bool DELTA, int MODE>
+__global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(LinArgs a, ChunkArgs c,
+                                                                             int32_t* ok_word) {
+  constexpr bool kOut = MODE != kEnds;
+  // a buffer: K, K^T, T, then Q and P, then the factors (offsets from the low
+  // part's base, or from the high part's for what follows it)
+  constexpr int kK = 0, kKt = 16 * kFrag, kQ = 32 * kFrag;
+  constexpr int kLow = (kOut ? 48 : 32) * kFrag;
+  constexpr int kT = 0, kP = kT + (DELTA ? kTParts * kLower * kFrag : 0);
+  constexpr int kFac = kP + (kOut ? kPParts * kLower * kFrag : 0);
+  constexpr int kBuffer = kLow + kFac + kFactors;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kBuffer];
+  uint32_t l0 = lds_addr(lds), l1 = l0 + kBuffer;  // this chunk's buffer, and the next one's
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, d = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int32_t part = blockIdx.x % c.parts, o = blockIdx.x / c.parts;  // o: head of the launch
+  const int32_t h = c.kh0 * a.group + o, kh = h / a.group;
+  // kEnds: the parts behind the value dims' are the rows of M
+  const bool ident = MODE == kEnds && part * 16 * WAVES >= kDim;
+  const int d0 = part * 16 * WAVES + 16 * wave - (ident ? kDim : 0);  // the wave's value dims
+  const bool first = blockIdx.x == 0 && c.kh0 == 0 && tid == 0;
+  const bool ok = offsets_ok(a.cu, a.n, a.tokens);
+  if (MODE != kEnds && first && blockIdx.y == 0) *ok_word = ok;
+  if (!ok) {
+    if (MODE != kEnds && first && blockIdx.y == 0) raise_err(a.err, MKV_DEVERR_TABLE);
+    return;
+  }
+  int32_t b = blockIdx.y;
+  if (MODE != kWhole) b = tile_sequence(a.cu, a.n, blockIdx.y, c.seg);
+  const int64_t q0 = ld_const(a.cu + b), q1 = ld_const(a.cu + b + 1);  // the sequence's rows
+  int64_t s0 = q0, s1 = q1;                                            // this workgroup's
+  int64_t seg = 0;
+  if (MODE != kWhole) {
+    seg = (int64_t)blockIdx.y - first_tile((int32_t)q0, b, c.seg);
+    s0 = q0 + seg * c.seg;
+    s1 = s0 + c.seg < q1 ? s0 + c.seg : q1;
+    if (s0 >= q1) return;  // uniform: no such segment
+  }
+  const bool last = s1 == q1;
+  const int32_t slot = ld_const(a.slots + b);
+  const int64_t out_row = (int64_t)a.hv * (kDim * 2);
+  uint8_t* outp = a.out + h * (kDim * 2) + (d0 + n) * 2;
+  if (slot < 0 || slot >= a.pool_slots) {  // uniform
+    if (!kOut) return;
+    if (first && s0 == q0) raise_err(a.err, MKV_DEVERR_STATE_SLOT);
+    for (int64_t t = s0 + d; t < s1; t += 4) *(uint16_t*)(outp + t * out_row) = 0;
+    return;
+  }
+  if (MODE == kEnds && (last || (ident && seg == 0))) return;  // uniform: not asked for
+  const int32_t chunks = (int32_t)((s1 - s0 + kChunk - 1) / kChunk);
+  if (chunks == 0) return;
+  const int64_t id0 = (q0 >> 6) + b + ((s0 - q0) >> 6);
+  const uint8_t* kimg = c.keys + (id0 * c.khs + (kh - c.kh0)) * kKeyImage;
+  const uint8_t* himg = c.heads + (id0 * c.khs * a.group + o) * head_image(DELTA);
+  const int64_t knext = (int64_t)c.khs * kKeyImage;
+  const int64_t hnext = (int64_t)c.khs * a.group * head_image(DELTA);
+
+  // A wave's loads of a chunk's images, in kLoads pieces of a few each: issued in
+  // one go they would hold the wave up until the address unit has taken them.
+  constexpr int kKeys = kLow / kFrag, kTs = (DELTA ? kTParts * kLower : 0);
+  constexpr int kFs = kFactors / kFrag, kPs = (kOut ? kPParts * kLower : 0) + kFs;  // P, factors
+  constexpr int kAll = kKeys + kTs + kPs, kEach = (kAll + WAVES - 1) / WAVES, kLoads = 3;
+  auto load_images = [&](int32_t ci, uint32_t to, int piece) __attribute__((always_inline)) {
+    const uint8_t* kp = kimg + ci * knext;
+    const uint8_t* hp = himg + ci * hnext;
+#pragma unroll
+    for (int f = piece * kEach / kLoads; f < (piece + 1) * kEach / kLoads; ++f) {
+      const int i = f * WAVES + wave;
+      if (f * WAVES + WAVES <= kKeys || i < kKeys) {  // images lie as K, Q, K^T
+        const int from = i < 16 ? i : i < 32 ? i + 16 : i - 16;
+        dma16(kp, from * kFrag + lane * 16, to + i * kFrag);
+      } else if (i < kAll) {
+        const int j = i - kKeys, from = kOut || j < kTs ? j : j + kPParts * kLower;
+        dma16(hp, from * kFrag + lane * 16, to + kLow + j * kFrag);
+      }
+    }
+  };
+  // A chunk's rows of v and out through buffer descriptors that end with the
+  // sequence: loads past it give zeros, stores past it are dropped, and the 16
+  // rows of a lane need one address register.
+  auto rows_of = [&](const uint8_t* base, int64_t stride, int32_t ci) __attribute__((always_inline)) {
+    const int64_t t0 = s0 + (int64_t)ci * kChunk;
+    const int32_t len = (int32_t)(s1 - t0 < kChunk ? s1 - t0 : kChunk);
+    return __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(base + t0 * stride + h * (kDim * 2)), (short)0,
+        (int)((len - 1) * (int32_t)stride + kDim * 2), 0x00020000);
+  };
+  const int32_t vs = (int32_t)a.v_stride, os = (int32_t)out_row;
+  const uint32_t vat = (uint32_t)(4 * d * vs + (d0 + n) * 2), oat = (uint32_t)(4 * d * os + (d0 + n) * 2);
+  // bf16 of this lane's value dim: tokens 16 x + 4 d + r of the next chunk, and two each of this one
+  uint32_t v[8], vnext[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) vnext[i] = 0;
+  auto load_v = [&](int32_t ci) __attribute__((always_inline)) {
+    if (MODE == kEnds && ident) return;  // uniform
+    const __amdgpu_buffer_rsrc_t rows = rows_of(a.v, a.v_stride, ci);
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      vnext[i] = __builtin_amdgcn_raw_buffer_load_b16(rows, vat, (16 * (i >> 2) + (i & 3)) * vs, 0);
+  };
+
+  const int64_t row0 = (int64_t)(d0 + n) * kDim + 4 * d;  // this lane's first key of its value dim
+  float* st = a.state + ((int64_t)slot * a.hv + h) * kStateHead + row0;
+  const int64_t segment = ((int64_t)blockIdx.y * c.khs * a.group + o) * kStateHead;
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) load_images(0, l0, i);
+  load_v(0);
+  f32x4 s[8];
+  if (MODE == kEnds && (ident || seg > 0)) {
+#pragma unroll
+    for (int x = 0; x < 8; ++x)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[x][r] = ident && 16 * x + 4 * d + r == d0 + n ? 1.f : 0.f;
+  } else {
+    const float* from = MODE == kRows && !(seg == 0 && last) ? c.ends + segment + row0 : st;
+#pragma unroll
+    for (int x = 0; x < 8; ++x)
+      s[x] = __builtin_bit_cast(f32x4, ld16((const uint8_t*)(from + 16 * x)));
+  }
+  float whole = 1.f;  // kEnds without the delta rule: the segment's decay
+
+  // The state times f. Its scale is what came before a chunk, so that a value
+  // far above it is seen as such: after every chunk the state's largest element
+  // if that has left its range, for a first chunk on zeros its first token's.
+  float f = 1.f, inv_f = 1.f;
+  auto over_wave = [&](float x) __attribute__((always_inline)) {
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) x = fmaxf(x, __shfl_xor(x, o));
+    return x;
+  };
+  auto lane_most = [&]() __attribute__((always_inline)) {
+    float x = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x = most_of(most_of(x, s[i][0], s[i][1]), s[i][2], s[i][3]);
+    return x;
+  };
+  bool large = false;  // the state does not fit fp16 (infinities)
+  auto rescale = [&](float most) __attribute__((always_inline)) {  // the wave's largest |s|
+    if (most > 0x1p-100f && most < 0x1p100f) {
+      const float to = bits_f32(0x7f000000u - (f32_bits(most) & 0x7f800000u));  // most: [1, 2)
+      const float g = f * to;
+      if (g > 0x1p-100f && g < 0x1p100f) {
+        f = g;
+        inv_f = 1.f / g;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[i][r] *= to;
+        most *= to;
+      }
+    }
+    large = !(most < kMostState);
+  };
+
+  uint32_t ob[8];  // O in bf16, tokens 16 x + 4 d + (2 y, 2 y + 1) at 2 x + y
+  auto store_o = [&](int32_t ci) __attribute__((always_inline)) {
+    const __amdgpu_buffer_rsrc_t rows = rows_of(a.out, out_row, ci);
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      __builtin_amdgcn_raw_buffer_store_b16((uint16_t)(i & 1 ? ob[i >> 1] >> 16 : ob[i >> 1]), rows,
+                                            oat, (16 * (i >> 2) + (i & 3)) * os, 0);
+  };
+  bool stored = true;
+  for (int32_t ci = 0; ci < chunks; ++ci) {
+    const int64_t t0 = s0 + (int64_t)ci * kChunk;
+    const int32_t len = (int32_t)(s1 - t0 < kChunk ? s1 - t0 : kChunk);
+    arrive_all();  // the chunk's images and v are there; the other buffer is read
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[i] = vnext[2 * i] | (vnext[2 * i + 1] << 16);
+      asm volatile("" : "+v"(v[i]));
+    }
+    auto value = [&](int i) __attribute__((always_inline)) {
+      return bits_f32(i & 1 ? v[i >> 1] & 0xffff0000u : v[i >> 1] << 16);
+    };
+    if (ci == 0) {
+      float most = over_wave(lane_most());
+      if (most == 0.f && !ident) {
+        float x = fabsf(value(0));
+        if (d != 0) x = 0.f;
+        most = over_wave(x);
+        if (most == 0.f) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x = fmaxf(x, fabsf(value(i)));
+          most = over_wave(x);
+        }
+        most *= *(lds_f32*)(uintptr_t)(l0 + kLow + kFac + kFacMax * 4);
+      }
+      rescale(most);
+    }
+    const bool more = ci + 1 < chunks;
+    // lane bases of the buffer's two parts: operands lie at constants from them
+    uint32_t low = l0 + lane * 16, high = l0 + kLow + lane * 16;
+    asm volatile("" : "+v"(low), "+v"(high));
+    uint32_t fac = l0 + kLow + kFac + d * 16;
+    asm volatile("" : "+v"(fac));
+    auto frag = [&](int at) __attribute__((always_inline)) { return lds_ld16(low + at); };
+    auto later = [&](int at) __attribute__((always_inline)) { return lds_ld16(high + at); };
+    // X = K S0^T, Y = Q S0^T. Operand reads run a step ahead of their use, and
+    // the vector unit cuts the next step's state while the matrix cores run.
+    f32x4 xa[4], ya[4];
+    u32x4 kf[2][4], qf[2][4], sp[2][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) xa[i] = ya[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto read_kq = [&](int ks) __attribute__((always_inline)) {
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        if (DELTA) kf[ks & 1][mt] = frag(kK + (4 * mt + ks) * kFrag);
+        if (kOut) qf[ks & 1][mt] = frag(kQ + (4 * mt + ks) * kFrag);
+      }
+    };
+    auto cut_state = [&](int ks) __attribute__((always_inline)) {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = s[2 * ks + (j >> 2)][j & 3];
+      if (DELTA) {
+        sp[ks & 1][0] = cut(x);
+        sp[ks & 1][1] = upper(x);
+      } else {
+        sp[ks & 1][0] = upper(x);
+      }
+    };
+    f32x4 cf[4], bf[4], ef[4];
+    u32x4 tq[2][4];  // T's parts of two row blocks: (0, 1; step 0), (2, 3; 0), (2, 3; 1)
+    auto read_t = [&](int to, int mt0, int ks) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+          tq[to][2 * i + p] = later(kT + (p * kLower + lower(mt0 + i, ks)) * kFrag);
+    };
+    if (DELTA || kOut) {
+      read_kq(0);
+      cut_state(0);
+    }
+    if (more) load_v(ci + 1);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      if (ks < 3) {
+        if (DELTA || kOut) {
+          read_kq(ks + 1);
+          cut_state(ks + 1);
+        }
+      } else if (DELTA) {
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) {
+          cf[mt] = lds_ldf4(fac + (kFacX + 16 * mt) * 4);
+          bf[mt] = lds_ldf4(fac + (kFacV + 16 * mt) * 4);
+        }
+        read_t(0, 0, 0);
+      }
+      if (DELTA || kOut) {
+#pragma unroll
+        for (int p = DELTA ? 1 : 0; p >= 0; --p) {
+          if (DELTA)
+#pragma unroll
+            for (int mt = 0; mt < 4; ++mt) xa[mt] = mfma16(kf[ks & 1][mt], sp[ks & 1][p], xa[mt]);
+          if (kOut && p == 0)
+#pragma unroll
+            for (int mt = 0; mt < 4; ++mt) ya[mt] = mfma16(qf[ks & 1][mt], sp[ks & 1][p], ya[mt]);
+        }
+        if (ks < 3) {
+          __builtin_amdgcn_sched_group_barrier(kSchedDsRead, (DELTA ? 4 : 0) + (kOut ? 4 : 0), 0);
+#pragma unroll
+          for (int i = 0; i < (DELTA ? 8 : 0) + (kOut ? 4 : 0); ++i) {
+            __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(kSchedValu, 2, 0);
+          }
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (ks < kLoads && more) load_images(ci + 1, l1, ks);
+    }
+    const int32_t walk = __builtin_amdgcn_readfirstlane(
+        *(__attribute__((address_space(3))) int32_t*)(uintptr_t)(l0 + kLow + kFac + kFacWalk * 4));
+    const float decay = *(lds_f32*)(uintptr_t)(l0 + kLow + kFac + kFacAll * 4);
+    if (MODE == kEnds && !DELTA) whole *= decay;
+    const uint32_t lnow = l0;
+    l0 = l1;
+    l1 = lnow;
+    f32x4 u[4], rhs[4];
+    bool big;  // operands past their limits, infinities and NaN
+    u32x4 pf[4], tf[8];  // operands of P and of K^T
+    auto read_p = [&](int ks) __attribute__((always_inline)) {
+      if (!kOut) return;
+#pragma unroll
+      for (int mt = 2 * ks; mt < 4; ++mt) pf[mt] = later(kP + lower(mt, ks) * kFrag);
+    };
+    auto read_kt = [&](int ks) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) tf[i] = frag(kKt + (2 * i + ks) * kFrag);
+    };
+    if (DELTA) {
+      read_t(1, 2, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      float most = 0.f;
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          rhs[mt][r] = fmaf(value(4 * mt + r), bf[mt][r] * f, -cf[mt][r] * xa[mt][r]);
+        most = any_of(any_of(most, rhs[mt][0], rhs[mt][1]), rhs[mt][2], rhs[mt][3]);
+      }
+      big = !(most < kMostValue);
+    } else {
+      const float bf = *(lds_f32*)(uintptr_t)(lnow + kLow + kFac + kFacV * 4) * f;
+      float most = 0.f;
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) u[mt][r] = value(4 * mt + r) * bf;
+        most = any_of(any_of(most, u[mt][0], u[mt][1]), u[mt][2], u[mt][3]);
+      }
+      big = !(most < kMostValue);
+    }
+    u32x4 r0[2], r1[2];
+    if (DELTA) {
+      auto mul_t = [&](int from, int mt0, const u32x4 (&r)[2]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int p = 2; p >= 0; --p)  // lower x upper, upper x lower, upper x upper
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            u[mt0 + i] = mfma16(tq[from][2 * i + (p == 2)], r[p == 1], u[mt0 + i]);
+      };
+      auto cut_rhs = [&](int ks, u32x4 (&to)[2]) __attribute__((always_inline)) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = rhs[2 * ks + (j >> 2)][j & 3];
+        to[0] = cut(x);
+        to[1] = upper(x);
+      };
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) u[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      cut_rhs(0, r0);
+      __builtin_amdgcn_sched_barrier(0);
+      cut_rhs(1, r1);
+      mul_t(0, 0, r0);
+      mul_t(1, 2, r0);
+#pragma unroll
+      for (int i = 0; i < 12; ++i) {
+        __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kSchedValu, 2, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      // (T's last blocks have been waited for; the others' use comes after more work)
+      read_t(0, 2, 1);
+    }
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) ef[mt] = lds_ldf4(fac + (kFacU + 16 * mt) * 4);
+    read_p(0);
+    __builtin_amdgcn_sched_barrier(0);
+    if (kOut && !stored) store_o(ci - 1);
+    stored = false;
+    if (DELTA) {
+#pragma unroll
+      for (int p = 2; p >= 0; --p)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          u[2 + i] = mfma16(tq[0][2 * i + (p == 2)], r1[p == 1], u[2 + i]);
+    }
+    // (fp16 operands: limits of u, and of u times its factors in the state)
+    {
+      float most = 0.f;
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) ef[mt][r] *= u[mt][r];
+        most = most_of(most_of(most, u[mt][0], u[mt][1]), u[mt][2], u[mt][3]);
+        most = most_of(most_of(most, ef[mt][0], ef[mt][1]), ef[mt][2], ef[mt][3]);
+      }
+      big |= !(most < kMostPart);
+    }
+    if (__builtin_expect(walk != 0 || large || __builtin_amdgcn_ballot_w64(big) != 0, 0)) {
+      // token by token: sums over keys in the lane's registers and the 4 lanes of its value dim
+      auto over_keys = [&](float x) __attribute__((always_inline)) {
+        x += __shfl_xor(x, 16);
+        x += __shfl_xor(x, 32);
+        return x;
+      };
+#pragma unroll 1
+      for (int32_t t = 0; t < len; ++t) {
+        const int64_t token = t0 + t;
+        const uint8_t* kp = a.k + token * a.k_stride + kh * (kDim * 2) + d * 8;
+        const uint8_t* qp = a.q + token * a.q_stride + kh * (kDim * 2) + d * 8;
+        float kx[8][4], kk = 0.f, qq = 0.f, kq = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float qx[4];
+          load4(kp + 32 * i, kx[i]);
+          if (kOut) load4(qp + 32 * i, qx);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            kk = fmaf(kx[i][r], kx[i][r], kk);
+            x = fmaf(s[i][r], kx[i][r], x);
+            if (kOut) {
+              qq = fmaf(qx[r], qx[r], qq);
+              kq = fmaf(kx[i][r], qx[r], kq);
+              y = fmaf(s[i][r], qx[r], y);
+            }
+          }
+        }
+        float rk = 1.f, rq = 1.f, g, beta;
+        if (a.qk_norm) {
+          rk = 1.f / sqrtf(over_keys(kk) + kL2Eps);
+          if (kOut) rq = 1.f / sqrtf(over_keys(qq) + kL2Eps);
+        }
+        load_gates(a, token, h, g, beta);
+        const float e = expf(g);
+        const float vt =
+            ident ? 0.f : f * bf16_at(a.v + token * a.v_stride + (h * kDim + d0 + n) * 2);
+        const float u = DELTA ? beta * (vt - e * rk * over_keys(x)) : vt;
+        if (kOut) {
+          const float out = a.scale * inv_f * (e * rq * over_keys(y) + u * (over_keys(kq) * rk * rq));
+          if (d == 0) *(uint16_t*)(outp + token * out_row) = f32_to_bf16_rne(out);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[i][r] = fmaf(u * rk, kx[i][r], e * s[i][r]);
+      }
+      stored = true;
+      rescale(over_wave(lane_most()));
+      continue;
+    }
+    // S = e^G S0 + (e^(G_63 - G) u) k^T; O = e^G Y + P U
+    f32x4 eg[4], of[4];
+    if (kOut) {
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) eg[mt] = lds_ldf4(fac + (kFacG + 16 * mt) * 4);
+    }
+    read_kt(0);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = ef[2 * ks + (j >> 2)][j & 3];
+      u32x4 w[2];
+      w[0] = cut(x);
+      w[1] = upper(x);
+      if (ks == 0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[i][r] *= decay;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      // the state's products while the vector unit rounds u and scales Y for the output's
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = u[2 * ks + (j >> 2)][j & 3];
+      const u32x4 uh = upper(x);
+      if (kOut && ks == 0) {
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) ya[mt][r] *= eg[mt][r];
+      }
+#pragma unroll
+      for (int p = 1; p >= 0; --p)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i] = mfma16(tf[i], w[p], s[i]);
+      if (kOut) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(kSchedValu, 2, 0);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (ks == 0) read_kt(1);
+      if (kOut) {
+#pragma unroll
+        for (int mt = 2 * ks; mt < 4; ++mt) ya[mt] = mfma16(pf[mt], uh, ya[mt]);
+        if (ks == 0) {
+          read_p(1);
+#pragma unroll
+          for (int mt = 0; mt < 4; ++mt) of[mt] = lds_ldf4(fac + (kFacO + 16 * mt) * 4);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (kOut) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int mt = i >> 1, j = 2 * (i & 1);
+        ob[i] = pack_bf16(ya[mt][j] * (of[mt][j] * inv_f), ya[mt][j + 1] * (of[mt][j + 1] * inv_f));
+      }
+    }
+    const float most = lane_most();
+    if (__builtin_amdgcn_ballot_w64(!(most < kHighState)) != 0 ||
+        __builtin_amdgcn_ballot_w64(most >= kLowState) == 0)
+      rescale(over_wave(most));
+  }
+  if (kOut && !stored) store_o(chunks - 1);
+#pragma unroll
+  for (int x = 0; x < 8; ++x)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s[x][r] *= inv_f;
+  if (MODE == kEnds) {
+    if (ident) {  // transposed, [key][row]: as linear_join_kernel reads it
+#pragma unroll
+      for (int x = 0; x < 8; ++x)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          c.steps[segment + (16 * x + 4 * d + r) * kDim + d0 + n] = s[x][r];
+    } else {
+#pragma unroll
+      for (int x = 0; x < 8; ++x)
+        st16((uint8_t*)(c.ends + segment + row0 + 16 * x), __builtin_bit_cast(u32x4, s[x]));
+      if (!DELTA && tid == 0 && part == 0)
+        c.steps[(int64_t)blockIdx.y * c.khs * a.group + o] = whole;
+    }
+  } else if (last) {
+#pragma unroll
+    for (int x = 0; x < 8; ++x) st16((uint8_t*)(st + 16 * x), __builtin_bit_cast(u32x4, s[x]));
+  }
+}
+
+// The first states of a sequence's segments, in the place of their B: one
+// workgroup per 16 value dims of a (head, sequence). S -> S M + B runs in fp32
+// matrix instructions (16x16x4), each wave making 32 of the 128 keys; the state
+// is handed round through LDS. Without the delta rule M is a factor.
+template <bool DELTA>
+__global__ __launch_bounds__(256) void linear_join_kernel(LinArgs a, ChunkArgs c) {
+  __shared__ __attribute__((aligned(16))) float state[2][kDim / 4][64];  // 4-key groups x (dim, key)
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, d = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int32_t part = blockIdx.x % (kDim / 16), o = blockIdx.x / (kDim / 16);
+  const int32_t h = c.kh0 * a.group + o, b = blockIdx.y;
+  if (!offsets_ok(a.cu, a.n, a.tokens)) return;
+  const int64_t q0 = ld_const(a.cu + b), q1 = ld_const(a.cu + b + 1);
+  const int32_t segs = (int32_t)((q1 - q0 + c.seg - 1) / c.seg);
+  const int64_t seg0 = first_tile((int32_t)q0, b, c.seg);
+  const int32_t slot = ld_const(a.slots + b);
+  if (segs < 2 || slot < 0 || slot >= a.pool_slots) return;  // uniform
+  const int64_t next = (int64_t)c.khs * a.group * kStateHead;
+  const int64_t row = (int64_t)(16 * part + n) * kDim + 4 * d + 32 * wave;  // this wave's keys
+  const int64_t at = seg0 * next + (int64_t)o * kStateHead;
+  float* ends = c.ends + at + row;
+  const float* slot0 = a.state + ((int64_t)slot * a.hv + h) * kStateHead + row;
+  f32x4 s[2], init[2];  // keys 32 wave + 16 y + 4 d + r of value dim n
+#pragma unroll
+  for (int y = 0; y < 2; ++y) {
+    s[y] = __builtin_bit_cast(f32x4, ld16((const uint8_t*)(ends + 16 * y)));
+    init[y] = __builtin_bit_cast(f32x4, ld16((const uint8_t*)(slot0 + 16 * y)));
+  }
+#pragma unroll
+  for (int y = 0; y < 2; ++y) st16((uint8_t*)(ends + 16 * y), __builtin_bit_cast(u32x4, init[y]));
+  // A operand rows: keys 32 wave + 16 y + n of M^T, columns 16 x + 4 d + r; they
+  // and B are read a segment ahead
+  const float* mt = c.steps + at + (32 * wave + n) * kDim + 4 * d;
+  // two segments ahead (three sets of registers, in turn)
+  f32x4 m[3][2][8], acc[3][2];
+  auto read_step = [&](int32_t i, f32x4 (&mi)[2][8], f32x4 (&bi)[2]) __attribute__((always_inline)) {
+    if (i + 1 >= segs) return;  // uniform; the last segment's B and M are not asked for
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      bi[y] = __builtin_bit_cast(f32x4, ld16((const uint8_t*)(ends + i * next + 16 * y)));
+      if (DELTA)
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+          mi[y][x] = __builtin_bit_cast(
+              f32x4, ld16((const uint8_t*)(mt + i * next + 16 * y * kDim + 16 * x)));
+    }
+  };
+  auto step = [&](int32_t i, f32x4 (&mi)[2][8], f32x4 (&bi)[2], f32x4 (&m2)[2][8],
+                  f32x4 (&b2)[2]) __attribute__((always_inline)) {
+    // this lane's B of the segment is read: the segment's first state takes its place
+#pragma unroll
+    for (int y = 0; y < 2; ++y)
+      st16((uint8_t*)(ends + i * next + 16 * y), __builtin_bit_cast(u32x4, s[y]));
+    if (i + 1 >= segs) return;
+    read_step(i + 2, m2, b2);
+    f32x4 sum[2] = {bi[0], bi[1]};
+    if (DELTA) {
+      float* to = &state[i & 1][0][0] + (8 * wave + d) * 64 + n * 4;
+#pragma unroll
+      for (int y = 0; y < 2; ++y) *(f32x4*)(to + y * 4 * 64) = s[y];
+      // (a barrier for LDS alone: the loads stay in flight)
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      const float* from = &state[i & 1][0][0] + d * 64 + n * 4;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const f32x4 k = *(const f32x4*)(from + x * 4 * 64);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+            sum[y] = __builtin_amdgcn_mfma_f32_16x16x4f32(mi[y][x][r], k[r], sum[y], 0, 0, 0);
+      }
+    } else {
+      const float f = c.steps[(seg0 + i) * c.khs * a.group + o];
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum[y][r] = fmaf(f, s[y][r], sum[y][r]);
+    }
+#pragma unroll
+    for (int y = 0; y < 2; ++y) s[y] = sum[y];
+  };
+  read_step(1, m[0], acc[0]);
+  read_step(2, m[1], acc[1]);
+  for (int32_t i = 1; i < segs; i += 3) {
+    step(i, m[0], acc[0], m[2], acc[2]);
+    if (i + 1 < segs) step(i + 1, m[1], acc[1], m[0], acc[0]);
+    if (i + 2 < segs) step(i + 2, m[2], acc[2], m[1], acc[1]);
+  }
+}
+
+// ---------------------------------------------------------------------------
 // y = x / sqrt(mean(x^2) + eps) w silu(z), a row of `dim` values at a time
 // ---------------------------------------------------------------------------
 struct NormArgs {
@@ -308,17 +1402,17 @@ __global__ __launch_bounds__(kThreads) void gated_norm_kernel(NormArgs a) {
   constexpr int kRowsPerWg = kThreads / LANES;
   const int lane = threadIdx.x % LANES;
   const int64_t row = (int64_t)blockIdx.x * kRowsPerWg + threadIdx.x / LANES;
-  const bool there = row < a.rows;
-  const int64_t at = there ? row : 0;
-  const int64_t token = a.heads == 1 ? at : at / a.heads;
-  const int64_t head = at - token * a.heads;
+  const bool there = row < a.rows;  // (at most 2^32 of them)
+  const uint32_t at = there ? (uint32_t)row : 0, heads = (uint32_t)a.heads;
+  const uint32_t token = heads == 1 ? at : at / heads, head = at - token * heads;
   if (a.cu) {  // rows outside the sequences stay as they are
-    if (!*a.ok || !there || token < a.cu[0] || token >= a.cu[a.n]) return;
+    if (!*a.ok || !there || token < (uint32_t)a.cu[0] || token >= (uint32_t)a.cu[a.n]) return;
   } else if (!there) {
     return;
   }
-  const uint8_t* xp = a.x + token * a.x_stride + head * a.dim * 2;
-  const uint8_t* zp = a.z + token * a.z_stride + head * a.dim * 2;
+  const int64_t off = (int64_t)head * a.dim * 2;
+  const uint8_t* xp = a.x + token * a.x_stride + off;
+  const uint8_t* zp = a.z + token * a.z_stride + off;
   u32x4 xv[STEPS], zv[STEPS];
 #pragma unroll
   for (int s = 0; s < STEPS; ++s) {
@@ -350,9 +1444,9 @@ __global__ __launch_bounds__(kThreads) void gated_norm_kernel(NormArgs a) {
     for (int j = 0; j < 4; ++j) {
       const float x0 = bits_f32(xv[s][j] << 16), x1 = bits_f32(xv[s][j] & 0xffff0000u);
       const float z0 = bits_f32(zv[s][j] << 16), z1 = bits_f32(zv[s][j] & 0xffff0000u);
-      const float y0 = x0 * r * weight_at(a.w, a.w_bf16, d + 2 * j) * silu(z0);
-      const float y1 = x1 * r * weight_at(a.w, a.w_bf16, d + 2 * j + 1) * silu(z1);
-      y[j] = (uint32_t)f32_to_bf16_rne(y0) | ((uint32_t)f32_to_bf16_rne(y1) << 16);
+      const float y0 = x0 * r * weight_at(a.w, a.w_bf16, d + 2 * j) * silu_bf16(z0);
+      const float y1 = x1 * r * weight_at(a.w, a.w_bf16, d + 2 * j + 1) * silu_bf16(z1);
+      y[j] = pack_bf16(y0, y1);
     }
     st16(a.out + (row * a.dim + d) * 2, y);
   }
@@ -489,16 +1583,152 @@ extern "C" int mkv_linear_attn_decode(
 
 namespace mkv {
 namespace {
-constexpr int64_t kHeadBytes = 16;  // the workspace's first bytes: the offsets' verdict
+
+constexpr int64_t kHeadBytes = 1024;  // the workspace's first bytes: the offsets' verdict
+// Images of one launch at most: more key heads are run in turn in the same space
+constexpr int64_t kImageBytes = 512ll << 20;
+constexpr int32_t kScanTokens = 8;  // up to so many tokens per sequence are walked one by one
+
+struct Prefill {
+  bool chunked;
+  int64_t ids;    // tiles
+  int32_t waves;  // of a workgroup that writes outputs (a head's value dims take 8)
+  int32_t seg;    // tokens of a segment; 0: whole sequences
+  int64_t segs;   // segment ids
+  int32_t khs;    // key heads of a launch
+  int64_t key_bytes, head_bytes, end_bytes, step_bytes, total;
+};
+
+// What a pass takes (us on MI355X, fitted to 12 shapes of 1 to 32 sequences of
+// 300 to 32768 tokens under all choices): so many a chunk where up to half the
+// CUs have a workgroup, and where all have; a join so many a segment.
+struct ChunkCosts {
+  float rows4[2], rows8[2], ends[2], join;
+};
+constexpr ChunkCosts kDeltaCosts = {{2.9f, 3.8f}, {4.0f, 5.3f}, {3.4f, 3.8f}, 1.2f};
+constexpr ChunkCosts kDecayCosts = {{2.2f, 2.9f}, {2.8f, 3.6f}, {2.0f, 2.4f}, 0.6f};
+constexpr float kPassStart = 6.f;  // a pass's launch, its first loads and its last stores
+
+// A pass of `wgs` workgroups of at most `chunks` chunks each, one per CU at a time.
+float pass_time(const float (&cost)[2], double wgs, double chunks, int cus) {
+  const double half = cus / 2.0, load = wgs <= half ? 0. : wgs >= cus ? 1. : (wgs - half) / half;
+  const double rounds = wgs <= cus ? 1. : ceil(wgs / cus);
+  return (float)(kPassStart + rounds * chunks * (cost[0] + load * (cost[1] - cost[0])));
 }
+
+// Whole sequences or segments of them, and workgroups of half a head or of one,
+// by those costs. The batch is taken as its longest sequence and others alike.
+// (1 x 32768 tokens, 8 heads: whole 1505, in 32 segments 320, in 16 300; 8 x
+// 4096: whole 248, in 3 segments 238, in 8 311; 32 x 1024: half heads 192, whole
+// ones 164, in 2 segments 295; 1 x 1024: whole 71, in 4 segments 68.)
+void choose_walk(Prefill& p, int64_t tokens, int32_t n, int32_t longest, double heads, bool delta) {
+  const ChunkCosts& c = delta ? kDeltaCosts : kDecayCosts;
+  const int cus = device_cus();
+  const double most = longest > 0 && longest < tokens ? longest : tokens;
+  const double rest = n > 1 ? (tokens - most) / (n - 1) : 0;
+  const double long_chunks = ceil(most / kChunk), rest_chunks = ceil(rest / kChunk);
+  const double work = long_chunks + (n - 1) * rest_chunks;  // chunks of one head
+  float best = 3e38f;
+  for (int32_t waves = 4; waves <= 8; waves += 4) {
+    const float (&cost)[2] = waves == 4 ? c.rows4 : c.rows8;
+    const double parts = 8.0 / waves, wgs = heads * parts * n;
+    // (rounds of sequences of different lengths fill up: at least the longest one)
+    const double each = wgs <= cus ? long_chunks : fmax(long_chunks, work * heads * parts / cus);
+    const float t = pass_time(cost, wgs <= cus ? wgs : cus, each, cus);
+    if (t < best) {
+      best = t;
+      p.waves = waves;
+      p.seg = 0;
+    }
+  }
+  for (int32_t len = 4; len < long_chunks; len += len < 16 ? 1 : len < 64 ? 2 : 8) {
+    const int64_t ids = tile_ids(tokens, n, len * kChunk);
+    if (ids > 65535) continue;  // (grid.y)
+    const double of_long = ceil(long_chunks / len), of_rest = ceil(rest_chunks / len);
+    const double segs = of_long + (n - 1) * of_rest;
+    const double starts = segs - n;  // segments whose end is asked for
+    const double steps = delta ? fmax(of_long - 2, 0) + (n - 1) * fmax(of_rest - 2, 0) : 0;
+    const float before = pass_time(c.ends, heads * (starts + steps), len, cus) + kPassStart +
+                         (float)of_long * c.join;
+    for (int32_t waves = 4; waves <= 8; waves += 4) {
+      const float t =
+          before + pass_time(waves == 4 ? c.rows4 : c.rows8, heads * (8 / waves) * segs, len, cus);
+      if (t < best) {
+        best = t;
+        p.waves = waves;
+        p.seg = len * kChunk;
+      }
+    }
+  }
+}
+
+Prefill plan_prefill(int64_t tokens, int32_t n, int32_t longest, int32_t hk, int32_t hv,
+                     bool delta) {
+  Prefill p{};
+  p.total = kHeadBytes;
+  p.chunked = tokens > 0 && n > 0 && (longest == 0 || longest > kScanTokens);
+  if (!p.chunked) return p;
+  p.ids = tile_ids(tokens, n);
+  const int64_t images = p.ids * (kKeyImage + (int64_t)(hv / hk) * head_image(delta));
+  p.khs = (int32_t)(kImageBytes / images < 1    ? 1
+                    : kImageBytes / images > hk ? hk
+                                                : kImageBytes / images);
+  const int64_t heads = (int64_t)p.khs * (hv / hk);
+  choose_walk(p, tokens, n, longest, (double)heads, delta);
+  if (p.seg) p.segs = tile_ids(tokens, n, p.seg);
+  p.key_bytes = p.ids * p.khs * kKeyImage;
+  p.head_bytes = p.ids * heads * head_image(delta);
+  p.end_bytes = p.segs * heads * kStateHead * 4;
+  p.step_bytes = delta ? p.end_bytes : p.segs * heads * 4;
+  p.total = kHeadBytes + p.key_bytes + p.head_bytes + p.end_bytes + p.step_bytes;
+  return p;
+}
+
+template <bool DELTA>
+void run_chunks(const LinArgs& a, const Prefill& p, uint8_t* ws, hipStream_t s) {
+  ChunkArgs c{};
+  c.keys = ws + kHeadBytes;
+  c.heads = c.keys + p.key_bytes;
+  c.ends = (float*)(c.heads + p.head_bytes);
+  c.steps = (float*)((uint8_t*)c.ends + p.end_bytes);
+  c.seg = p.seg;
+  int32_t* ok = (int32_t*)ws;
+  for (int32_t kh0 = 0; kh0 < a.hk; kh0 += p.khs) {
+    c.kh0 = kh0;
+    c.khs = a.hk - kh0 < p.khs ? a.hk - kh0 : p.khs;
+    const unsigned heads = (unsigned)(c.khs * a.group), n = (unsigned)a.n;
+    hipLaunchKernelGGL(linear_prep_kernel<DELTA>, dim3((unsigned)p.ids, (unsigned)c.khs), dim3(256),
+                       0, s, a, c);
+    if (p.seg) {
+      c.parts = DELTA ? 2 : 1;
+      hipLaunchKernelGGL((linear_chunk_kernel<8, DELTA, kEnds>),
+                         dim3(heads * c.parts, (unsigned)p.segs), dim3(512), 0, s, a, c, ok);
+      hipLaunchKernelGGL(linear_join_kernel<DELTA>, dim3(heads * (kDim / 16), n), dim3(256), 0, s,
+                         a, c);
+    }
+    c.parts = 8 / p.waves;
+    const dim3 grid(heads * c.parts, p.seg ? (unsigned)p.segs : n), block(64 * p.waves);
+    if (p.seg && p.waves == 8)
+      hipLaunchKernelGGL((linear_chunk_kernel<8, DELTA, kRows>), grid, block, 0, s, a, c, ok);
+    else if (p.seg)
+      hipLaunchKernelGGL((linear_chunk_kernel<4, DELTA, kRows>), grid, block, 0, s, a, c, ok);
+    else if (p.waves == 8)
+      hipLaunchKernelGGL((linear_chunk_kernel<8, DELTA, kWhole>), grid, block, 0, s, a, c, ok);
+    else
+      hipLaunchKernelGGL((linear_chunk_kernel<4, DELTA, kWhole>), grid, block, 0, s, a, c, ok);
+  }
+}
+
+}  // namespace
 }  // namespace mkv
 
 extern "C" int64_t mkv_linear_attn_prefill_workspace_bytes(int64_t num_tokens, int32_t batch,
                                                            int32_t max_seqlen, int32_t num_k_heads,
                                                            int32_t num_v_heads, int32_t delta) {
-  if (num_tokens < 0 || batch < 0 || max_seqlen < 0 || num_k_heads <= 0 || num_v_heads <= 0)
+  if (num_tokens < 0 || num_tokens >= (1ll << 31) || batch < 0 || max_seqlen < 0 ||
+      num_k_heads <= 0 || num_v_heads <= 0 || num_v_heads % num_k_heads != 0)
     return -1;
-  return kHeadBytes;
+  return plan_prefill(num_tokens, batch, max_seqlen, num_k_heads, num_v_heads, delta != 0).total;
 }
 
 extern "C" int mkv_linear_attn_prefill(
@@ -519,19 +1749,25 @@ extern "C" int mkv_linear_attn_prefill(
                              z_stride, norm_weight, weight_bf16, norm_eps, out, err, a);
   if (rc != MKV_OK) return rc;
   MKV_REQUIRE(num_tokens < (1ll << 31) && max_seqlen >= 0, MKV_E_INVALID, "%s: bad sizes", fn);
+  MKV_REQUIRE(v_stride <= (1 << 24), MKV_E_UNSUPPORTED, "%s: rows of v more than 16 MiB apart", fn);
   if (batch == 0 || num_tokens == 0) return MKV_OK;
-  const int64_t need = mkv_linear_attn_prefill_workspace_bytes(
-      num_tokens, batch, max_seqlen, num_k_heads, num_v_heads, beta != nullptr);
+  const Prefill p =
+      plan_prefill(num_tokens, batch, max_seqlen, num_k_heads, num_v_heads, beta != nullptr);
   MKV_REQUIRE(cu_seqlens && workspace && aligned4(cu_seqlens), MKV_E_INVALID, "%s: null pointer",
               fn);
-  MKV_REQUIRE(aligned16(workspace) && workspace_bytes >= need, MKV_E_INVALID,
+  MKV_REQUIRE(aligned16(workspace) && workspace_bytes >= p.total, MKV_E_INVALID,
               "%s: the workspace must be 16-byte aligned and hold %lld bytes", fn,
-              (long long)need);
+              (long long)p.total);
   a.cu = cu_seqlens;
   const hipStream_t s = as_stream(stream);
   int32_t* ok = (int32_t*)workspace;
-  hipLaunchKernelGGL(linear_scan_kernel, dim3((unsigned)num_v_heads * 2, (unsigned)batch),
-                     dim3(256), 0, s, a, ok);
+  if (!p.chunked)
+    hipLaunchKernelGGL(linear_scan_kernel, dim3((unsigned)num_v_heads * 2, (unsigned)batch),
+                       dim3(256), 0, s, a, ok);
+  else if (a.beta)
+    run_chunks<true>(a, p, (uint8_t*)workspace, s);
+  else
+    run_chunks<false>(a, p, (uint8_t*)workspace, s);
   const int launched = check_launch(fn);
   if (launched != MKV_OK || !a.z) return launched;
   NormArgs m{a.out, a.z, a.w, (int64_t)a.hv * kDim * 2, a.z_stride, a.hv, kDim, a.w_bf16, a.eps,

@@ -314,7 +314,7 @@ __global__ __launch_bounds__(kThreads) void conv_prefill_kernel(ConvPrefillArgs 
   }
   const int32_t b = tile_sequence(p.cu, a.batch, blockIdx.x);
   const int64_t end = p.cu[b + 1], seq0 = p.cu[b];
-  const int64_t tile = (int64_t)blockIdx.x - first_tile(p.cu, b);
+  const int64_t tile = (int64_t)blockIdx.x - first_tile(p.cu[b], b);
   const int64_t t0 = seq0 + tile * 64 + (threadIdx.x >> 6) * kConvRows;
   const int64_t g = (int64_t)blockIdx.y * 64 + (threadIdx.x & 63);  // group of 8 channels
   if (t0 >= end || g * 8 >= a.channels) return;
@@ -376,15 +376,19 @@ __global__ __launch_bounds__(kThreads) void conv_prefill_kernel(ConvPrefillArgs 
   }
 #pragma unroll
   for (int i = 0; i < kConvRows; ++i) {
-    u32x4 y = u32x4{0u, 0u, 0u, 0u};
+    u32x4 y;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float acc = 0.f;
+    for (int e = 0; e < 8; e += 2) {
+      float acc[2];
 #pragma unroll
-      for (int k = 0; k < kConvK; ++k)
-        acc = fmaf(bits_f32(half16(wv, e * kConvK + k) << 16),
-                   bits_f32(half16(&xv[i + k], e) << 16), acc);
-      y[e >> 1] |= (uint32_t)f32_to_bf16_rne(acc / (1.0f + expf(-acc))) << (16 * (e & 1));
+      for (int j = 0; j < 2; ++j) {
+        acc[j] = 0.f;
+#pragma unroll
+        for (int k = 0; k < kConvK; ++k)
+          acc[j] = fmaf(bits_f32(half16(wv, (e + j) * kConvK + k) << 16),
+                        bits_f32(half16(&xv[i + k], e + j) << 16), acc[j]);
+      }
+      y[e >> 1] = pack_bf16(silu_bf16(acc[0]), silu_bf16(acc[1]));
     }
     if (i < rows) st16(outp + i * row, y);
   }

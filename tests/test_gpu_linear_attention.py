@@ -101,6 +101,135 @@ def test_prompts_with_the_norm(max_seqlen):
     check_prompts(x, [70, 0, 180], [3, 1, 0], norm=True, first=4, max_seqlen=max_seqlen)
 
 
+@pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("what", ["v", "k", "q", "g", "beta", "big v", "large v", "larger v",
+                                  "no decay left", "growth"])
+def test_what_is_not_finite_reaches_later_tokens_only(what, delta):
+    """An infinity or NaN of one token leaves the tokens before it, the other
+    heads, value dims (for v) and sequences as they were without it."""
+    case(f"linear attention prompts with {what} of one token, delta {delta}")
+    if what == "beta" and not delta:
+        return
+    lens, at, hk, hv = [70, 130, 40], 70 + 64 + 21, 2, 8
+    x = lu.inputs(5, 240, hk, hv, slots=3, raw=False, delta=delta)
+    clean = {n: t.clone() if isinstance(t, torch.Tensor) else t for n, t in x.items()}
+    q, k, v = lu.split(x["mixed"], hk, hv)
+    if what == "v":
+        v[at, 5, 17], v[at, 5, 90] = float("inf"), float("nan")
+    elif what == "k":
+        k[at, 1, 3] = float("nan")
+    elif what == "q":
+        q[at, 1, 3] = float("inf")
+    elif what == "g":
+        x["g"][at, 5] = float("nan")
+    elif what == "beta":
+        x["beta"][at, 5] = float("nan")
+    elif what == "big v":
+        v[at, 5, 17] = 2.0 ** 100
+    elif what == "large v":
+        v[at, 5, 17] = 2.0 ** 24
+    elif what == "larger v":
+        v[at, 5, 17] = 2.0 ** 50
+    elif what == "no decay left":  # everything before it is forgotten: still finite
+        x["g"][at, 5] = -float("inf")
+    elif what == "growth":
+        x["g"][at, 5] = 60.0
+    gx = lu.on_gpu(x)
+    out = prompt(gx, ints([0, 1, 2]), ints([0, 70, 200, 240]), gx["state"])
+    la.check_errors(DEV)
+    assert torch.isfinite(out[:at].float()).all() and torch.isfinite(out[200:].float()).all()
+    if what in ("no decay left", "growth"):
+        assert torch.isfinite(out.float()).all()
+    hit = [4, 5, 6, 7] if what in ("k", "q") else [5]
+    for b, (r0, r1) in enumerate(((0, 70), (70, 200), (200, 240))):
+        o, st, s_tol, o_tol = lu.want_sequence(clean, slice(r0, r1), clean["state"][b])
+        for h in range(hv):
+            to = min(r1, at) if h in hit else r1
+            if to > r0:
+                lu.close(out[r0:to, h], o[:to - r0, h], o_tol[:to - r0, h], f"{b} head {h}")
+            if h not in hit or b != 1:
+                lu.close_state(gx["state"][b, h:h + 1], st[h:h + 1], s_tol[h:h + 1], f"state {b}")
+    got = out[at:200, 5].float()
+    if what == "v":  # an infinite or NaN value stays in its value dim
+        others = [i for i in range(D) if i not in (17, 90)]
+        assert torch.isfinite(got[:, others]).all() and not torch.isfinite(got[:, 90]).any()
+        assert not torch.isfinite(got[0, 17])
+    elif what in ("k", "g", "beta"):
+        assert got.isnan().all() and not torch.isfinite(gx["state"][1, 5]).any()
+    elif what == "q":  # a query is its own token's
+        assert not torch.isfinite(got[0]).any() and torch.isfinite(got[1:]).all()
+    elif what in ("no decay left", "growth"):
+        o, st, s_tol, o_tol = lu.want_sequence(x, slice(70, 200), x["state"][1])
+        if what == "no decay left":
+            lu.close(out[70:200], o, o_tol, what)
+            lu.close_state(gx["state"][1], st, s_tol, what)
+        else:  # e^60: sizes are relative to the state's own, about its largest
+            want = st[5]
+            assert float((gx["state"][1, 5].double().cpu() - want).norm() / want.norm()) < 1e-4
+
+
+@pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("size", [dict(v=1e-4), dict(v=2.0 ** 40), dict(beta=1e-3), dict(q=1e-5),
+                                  dict(q=1e4), dict(k=1e-5), dict(k=1e-2, v=1e3),
+                                  dict(state=1e-6), dict(state=1e6), dict(state=0.0),
+                                  dict(v=0.0), dict(first=1e-7), dict(first=0.0), dict(last=3e4)],
+                         ids=str)
+def test_sizes(size, delta):
+    """Inputs far from 1, all of them or the first or last tokens' alone."""
+    case(f"linear attention prompts with inputs of other sizes, {size}, delta {delta}")
+    x = lu.inputs(12, 150, 2, 8, raw=False, delta=delta, qk_norm="q" not in size and "k" not in size)
+    q, k, v = lu.split(x["mixed"], 2, 8)
+    for name, f in size.items():
+        if name in ("q", "k", "v"):
+            {"q": q, "k": k, "v": v}[name].mul_(f)
+        elif name == "first":
+            v[:3] *= f
+        elif name == "last":
+            v[140:] *= f
+        elif x[name] is not None:
+            x[name] *= f
+    check_prompts(x, [150], [0])
+
+
+def test_strong_decays_keep_their_ratios():
+    """Log decays of -50 a token next to ones of -0.01: sums far from 0 whose
+    differences are small."""
+    case("linear attention prompts under strong decays")
+    x = lu.inputs(6, 200, 2, 8, raw=False, slots=1)
+    gen = torch.Generator().manual_seed(1)
+    strong = torch.rand(200, 8, generator=gen) < 0.3
+    x["g"] = torch.where(strong, torch.full_like(x["g"], -50.0), x["g"] * 0.1)
+    x["g"][100:110] = -3e38
+    check_prompts(x, [200], [0])
+
+
+def test_large_launches_run_their_heads_in_turn():
+    """More images than one launch holds: key heads in turn, with each key head's
+    share alone as the reference. Its walk may be cut otherwise: outputs differ by
+    two roundings to bf16 (2^-8 relative each), states by what fp32 sums do."""
+    case("linear attention prompts, 16/64 heads x 12800 tokens in several launches")
+    T, hk, hv = 12800, 16, 64
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    q, k = (torch.randn(T, hk, D, generator=gen, device=DEV).bfloat16() for _ in range(2))
+    v = torch.randn(T, hv, D, generator=gen, device=DEV).bfloat16()
+    g = -torch.rand(T, hv, generator=gen, device=DEV)
+    beta = torch.rand(T, hv, generator=gen, device=DEV)
+    state = torch.randn(2, hv, D, D, generator=gen, device=DEV)
+    cu, at = ints([0, 7000, T]), ints([1, 0])
+    want = state.clone()
+    out = la.linear_attn_prefill(q, k, v, g, beta, state, at, cu, qk_norm=True)
+    for kh in (0, 7, 15):
+        vh = slice(4 * kh, 4 * kh + 4)
+        st = want[:, vh].contiguous()
+        some = la.linear_attn_prefill(q[:, kh:kh + 1].contiguous(), k[:, kh:kh + 1].contiguous(),
+                                      v[:, vh].contiguous(), g[:, vh].contiguous(),
+                                      beta[:, vh].contiguous(), st, at, cu, qk_norm=True)
+        for got, ref_, tol in ((out[:, vh], some, 2.0 ** -7), (state[:, vh], st, 1e-5)):
+            ref_ = ref_.double()
+            assert (got.double() - ref_).norm() <= tol * ref_.norm()
+    la.check_errors(DEV)
+
+
 def test_prompt_in_pieces_and_steps():
     """A prompt in chunks and then token by token gives what one call gives."""
     case("linear attention prompt whole, in pieces, and step by step")

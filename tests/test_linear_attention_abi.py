@@ -59,6 +59,7 @@ def test_prefill_refused():
     assert prefill(cu=None)[0] == -1
     assert prefill(tokens=1 << 31)[0] == -1
     assert prefill(longest=-1)[0] == -1
+    assert prefill(vs=(1 << 24) + 16)[0] == -3
     rc, msg = prefill(wsb=8)
     assert rc == -1 and "workspace" in msg
     rc, msg = prefill(ws=FAKE + 8)
