@@ -1396,88 +1396,132 @@ struct NormArgs {
   const int32_t* ok;
 };
 
-// LANES lanes per row, 8 values (16 bytes) per lane and step.
-template <int LANES, int STEPS>
-__global__ __launch_bounds__(kThreads) void gated_norm_kernel(NormArgs a) {
-  constexpr int kRowsPerWg = kThreads / LANES;
-  const int lane = threadIdx.x % LANES;
-  const int64_t row = (int64_t)blockIdx.x * kRowsPerWg + threadIdx.x / LANES;
-  const bool there = row < a.rows;  // (at most 2^32 of them)
-  const uint32_t at = there ? (uint32_t)row : 0, heads = (uint32_t)a.heads;
-  const uint32_t token = heads == 1 ? at : at / heads, head = at - token * heads;
-  if (a.cu) {  // rows outside the sequences stay as they are
-    if (!*a.ok || !there || token < (uint32_t)a.cu[0] || token >= (uint32_t)a.cu[a.n]) return;
-  } else if (!there) {
-    return;
-  }
-  const int64_t off = (int64_t)head * a.dim * 2;
-  const uint8_t* xp = a.x + token * a.x_stride + off;
-  const uint8_t* zp = a.z + token * a.z_stride + off;
-  u32x4 xv[STEPS], zv[STEPS];
+// 8 weights as floats
+template <bool BF16>
+__device__ __forceinline__ void load_weights(const uint8_t* w, int d, float (&x)[8]) {
+  if (BF16) {  // (aligned to 2 bytes)
 #pragma unroll
-  for (int s = 0; s < STEPS; ++s) {
-    const int d = (s * LANES + lane) * 8;
-    xv[s] = zv[s] = u32x4{0u, 0u, 0u, 0u};
-    if (d < a.dim) {
-      xv[s] = ld16(xp + 2 * d);
-      zv[s] = ld16(zp + 2 * d);
-    }
-  }
-  float q = 0.f;
+    for (int j = 0; j < 8; ++j) x[j] = bf16_at(w + 2 * (d + j));
+  } else {
 #pragma unroll
-  for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float lo = bits_f32(xv[s][j] << 16), hi = bits_f32(xv[s][j] & 0xffff0000u);
-      q = fmaf(lo, lo, q);
-      q = fmaf(hi, hi, q);
-    }
-#pragma unroll
-  for (int o = 1; o < LANES; o *= 2) q += __shfl_xor(q, o);
-  const float r = 1.f / sqrtf(q / (float)a.dim + a.eps);
-#pragma unroll
-  for (int s = 0; s < STEPS; ++s) {
-    const int d = (s * LANES + lane) * 8;
-    if (d >= a.dim) continue;
-    u32x4 y;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float x0 = bits_f32(xv[s][j] << 16), x1 = bits_f32(xv[s][j] & 0xffff0000u);
-      const float z0 = bits_f32(zv[s][j] << 16), z1 = bits_f32(zv[s][j] & 0xffff0000u);
-      const float y0 = x0 * r * weight_at(a.w, a.w_bf16, d + 2 * j) * silu_bf16(z0);
-      const float y1 = x1 * r * weight_at(a.w, a.w_bf16, d + 2 * j + 1) * silu_bf16(z1);
-      y[j] = pack_bf16(y0, y1);
-    }
-    st16(a.out + (row * a.dim + d) * 2, y);
+    for (int j = 0; j < 8; ++j) x[j] = *(const float*)(w + 4 * (d + j));
   }
 }
 
-template <int LANES, int STEPS>
-void launch_norm(const NormArgs& a, hipStream_t stream) {
+// LANES lanes per row, 8 values (16 bytes) per lane and step; a thread takes
+// ROWS rows one workgroup's span apart, all loaded before the first is used.
+template <int LANES, int STEPS, int ROWS, bool BF16>
+__global__ __launch_bounds__(kThreads) void gated_norm_kernel(NormArgs a) {
   constexpr int kRowsPerWg = kThreads / LANES;
-  hipLaunchKernelGGL((gated_norm_kernel<LANES, STEPS>),
-                     dim3((unsigned)((a.rows + kRowsPerWg - 1) / kRowsPerWg)), dim3(kThreads), 0,
-                     stream, a);
+  const int lane = threadIdx.x % LANES;
+  const uint32_t heads = (uint32_t)a.heads;
+  float w[STEPS][8];
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    const int d = (s * LANES + lane) * 8;
+    if (d < a.dim) load_weights<BF16>(a.w, d, w[s]);
+  }
+  bool there[ROWS];
+  u32x4 xv[ROWS][STEPS], zv[ROWS][STEPS];
+  uint32_t first = 0, end = 0xffffffffu;
+  if (a.cu) {  // rows outside the sequences stay as they are
+    if (!*a.ok) return;
+    first = (uint32_t)a.cu[0];
+    end = (uint32_t)a.cu[a.n];
+  }
+  const int64_t row0 = (int64_t)blockIdx.x * (kRowsPerWg * ROWS) + threadIdx.x / LANES;
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int64_t row = row0 + i * kRowsPerWg;
+    there[i] = row < a.rows;  // (at most 2^32 of them)
+    const uint32_t at = there[i] ? (uint32_t)row : 0;
+    const uint32_t token = heads == 1 ? at : at / heads, head = at - token * heads;
+    there[i] &= token >= first && token < end;
+    const int64_t off = (int64_t)head * a.dim * 2;
+    const uint8_t* xp = a.x + token * a.x_stride + off;
+    const uint8_t* zp = a.z + token * a.z_stride + off;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      const int d = (s * LANES + lane) * 8;
+      xv[i][s] = zv[i][s] = u32x4{0u, 0u, 0u, 0u};
+      if (there[i] && d < a.dim) {
+        xv[i][s] = ld16(xp + 2 * d);
+        zv[i][s] = ld_nt(zp + 2 * d);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    float q = 0.f;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float lo = bits_f32(xv[i][s][j] << 16), hi = bits_f32(xv[i][s][j] & 0xffff0000u);
+        q = fmaf(lo, lo, q);
+        q = fmaf(hi, hi, q);
+      }
+#pragma unroll
+    for (int o = 1; o < LANES; o *= 2) q += __shfl_xor(q, o);
+    const float r = 1.f / sqrtf(q / (float)a.dim + a.eps);
+    if (!there[i]) continue;
+    uint8_t* out = a.out + (row0 + i * kRowsPerWg) * a.dim * 2;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      const int d = (s * LANES + lane) * 8;
+      if (d >= a.dim) continue;
+      u32x4 y;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t x = xv[i][s][j], z = zv[i][s][j];
+        y[j] = pack_bf16(
+            bits_f32(x << 16) * r * w[s][2 * j] * silu_bf16(bits_f32(z << 16)),
+            bits_f32(x & 0xffff0000u) * r * w[s][2 * j + 1] * silu_bf16(bits_f32(z & 0xffff0000u)));
+      }
+      st16(out + 2 * d, y);
+    }
+  }
+}
+
+template <int LANES, int STEPS, int ROWS>
+void launch_norm(const NormArgs& a, hipStream_t stream) {
+  constexpr int kRowsPerWg = kThreads / LANES * ROWS;
+  const dim3 grid((unsigned)((a.rows + kRowsPerWg - 1) / kRowsPerWg));
+  if (a.w_bf16)
+    hipLaunchKernelGGL((gated_norm_kernel<LANES, STEPS, ROWS, true>), grid, dim3(kThreads), 0,
+                       stream, a);
+  else
+    hipLaunchKernelGGL((gated_norm_kernel<LANES, STEPS, ROWS, false>), grid, dim3(kThreads), 0,
+                       stream, a);
 }
 
 constexpr int kNormMaxDim = 4096;
 
+// Several rows per thread where that leaves every CU a few workgroups.
+template <int LANES, int STEPS>
+void pick_rows(const NormArgs& a, hipStream_t stream) {
+  if (a.rows >= (int64_t)device_cus() * (kThreads / LANES) * 4 * 4)
+    launch_norm<LANES, STEPS, 4>(a, stream);
+  else
+    launch_norm<LANES, STEPS, 1>(a, stream);
+}
+
 void run_norm(const NormArgs& a, hipStream_t stream) {
   const int32_t d = a.dim;
   if (d <= 64)
-    launch_norm<8, 1>(a, stream);
+    pick_rows<8, 1>(a, stream);
   else if (d <= 128)
-    launch_norm<16, 1>(a, stream);
+    pick_rows<16, 1>(a, stream);
   else if (d <= 256)
-    launch_norm<32, 1>(a, stream);
+    pick_rows<32, 1>(a, stream);
   else if (d <= 512)
-    launch_norm<64, 1>(a, stream);
+    pick_rows<64, 1>(a, stream);
   else if (d <= 1024)
-    launch_norm<64, 2>(a, stream);
+    launch_norm<64, 2, 1>(a, stream);
   else if (d <= 2048)
-    launch_norm<64, 4>(a, stream);
+    launch_norm<64, 4, 1>(a, stream);
   else
-    launch_norm<64, 8>(a, stream);
+    launch_norm<64, 8, 1>(a, stream);
 }
 
 // ---------------------------------------------------------------------------

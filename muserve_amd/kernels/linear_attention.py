@@ -56,6 +56,26 @@ def _call(dev: torch.device, name: str, *args) -> None:
             _lib.call(name, *args, _lib.stream_of(dev))
 
 
+# What a call's arguments come to, by their types, shapes, strides and devices
+# alone: checking them anew takes 9 us, as long as a small call's kernel.
+_plans: dict[tuple, tuple] = {}
+_PLANS = 4096
+
+
+def _sig(t: torch.Tensor | None):
+    return None if t is None else (t.dtype, t.shape, t.stride(), t.get_device())
+
+
+def _planned(key: tuple, check, *args) -> tuple:
+    plan = _plans.get(key)
+    if plan is None:
+        plan = check(*args)  # (raises for what is refused)
+        if len(_plans) >= _PLANS:
+            _plans.clear()
+        _plans[key] = plan
+    return plan
+
+
 def _rows(name: str, t: torch.Tensor, heads: int, dim: int) -> int:
     """Bytes between the token rows of t [tokens, heads, dim] bf16, whose heads
     follow each other."""
@@ -89,6 +109,9 @@ def _gate(name: str, t: torch.Tensor, tokens: int, heads: int, dtype: torch.dtyp
 
 
 def _ids(name: str, t: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    if t.dtype is torch.int32 and t.get_device() == dev.index and t.dim() == 1 \
+            and t.is_contiguous():
+        return t
     if t.dim() != 1 or t.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{name} must be a list of int32 (or int64) values")
     if t.dtype != torch.int32 or t.device != dev:
@@ -104,8 +127,9 @@ def _weight(w: torch.Tensor, dim: int) -> int:
     return 1 if w.dtype == torch.bfloat16 else 0
 
 
-def _common(q, k, v, g, beta, state, slots, a_log, dt_bias, scale, z, norm_weight, out):
-    """What both forms check; the library's arguments from q on, up to out."""
+def _check_common(q, k, v, g, beta, state, slots, a_log, dt_bias, z, norm_weight, out):
+    """What both forms check: (device, tokens, key heads, value heads, q to
+    norm_weight's strides and types, pool slots)."""
     dev = _lib.require_gpu(q, k, v, g, beta, state, a_log, dt_bias, z, norm_weight, out)
     if state.dtype != torch.float32 or state.dim() != 4 or not state.is_contiguous():
         raise ValueError("state must be contiguous fp32 [slots, value heads, 128, 128]")
@@ -136,21 +160,31 @@ def _common(q, k, v, g, beta, state, slots, a_log, dt_bias, scale, z, norm_weigh
         if z.shape[0] != tokens:
             raise ValueError("z must have the tokens of q")
         zs, wb = _rows("z", z, hv, HEAD_DIM), _weight(norm_weight, HEAD_DIM)
-    if out is None:
-        out = torch.empty((tokens, hv, HEAD_DIM), dtype=torch.bfloat16, device=dev)
-    elif out.shape != (tokens, hv, HEAD_DIM) or out.dtype != torch.bfloat16 \
-            or not out.is_contiguous():
+    if out is not None and (out.shape != (tokens, hv, HEAD_DIM) or out.dtype != torch.bfloat16
+                            or not out.is_contiguous()):
         raise ValueError(f"out must be contiguous bf16 [{tokens}, {hv}, {HEAD_DIM}]")
-    slots = _ids("slots", slots, dev)
-    scale = HEAD_DIM ** -0.5 if scale is None else float(scale)
+    return (dev, tokens, hk, hv, state.shape[0], qs, ks, vs, gs, bs, zs, wb,
+            1 if g.dtype == torch.bfloat16 else 0)
 
-    def args(qk_norm, eps):
-        return (q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, g.data_ptr(), gs,
-                _lib.ptr(beta), bs, 1 if g.dtype == torch.bfloat16 else 0, _lib.ptr(a_log),
-                _lib.ptr(dt_bias), 1 if qk_norm else 0, scale, _lib.ptr(z), zs,
-                _lib.ptr(norm_weight), wb, float(eps), out.data_ptr())
 
-    return dev, tokens, hk, hv, slots, out, args
+def _common(q, k, v, g, beta, state, slots, a_log, dt_bias, z, norm_weight, out):
+    key = (_sig(q), _sig(k), _sig(v), _sig(g), _sig(beta), _sig(state), _sig(a_log), _sig(dt_bias),
+           _sig(z), _sig(norm_weight), _sig(out))
+    return _planned(key, _check_common, q, k, v, g, beta, state, slots, a_log, dt_bias, z,
+                    norm_weight, out)
+
+
+def _args(plan, q, k, v, g, beta, a_log, dt_bias, qk_norm, scale, z, norm_weight, eps, out):
+    """The library's arguments from q on, up to out."""
+    qs, ks, vs, gs, bs, zs, wb, gates_bf16 = plan[5:]
+    return (q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, g.data_ptr(), gs,
+            None if beta is None else beta.data_ptr(), bs, gates_bf16,
+            None if a_log is None else a_log.data_ptr(),
+            None if dt_bias is None else dt_bias.data_ptr(), 1 if qk_norm else 0,
+            HEAD_DIM ** -0.5 if scale is None else float(scale),
+            None if z is None else z.data_ptr(), zs,
+            None if norm_weight is None else norm_weight.data_ptr(), wb, float(eps),
+            out.data_ptr())
 
 
 def linear_attn_decode(
@@ -185,12 +219,17 @@ def linear_attn_decode(
     ``norm_weight`` the output is o / sqrt(mean(o^2) + norm_eps) * norm_weight
     * silu(z). q, k, v and z may be views with strided token rows. A slot
     outside the pool gives zeros and a device fault; slots must be unique."""
-    dev, B, hk, hv, slots, out, args = _common(q, k, v, g, beta, state, slots, a_log, dt_bias,
-                                               scale, z, norm_weight, out)
+    plan = _common(q, k, v, g, beta, state, slots, a_log, dt_bias, z, norm_weight, out)
+    dev, B, hk, hv, pool = plan[:5]
+    slots = _ids("slots", slots, dev)
+    if out is None:
+        out = torch.empty((B, hv, HEAD_DIM), dtype=torch.bfloat16, device=dev)
     if slots.numel() != B:
         raise ValueError(f"slots must name a slot for each of {B} requests")
-    _call(dev, "mkv_linear_attn_decode", state.data_ptr(), state.shape[0], hk, hv, HEAD_DIM,
-          slots.data_ptr(), B, *args(qk_norm, norm_eps), (errors or _errword(dev)).ptr())
+    _call(dev, "mkv_linear_attn_decode", state.data_ptr(), pool, hk, hv, HEAD_DIM,
+          slots.data_ptr(), B,
+          *_args(plan, q, k, v, g, beta, a_log, dt_bias, qk_norm, scale, z, norm_weight, norm_eps,
+                 out), (errors or _errword(dev)).ptr())
     return out
 
 
@@ -235,8 +274,11 @@ def linear_attn_prefill(
     computation. With ``z`` the output is rounded to bf16 before the norm too.
     Offsets that do not hold together are a device fault, and the call then
     writes nothing."""
-    dev, tokens, hk, hv, slots, out, args = _common(q, k, v, g, beta, state, slots, a_log,
-                                                    dt_bias, scale, z, norm_weight, out)
+    plan = _common(q, k, v, g, beta, state, slots, a_log, dt_bias, z, norm_weight, out)
+    dev, tokens, hk, hv, pool = plan[:5]
+    slots = _ids("slots", slots, dev)
+    if out is None:
+        out = torch.empty((tokens, hv, HEAD_DIM), dtype=torch.bfloat16, device=dev)
     cu = _ids("cu_seqlens", cu_seqlens, dev)
     batch = slots.numel()
     if cu.numel() != batch + 1:
@@ -249,10 +291,32 @@ def linear_attn_prefill(
     # keeps it with a graph under capture
     need = _prefill_bytes(tokens, batch, longest, hk, hv, beta is not None, dev)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    _call(dev, "mkv_linear_attn_prefill", state.data_ptr(), state.shape[0], hk, hv, HEAD_DIM,
-          slots.data_ptr(), cu.data_ptr(), batch, tokens, longest, *args(qk_norm, norm_eps),
-          ws.data_ptr(), need, (errors or _errword(dev)).ptr())
+    _call(dev, "mkv_linear_attn_prefill", state.data_ptr(), pool, hk, hv, HEAD_DIM,
+          slots.data_ptr(), cu.data_ptr(), batch, tokens, longest,
+          *_args(plan, q, k, v, g, beta, a_log, dt_bias, qk_norm, scale, z, norm_weight, norm_eps,
+                 out), ws.data_ptr(), need, (errors or _errword(dev)).ptr())
     return out
+
+
+def _check_conv(x, weight, conv_state, out):
+    dev = _lib.require_gpu(x, weight, conv_state, out)
+    if x.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16 \
+            or conv_state.dtype != torch.bfloat16:
+        raise TypeError("causal_conv_prefill takes bf16 x, weight and conv states")
+    if conv_state.dim() != 3 or not conv_state.is_contiguous():
+        raise ValueError("conv_state must be contiguous [slots, channels, width]")
+    C, W = conv_state.shape[1], conv_state.shape[2]
+    if x.dim() != 2 or x.shape[1] != C:
+        raise ValueError(f"x must be [tokens, {C}], not {tuple(x.shape)}")
+    T = x.shape[0]
+    if x.numel() and (x.stride(1) != 1 or (T > 1 and x.stride(0) < C)):
+        raise ValueError("x: the channels of a token must follow each other")
+    if weight.dim() not in (2, 3) or weight.shape[0] != C or weight.numel() != C * weight.shape[-1]:
+        raise ValueError(f"weight must be [{C}, 1, K] or [{C}, K]")
+    if out is not None and (out.shape != (T, C) or out.dtype != x.dtype
+                            or not out.is_contiguous()):
+        raise ValueError(f"out must be contiguous bf16 [{T}, {C}]")
+    return dev, T, C, W, weight.shape[-1], x.stride(0) * 2 if T > 1 else C * 2
 
 
 def causal_conv_prefill(
@@ -270,26 +334,11 @@ def causal_conv_prefill(
     for each channel, the inputs before a sequence's first row taken from
     slots[b], which is left with the sequence's last inputs. Rows of x may be
     strided; rows of ``out`` outside the sequences are left as they were."""
-    dev = _lib.require_gpu(x, weight, conv_state, out)
-    if x.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16 \
-            or conv_state.dtype != torch.bfloat16:
-        raise TypeError("causal_conv_prefill takes bf16 x, weight and conv states")
-    if conv_state.dim() != 3 or not conv_state.is_contiguous():
-        raise ValueError("conv_state must be contiguous [slots, channels, width]")
-    C, W = conv_state.shape[1], conv_state.shape[2]
-    if x.dim() != 2 or x.shape[1] != C:
-        raise ValueError(f"x must be [tokens, {C}], not {tuple(x.shape)}")
-    T = x.shape[0]
-    if x.numel() and (x.stride(1) != 1 or (T > 1 and x.stride(0) < C)):
-        raise ValueError("x: the channels of a token must follow each other")
-    w = weight.reshape(weight.shape[0], -1)
-    if w.shape[0] != C:
-        raise ValueError(f"weight must be [{C}, 1, K]")
-    w = w.contiguous()
+    key = (_sig(x), _sig(weight), _sig(conv_state), _sig(out))
+    dev, T, C, W, K, xs = _planned(key, _check_conv, x, weight, conv_state, out)
+    w = weight if weight.is_contiguous() else weight.contiguous()
     if out is None:
         out = torch.empty((T, C), dtype=x.dtype, device=dev)
-    elif out.shape != (T, C) or out.dtype != x.dtype or not out.is_contiguous():
-        raise ValueError(f"out must be contiguous bf16 [{T}, {C}]")
     elif T and out.data_ptr() == x.data_ptr():
         raise ValueError("out must not be x: other rows of it are still to be read")
     slots, cu = _ids("slots", slots, dev), _ids("cu_seqlens", cu_seqlens, dev)
@@ -297,10 +346,27 @@ def causal_conv_prefill(
     if cu.numel() != batch + 1:
         raise ValueError(f"cu_seqlens must hold {batch + 1} offsets for {batch} slots")
     _call(dev, "mkv_gdn_conv_prefill", conv_state.data_ptr(), conv_state.shape[0], C, W,
-          slots.data_ptr(), cu.data_ptr(), batch, T, x.data_ptr(),
-          x.stride(0) * 2 if T > 1 else C * 2, w.data_ptr(), w.shape[1], out.data_ptr(),
+          slots.data_ptr(), cu.data_ptr(), batch, T, x.data_ptr(), xs, w.data_ptr(), K,
+          out.data_ptr(),
           (errors or _errword(dev)).ptr())
     return out
+
+
+def _check_norm(x, z, weight, out):
+    dev = _lib.require_gpu(x, z, weight, out)
+    if x.dim() not in (2, 3) or z.shape != x.shape:
+        raise ValueError(f"x and z must be [tokens, heads, D] or [rows, D] alike, not "
+                         f"{tuple(x.shape)} and {tuple(z.shape)}")
+    D = x.shape[-1]
+    if D == 0 or D % 8 or D > 4096:
+        raise ValueError(f"unsupported rows of {D} values (a multiple of 8, at most 4096)")
+    x3, z3 = (x, z) if x.dim() == 3 else (x.unsqueeze(1), z.unsqueeze(1))
+    T, H = x3.shape[:2]
+    xs, zs, wb = _rows("x", x3, H, D), _rows("z", z3, H, D), _weight(weight, D)
+    if out is not None and (out.shape != x.shape or out.dtype != x.dtype
+                            or not out.is_contiguous()):
+        raise ValueError("out must be a contiguous tensor shaped like x")
+    return dev, T if H else 0, H, D, xs, zs, wb
 
 
 def gated_rms_norm(
@@ -314,23 +380,11 @@ def gated_rms_norm(
     """x / sqrt(mean(x^2) + eps) * weight * silu(z) over the last dimension (a
     multiple of 8, at most 4096), in fp32, rounded once. The rows of a token
     follow each other; tokens may be strided. ``out`` may be x."""
-    dev = _lib.require_gpu(x, z, weight, out)
-    if x.dim() not in (2, 3) or z.shape != x.shape:
-        raise ValueError(f"x and z must be [tokens, heads, D] or [rows, D] alike, not "
-                         f"{tuple(x.shape)} and {tuple(z.shape)}")
-    D = x.shape[-1]
-    if D == 0 or D % 8 or D > 4096:
-        raise ValueError(f"unsupported rows of {D} values (a multiple of 8, at most 4096)")
-    shape = x.shape
-    x3, z3 = (x, z) if x.dim() == 3 else (x.unsqueeze(1), z.unsqueeze(1))
-    T, H = x3.shape[:2]
-    xs, zs, wb = _rows("x", x3, H, D), _rows("z", z3, H, D), _weight(weight, D)
+    key = (_sig(x), _sig(z), _sig(weight), _sig(out))
+    dev, T, H, D, xs, zs, wb = _planned(key, _check_norm, x, z, weight, out)
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=dev)
-    elif out.shape != shape or out.dtype != x.dtype or not out.is_contiguous():
-        raise ValueError("out must be a contiguous tensor shaped like x")
-    if x.numel() == 0:
-        return out
-    _call(dev, "mkv_gated_rms_norm", x.data_ptr(), xs, z.data_ptr(), zs, T, H, D,
-          weight.data_ptr(), wb, float(eps), out.data_ptr())
+        out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    if T:
+        _call(dev, "mkv_gated_rms_norm", x.data_ptr(), xs, z.data_ptr(), zs, T, H, D,
+              weight.data_ptr(), wb, float(eps), out.data_ptr())
     return out
