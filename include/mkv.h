@@ -331,7 +331,8 @@ int mkv_gdn_decode_gather(const void* state_pool, int64_t state_bytes, void* sta
  * with the sequence's last `width` inputs (and the newest of its old ones
  * where the sequence is shorter). A sequence without rows leaves its slot.
  * Rows of out [num_tokens, channels] outside the sequences are left as they
- * were. Requirements as mkv_gdn_conv_decode's, x_stride a multiple of 16.
+ * were. Requirements as mkv_gdn_conv_decode's, x_stride a multiple of 16, at
+ * most 4096 sequences (MKV_E_UNSUPPORTED); out does not overlap x.
  * Offsets below 0, falling or above num_tokens set MKV_DEVERR_TABLE, and the
  * call writes nothing; a slot outside [0, pool_slots) gives zeros and sets
  * MKV_DEVERR_STATE_SLOT.
@@ -365,8 +366,8 @@ int mkv_gdn_conv_prefill(void* conv_pool, int64_t pool_slots, int32_t channels, 
  *       o / sqrt(mean(o^2) + norm_eps) * norm_weight * silu(z), still rounded once.
  * Requirements: head_dim 128, num_v_heads a multiple of num_k_heads and at
  * most 1024, batch <= 65535 (MKV_E_UNSUPPORTED); rows, strides and the state
- * 16-byte aligned (MKV_E_ALIGN); slots unique. A slot outside [0, pool_slots)
- * gives zeros and sets MKV_DEVERR_STATE_SLOT.
+ * 16-byte aligned (MKV_E_ALIGN); slots unique; out overlaps no other argument.
+ * A slot outside [0, pool_slots) gives zeros and sets MKV_DEVERR_STATE_SLOT.
  */
 int mkv_linear_attn_decode(void* state, int64_t pool_slots, int32_t num_k_heads,
                            int32_t num_v_heads, int32_t head_dim, const int32_t* slots,
@@ -387,8 +388,10 @@ int mkv_linear_attn_decode(void* state, int64_t pool_slots, int32_t num_k_heads,
  * without rows leaves its slot; rows of out outside the sequences are left as
  * they were. max_seqlen is a hint of the longest sequence (0: not known) that
  * chooses between forms of the computation; any value is right. With z the
- * output is rounded to bf16 before the norm as well. Arguments and
- * requirements otherwise as above, batch <= 65535, num_tokens < 2^31.
+ * output is rounded to bf16 before the norm as well (rows of a slot outside the
+ * pool are zeros before it). Arguments and requirements otherwise as above,
+ * batch <= 4096, num_tokens < 2^31, num_tokens * num_v_heads <= 2^30, rows of v
+ * at most 16 MiB apart (MKV_E_UNSUPPORTED).
  * Offsets below 0, falling or above num_tokens set MKV_DEVERR_TABLE, and the
  * call writes neither rows nor states. The workspace must be 16-byte aligned
  * and hold mkv_linear_attn_prefill_workspace_bytes (-1: bad sizes) for the
@@ -414,9 +417,10 @@ int64_t mkv_linear_attn_prefill_workspace_bytes(int64_t num_tokens, int32_t batc
  * values of x, z and out [tokens, heads, dim] bf16 (fp32 arithmetic, rounded
  * once): the norm behind a linear-attention layer. x and z rows are x_stride
  * and z_stride bytes apart, a token's heads follow each other; out is
- * contiguous and may be x. weight is [dim] fp32, or bf16 with weight_bf16.
- * dim is a multiple of 8 up to 4096, tokens * heads at most 2^32
- * (MKV_E_UNSUPPORTED); rows and strides 16-byte aligned (MKV_E_ALIGN).
+ * contiguous and may be x or z (without gaps then), but overlap neither
+ * otherwise. weight is [dim] fp32, or bf16 with weight_bf16. dim is a multiple
+ * of 8 up to 4096, tokens * heads at most 2^30 (MKV_E_UNSUPPORTED); rows and
+ * strides 16-byte aligned (MKV_E_ALIGN).
  */
 int mkv_gated_rms_norm(const void* x, int64_t x_stride, const void* z, int64_t z_stride,
                        int64_t tokens, int32_t heads, int32_t dim, const void* weight,

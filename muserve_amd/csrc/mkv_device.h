@@ -50,12 +50,23 @@ __device__ __forceinline__ void raise_err(int32_t* err, int32_t bit) { atomicOr(
 // more, never falling, at most `rows`. Every thread of the workgroup calls.
 __device__ __forceinline__ bool offsets_ok(const int32_t* cu, int32_t n, int64_t rows) {
   bool bad = false;
+  if (n < 64) {  // each wave by itself, without a barrier
+    const int32_t i = threadIdx.x & 63;
+    if (i <= n) {
+      const int32_t x = cu[i];
+      bad = x < 0 || x > rows || (i > 0 && cu[i - 1] > x);
+    }
+    return __builtin_amdgcn_ballot_w64(bad) == 0;
+  }
   for (int32_t i = threadIdx.x; i <= n; i += blockDim.x) {
     const int32_t x = cu[i];
     bad |= x < 0 || x > rows || (i > 0 && cu[i - 1] > x);
   }
   return !__syncthreads_or(bad);
 }
+
+// Sequences of one call: each workgroup reads all offsets.
+constexpr int32_t kMaxSequences = 4096;
 
 // Tiles of R rows of packed sequences without a list of them: tile c of
 // sequence b has the id cu[b] / R + b + c. Ids never meet (a sequence of m rows
@@ -65,18 +76,42 @@ __device__ __forceinline__ int32_t first_tile(int32_t row, int32_t b, int32_t r 
   return row / r + b;
 }
 inline int64_t tile_ids(int64_t rows, int32_t n, int32_t r = 64) { return rows / r + n; }
-// The sequence that a tile id would belong to.
-__device__ __forceinline__ int32_t tile_sequence(const int32_t* cu, int32_t n, int64_t id,
-                                                 int32_t r = 64) {
-  int32_t lo = 0, hi = n - 1;
-  while (lo < hi) {
-    const int32_t mid = (lo + hi + 1) >> 1;
-    if (first_tile(cu[mid], mid, r) <= id)
-      lo = mid;
-    else
-      hi = mid - 1;
+// The sequence that a tile id would belong to, or -1 if the offsets do not hold
+// together. Every thread of the workgroup calls, once a kernel: all offsets are
+// read side by side (a binary search waits for log2 n loads, one after another).
+__device__ __forceinline__ int32_t tile_sequence(const int32_t* cu, int32_t n, int64_t rows,
+                                                 int64_t id, int32_t r = 64) {
+  if (n < 64) {
+    const int32_t i = threadIdx.x & 63;
+    bool bad = false, before = false;
+    if (i <= n) {
+      const int32_t x = cu[i];
+      bad = x < 0 || x > rows || (i > 0 && cu[i - 1] > x);
+      before = i < n && first_tile(x, i, r) <= id;
+    }
+    if (__builtin_amdgcn_ballot_w64(bad) != 0) return -1;
+    const int32_t of = __builtin_popcountll(__builtin_amdgcn_ballot_w64(before));
+    return of > 0 ? of - 1 : 0;  // (ids before the first sequence's first tile belong to none)
   }
-  return lo;
+  constexpr int32_t kBad = 0x7fffffff;
+  __shared__ int32_t last[16];
+  int32_t at = 0;  // the last sequence whose first tile is not behind id
+  for (int32_t i = threadIdx.x; i <= n; i += blockDim.x) {
+    const int32_t x = cu[i];
+    if (x < 0 || x > rows || (i > 0 && cu[i - 1] > x))
+      at = kBad;
+    else if (i < n && first_tile(x, i, r) <= id)
+      at = at > i ? at : i;
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    const int32_t x = __shfl_xor(at, o);
+    at = at > x ? at : x;
+  }
+  if ((threadIdx.x & 63) == 0) last[threadIdx.x >> 6] = at;
+  __syncthreads();
+  for (uint32_t i = 0; i < blockDim.x / 64; ++i) at = at > last[i] ? at : last[i];
+  return __builtin_amdgcn_readfirstlane(at == kBad ? -1 : at);
 }
 
 // x / (1 + e^-x) by the hardware's 2^x and reciprocal, both within an fp32 step

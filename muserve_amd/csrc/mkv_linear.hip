@@ -153,10 +153,11 @@ __device__ __forceinline__ float weight_at(const uint8_t* w, int32_t bf16, int64
 
 // One workgroup per (value head, request): the head's 64 KiB state is read
 // once, updated in registers and written back. Bound by HBM: 128 KiB per
-// (request, head) against 0.8 KiB of everything else.
-template <int THREADS>
-__global__ __launch_bounds__(THREADS) void linear_decode_kernel(LinArgs a) {
-  constexpr int kGroups = THREADS / 8, kRows = kDim / kGroups;
+// (request, head) against 0.8 KiB of everything else; 256 requests of 8 heads
+// take 53 us, 5.1 TB/s. A lone request (7.4 us) is bound by its two trips to
+// memory: 1024 threads a head, with 4 rows' loads less each, were no faster.
+__global__ __launch_bounds__(kThreads) void linear_decode_kernel(LinArgs a) {
+  constexpr int kGroups = kThreads / 8, kRows = kDim / kGroups;
   const int tid = threadIdx.x, l = tid & 7, r0 = tid >> 3;
   const int32_t h = blockIdx.x, kh = h / a.group;
   const int64_t b = blockIdx.y;
@@ -195,7 +196,7 @@ __global__ __launch_bounds__(THREADS) void linear_decode_kernel(LinArgs a) {
       st_stream((uint8_t*)st, (uint32_t)((r0 + kGroups * i) * kDim + 32 * c + 4 * l) * 4, x);
     }
   if (a.z) {  // uniform: o / sqrt(mean(o^2) + eps) w silu(z)
-    __shared__ float part[THREADS / 64];
+    __shared__ float part[kThreads / 64];
     float q = 0.f;
 #pragma unroll
     for (int i = 0; i < kRows; ++i) q = fmaf(o[i], o[i], q);
@@ -206,7 +207,7 @@ __global__ __launch_bounds__(THREADS) void linear_decode_kernel(LinArgs a) {
     __syncthreads();
     q = 0.f;
 #pragma unroll
-    for (int i = 0; i < THREADS / 64; ++i) q += part[i];
+    for (int i = 0; i < kThreads / 64; ++i) q += part[i];
     const float r = 1.f / sqrtf(q * (1.f / kDim) + a.eps);
     const uint8_t* zp = a.z + b * a.z_stride + h * (kDim * 2);
 #pragma unroll
@@ -240,6 +241,7 @@ __global__ __launch_bounds__(256) void linear_scan_kernel(LinArgs a, int32_t* ok
     return;
   }
   const int64_t t0 = a.cu[b], t1 = a.cu[b + 1];
+  if (t0 == t1) return;  // uniform
   const int32_t slot = a.slots[b];
   if (slot < 0 || slot >= a.pool_slots) {  // uniform
     if (first) raise_err(a.err, MKV_DEVERR_STATE_SLOT);
@@ -247,7 +249,6 @@ __global__ __launch_bounds__(256) void linear_scan_kernel(LinArgs a, int32_t* ok
       *(uint32_t*)(a.out + (t * a.hv + h) * (kDim * 2) + d0 * 2 + 4 * (tid & 31)) = 0u;
     return;
   }
-  if (t0 == t1) return;
   float* st = a.state + ((int64_t)slot * a.hv + h) * kStateHead + (int64_t)d0 * kDim;
   Rows<kRows> m;
 #pragma unroll
@@ -326,7 +327,6 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 typedef __attribute__((address_space(3))) u32x2 lds_u32x2;
 typedef __attribute__((address_space(3))) float lds_f32;
-typedef __attribute__((address_space(3))) double lds_f64;
 typedef __attribute__((address_space(3))) uint16_t lds_u16;
 
 constexpr int kChunk = 64;
@@ -339,10 +339,10 @@ constexpr int kKeyImage = 48 * kFrag;  // of a chunk's key head: K, Q (4 row blo
 constexpr int kLower = 6;              // operands of a 64 x 64 lower triangle
 constexpr int kTParts = 2, kPParts = 1;
 // The factors of a chunk's tokens, [64] each: of K S0^T in the right-hand side,
-// of u in the state, e^G, of the output, of v; then e^G_63, whether to walk, and
-// the largest factor of v.
+// of u in the state, e^G, of the output, of v; then e^G_63, whether to walk (two
+// words), and the largest factor of v.
 constexpr int kFactors = 2048, kFacX = 0, kFacU = 64, kFacG = 128, kFacO = 192, kFacV = 256;
-constexpr int kFacAll = 320, kFacWalk = 321, kFacMax = 322;
+constexpr int kFacAll = 320, kFacWalk = 322, kFacMax = 324;
 constexpr int head_image(bool delta) {
   return (delta ? kTParts * kLower * kFrag : 0) + kPParts * kLower * kFrag + kFactors;
 }
@@ -355,14 +355,17 @@ constexpr float kMostPart = 0x1p15f;    // of operands of fp16 parts (fp16 ends 
 constexpr float kMostValue = 0x1p13f;   // of right-hand sides and u, in units of the state's scale
 constexpr float kMostState = 0x1p12f, kHighState = 0x1p9f, kLowState = 0x1p-2f;
 
+constexpr uint32_t kXcds = 8;
+
 struct ChunkArgs {
   uint8_t* keys;   // [ids][khs] key images
   uint8_t* heads;  // [ids][khs * group] head images
   int32_t kh0, khs;  // key heads of this launch
   int32_t parts;     // workgroups per head
+  int32_t rows;      // sequences, or segments
   int32_t seg;       // tokens of a segment (a multiple of 64)
   float* ends;       // [segment ids][heads of the launch][128][128]: B, then the first states
-  float* steps;      // as ends: M transposed; without the delta rule one factor each
+  float* steps;      // as ends: M's operand blocks; without the delta rule one factor each
 };
 
 __device__ __forceinline__ uint32_t lds_addr(const void* p) {
@@ -437,35 +440,42 @@ __device__ __forceinline__ bool huge(u32x4 w) {  // any of 8 bf16
 }
 
 // One workgroup per (chunk, key head): K and Q rows through LDS, their images;
-// then each wave takes value heads of the group in turn. A wave keeps A as 10
-// 16 x 16 blocks in LDS (row-major, 16-byte chunks XORed by row / 4). The
-// inverse runs by blocks: the diagonal ones by forward substitution, a lane per
-// column, and the rest in fp32 matrix instructions (16x16x4).
+// then the value heads of the group, four at a time: a wave makes a head's P and
+// factors, and with the delta rule another one A and T. That wave keeps A as 10
+// 16 x 16 blocks in LDS (row-major, 16-byte chunks XORed by row / 4) and inverts
+// by blocks: the diagonal ones by forward substitution, a lane per column, the
+// rest in fp32 matrix instructions (16x16x4). Bound by the latency of these
+// chains: 512 chunks of 8 heads take 44 us, a lone one 13; with one wave for
+// both parts of a head (2 waves per SIMD, not 4) 48 and 17.
 constexpr int kRowB = 272;  // bytes of a staged row: 256 and a pad against bank conflicts
 constexpr int kBlocks = 10;
+constexpr int kSlots = 4;   // heads at a time
 
 template <bool DELTA>
-__global__ __launch_bounds__(256) void linear_prep_kernel(LinArgs a, ChunkArgs c) {
+__global__ __launch_bounds__(DELTA ? 512 : 256, 4) void linear_prep_kernel(LinArgs a, ChunkArgs c) {
+  constexpr int kWaves = DELTA ? 8 : 4;
   __shared__ __attribute__((aligned(16))) uint8_t stage[2 * kChunk * kRowB];
-  __shared__ __attribute__((aligned(16))) uint8_t blocks[4][DELTA ? kBlocks * kFrag : kFrag];
-  __shared__ double run[4][kChunk];
-  __shared__ float strength[4][kChunk];
-  __shared__ float inv[2][kChunk];  // 1 / norms of k, q
+  __shared__ __attribute__((aligned(16))) uint8_t blocks[kSlots][DELTA ? kBlocks * kFrag : 16];
+  __shared__ double run[kSlots][kChunk];
+  // e^(G_16 mt - G_j) for j < 16 mt: 16, 32 and 48 of them
+  __shared__ __attribute__((aligned(16))) float since[kSlots][96];
+  __shared__ float inv[2][kChunk];   // 1 / norms of k, q
   __shared__ float unit[2][kChunk];  // the powers of two that bring rows of k, q near 1
   const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, d = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t id = blockIdx.x;
   const int32_t kh = c.kh0 + blockIdx.y;
-  const int32_t b = tile_sequence(a.cu, a.n, id);
+  const int32_t b = tile_sequence(a.cu, a.n, a.tokens, id);
+  if (b < 0) return;  // uniform; bad offsets
   const int64_t s0 = a.cu[b], s1 = a.cu[b + 1];
   const int64_t t0 = s0 + (id - first_tile((int32_t)s0, b)) * kChunk;
-  if (s0 < 0 || s1 > a.tokens || t0 < s0 || t0 >= s1) return;  // uniform; no tile, or bad offsets
+  if (t0 < s0 || t0 >= s1) return;  // uniform; no such tile
   const int32_t len = (int32_t)(s1 - t0 < kChunk ? s1 - t0 : kChunk);
 
   bool odd = false;
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {  // 16 chunks of 16 bytes per row
-    const int r = (tid >> 4) + 16 * u, ch = tid & 15;
+  for (int u = 0; u < 16 / kWaves; ++u) {  // 16 chunks of 16 bytes per row
+    const int r = (tid >> 4) + 4 * kWaves * u, ch = tid & 15;
     u32x4 kv = u32x4{0u, 0u, 0u, 0u}, qv = kv;
     if (r < len) {
       kv = ld16(a.k + (t0 + r) * a.k_stride + kh * (kDim * 2) + ch * 16);
@@ -508,29 +518,27 @@ __global__ __launch_bounds__(256) void linear_prep_kernel(LinArgs a, ChunkArgs c
       return f16_pack(bits_f32(w << 16) * u, bits_f32(w & 0xffff0000u) * u);
     };
 #pragma unroll
-    for (int f = 0; f < 4; ++f) {  // row block `wave`, step f
-      const uint32_t at = (16 * wave + m) * kRowB + (32 * f + 4 * d) * 2;
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const uint32_t from = (x ? sq : sk) + at;
-        const float u = unit[x][16 * wave + m];
-        const u32x2 lo = *(lds_u32x2*)(uintptr_t)from, hi = *(lds_u32x2*)(uintptr_t)(from + 32);
-        st16(img + (x * 16 + 4 * wave + f) * kFrag,
-             u32x4{two(lo.x, u), two(lo.y, u), two(hi.x, u), two(hi.y, u)});
-      }
+    for (int u = 0; u < 32 / kWaves; ++u) {  // K and Q: row block f / 4 % 4, step f % 4
+      const int f = wave * (32 / kWaves) + u;
+      const int row = 16 * ((f >> 2) & 3) + m;
+      const uint32_t from = (f >= 16 ? sq : sk) + row * kRowB + (32 * (f & 3) + 4 * d) * 2;
+      const float x = unit[f >> 4][row];
+      const u32x2 lo = *(lds_u32x2*)(uintptr_t)from, hi = *(lds_u32x2*)(uintptr_t)(from + 32);
+      st16(img + f * kFrag, u32x4{two(lo.x, x), two(lo.y, x), two(hi.x, x), two(hi.y, x)});
     }
 #pragma unroll
-    for (int f = 0; f < 4; ++f) {  // K^T: keys 16 (2 wave + f / 2) + m, tokens of step f % 2
+    for (int u = 0; u < 16 / kWaves; ++u) {  // K^T: keys 16 (f / 2) + m, tokens of step f % 2
+      const int f = wave * (16 / kWaves) + u;
       u32x4 w;
 #pragma unroll
       for (int j = 0; j < 8; j += 2) {
         const int t = 32 * (f & 1) + 16 * (j >> 2) + 4 * d + (j & 3);
-        const uint32_t at = sk + t * kRowB + (16 * (2 * wave + (f >> 1)) + m) * 2;
+        const uint32_t at = sk + t * kRowB + (16 * (f >> 1) + m) * 2;
         w[j >> 1] = f16_pack(
             bits_f32((uint32_t) * (lds_u16*)(uintptr_t)at << 16) * unit[0][t],
             bits_f32((uint32_t) * (lds_u16*)(uintptr_t)(at + kRowB) << 16) * unit[0][t + 1]);
       }
-      st16(img + (32 + 4 * wave + f) * kFrag, w);
+      st16(img + (32 + f) * kFrag, w);
     }
   }
   // without norms, keys far from 1 would put u far from the state's scale: u
@@ -543,19 +551,28 @@ __global__ __launch_bounds__(256) void linear_prep_kernel(LinArgs a, ChunkArgs c
     size = fmaxf(1.f / x, 0x1p-30f);
   }
 
-  const uint32_t blk = lds_addr(blocks[wave]);
-  // element (row i, 4 columns from 4 x) of block n
-  auto block4 = [&](int n, int i, int x) __attribute__((always_inline)) {
-    return blk + (uint32_t)(n * kFrag + i * 64 + ((x ^ ((i >> 2) & 3)) << 4));
+  const int slot = wave & (kSlots - 1);
+  const bool makes_t = wave >= kSlots;  // uniform
+  // rows 16 t + m of K or Q as operands, and their products with the rows of block nt:
+  // lane (m, d) has those of row 16 mt + m with rows 16 nt + 4 d + r
+  auto rows_of = [&](uint32_t base, int t, u32x4 (&x)[4]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) x[s] = lds_ld16(base + (16 * t + m) * kRowB + (32 * s + 8 * d) * 2);
   };
-  // e^(G_16 mt - G_j) for j < 16 mt, mt from 1 on: in the last block's place, which is written last
-  const uint32_t since = blk + (DELTA ? (kBlocks - 1) * kFrag : 0);
-  for (int32_t o = wave; o < a.group; o += 4) {
-    const int32_t h = kh * a.group + o;
-    uint8_t* img = c.heads + ((id * c.khs + blockIdx.y) * a.group + o) * head_image(DELTA);
+  auto products = [&](int nt, const u32x4 (&x)[4]) __attribute__((always_inline)) {
+    u32x4 kn[4];
+    rows_of(sk, nt, kn);
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < 4; ++s) sum = mfma(kn[s], x[s], sum);
+    return sum;
+  };
+  for (int32_t o0 = 0; o0 < a.group; o0 += kSlots) {
+    const int32_t o = o0 + slot, h = kh * a.group + o;
+    const bool there = o < a.group;  // uniform
     // lane i has token i's gates
     float g = 0.f, beta = 0.f;
-    if (lane < len) load_gates(a, t0 + lane, h, g, beta);
+    if (there && lane < len) load_gates(a, t0 + lane, h, g, beta);
     float grow = fmaxf(g, 0.f);
 #pragma unroll
     for (int s = 1; s < 64; s *= 2) grow += __shfl_xor(grow, s);
@@ -567,82 +584,103 @@ __global__ __launch_bounds__(256) void linear_prep_kernel(LinArgs a, ChunkArgs c
       const double x = __shfl_up(gsum, s);
       if (lane >= s) gsum += x;
     }
-    const double all = __shfl(gsum, 63);
-    const float rk = inv[0][lane] / unit[0][lane], rq = inv[1][lane] / unit[1][lane];
-    const float head = exp_of(gsum), strong = DELTA ? beta * size : size;
-    wave_sync();  // the last head's readers are done
-    run[wave][lane] = gsum;
-    strength[wave][lane] = beta;
-    wave_sync();
+    if (o0 > 0) __syncthreads();  // the last heads' readers are done
+    if (!makes_t) {
+      run[slot][lane] = gsum;
 #pragma unroll
-    for (int mt = 1; mt < 4; ++mt) {
-      const double x = run[wave][16 * mt] - gsum;
-      *(lds_f32*)(uintptr_t)(since + ((mt - 1) * kChunk + lane) * 4) = lane < 16 * mt ? exp_of(x) : 0.f;
-    }
-    wave_sync();
-    float* fac = (float*)(img + head_image(DELTA) - kFactors);
-    fac[kFacX + lane] = head * rk * strong;
-    fac[kFacU + lane] = exp_of(all - gsum) * rk / size;
-    fac[kFacG + lane] = head;
-    fac[kFacO + lane] = a.scale * rq;
-    fac[kFacV + lane] = strong;
-    float most = fabsf(strong), largest = 0.f;  // largest: of the operands written below
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) most = fmaxf(most, __shfl_xor(most, o));
-    uint8_t* pimg = img + (DELTA ? kTParts * kLower * kFrag : 0) + lane * 16;
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      u32x4 km[4], qm[4];  // rows 16 mt + m of K and Q as B operands
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        km[s] = lds_ld16(sk + (16 * mt + m) * kRowB + (32 * s + 8 * d) * 2);
-        qm[s] = lds_ld16(sq + (16 * mt + m) * kRowB + (32 * s + 8 * d) * 2);
+      for (int mt = 1; mt < 4; ++mt) {
+        const double x = __shfl(gsum, 16 * mt) - gsum;
+        if (lane < 16 * mt) since[slot][8 * mt * (mt - 1) + lane] = exp_of(x);
       }
-      const int i = 16 * mt + m;
-      // e^(G_i - G_j) below the diagonal block: by way of the block's first token
-      const double gi = run[wave][i];
-      const float from = exp_of(gi - run[wave][16 * mt]);
-      const float ki = inv[0][i] * strength[wave][i], qi = unit[1][i] / size;
-      float p[8];
+    }
+    __syncthreads();
+    if (!there) continue;
+    // e^(G_i - G_j), i = 16 mt + m, j = 16 nt + 4 d + r; below the diagonal
+    // block by way of the row block's first token
+    auto decays = [&](int mt, int nt, double gi, float from) __attribute__((always_inline)) {
+      f32x4 e;
+      if (nt < mt) {
+        e = *(const f32x4*)&since[slot][8 * mt * (mt - 1) + 16 * nt + 4 * d];
 #pragma unroll
-      for (int nt = 0; nt <= mt; ++nt) {
-        // k_i . k_j and q_i . k_j for j = 16 nt + 4 d + r
-        f32x4 kk = {0.f, 0.f, 0.f, 0.f}, qk = kk;
+        for (int r = 0; r < 4; ++r) e[r] *= from;
+      } else {
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          const u32x4 kn = lds_ld16(sk + (16 * nt + m) * kRowB + (32 * s + 8 * d) * 2);
-          if (DELTA) kk = mfma(kn, km[s], kk);
-          qk = mfma(kn, qm[s], qk);
-        }
-        f32x4 av, decay;
-        if (nt < mt) {
-          decay = lds_ldf4(since + ((mt - 1) * kChunk + 16 * nt + 4 * d) * 4);
+        for (int r = 0; r < 4; ++r)
+          e[r] = exp_of(4 * d + r <= m ? gi - run[slot][16 * nt + 4 * d + r] : 0.);
+      }
 #pragma unroll
-          for (int r = 0; r < 4; ++r) decay[r] *= from;
-        } else {
+      for (int r = 0; r < 4; ++r) e[r] *= inv[0][16 * nt + 4 * d + r];
+      return e;
+    };
+    uint8_t* img = c.heads + ((id * c.khs + blockIdx.y) * a.group + o) * head_image(DELTA);
+    float* fac = (float*)(img + head_image(DELTA) - kFactors);
+    float largest = 0.f;  // of the operands written below
+    if (!makes_t) {
+      const double all = __shfl(gsum, 63);
+      const float rk = inv[0][lane] / unit[0][lane], rq = inv[1][lane] / unit[1][lane];
+      const float head = exp_of(gsum), strong = DELTA ? beta * size : size;
+      fac[kFacX + lane] = head * rk * strong;
+      fac[kFacU + lane] = exp_of(all - gsum) * rk / size;
+      fac[kFacG + lane] = head;
+      fac[kFacO + lane] = a.scale * rq;
+      fac[kFacV + lane] = strong;
+      float most = fabsf(strong);
+#pragma unroll
+      for (int x = 1; x < 64; x *= 2) most = fmaxf(most, __shfl_xor(most, x));
+      uint8_t* pimg = img + (DELTA ? kTParts * kLower * kFrag : 0) + lane * 16;
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        u32x4 qm[4];
+        rows_of(sq, mt, qm);
+        const double gi = run[slot][16 * mt + m];
+        const float from = exp_of(gi - run[slot][16 * mt]), qi = unit[1][16 * mt + m] / size;
+        float p[8];
+#pragma unroll
+        for (int nt = 0; nt <= mt; ++nt) {
+          const f32x4 qk = products(nt, qm), e = decays(mt, nt, gi, from);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int j = 16 * nt + 4 * d + r;
-            decay[r] = exp_of(j <= i ? gi - run[wave][j] : 0.);
+            p[4 * (nt & 1) + r] = nt < mt || 4 * d + r <= m ? qi * e[r] * qk[r] : 0.f;
+            if (!(nt & 1)) p[4 + r] = 0.f;
           }
-        }
+          if ((nt & 1) || nt == mt) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int j = 16 * nt + 4 * d + r;
-          const float w = inv[0][j] * decay[r];
-          av[r] = j < i ? ki * w * kk[r] : 0.f;
-          p[4 * (nt & 1) + r] = j <= i ? qi * w * qk[r] : 0.f;
-          if (!(nt & 1)) p[4 + r] = 0.f;
-        }
-        if (DELTA) lds_st16(block4(mt * (mt + 1) / 2 + nt, m, d), __builtin_bit_cast(u32x4, av));
-        if ((nt & 1) || nt == mt) {
-#pragma unroll
-          for (int r = 0; r < 8; ++r) largest = fmaxf(largest, fabsf(p[r]));
-          st16(pimg + lower(mt, nt >> 1) * kFrag, upper(p));
+            for (int r = 0; r < 8; r += 2) largest = most_of(largest, p[r], p[r + 1]);
+            st16(pimg + lower(mt, nt >> 1) * kFrag, upper(p));
+          }
+          __builtin_amdgcn_sched_barrier(0);  // (registers: one block's reads at a time)
         }
       }
-    }
-    if (DELTA) {
+      walk |= __builtin_amdgcn_ballot_w64(!(largest < kMostPart)) != 0;
+      if (lane == 0) {
+        fac[kFacAll] = exp_of(all);
+        fac[kFacMax] = most;
+        ((int32_t*)fac)[kFacWalk] = walk;
+        if (!DELTA) ((int32_t*)fac)[kFacWalk + 1] = 0;
+      }
+    } else if (DELTA) {
+      const uint32_t blk = lds_addr(blocks[slot]);
+      // element (row i, 4 columns from 4 x) of block n
+      auto block4 = [&](int n, int i, int x) __attribute__((always_inline)) {
+        return blk + (uint32_t)(n * kFrag + i * 64 + ((x ^ ((i >> 2) & 3)) << 4));
+      };
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        u32x4 km[4];
+        rows_of(sk, mt, km);
+        const double gi = run[slot][16 * mt + m];
+        const float from = exp_of(gi - run[slot][16 * mt]);
+        const float ki = inv[0][16 * mt + m] * __shfl(beta, 16 * mt + m);
+#pragma unroll
+        for (int nt = 0; nt <= mt; ++nt) {
+          f32x4 av = products(nt, km);
+          const f32x4 e = decays(mt, nt, gi, from);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) av[r] = nt < mt || 4 * d + r < m ? ki * e[r] * av[r] : 0.f;
+          lds_st16(block4(mt * (mt + 1) / 2 + nt, m, d), __builtin_bit_cast(u32x4, av));
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
       wave_sync();
       {  // the diagonal blocks' inverses: lane (m, d) has column m of block d's
         float t[16];
@@ -689,20 +727,17 @@ __global__ __launch_bounds__(256) void linear_prep_kernel(LinArgs a, ChunkArgs c
           for (int s = 0; s < 4; ++s)
             res = __builtin_amdgcn_mfma_f32_16x16x4f32(-left[s], acc[s], res, 0, 0, 0);
           tb[mt * (mt + 1) / 2 + nt] = res;
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
       wave_sync();
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt)
+      for (int n = 0; n < kBlocks; ++n) {
+        largest = most_of(most_of(largest, tb[n][0], tb[n][1]), tb[n][2], tb[n][3]);
 #pragma unroll
-        for (int nt = 0; nt <= mt; ++nt) {
-          const int n = mt * (mt + 1) / 2 + nt;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            largest = fmaxf(largest, fabsf(tb[n][r]));
-            *(lds_f32*)(uintptr_t)(block4(n, 4 * d + r, m >> 2) + (m & 3) * 4) = tb[n][r];
-          }
-        }
+        for (int r = 0; r < 4; ++r)
+          *(lds_f32*)(uintptr_t)(block4(n, 4 * d + r, m >> 2) + (m & 3) * 4) = tb[n][r];
+      }
       wave_sync();
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt)
@@ -723,12 +758,8 @@ __global__ __launch_bounds__(256) void linear_prep_kernel(LinArgs a, ChunkArgs c
             st16(img + lane * 16 + (part * kLower + lower(mt, s)) * kFrag, w);
           }
         }
-    }
-    walk |= __builtin_amdgcn_ballot_w64(!(largest < kMostPart)) != 0;
-    if (lane == 0) {
-      fac[kFacAll] = exp_of(all);
-      ((int32_t*)fac)[kFacWalk] = walk;
-      fac[kFacMax] = most;
+      const bool out_of_range = __builtin_amdgcn_ballot_w64(!(largest < kMostPart)) != 0;
+      if (lane == 0) ((int32_t*)fac)[kFacWalk + 1] = out_of_range;
     }
   }
 }
@@ -773,6 +804,9 @@ template <int WAVES, bool DELTA, int MODE>
 __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(LinArgs a, ChunkArgs c,
                                                                              int32_t* ok_word) {
   constexpr bool kOut = MODE != kEnds;
+  // With 4 waves per SIMD these hide each other's waits in 128 registers; with
+  // fewer, operands are read a step ahead.
+  constexpr bool kAhead = WAVES < 16;
   // a buffer: K, K^T, T, then Q and P, then the factors (offsets from the low
   // part's base, or from the high part's for what follows it)
   constexpr int kK = 0, kKt = 16 * kFrag, kQ = 32 * kFrag;
@@ -784,29 +818,41 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
   uint32_t l0 = lds_addr(lds), l1 = l0 + kBuffer;  // this chunk's buffer, and the next one's
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, d = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int32_t part = blockIdx.x % c.parts, o = blockIdx.x / c.parts;  // o: head of the launch
+  // Workgroups are dealt to the 8 XCDs in turn. The value heads of a key head
+  // read the same K, Q and K^T: they go to one XCD, whose L2 reads them once (8
+  // x 4096 tokens: 2 to 3 % less time than one XCD a head).
+  const uint32_t members = (uint32_t)(a.group * c.parts), lot = blockIdx.x / kXcds;
+  const uint32_t pair = lot / members * kXcds + blockIdx.x % kXcds;  // (key head, row of the launch)
+  const uint32_t member = lot % members, khl = pair % (uint32_t)c.khs;
+  const int32_t y = (int32_t)(pair / (uint32_t)c.khs);  // sequence, or segment
+  if (y >= c.rows) return;                              // uniform
+  const int32_t part = (int32_t)(member % (uint32_t)c.parts);
+  const int32_t o = (int32_t)(khl * a.group + member / c.parts);  // head of the launch
   const int32_t h = c.kh0 * a.group + o, kh = h / a.group;
-  // kEnds: the parts behind the value dims' are the rows of M
-  const bool ident = MODE == kEnds && part * 16 * WAVES >= kDim;
-  const int d0 = part * 16 * WAVES + 16 * wave - (ident ? kDim : 0);  // the wave's value dims
-  const bool first = blockIdx.x == 0 && c.kh0 == 0 && tid == 0;
-  const bool ok = offsets_ok(a.cu, a.n, a.tokens);
-  if (MODE != kEnds && first && blockIdx.y == 0) *ok_word = ok;
-  if (!ok) {
-    if (MODE != kEnds && first && blockIdx.y == 0) raise_err(a.err, MKV_DEVERR_TABLE);
+  // kEnds: the waves behind the value dims' have the rows of M
+  const int at_dim = part * 16 * WAVES + 16 * wave;
+  const bool ident = MODE == kEnds && at_dim >= kDim;
+  const int d0 = at_dim - (ident ? kDim : 0);  // the wave's value dims
+  const bool first = o == 0 && part == 0 && c.kh0 == 0 && tid == 0;
+  int32_t b = y;
+  if (MODE != kWhole)
+    b = tile_sequence(a.cu, a.n, a.tokens, y, c.seg);
+  else if (!offsets_ok(a.cu, a.n, a.tokens))
+    b = -1;
+  if (MODE != kEnds && first && y == 0) *ok_word = b >= 0;
+  if (b < 0) {
+    if (MODE != kEnds && first && y == 0) raise_err(a.err, MKV_DEVERR_TABLE);
     return;
   }
-  int32_t b = blockIdx.y;
-  if (MODE != kWhole) b = tile_sequence(a.cu, a.n, blockIdx.y, c.seg);
   const int64_t q0 = ld_const(a.cu + b), q1 = ld_const(a.cu + b + 1);  // the sequence's rows
   int64_t s0 = q0, s1 = q1;                                            // this workgroup's
   int64_t seg = 0;
   if (MODE != kWhole) {
-    seg = (int64_t)blockIdx.y - first_tile((int32_t)q0, b, c.seg);
+    seg = y - first_tile((int32_t)q0, b, c.seg);
     s0 = q0 + seg * c.seg;
     s1 = s0 + c.seg < q1 ? s0 + c.seg : q1;
-    if (s0 >= q1) return;  // uniform: no such segment
   }
+  if (s0 >= q1) return;  // uniform: no rows, or no such segment
   const bool last = s1 == q1;
   const int32_t slot = ld_const(a.slots + b);
   const int64_t out_row = (int64_t)a.hv * (kDim * 2);
@@ -817,9 +863,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
     for (int64_t t = s0 + d; t < s1; t += 4) *(uint16_t*)(outp + t * out_row) = 0;
     return;
   }
-  if (MODE == kEnds && (last || (ident && seg == 0))) return;  // uniform: not asked for
+  if (MODE == kEnds && last) return;  // uniform: not asked for
   const int32_t chunks = (int32_t)((s1 - s0 + kChunk - 1) / kChunk);
-  if (chunks == 0) return;
   const int64_t id0 = (q0 >> 6) + b + ((s0 - q0) >> 6);
   const uint8_t* kimg = c.keys + (id0 * c.khs + (kh - c.kh0)) * kKeyImage;
   const uint8_t* himg = c.heads + (id0 * c.khs * a.group + o) * head_image(DELTA);
@@ -839,10 +884,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
       const int i = f * WAVES + wave;
       if (f * WAVES + WAVES <= kKeys || i < kKeys) {  // images lie as K, Q, K^T
         const int from = i < 16 ? i : i < 32 ? i + 16 : i - 16;
-        dma16(kp, from * kFrag + lane * 16, to + i * kFrag);
+        dma16(kp + from * kFrag, lane * 16, to + i * kFrag);
       } else if (i < kAll) {
         const int j = i - kKeys, from = kOut || j < kTs ? j : j + kPParts * kLower;
-        dma16(hp, from * kFrag + lane * 16, to + kLow + j * kFrag);
+        dma16(hp + from * kFrag, lane * 16, to + kLow + j * kFrag);
       }
     }
   };
@@ -857,22 +902,34 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
         (int)((len - 1) * (int32_t)stride + kDim * 2), 0x00020000);
   };
   const int32_t vs = (int32_t)a.v_stride, os = (int32_t)out_row;
-  const uint32_t vat = (uint32_t)(4 * d * vs + (d0 + n) * 2), oat = (uint32_t)(4 * d * os + (d0 + n) * 2);
-  // bf16 of this lane's value dim: tokens 16 x + 4 d + r of the next chunk, and two each of this one
-  uint32_t v[8], vnext[16];
+  // Memory has a token's value dims next to each other, a lane two tokens of one
+  // dim: lanes in pairs move two dims each, the even one of the first token and
+  // the odd one of the second, and swap halves.
+  const int odd = n & 1;
+  const uint32_t vat = (uint32_t)((4 * d + odd) * vs + (d0 + n - odd) * 2);
+  const uint32_t oat = (uint32_t)((4 * d + odd) * os + (d0 + n - odd) * 2);
+  const uint32_t halves = odd ? 0x03020706u : 0x05040100u;
+  auto swap_pair = [&](uint32_t w) __attribute__((always_inline)) {
+    const uint32_t other = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0xb1, 0xf, 0xf, true);
+    return __builtin_amdgcn_perm(other, w, halves);
+  };
+  // bf16 of this lane's value dim, tokens 16 x + 4 d + (2 y, 2 y + 1) at 2 x + y; of
+  // the next chunk as they come
+  uint32_t v[8], vnext[8];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) vnext[i] = 0;
+  for (int i = 0; i < 8; ++i) vnext[i] = 0;
   auto load_v = [&](int32_t ci) __attribute__((always_inline)) {
     if (MODE == kEnds && ident) return;  // uniform
     const __amdgpu_buffer_rsrc_t rows = rows_of(a.v, a.v_stride, ci);
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      vnext[i] = __builtin_amdgcn_raw_buffer_load_b16(rows, vat, (16 * (i >> 2) + (i & 3)) * vs, 0);
+    for (int i = 0; i < 8; ++i)
+      vnext[i] =
+          __builtin_amdgcn_raw_buffer_load_b32(rows, vat, (16 * (i >> 1) + 2 * (i & 1)) * vs, 0);
   };
 
   const int64_t row0 = (int64_t)(d0 + n) * kDim + 4 * d;  // this lane's first key of its value dim
   float* st = a.state + ((int64_t)slot * a.hv + h) * kStateHead + row0;
-  const int64_t segment = ((int64_t)blockIdx.y * c.khs * a.group + o) * kStateHead;
+  const int64_t segment = ((int64_t)y * c.khs * a.group + o) * kStateHead;
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) load_images(0, l0, i);
   load_v(0);
@@ -923,13 +980,13 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
     large = !(most < kMostState);
   };
 
-  uint32_t ob[8];  // O in bf16, tokens 16 x + 4 d + (2 y, 2 y + 1) at 2 x + y
+  uint32_t ob[8];  // O in bf16, as v
   auto store_o = [&](int32_t ci) __attribute__((always_inline)) {
     const __amdgpu_buffer_rsrc_t rows = rows_of(a.out, out_row, ci);
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      __builtin_amdgcn_raw_buffer_store_b16((uint16_t)(i & 1 ? ob[i >> 1] >> 16 : ob[i >> 1]), rows,
-                                            oat, (16 * (i >> 2) + (i & 3)) * os, 0);
+    for (int i = 0; i < 8; ++i)
+      __builtin_amdgcn_raw_buffer_store_b32(swap_pair(ob[i]), rows, oat,
+                                            (16 * (i >> 1) + 2 * (i & 1)) * os, 0);
   };
   bool stored = true;
   for (int32_t ci = 0; ci < chunks; ++ci) {
@@ -938,7 +995,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
     arrive_all();  // the chunk's images and v are there; the other buffer is read
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      v[i] = vnext[2 * i] | (vnext[2 * i + 1] << 16);
+      v[i] = swap_pair(vnext[i]);
       asm volatile("" : "+v"(v[i]));
     }
     auto value = [&](int i) __attribute__((always_inline)) {
@@ -970,14 +1027,15 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
     // X = K S0^T, Y = Q S0^T. Operand reads run a step ahead of their use, and
     // the vector unit cuts the next step's state while the matrix cores run.
     f32x4 xa[4], ya[4];
-    u32x4 kf[2][4], qf[2][4], sp[2][2];
+    constexpr int kSets = kAhead ? 2 : 1;
+    u32x4 kf[kSets][4], qf[kSets][4], sp[kSets][2];
 #pragma unroll
     for (int i = 0; i < 4; ++i) xa[i] = ya[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     auto read_kq = [&](int ks) __attribute__((always_inline)) {
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
-        if (DELTA) kf[ks & 1][mt] = frag(kK + (4 * mt + ks) * kFrag);
-        if (kOut) qf[ks & 1][mt] = frag(kQ + (4 * mt + ks) * kFrag);
+        if (DELTA) kf[ks % kSets][mt] = frag(kK + (4 * mt + ks) * kFrag);
+        if (kOut) qf[ks % kSets][mt] = frag(kQ + (4 * mt + ks) * kFrag);
       }
     };
     auto cut_state = [&](int ks) __attribute__((always_inline)) {
@@ -985,10 +1043,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = s[2 * ks + (j >> 2)][j & 3];
       if (DELTA) {
-        sp[ks & 1][0] = cut(x);
-        sp[ks & 1][1] = upper(x);
+        sp[ks % kSets][0] = cut(x);
+        sp[ks % kSets][1] = upper(x);
       } else {
-        sp[ks & 1][0] = upper(x);
+        sp[ks % kSets][0] = upper(x);
       }
     };
     f32x4 cf[4], bf[4], ef[4];
@@ -1000,20 +1058,25 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
         for (int p = 0; p < 2; ++p)
           tq[to][2 * i + p] = later(kT + (p * kLower + lower(mt0 + i, ks)) * kFrag);
     };
-    if (DELTA || kOut) {
+    if (kAhead && (DELTA || kOut)) {
       read_kq(0);
       cut_state(0);
     }
     if (more) load_v(ci + 1);
-    __builtin_amdgcn_sched_barrier(0);
+    if (kAhead) __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
-      if (ks < 3) {
+      if (!kAhead && (DELTA || kOut)) {
+        read_kq(ks);
+        cut_state(ks);
+      } else if (ks < 3) {
         if (DELTA || kOut) {
           read_kq(ks + 1);
           cut_state(ks + 1);
         }
-      } else if (DELTA) {
+      }
+      if (kAhead && DELTA && ks == 3) {
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt) {
           cf[mt] = lds_ldf4(fac + (kFacX + 16 * mt) * 4);
@@ -1026,12 +1089,12 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
         for (int p = DELTA ? 1 : 0; p >= 0; --p) {
           if (DELTA)
 #pragma unroll
-            for (int mt = 0; mt < 4; ++mt) xa[mt] = mfma16(kf[ks & 1][mt], sp[ks & 1][p], xa[mt]);
+            for (int mt = 0; mt < 4; ++mt) xa[mt] = mfma16(kf[ks % kSets][mt], sp[ks % kSets][p], xa[mt]);
           if (kOut && p == 0)
 #pragma unroll
-            for (int mt = 0; mt < 4; ++mt) ya[mt] = mfma16(qf[ks & 1][mt], sp[ks & 1][p], ya[mt]);
+            for (int mt = 0; mt < 4; ++mt) ya[mt] = mfma16(qf[ks % kSets][mt], sp[ks % kSets][p], ya[mt]);
         }
-        if (ks < 3) {
+        if (kAhead && ks < 3) {
           __builtin_amdgcn_sched_group_barrier(kSchedDsRead, (DELTA ? 4 : 0) + (kOut ? 4 : 0), 0);
 #pragma unroll
           for (int i = 0; i < (DELTA ? 8 : 0) + (kOut ? 4 : 0); ++i) {
@@ -1043,8 +1106,9 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
       __builtin_amdgcn_sched_barrier(0);
       if (ks < kLoads && more) load_images(ci + 1, l1, ks);
     }
-    const int32_t walk = __builtin_amdgcn_readfirstlane(
-        *(__attribute__((address_space(3))) int32_t*)(uintptr_t)(l0 + kLow + kFac + kFacWalk * 4));
+    __builtin_amdgcn_s_setprio(0);
+    const u32x2 walks = *(lds_u32x2*)(uintptr_t)(l0 + kLow + kFac + kFacWalk * 4);
+    const uint32_t walk = __builtin_amdgcn_readfirstlane(walks.x | walks.y);
     const float decay = *(lds_f32*)(uintptr_t)(l0 + kLow + kFac + kFacAll * 4);
     if (MODE == kEnds && !DELTA) whole *= decay;
     const uint32_t lnow = l0;
@@ -1058,13 +1122,21 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
 #pragma unroll
       for (int mt = 2 * ks; mt < 4; ++mt) pf[mt] = later(kP + lower(mt, ks) * kFrag);
     };
-    auto read_kt = [&](int ks) __attribute__((always_inline)) {
+    auto read_kt = [&](int ks, int from, int to) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) tf[i] = frag(kKt + (2 * i + ks) * kFrag);
+      for (int i = from; i < to; ++i) tf[i] = frag(kKt + (2 * i + ks) * kFrag);
     };
     if (DELTA) {
-      read_t(1, 2, 0);
-      __builtin_amdgcn_sched_barrier(0);
+      if (!kAhead) {
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) {
+          cf[mt] = lds_ldf4(fac + (kFacX + 16 * mt) * 4);
+          bf[mt] = lds_ldf4(fac + (kFacV + 16 * mt) * 4);
+        }
+      } else {
+        read_t(1, 2, 0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
       float most = 0.f;
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
@@ -1104,14 +1176,23 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) u[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
       cut_rhs(0, r0);
-      __builtin_amdgcn_sched_barrier(0);
+      if (kAhead)
+        __builtin_amdgcn_sched_barrier(0);
+      else
+        read_t(0, 0, 0);
       cut_rhs(1, r1);
       mul_t(0, 0, r0);
+      if (!kAhead) {
+        __builtin_amdgcn_sched_barrier(0);
+        read_t(1, 2, 0);
+      }
       mul_t(1, 2, r0);
+      if (kAhead) {
 #pragma unroll
-      for (int i = 0; i < 12; ++i) {
-        __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(kSchedValu, 2, 0);
+        for (int i = 0; i < 12; ++i) {
+          __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(kSchedValu, 2, 0);
+        }
       }
       __builtin_amdgcn_sched_barrier(0);
       // (T's last blocks have been waited for; the others' use comes after more work)
@@ -1120,7 +1201,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) ef[mt] = lds_ldf4(fac + (kFacU + 16 * mt) * 4);
     read_p(0);
-    __builtin_amdgcn_sched_barrier(0);
+    if (kAhead) __builtin_amdgcn_sched_barrier(0);
     if (kOut && !stored) store_o(ci - 1);
     stored = false;
     if (DELTA) {
@@ -1200,7 +1281,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) eg[mt] = lds_ldf4(fac + (kFacG + 16 * mt) * 4);
     }
-    read_kt(0);
+    if (kAhead) read_kt(0, 0, 8);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
@@ -1217,6 +1298,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
           for (int r = 0; r < 4; ++r) s[i][r] *= decay;
       }
       __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(1);
       // the state's products while the vector unit rounds u and scales Y for the output's
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = u[2 * ks + (j >> 2)][j & 3];
@@ -1228,9 +1310,15 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
           for (int r = 0; r < 4; ++r) ya[mt][r] *= eg[mt][r];
       }
 #pragma unroll
-      for (int p = 1; p >= 0; --p)
+      for (int half = 0; half < (kAhead ? 1 : 2); ++half) {
+        const int from = kAhead ? 0 : 4 * half, to = kAhead ? 8 : 4 * half + 4;
+        if (!kAhead) read_kt(ks, from, to);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s[i] = mfma16(tf[i], w[p], s[i]);
+        for (int p = 1; p >= 0; --p)
+#pragma unroll
+          for (int i = from; i < to; ++i) s[i] = mfma16(tf[i], w[p], s[i]);
+        if (!kAhead) __builtin_amdgcn_sched_barrier(0);
+      }
       if (kOut) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -1239,7 +1327,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
         }
       }
       __builtin_amdgcn_sched_barrier(0);
-      if (ks == 0) read_kt(1);
+      __builtin_amdgcn_s_setprio(0);
+      if (kAhead && ks == 0) read_kt(1, 0, 8);
       if (kOut) {
 #pragma unroll
         for (int mt = 2 * ks; mt < 4; ++mt) ya[mt] = mfma16(pf[mt], uh, ya[mt]);
@@ -1269,18 +1358,21 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
 #pragma unroll
     for (int r = 0; r < 4; ++r) s[x][r] *= inv_f;
   if (MODE == kEnds) {
-    if (ident) {  // transposed, [key][row]: as linear_join_kernel reads it
+    if (ident && seg == 0) return;
+    if (ident) {
+      // as linear_join_kernel's operands: row block x of M^T, columns 16 y; lane
+      // (m, e) has row m, columns 4 e .. +3. This lane has column n of y = d0 / 16.
+      float* to = c.steps + segment + (d0 / 16) * 256 + (n >> 2) * 64 + (n & 3);
 #pragma unroll
       for (int x = 0; x < 8; ++x)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          c.steps[segment + (16 * x + 4 * d + r) * kDim + d0 + n] = s[x][r];
+        for (int r = 0; r < 4; ++r) to[x * 8 * 256 + (4 * d + r) * 4] = s[x][r];
     } else {
 #pragma unroll
       for (int x = 0; x < 8; ++x)
         st16((uint8_t*)(c.ends + segment + row0 + 16 * x), __builtin_bit_cast(u32x4, s[x]));
       if (!DELTA && tid == 0 && part == 0)
-        c.steps[(int64_t)blockIdx.y * c.khs * a.group + o] = whole;
+        c.steps[(int64_t)y * c.khs * a.group + o] = whole;
     }
   } else if (last) {
 #pragma unroll
@@ -1318,9 +1410,9 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinArgs a, ChunkArgs c
   }
 #pragma unroll
   for (int y = 0; y < 2; ++y) st16((uint8_t*)(ends + 16 * y), __builtin_bit_cast(u32x4, init[y]));
-  // A operand rows: keys 32 wave + 16 y + n of M^T, columns 16 x + 4 d + r; they
-  // and B are read a segment ahead
-  const float* mt = c.steps + at + (32 * wave + n) * kDim + 4 * d;
+  // A operand rows: keys 32 wave + 16 y + n of M^T, columns 16 x + 4 d + r, 1 KiB
+  // blocks in this order; they and B are read
+  const float* mt = c.steps + at + 2 * wave * 8 * 256 + lane * 4;
   // two segments ahead (three sets of registers, in turn)
   f32x4 m[3][2][8], acc[3][2];
   auto read_step = [&](int32_t i, f32x4 (&mi)[2][8], f32x4 (&bi)[2]) __attribute__((always_inline)) {
@@ -1332,7 +1424,7 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinArgs a, ChunkArgs c
 #pragma unroll
         for (int x = 0; x < 8; ++x)
           mi[y][x] = __builtin_bit_cast(
-              f32x4, ld16((const uint8_t*)(mt + i * next + 16 * y * kDim + 16 * x)));
+              f32x4, ld16((const uint8_t*)(mt + i * next + (y * 8 + x) * 256)));
     }
   };
   auto step = [&](int32_t i, f32x4 (&mi)[2][8], f32x4 (&bi)[2], f32x4 (&m2)[2][8],
@@ -1408,11 +1500,11 @@ __device__ __forceinline__ void load_weights(const uint8_t* w, int d, float (&x)
   }
 }
 
-// LANES lanes per row, 8 values (16 bytes) per lane and step; a thread takes
-// ROWS rows one workgroup's span apart, all loaded before the first is used.
-template <int LANES, int STEPS, int ROWS, bool BF16>
+// LANES lanes per row, 8 values (16 bytes) per lane and step. Bound by HBM: 2^20
+// rows of 128 take 130 us, 6.2 TB/s over x, z and out (four rows a thread, all
+// loaded before the first is used: 139); 2048 rows 2.7 us, a launch.
+template <int LANES, int STEPS, bool BF16>
 __global__ __launch_bounds__(kThreads) void gated_norm_kernel(NormArgs a) {
-  constexpr int kRowsPerWg = kThreads / LANES;
   const int lane = threadIdx.x % LANES;
   const uint32_t heads = (uint32_t)a.heads;
   float w[STEPS][8];
@@ -1421,107 +1513,92 @@ __global__ __launch_bounds__(kThreads) void gated_norm_kernel(NormArgs a) {
     const int d = (s * LANES + lane) * 8;
     if (d < a.dim) load_weights<BF16>(a.w, d, w[s]);
   }
-  bool there[ROWS];
-  u32x4 xv[ROWS][STEPS], zv[ROWS][STEPS];
   uint32_t first = 0, end = 0xffffffffu;
   if (a.cu) {  // rows outside the sequences stay as they are
     if (!*a.ok) return;
     first = (uint32_t)a.cu[0];
     end = (uint32_t)a.cu[a.n];
   }
-  const int64_t row0 = (int64_t)blockIdx.x * (kRowsPerWg * ROWS) + threadIdx.x / LANES;
+  const int64_t wg = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+  const int64_t row = wg * (kThreads / LANES) + threadIdx.x / LANES;
+  const uint32_t at = row < a.rows ? (uint32_t)row : 0;
+  const uint32_t token = heads == 1 ? at : at / heads, head = at - token * heads;
+  const bool there = row < a.rows && token >= first && token < end;
+  const int64_t off = (int64_t)head * a.dim * 2;
+  const uint8_t* xp = a.x + token * a.x_stride + off;
+  const uint8_t* zp = a.z + token * a.z_stride + off;
+  u32x4 xv[STEPS], zv[STEPS];
 #pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    const int64_t row = row0 + i * kRowsPerWg;
-    there[i] = row < a.rows;  // (at most 2^32 of them)
-    const uint32_t at = there[i] ? (uint32_t)row : 0;
-    const uint32_t token = heads == 1 ? at : at / heads, head = at - token * heads;
-    there[i] &= token >= first && token < end;
-    const int64_t off = (int64_t)head * a.dim * 2;
-    const uint8_t* xp = a.x + token * a.x_stride + off;
-    const uint8_t* zp = a.z + token * a.z_stride + off;
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      const int d = (s * LANES + lane) * 8;
-      xv[i][s] = zv[i][s] = u32x4{0u, 0u, 0u, 0u};
-      if (there[i] && d < a.dim) {
-        xv[i][s] = ld16(xp + 2 * d);
-        zv[i][s] = ld_nt(zp + 2 * d);
-      }
+  for (int s = 0; s < STEPS; ++s) {
+    const int d = (s * LANES + lane) * 8;
+    xv[s] = zv[s] = u32x4{0u, 0u, 0u, 0u};
+    if (there && d < a.dim) {
+      xv[s] = ld16(xp + 2 * d);
+      zv[s] = ld_nt(zp + 2 * d);
     }
   }
+  float q = 0.f;
 #pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    float q = 0.f;
+  for (int s = 0; s < STEPS; ++s)
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float lo = bits_f32(xv[i][s][j] << 16), hi = bits_f32(xv[i][s][j] & 0xffff0000u);
-        q = fmaf(lo, lo, q);
-        q = fmaf(hi, hi, q);
-      }
-#pragma unroll
-    for (int o = 1; o < LANES; o *= 2) q += __shfl_xor(q, o);
-    const float r = 1.f / sqrtf(q / (float)a.dim + a.eps);
-    if (!there[i]) continue;
-    uint8_t* out = a.out + (row0 + i * kRowsPerWg) * a.dim * 2;
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      const int d = (s * LANES + lane) * 8;
-      if (d >= a.dim) continue;
-      u32x4 y;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t x = xv[i][s][j], z = zv[i][s][j];
-        y[j] = pack_bf16(
-            bits_f32(x << 16) * r * w[s][2 * j] * silu_bf16(bits_f32(z << 16)),
-            bits_f32(x & 0xffff0000u) * r * w[s][2 * j + 1] * silu_bf16(bits_f32(z & 0xffff0000u)));
-      }
-      st16(out + 2 * d, y);
+    for (int j = 0; j < 4; ++j) {
+      const float lo = bits_f32(xv[s][j] << 16), hi = bits_f32(xv[s][j] & 0xffff0000u);
+      q = fmaf(lo, lo, q);
+      q = fmaf(hi, hi, q);
     }
+#pragma unroll
+  for (int o = 1; o < LANES; o *= 2) q += __shfl_xor(q, o);
+  const float r = 1.f / sqrtf(q / (float)a.dim + a.eps);
+  if (!there) return;
+  uint8_t* out = a.out + row * a.dim * 2;
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    const int d = (s * LANES + lane) * 8;
+    if (d >= a.dim) continue;
+    u32x4 y;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t x = xv[s][j], z = zv[s][j];
+      y[j] = pack_bf16(
+          bits_f32(x << 16) * r * w[s][2 * j] * silu_bf16(bits_f32(z << 16)),
+          bits_f32(x & 0xffff0000u) * r * w[s][2 * j + 1] * silu_bf16(bits_f32(z & 0xffff0000u)));
+    }
+    st16(out + 2 * d, y);
   }
 }
 
-template <int LANES, int STEPS, int ROWS>
+template <int LANES, int STEPS>
 void launch_norm(const NormArgs& a, hipStream_t stream) {
-  constexpr int kRowsPerWg = kThreads / LANES * ROWS;
-  const dim3 grid((unsigned)((a.rows + kRowsPerWg - 1) / kRowsPerWg));
+  constexpr int kRowsPerWg = kThreads / LANES;
+  const int64_t wgs = (a.rows + kRowsPerWg - 1) / kRowsPerWg;
+  constexpr int64_t kWide = 1 << 20;  // (a grid dimension has less than 2^32 threads)
+  const dim3 grid((unsigned)(wgs < kWide ? wgs : kWide), (unsigned)((wgs + kWide - 1) / kWide));
   if (a.w_bf16)
-    hipLaunchKernelGGL((gated_norm_kernel<LANES, STEPS, ROWS, true>), grid, dim3(kThreads), 0,
-                       stream, a);
+    hipLaunchKernelGGL((gated_norm_kernel<LANES, STEPS, true>), grid, dim3(kThreads), 0, stream, a);
   else
-    hipLaunchKernelGGL((gated_norm_kernel<LANES, STEPS, ROWS, false>), grid, dim3(kThreads), 0,
-                       stream, a);
+    hipLaunchKernelGGL((gated_norm_kernel<LANES, STEPS, false>), grid, dim3(kThreads), 0, stream,
+                       a);
 }
 
 constexpr int kNormMaxDim = 4096;
-
-// Several rows per thread where that leaves every CU a few workgroups.
-template <int LANES, int STEPS>
-void pick_rows(const NormArgs& a, hipStream_t stream) {
-  if (a.rows >= (int64_t)device_cus() * (kThreads / LANES) * 4 * 4)
-    launch_norm<LANES, STEPS, 4>(a, stream);
-  else
-    launch_norm<LANES, STEPS, 1>(a, stream);
-}
+constexpr int64_t kNormMaxRows = 1ll << 30;
 
 void run_norm(const NormArgs& a, hipStream_t stream) {
   const int32_t d = a.dim;
   if (d <= 64)
-    pick_rows<8, 1>(a, stream);
+    launch_norm<8, 1>(a, stream);
   else if (d <= 128)
-    pick_rows<16, 1>(a, stream);
+    launch_norm<16, 1>(a, stream);
   else if (d <= 256)
-    pick_rows<32, 1>(a, stream);
+    launch_norm<32, 1>(a, stream);
   else if (d <= 512)
-    pick_rows<64, 1>(a, stream);
+    launch_norm<64, 1>(a, stream);
   else if (d <= 1024)
-    launch_norm<64, 2, 1>(a, stream);
+    launch_norm<64, 2>(a, stream);
   else if (d <= 2048)
-    launch_norm<64, 4, 1>(a, stream);
+    launch_norm<64, 4>(a, stream);
   else
-    launch_norm<64, 8, 1>(a, stream);
+    launch_norm<64, 8>(a, stream);
 }
 
 // ---------------------------------------------------------------------------
@@ -1621,7 +1698,7 @@ extern "C" int mkv_linear_attn_decode(
   if (rc != MKV_OK) return rc;
   if (batch == 0) return MKV_OK;
   const dim3 grid((unsigned)num_v_heads, (unsigned)batch);
-  hipLaunchKernelGGL(linear_decode_kernel<256>, grid, dim3(256), 0, as_stream(stream), a);
+  hipLaunchKernelGGL(linear_decode_kernel, grid, dim3(kThreads), 0, as_stream(stream), a);
   return check_launch(fn);
 }
 
@@ -1629,29 +1706,36 @@ namespace mkv {
 namespace {
 
 constexpr int64_t kHeadBytes = 1024;  // the workspace's first bytes: the offsets' verdict
-// Images of one launch at most: more key heads are run in turn in the same space
-constexpr int64_t kImageBytes = 512ll << 20;
-constexpr int32_t kScanTokens = 8;  // up to so many tokens per sequence are walked one by one
+// Images of one launch at most: more key heads are run in turn in the same
+// space, which leaves CUs idle (64 heads, 32768 tokens, 1 GiB of images: 1034 us
+// at once, 1411 in two launches, 1544 in three).
+constexpr int64_t kImageBytes = 2048ll << 20;
+// Up to so many tokens per sequence are walked one by one (8 heads; token by
+// token, in chunks: 1 sequence of 8 tokens 18 us, 20; of 12 25, 20; 64 of 8 37,
+// 44; of 12 51, 44; 256 of 4 77, 121; of 8 123, 121).
+constexpr int32_t kScanTokens = 8;
 
 struct Prefill {
   bool chunked;
   int64_t ids;    // tiles
   int32_t waves;  // of a workgroup that writes outputs (a head's value dims take 8)
   int32_t seg;    // tokens of a segment; 0: whole sequences
+  int32_t end_waves;  // of a workgroup that computes segments' ends
   int64_t segs;   // segment ids
   int32_t khs;    // key heads of a launch
   int64_t key_bytes, head_bytes, end_bytes, step_bytes, total;
 };
 
 // What a pass takes (us on MI355X, fitted to 12 shapes of 1 to 32 sequences of
-// 300 to 32768 tokens under all choices): so many a chunk where up to half the
-// CUs have a workgroup, and where all have; a join so many a segment.
+// 300 to 32768 tokens under all choices, 5 % off on average): so many a chunk
+// where up to half the CUs have a workgroup, and where all have; a join so many
+// a segment.
 struct ChunkCosts {
-  float rows4[2], rows8[2], ends[2], join;
+  float rows4[2], rows8[2], ends8[2], ends16[2], join;
 };
-constexpr ChunkCosts kDeltaCosts = {{2.9f, 3.8f}, {4.0f, 5.3f}, {3.4f, 3.8f}, 1.2f};
-constexpr ChunkCosts kDecayCosts = {{2.2f, 2.9f}, {2.8f, 3.6f}, {2.0f, 2.4f}, 0.6f};
-constexpr float kPassStart = 6.f;  // a pass's launch, its first loads and its last stores
+constexpr ChunkCosts kDeltaCosts = {{2.7f, 3.2f}, {3.4f, 4.9f}, {2.4f, 3.0f}, {3.8f, 5.5f}, 1.6f};
+constexpr ChunkCosts kDecayCosts = {{1.9f, 2.1f}, {2.4f, 2.8f}, {1.4f, 2.5f}, {1.4f, 2.5f}, 0.4f};
+constexpr float kPassStart = 7.f;  // a pass's launch, its first loads and its last stores
 
 // A pass of `wgs` workgroups of at most `chunks` chunks each, one per CU at a time.
 float pass_time(const float (&cost)[2], double wgs, double chunks, int cus) {
@@ -1662,9 +1746,11 @@ float pass_time(const float (&cost)[2], double wgs, double chunks, int cus) {
 
 // Whole sequences or segments of them, and workgroups of half a head or of one,
 // by those costs. The batch is taken as its longest sequence and others alike.
-// (1 x 32768 tokens, 8 heads: whole 1505, in 32 segments 320, in 16 300; 8 x
-// 4096: whole 248, in 3 segments 238, in 8 311; 32 x 1024: half heads 192, whole
-// ones 164, in 2 segments 295; 1 x 1024: whole 71, in 4 segments 68.)
+// (us, prep and all, 8 heads: 1 x 32768 tokens whole 1507, segments of 8 chunks
+// 345, of 16 269, of 32 288; 8 x 4096 whole 242, segments of 16 chunks 232; 32 x
+// 1024 half heads 186, whole ones 145, segments of 8 chunks 227; 1 x 1024 whole
+// 70, segments of 4 chunks 64; 6 of 80 to 3000 whole 160, segments of 6 to 8
+// chunks 106 to 118.)
 void choose_walk(Prefill& p, int64_t tokens, int32_t n, int32_t longest, double heads, bool delta) {
   const ChunkCosts& c = delta ? kDeltaCosts : kDecayCosts;
   const int cus = device_cus();
@@ -1688,18 +1774,21 @@ void choose_walk(Prefill& p, int64_t tokens, int32_t n, int32_t longest, double 
   for (int32_t len = 4; len < long_chunks; len += len < 16 ? 1 : len < 64 ? 2 : 8) {
     const int64_t ids = tile_ids(tokens, n, len * kChunk);
     if (ids > 65535) continue;  // (grid.y)
-    const double of_long = ceil(long_chunks / len), of_rest = ceil(rest_chunks / len);
+    const double of_long = ceil(long_chunks / len);
+    // (others of different lengths end inside a segment, half of one on average)
+    const double of_rest = rest_chunks == long_chunks ? of_long : rest_chunks / len + .5;
     const double segs = of_long + (n - 1) * of_rest;
     const double starts = segs - n;  // segments whose end is asked for
-    const double steps = delta ? fmax(of_long - 2, 0) + (n - 1) * fmax(of_rest - 2, 0) : 0;
-    const float before = pass_time(c.ends, heads * (starts + steps), len, cus) + kPassStart +
-                         (float)of_long * c.join;
+    const float join = kPassStart + (float)of_long * c.join;
+    const float by8 = pass_time(c.ends8, heads * starts * (delta ? 2 : 1), len, cus);
+    const float by16 = pass_time(c.ends16, heads * starts, len, cus);
     for (int32_t waves = 4; waves <= 8; waves += 4) {
-      const float t =
-          before + pass_time(waves == 4 ? c.rows4 : c.rows8, heads * (8 / waves) * segs, len, cus);
+      const float t = join + (delta && by16 < by8 ? by16 : by8) +
+                      pass_time(waves == 4 ? c.rows4 : c.rows8, heads * (8 / waves) * segs, len, cus);
       if (t < best) {
         best = t;
         p.waves = waves;
+        p.end_waves = delta && by16 < by8 ? 16 : 8;
         p.seg = len * kChunk;
       }
     }
@@ -1728,6 +1817,11 @@ Prefill plan_prefill(int64_t tokens, int32_t n, int32_t longest, int32_t hk, int
   return p;
 }
 
+dim3 walk_grid(const LinArgs& a, const ChunkArgs& c) {
+  const int64_t pairs = (int64_t)c.khs * c.rows;
+  return dim3((unsigned)((pairs + kXcds - 1) / kXcds * kXcds * a.group * c.parts));
+}
+
 template <bool DELTA>
 void run_chunks(const LinArgs& a, const Prefill& p, uint8_t* ws, hipStream_t s) {
   ChunkArgs c{};
@@ -1741,17 +1835,23 @@ void run_chunks(const LinArgs& a, const Prefill& p, uint8_t* ws, hipStream_t s) 
     c.kh0 = kh0;
     c.khs = a.hk - kh0 < p.khs ? a.hk - kh0 : p.khs;
     const unsigned heads = (unsigned)(c.khs * a.group), n = (unsigned)a.n;
-    hipLaunchKernelGGL(linear_prep_kernel<DELTA>, dim3((unsigned)p.ids, (unsigned)c.khs), dim3(256),
-                       0, s, a, c);
+    hipLaunchKernelGGL(linear_prep_kernel<DELTA>, dim3((unsigned)p.ids, (unsigned)c.khs),
+                       dim3(DELTA ? 512 : 256), 0, s, a, c);
     if (p.seg) {
-      c.parts = DELTA ? 2 : 1;
-      hipLaunchKernelGGL((linear_chunk_kernel<8, DELTA, kEnds>),
-                         dim3(heads * c.parts, (unsigned)p.segs), dim3(512), 0, s, a, c, ok);
+      c.rows = (int32_t)p.segs;
+      c.parts = DELTA && p.end_waves == 8 ? 2 : 1;  // (with the delta rule M's 128 rows too)
+      if (p.end_waves == 16)
+        hipLaunchKernelGGL((linear_chunk_kernel<DELTA ? 16 : 8, DELTA, kEnds>), walk_grid(a, c),
+                           dim3(DELTA ? 1024 : 512), 0, s, a, c, ok);
+      else
+        hipLaunchKernelGGL((linear_chunk_kernel<8, DELTA, kEnds>), walk_grid(a, c), dim3(512), 0, s,
+                           a, c, ok);
       hipLaunchKernelGGL(linear_join_kernel<DELTA>, dim3(heads * (kDim / 16), n), dim3(256), 0, s,
                          a, c);
     }
     c.parts = 8 / p.waves;
-    const dim3 grid(heads * c.parts, p.seg ? (unsigned)p.segs : n), block(64 * p.waves);
+    c.rows = p.seg ? (int32_t)p.segs : a.n;
+    const dim3 grid = walk_grid(a, c), block(64 * p.waves);
     if (p.seg && p.waves == 8)
       hipLaunchKernelGGL((linear_chunk_kernel<8, DELTA, kRows>), grid, block, 0, s, a, c, ok);
     else if (p.seg)
@@ -1793,6 +1893,9 @@ extern "C" int mkv_linear_attn_prefill(
                              z_stride, norm_weight, weight_bf16, norm_eps, out, err, a);
   if (rc != MKV_OK) return rc;
   MKV_REQUIRE(num_tokens < (1ll << 31) && max_seqlen >= 0, MKV_E_INVALID, "%s: bad sizes", fn);
+  MKV_REQUIRE(batch <= kMaxSequences, MKV_E_UNSUPPORTED, "%s: more than %d sequences", fn,
+              kMaxSequences);
+  MKV_REQUIRE(num_tokens <= kNormMaxRows / num_v_heads, MKV_E_UNSUPPORTED, "%s: too many rows", fn);
   MKV_REQUIRE(v_stride <= (1 << 24), MKV_E_UNSUPPORTED, "%s: rows of v more than 16 MiB apart", fn);
   if (batch == 0 || num_tokens == 0) return MKV_OK;
   const Prefill p =
@@ -1837,7 +1940,7 @@ extern "C" int mkv_gated_rms_norm(const void* x, int64_t x_stride, const void* z
   MKV_REQUIRE(aligned16(x) && aligned16(z) && aligned16(out) && x_stride % 16 == 0 &&
                   z_stride % 16 == 0 && (uintptr_t)weight % (weight_bf16 ? 2 : 4) == 0,
               MKV_E_ALIGN, "%s: rows must be 16-byte aligned, the weight to its type", fn);
-  MKV_REQUIRE(tokens <= (1ll << 32) / heads, MKV_E_UNSUPPORTED, "%s: too many rows", fn);
+  MKV_REQUIRE(tokens <= kNormMaxRows / heads, MKV_E_UNSUPPORTED, "%s: too many rows", fn);
   NormArgs a{(const uint8_t*)x, (const uint8_t*)z, (const uint8_t*)weight, x_stride, z_stride,
              heads, dim, weight_bf16, eps, (uint8_t*)out, tokens * heads, nullptr, 0, nullptr};
   run_norm(a, as_stream(stream));

@@ -307,12 +307,11 @@ constexpr int kConvRows = 16;
 template <int W>
 __global__ __launch_bounds__(kThreads) void conv_prefill_kernel(ConvPrefillArgs p) {
   const ConvArgs& a = p.c;
-  const bool ok = offsets_ok(p.cu, a.batch, p.tokens);
-  if (!ok) {  // uniform
+  const int32_t b = tile_sequence(p.cu, a.batch, p.tokens, blockIdx.x);
+  if (b < 0) {  // uniform
     if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0) raise_err(a.err, MKV_DEVERR_TABLE);
     return;
   }
-  const int32_t b = tile_sequence(p.cu, a.batch, blockIdx.x);
   const int64_t end = p.cu[b + 1], seq0 = p.cu[b];
   const int64_t tile = (int64_t)blockIdx.x - first_tile(p.cu[b], b);
   const int64_t t0 = seq0 + tile * 64 + (threadIdx.x >> 6) * kConvRows;
@@ -565,6 +564,8 @@ extern "C" int mkv_gdn_conv_prefill(void* conv_pool, int64_t pool_slots, int32_t
   const int rc = conv_args(fn, conv_pool, pool_slots, channels, width, slots,
                            num_tokens == 0 ? 0 : batch, x, weight, kernel_size, out, err, p.c);
   if (rc != MKV_OK) return rc == kEmpty ? MKV_OK : rc;
+  MKV_REQUIRE(batch <= kMaxSequences, MKV_E_UNSUPPORTED, "%s: more than %d sequences", fn,
+              kMaxSequences);
   MKV_REQUIRE(cu_seqlens && aligned4(cu_seqlens), MKV_E_INVALID, "%s: null pointer", fn);
   MKV_REQUIRE(x_stride >= (int64_t)channels * 2, MKV_E_INVALID,
               "%s: a stride is shorter than its row", fn);

@@ -66,6 +66,23 @@ def _sig(t: torch.Tensor | None):
     return None if t is None else (t.dtype, t.shape, t.stride(), t.get_device())
 
 
+def _span(t: torch.Tensor | None) -> int:
+    """Bytes from the first element of t to behind the last."""
+    if t is None or t.numel() == 0:
+        return 0
+    return (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+
+
+def _apart(out: torch.Tensor, others, spans, names=("q", "k", "v", "g", "beta", "z")) -> None:
+    """out is written while other workgroups still read."""
+    at = out.data_ptr()
+    end = at + out.numel() * out.element_size()
+    for t, n, name in zip(others, spans, names):
+        if n and t.data_ptr() < end and at < t.data_ptr() + n:
+            raise ValueError(f"out must not be {name} or overlap it: other rows of it are still "
+                             "to be read")
+
+
 def _planned(key: tuple, check, *args) -> tuple:
     plan = _plans.get(key)
     if plan is None:
@@ -128,8 +145,8 @@ def _weight(w: torch.Tensor, dim: int) -> int:
 
 
 def _check_common(q, k, v, g, beta, state, slots, a_log, dt_bias, z, norm_weight, out):
-    """What both forms check: (device, tokens, key heads, value heads, q to
-    norm_weight's strides and types, pool slots)."""
+    """What both forms check: (device, tokens, key heads, value heads, pool
+    slots, sizes of the inputs, their strides and types)."""
     dev = _lib.require_gpu(q, k, v, g, beta, state, a_log, dt_bias, z, norm_weight, out)
     if state.dtype != torch.float32 or state.dim() != 4 or not state.is_contiguous():
         raise ValueError("state must be contiguous fp32 [slots, value heads, 128, 128]")
@@ -163,7 +180,8 @@ def _check_common(q, k, v, g, beta, state, slots, a_log, dt_bias, z, norm_weight
     if out is not None and (out.shape != (tokens, hv, HEAD_DIM) or out.dtype != torch.bfloat16
                             or not out.is_contiguous()):
         raise ValueError(f"out must be contiguous bf16 [{tokens}, {hv}, {HEAD_DIM}]")
-    return (dev, tokens, hk, hv, state.shape[0], qs, ks, vs, gs, bs, zs, wb,
+    spans = tuple(_span(t) for t in (q, k, v, g, beta, z))
+    return (dev, tokens, hk, hv, state.shape[0], spans, qs, ks, vs, gs, bs, zs, wb,
             1 if g.dtype == torch.bfloat16 else 0)
 
 
@@ -176,7 +194,7 @@ def _common(q, k, v, g, beta, state, slots, a_log, dt_bias, z, norm_weight, out)
 
 def _args(plan, q, k, v, g, beta, a_log, dt_bias, qk_norm, scale, z, norm_weight, eps, out):
     """The library's arguments from q on, up to out."""
-    qs, ks, vs, gs, bs, zs, wb, gates_bf16 = plan[5:]
+    qs, ks, vs, gs, bs, zs, wb, gates_bf16 = plan[6:]
     return (q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, g.data_ptr(), gs,
             None if beta is None else beta.data_ptr(), bs, gates_bf16,
             None if a_log is None else a_log.data_ptr(),
@@ -224,6 +242,8 @@ def linear_attn_decode(
     slots = _ids("slots", slots, dev)
     if out is None:
         out = torch.empty((B, hv, HEAD_DIM), dtype=torch.bfloat16, device=dev)
+    else:
+        _apart(out, (q, k, v, g, beta, z), plan[5])
     if slots.numel() != B:
         raise ValueError(f"slots must name a slot for each of {B} requests")
     _call(dev, "mkv_linear_attn_decode", state.data_ptr(), pool, hk, hv, HEAD_DIM,
@@ -279,6 +299,8 @@ def linear_attn_prefill(
     slots = _ids("slots", slots, dev)
     if out is None:
         out = torch.empty((tokens, hv, HEAD_DIM), dtype=torch.bfloat16, device=dev)
+    else:
+        _apart(out, (q, k, v, g, beta, z), plan[5])
     cu = _ids("cu_seqlens", cu_seqlens, dev)
     batch = slots.numel()
     if cu.numel() != batch + 1:
@@ -316,7 +338,7 @@ def _check_conv(x, weight, conv_state, out):
     if out is not None and (out.shape != (T, C) or out.dtype != x.dtype
                             or not out.is_contiguous()):
         raise ValueError(f"out must be contiguous bf16 [{T}, {C}]")
-    return dev, T, C, W, weight.shape[-1], x.stride(0) * 2 if T > 1 else C * 2
+    return dev, T, C, W, weight.shape[-1], x.stride(0) * 2 if T > 1 else C * 2, (_span(x),)
 
 
 def causal_conv_prefill(
@@ -335,12 +357,12 @@ def causal_conv_prefill(
     slots[b], which is left with the sequence's last inputs. Rows of x may be
     strided; rows of ``out`` outside the sequences are left as they were."""
     key = (_sig(x), _sig(weight), _sig(conv_state), _sig(out))
-    dev, T, C, W, K, xs = _planned(key, _check_conv, x, weight, conv_state, out)
+    dev, T, C, W, K, xs, spans = _planned(key, _check_conv, x, weight, conv_state, out)
     w = weight if weight.is_contiguous() else weight.contiguous()
     if out is None:
         out = torch.empty((T, C), dtype=x.dtype, device=dev)
-    elif T and out.data_ptr() == x.data_ptr():
-        raise ValueError("out must not be x: other rows of it are still to be read")
+    else:
+        _apart(out, (x,), spans, ("x",))
     slots, cu = _ids("slots", slots, dev), _ids("cu_seqlens", cu_seqlens, dev)
     batch = slots.numel()
     if cu.numel() != batch + 1:
@@ -366,7 +388,10 @@ def _check_norm(x, z, weight, out):
     if out is not None and (out.shape != x.shape or out.dtype != x.dtype
                             or not out.is_contiguous()):
         raise ValueError("out must be a contiguous tensor shaped like x")
-    return dev, T if H else 0, H, D, xs, zs, wb
+    # (out may lie on x or z without gaps: a thread reads what it writes)
+    whole = H * D * 2
+    return (dev, T if H else 0, H, D, xs, zs, wb, (_span(x), _span(z)),
+            (xs == whole, zs == whole))
 
 
 def gated_rms_norm(
@@ -379,11 +404,15 @@ def gated_rms_norm(
 ) -> torch.Tensor:         # as x
     """x / sqrt(mean(x^2) + eps) * weight * silu(z) over the last dimension (a
     multiple of 8, at most 4096), in fp32, rounded once. The rows of a token
-    follow each other; tokens may be strided. ``out`` may be x."""
+    follow each other; tokens may be strided. ``out`` may be x or z."""
     key = (_sig(x), _sig(z), _sig(weight), _sig(out))
-    dev, T, H, D, xs, zs, wb = _planned(key, _check_norm, x, z, weight, out)
+    dev, T, H, D, xs, zs, wb, spans, whole = _planned(key, _check_norm, x, z, weight, out)
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    else:
+        at = out.data_ptr()
+        _apart(out, (x, z), [0 if w and t.data_ptr() == at else n
+                             for t, w, n in zip((x, z), whole, spans)], ("x", "z"))
     if T:
         _call(dev, "mkv_gated_rms_norm", x.data_ptr(), xs, z.data_ptr(), zs, T, H, D,
               weight.data_ptr(), wb, float(eps), out.data_ptr())

@@ -207,15 +207,15 @@ def test_large_launches_run_their_heads_in_turn():
     """More images than one launch holds: key heads in turn, with each key head's
     share alone as the reference. Its walk may be cut otherwise: outputs differ by
     two roundings to bf16 (2^-8 relative each), states by what fp32 sums do."""
-    case("linear attention prompts, 16/64 heads x 12800 tokens in several launches")
-    T, hk, hv = 12800, 16, 64
+    case("linear attention prompts, 16/64 heads x 66000 tokens in several launches")
+    T, hk, hv = 66000, 16, 64
     gen = torch.Generator(device=DEV).manual_seed(3)
     q, k = (torch.randn(T, hk, D, generator=gen, device=DEV).bfloat16() for _ in range(2))
     v = torch.randn(T, hv, D, generator=gen, device=DEV).bfloat16()
     g = -torch.rand(T, hv, generator=gen, device=DEV)
     beta = torch.rand(T, hv, generator=gen, device=DEV)
     state = torch.randn(2, hv, D, D, generator=gen, device=DEV)
-    cu, at = ints([0, 7000, T]), ints([1, 0])
+    cu, at = ints([0, 40000, T]), ints([1, 0])
     want = state.clone()
     out = la.linear_attn_prefill(q, k, v, g, beta, state, at, cu, qk_norm=True)
     for kh in (0, 7, 15):

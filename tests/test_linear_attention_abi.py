@@ -131,3 +131,17 @@ def test_oracle_closed_forms():
     assert (one == 0).all()
     g, beta = ref.gates(torch.zeros(1, 1), torch.zeros(1, 1), torch.zeros(1), torch.zeros(1))
     assert torch.allclose(g, torch.tensor(-0.6931471805599453).double()) and beta == 0.5
+
+
+def test_more_sequences_and_rows_than_a_call_takes():
+    assert prefill(batch=4096, cu=None)[0] == -1  # (4096 are taken: the next check speaks)
+    rc, msg = prefill(batch=4097)
+    assert rc == -3 and "more than 4096 sequences" in msg
+    rc, msg = prefill(tokens=(1 << 27) + 1)
+    assert rc == -3 and "too many rows" in msg
+    rc, msg = _rc("mkv_gdn_conv_prefill", FAKE, 4, 64, 4, FAKE, FAKE, 4097, 9, FAKE, 128, FAKE, 4,
+                  FAKE, FAKE, None)
+    assert rc == -3 and "more than 4096 sequences" in msg
+    rc, msg = _rc("mkv_gated_rms_norm", FAKE, 256, FAKE, 256, (1 << 29) + 1, 2, 64, FAKE, 0, 1e-6,
+                  FAKE, None)
+    assert rc == -3 and "too many rows" in msg
