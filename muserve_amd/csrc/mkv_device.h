@@ -46,6 +46,41 @@ __device__ __forceinline__ T ld_const(const T* p) {
 // Device error bits go through a vector-memory atomic on the caller's word.
 __device__ __forceinline__ void raise_err(int32_t* err, int32_t bit) { atomicOr(err, bit); }
 
+// x of another lane by the vector unit alone. Within 16 lanes: 0xb1 and 0x4e have
+// lane ^ 1 and ^ 2, 0x141 and 0x140 lane ^ 7 and ^ 15 (as good as ^ 4 and ^ 8
+// where 4 and 8 lanes hold the same).
+template <int CTRL, typename T>
+__device__ __forceinline__ T lane_of(T x) {
+  static_assert(sizeof(T) == 4, "one register");
+  return __builtin_bit_cast(
+      T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
+// op over each LANES lanes side by side, in all of them.
+template <int LANES, typename T, typename F>
+__device__ __forceinline__ T over_lanes(T x, F op) {
+  if (LANES > 1) x = op(x, lane_of<0xb1>(x));
+  if (LANES > 2) x = op(x, lane_of<0x4e>(x));
+  if (LANES > 4) x = op(x, lane_of<0x141>(x));
+  if (LANES > 8) x = op(x, lane_of<0x140>(x));
+  if (LANES > 16) {  // (a 16-lane row and its neighbour)
+    const uint32_t v = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    const uint32_t a = r[0], b = r[1];
+    x = op(__builtin_bit_cast(T, a), __builtin_bit_cast(T, b));
+  }
+  if (LANES > 32) {
+    const uint32_t v = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    const uint32_t a = r[0], b = r[1];
+    x = op(__builtin_bit_cast(T, a), __builtin_bit_cast(T, b));
+  }
+  return x;
+}
+template <int LANES>
+__device__ __forceinline__ float sum_lanes(float x) {
+  return over_lanes<LANES>(x, [](float a, float b) { return a + b; });
+}
+
 // Whether the offsets cu[0 .. n] of packed sequences hold together: from 0 or
 // more, never falling, at most `rows`. Every thread of the workgroup calls.
 __device__ __forceinline__ bool offsets_ok(const int32_t* cu, int32_t n, int64_t rows) {
@@ -103,11 +138,7 @@ __device__ __forceinline__ int32_t tile_sequence(const int32_t* cu, int32_t n, i
     else if (i < n && first_tile(x, i, r) <= id)
       at = at > i ? at : i;
   }
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
-    const int32_t x = __shfl_xor(at, o);
-    at = at > x ? at : x;
-  }
+  at = over_lanes<64>(at, [](int32_t a, int32_t b) { return a > b ? a : b; });
   if ((threadIdx.x & 63) == 0) last[threadIdx.x >> 6] = at;
   __syncthreads();
   for (uint32_t i = 0; i < blockDim.x / 64; ++i) at = at > last[i] ? at : last[i];

@@ -76,14 +76,6 @@ __device__ __forceinline__ void load4(const uint8_t* p, float (&x)[4]) {
   x[3] = bits_f32(w.y & 0xffff0000u);
 }
 
-// sum over the 8 lanes that share a row of the state
-__device__ __forceinline__ float sum8(float x) {
-  x += __shfl_xor(x, 1);
-  x += __shfl_xor(x, 2);
-  x += __shfl_xor(x, 4);
-  return x;
-}
-
 // The recurrence over a few tokens with a head's state in registers: a row of
 // S is 8 lanes x 16 floats (lane l holds columns 4 l + 32 c .. +3, whole
 // 128-byte lines per 8 lanes), a thread holds ROWS rows. S k and S q are both
@@ -116,11 +108,11 @@ struct Rows {
       qq = fmaf(qx[j], qx[j], qq);
       m = fmaf(kx[j], qx[j], m);
     }
-    m = sum8(m);
+    m = sum_lanes<8>(m);
     rk = rq = 1.f;
     if (a.qk_norm) {
-      rk = 1.f / sqrtf(sum8(kk) + kL2Eps);
-      rq = 1.f / sqrtf(sum8(qq) + kL2Eps);
+      rk = 1.f / sqrtf(sum_lanes<8>(kk) + kL2Eps);
+      rq = 1.f / sqrtf(sum_lanes<8>(qq) + kL2Eps);
     }
     kq = m * rk * rq;
   }
@@ -136,8 +128,8 @@ struct Rows {
         x = fmaf(s[i][j], kx[j], x);
         y = fmaf(s[i][j], qx[j], y);
       }
-      x = sum8(x);
-      y = sum8(y);
+      x = sum_lanes<8>(x);
+      y = sum_lanes<8>(y);
       const float u = a.beta ? beta * (v[i] - e * rk * x) : v[i];
       o[i] = a.scale * (e * rq * y + u * kq);
       const float w = u * rk;
@@ -154,7 +146,7 @@ __device__ __forceinline__ float weight_at(const uint8_t* w, int32_t bf16, int64
 // One workgroup per (value head, request): the head's 64 KiB state is read
 // once, updated in registers and written back. Bound by HBM: 128 KiB per
 // (request, head) against 0.8 KiB of everything else; 256 requests of 8 heads
-// take 53 us, 5.1 TB/s. A lone request (7.4 us) is bound by its two trips to
+// take 53 us, 5.1 TB/s. A lone request (7.0 us) is bound by its two trips to
 // memory: 1024 threads a head, with 4 rows' loads less each, were no faster.
 __global__ __launch_bounds__(kThreads) void linear_decode_kernel(LinArgs a) {
   constexpr int kGroups = kThreads / 8, kRows = kDim / kGroups;
@@ -200,9 +192,7 @@ __global__ __launch_bounds__(kThreads) void linear_decode_kernel(LinArgs a) {
     float q = 0.f;
 #pragma unroll
     for (int i = 0; i < kRows; ++i) q = fmaf(o[i], o[i], q);
-    q += __shfl_xor(q, 8);
-    q += __shfl_xor(q, 16);
-    q += __shfl_xor(q, 32);
+    q = sum_lanes<64>(l == 0 ? q : 0.f);  // (8 lanes have the same rows)
     if ((tid & 63) == 0) part[tid >> 6] = q;
     __syncthreads();
     q = 0.f;
@@ -431,6 +421,24 @@ __device__ __forceinline__ float exp_of(double x) {
   return __builtin_amdgcn_exp2f((float)(x * 1.4426950408889634074));
 }
 
+// x of the lane that a row shift or broadcast (as a DPP control) names, 0 where
+// there is none or a row of 16 lanes is not among ROWS
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ double lanes_below(double x) {
+  const u32x2 w = __builtin_bit_cast(u32x2, x);
+  const uint32_t lo = w.x, hi = w.y;
+  return __builtin_bit_cast(
+      double, u32x2{(uint32_t)__builtin_amdgcn_update_dpp(0, (int)lo, CTRL, ROWS, 0xf, true),
+                    (uint32_t)__builtin_amdgcn_update_dpp(0, (int)hi, CTRL, ROWS, 0xf, true)});
+}
+__device__ __forceinline__ double lane_at(double x, int lane) {
+  const u32x2 w = __builtin_bit_cast(u32x2, x);
+  const uint32_t lo = w.x, hi = w.y;
+  return __builtin_bit_cast(double,
+                            u32x2{(uint32_t)__builtin_amdgcn_readlane((int)lo, lane),
+                                  (uint32_t)__builtin_amdgcn_readlane((int)hi, lane)});
+}
+
 __device__ __forceinline__ bool huge(u32x4 w) {  // any of 8 bf16
   bool h = false;
 #pragma unroll
@@ -472,15 +480,26 @@ __global__ __launch_bounds__(DELTA ? 512 : 256, 4) void linear_prep_kernel(LinAr
   if (t0 < s0 || t0 >= s1) return;  // uniform; no such tile
   const int32_t len = (int32_t)(s1 - t0 < kChunk ? s1 - t0 : kChunk);
 
-  bool odd = false;
+  // lane i has token i's gates; their loads run with the first rows'
+  const int slot = wave & (kSlots - 1);
+  const bool makes_t = wave >= kSlots;  // uniform
+  float g = 0.f, beta = 0.f;
+  u32x4 rows[2][16 / kWaves];
 #pragma unroll
   for (int u = 0; u < 16 / kWaves; ++u) {  // 16 chunks of 16 bytes per row
     const int r = (tid >> 4) + 4 * kWaves * u, ch = tid & 15;
-    u32x4 kv = u32x4{0u, 0u, 0u, 0u}, qv = kv;
+    rows[0][u] = rows[1][u] = u32x4{0u, 0u, 0u, 0u};
     if (r < len) {
-      kv = ld16(a.k + (t0 + r) * a.k_stride + kh * (kDim * 2) + ch * 16);
-      qv = ld16(a.q + (t0 + r) * a.q_stride + kh * (kDim * 2) + ch * 16);
+      rows[0][u] = ld16(a.k + (t0 + r) * a.k_stride + kh * (kDim * 2) + ch * 16);
+      rows[1][u] = ld16(a.q + (t0 + r) * a.q_stride + kh * (kDim * 2) + ch * 16);
     }
+  }
+  if (slot < a.group && lane < len) load_gates(a, t0 + lane, kh * a.group + slot, g, beta);
+  bool odd = false;
+#pragma unroll
+  for (int u = 0; u < 16 / kWaves; ++u) {
+    const int r = (tid >> 4) + 4 * kWaves * u, ch = tid & 15;
+    const u32x4 kv = rows[0][u], qv = rows[1][u];
     odd |= huge(kv) || huge(qv);
     *(u32x4*)(stage + r * kRowB + ch * 16) = kv;
     *(u32x4*)(stage + (kChunk + r) * kRowB + ch * 16) = qv;
@@ -495,13 +514,11 @@ __global__ __launch_bounds__(DELTA ? 512 : 256, 4) void linear_prep_kernel(LinAr
       kk = fmaf(k0, k0, fmaf(k1, k1, kk));
       qq = fmaf(q0, q0, fmaf(q1, q1, qq));
     }
-#pragma unroll
-    for (int o = 1; o < 16; o *= 2) {
-      kk += __shfl_xor(kk, o);
-      qq += __shfl_xor(qq, o);
-      ke = max(ke, (uint32_t)__shfl_xor((int)ke, o));
-      qe = max(qe, (uint32_t)__shfl_xor((int)qe, o));
-    }
+    kk = sum_lanes<16>(kk);
+    qq = sum_lanes<16>(qq);
+    const auto most = [](uint32_t x, uint32_t y) { return x > y ? x : y; };
+    ke = over_lanes<16>(ke, most);
+    qe = over_lanes<16>(qe, most);
     if (ch == 0) {
       unit[0][r] = bits_f32(0x7f000000u - (ke << 16));  // 2^(127 - e) of exponent field e
       unit[1][r] = bits_f32(0x7f000000u - (qe << 16));
@@ -512,14 +529,14 @@ __global__ __launch_bounds__(DELTA ? 512 : 256, 4) void linear_prep_kernel(LinAr
   odd = __syncthreads_or(odd);
 
   const uint32_t sk = lds_addr(stage), sq = sk + kChunk * kRowB;
-  {
+  if (!makes_t) {  // (the waves with less to do afterwards)
     uint8_t* img = c.keys + (id * c.khs + blockIdx.y) * kKeyImage + lane * 16;
     auto two = [](uint32_t w, float u) __attribute__((always_inline)) {  // bf16 pair times u
       return f16_pack(bits_f32(w << 16) * u, bits_f32(w & 0xffff0000u) * u);
     };
 #pragma unroll
-    for (int u = 0; u < 32 / kWaves; ++u) {  // K and Q: row block f / 4 % 4, step f % 4
-      const int f = wave * (32 / kWaves) + u;
+    for (int u = 0; u < 8; ++u) {  // K and Q: row block f / 4 % 4, step f % 4
+      const int f = wave * 8 + u;
       const int row = 16 * ((f >> 2) & 3) + m;
       const uint32_t from = (f >= 16 ? sq : sk) + row * kRowB + (32 * (f & 3) + 4 * d) * 2;
       const float x = unit[f >> 4][row];
@@ -527,8 +544,8 @@ __global__ __launch_bounds__(DELTA ? 512 : 256, 4) void linear_prep_kernel(LinAr
       st16(img + f * kFrag, u32x4{two(lo.x, x), two(lo.y, x), two(hi.x, x), two(hi.y, x)});
     }
 #pragma unroll
-    for (int u = 0; u < 16 / kWaves; ++u) {  // K^T: keys 16 (f / 2) + m, tokens of step f % 2
-      const int f = wave * (16 / kWaves) + u;
+    for (int u = 0; u < 4; ++u) {  // K^T: keys 16 (f / 2) + m, tokens of step f % 2
+      const int f = wave * 4 + u;
       u32x4 w;
 #pragma unroll
       for (int j = 0; j < 8; j += 2) {
@@ -545,14 +562,11 @@ __global__ __launch_bounds__(DELTA ? 512 : 256, 4) void linear_prep_kernel(LinAr
   // goes in times the largest row's power of two
   float size = 1.f;
   if (!a.qk_norm) {
-    float x = unit[0][lane];  // (the reciprocals of the rows' sizes)
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) x = fminf(x, __shfl_xor(x, o));
+    // (unit: the reciprocals of the rows' sizes)
+    const float x = over_lanes<64>(unit[0][lane], [](float a, float b) { return fminf(a, b); });
     size = fmaxf(1.f / x, 0x1p-30f);
   }
 
-  const int slot = wave & (kSlots - 1);
-  const bool makes_t = wave >= kSlots;  // uniform
   // rows 16 t + m of K or Q as operands, and their products with the rows of block nt:
   // lane (m, d) has those of row 16 mt + m with rows 16 nt + 4 d + r
   auto rows_of = [&](uint32_t base, int t, u32x4 (&x)[4]) __attribute__((always_inline)) {
@@ -568,28 +582,28 @@ __global__ __launch_bounds__(DELTA ? 512 : 256, 4) void linear_prep_kernel(LinAr
     return sum;
   };
   for (int32_t o0 = 0; o0 < a.group; o0 += kSlots) {
-    const int32_t o = o0 + slot, h = kh * a.group + o;
+    const int32_t o = o0 + slot;
     const bool there = o < a.group;  // uniform
-    // lane i has token i's gates
-    float g = 0.f, beta = 0.f;
-    if (there && lane < len) load_gates(a, t0 + lane, h, g, beta);
-    float grow = fmaxf(g, 0.f);
-#pragma unroll
-    for (int s = 1; s < 64; s *= 2) grow += __shfl_xor(grow, s);
+    if (o0 > 0) {
+      g = beta = 0.f;
+      if (there && lane < len) load_gates(a, t0 + lane, kh * a.group + o, g, beta);
+    }
+    const float grow = sum_lanes<64>(fmaxf(g, 0.f));
     bool walk = odd || !(grow <= 2.f) ||
                 __builtin_amdgcn_ballot_w64(!(g <= 2.f) || !(fabsf(beta) < 0x1p20f)) != 0;
     double gsum = g < (float)kLeastDecay ? kLeastDecay : (double)g;
-#pragma unroll
-    for (int s = 1; s < 64; s *= 2) {
-      const double x = __shfl_up(gsum, s);
-      if (lane >= s) gsum += x;
-    }
+    gsum += lanes_below<0x111>(gsum);
+    gsum += lanes_below<0x112>(gsum);
+    gsum += lanes_below<0x114>(gsum);
+    gsum += lanes_below<0x118>(gsum);
+    gsum += lanes_below<0x142, 0xa>(gsum);  // the row before's last, in rows 1 and 3
+    gsum += lanes_below<0x143, 0xc>(gsum);  // lane 31's, in rows 2 and 3
     if (o0 > 0) __syncthreads();  // the last heads' readers are done
     if (!makes_t) {
       run[slot][lane] = gsum;
 #pragma unroll
       for (int mt = 1; mt < 4; ++mt) {
-        const double x = __shfl(gsum, 16 * mt) - gsum;
+        const double x = lane_at(gsum, 16 * mt) - gsum;
         if (lane < 16 * mt) since[slot][8 * mt * (mt - 1) + lane] = exp_of(x);
       }
     }
@@ -616,7 +630,7 @@ __global__ __launch_bounds__(DELTA ? 512 : 256, 4) void linear_prep_kernel(LinAr
     float* fac = (float*)(img + head_image(DELTA) - kFactors);
     float largest = 0.f;  // of the operands written below
     if (!makes_t) {
-      const double all = __shfl(gsum, 63);
+      const double all = lane_at(gsum, 63);
       const float rk = inv[0][lane] / unit[0][lane], rq = inv[1][lane] / unit[1][lane];
       const float head = exp_of(gsum), strong = DELTA ? beta * size : size;
       fac[kFacX + lane] = head * rk * strong;
@@ -624,9 +638,8 @@ __global__ __launch_bounds__(DELTA ? 512 : 256, 4) void linear_prep_kernel(LinAr
       fac[kFacG + lane] = head;
       fac[kFacO + lane] = a.scale * rq;
       fac[kFacV + lane] = strong;
-      float most = fabsf(strong);
-#pragma unroll
-      for (int x = 1; x < 64; x *= 2) most = fmaxf(most, __shfl_xor(most, x));
+      const float most =
+          over_lanes<64>(fabsf(strong), [](float x, float y) { return fmaxf(x, y); });
       uint8_t* pimg = img + (DELTA ? kTParts * kLower * kFrag : 0) + lane * 16;
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
@@ -952,9 +965,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
   // if that has left its range, for a first chunk on zeros its first token's.
   float f = 1.f, inv_f = 1.f;
   auto over_wave = [&](float x) __attribute__((always_inline)) {
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) x = fmaxf(x, __shfl_xor(x, o));
-    return x;
+    return over_lanes<64>(x, [](float y, float z) { return fmaxf(y, z); });
   };
   auto lane_most = [&]() __attribute__((always_inline)) {
     float x = 0.f;
@@ -1546,8 +1557,7 @@ __global__ __launch_bounds__(kThreads) void gated_norm_kernel(NormArgs a) {
       q = fmaf(lo, lo, q);
       q = fmaf(hi, hi, q);
     }
-#pragma unroll
-  for (int o = 1; o < LANES; o *= 2) q += __shfl_xor(q, o);
+  q = sum_lanes<LANES>(q);
   const float r = 1.f / sqrtf(q / (float)a.dim + a.eps);
   if (!there) return;
   uint8_t* out = a.out + row * a.dim * 2;
@@ -1711,8 +1721,8 @@ constexpr int64_t kHeadBytes = 1024;  // the workspace's first bytes: the offset
 // at once, 1411 in two launches, 1544 in three).
 constexpr int64_t kImageBytes = 2048ll << 20;
 // Up to so many tokens per sequence are walked one by one (8 heads; token by
-// token, in chunks: 1 sequence of 8 tokens 18 us, 20; of 12 25, 20; 64 of 8 37,
-// 44; of 12 51, 44; 256 of 4 77, 121; of 8 123, 121).
+// token, in chunks: 1 sequence of 8 tokens 15 us, 20; 32 of 8 23, 29; 64 of 8
+// 37, 44; of 12 51, 44; 256 of 4 77, 121; of 8 123, 121).
 constexpr int32_t kScanTokens = 8;
 
 struct Prefill {
