@@ -8,7 +8,9 @@ Drop-in modules with the reference's class names and signatures:
 * ``muserve_amd.memory.kv_cache`` -> ``KVCache`` (muserve/memory/kv_cache.py)
 * ``muserve_amd.model.prefix_cache`` -> ``PrefixCache``
                                      (muserve/model/prefix_cache.py)
-* ``muserve_amd.state_pool``      -> ``StatePool`` for GDN recurrent/conv states
+* ``muserve_amd.state_pool``      -> ``StatePool`` for GDN recurrent/conv states, with
+                                     the layer's conv and linear attention in place
+                                     (``muserve_amd.kernels.linear_attention``)
 * ``muserve_amd.block_manager``   -> ``BlockManager`` (refcounts, copy-on-write,
                                      prefix-hash table, LRU eviction)
 * ``muserve_amd.scheduler``       -> ``ContinuousBatchScheduler``,

