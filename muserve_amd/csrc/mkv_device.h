@@ -111,22 +111,27 @@ __device__ __forceinline__ int32_t first_tile(int32_t row, int32_t b, int32_t r 
   return row / r + b;
 }
 inline int64_t tile_ids(int64_t rows, int32_t n, int32_t r = 64) { return rows / r + n; }
-// The sequence that a tile id would belong to, or -1 if the offsets do not hold
-// together. Every thread of the workgroup calls, once a kernel: all offsets are
-// read side by side (a binary search waits for log2 n loads, one after another).
+// The sequence that a tile id would belong to and its rows [q0, q1), or -1 if the
+// offsets do not hold together. Every thread of the workgroup calls, once a
+// kernel: all offsets are read side by side (a binary search waits for log2 n
+// loads, one after another).
 __device__ __forceinline__ int32_t tile_sequence(const int32_t* cu, int32_t n, int64_t rows,
-                                                 int64_t id, int32_t r = 64) {
+                                                 int64_t id, int32_t r, int64_t& q0, int64_t& q1) {
   if (n < 64) {
     const int32_t i = threadIdx.x & 63;
     bool bad = false, before = false;
+    int32_t x = 0;
     if (i <= n) {
-      const int32_t x = cu[i];
+      x = cu[i];
       bad = x < 0 || x > rows || (i > 0 && cu[i - 1] > x);
       before = i < n && first_tile(x, i, r) <= id;
     }
     if (__builtin_amdgcn_ballot_w64(bad) != 0) return -1;
     const int32_t of = __builtin_popcountll(__builtin_amdgcn_ballot_w64(before));
-    return of > 0 ? of - 1 : 0;  // (ids before the first sequence's first tile belong to none)
+    const int32_t b = of > 0 ? of - 1 : 0;  // (ids before the first tile belong to none)
+    q0 = __builtin_amdgcn_readlane(x, b);
+    q1 = __builtin_amdgcn_readlane(x, b + 1);
+    return b;
   }
   constexpr int32_t kBad = 0x7fffffff;
   __shared__ int32_t last[16];
@@ -142,7 +147,11 @@ __device__ __forceinline__ int32_t tile_sequence(const int32_t* cu, int32_t n, i
   if ((threadIdx.x & 63) == 0) last[threadIdx.x >> 6] = at;
   __syncthreads();
   for (uint32_t i = 0; i < blockDim.x / 64; ++i) at = at > last[i] ? at : last[i];
-  return __builtin_amdgcn_readfirstlane(at == kBad ? -1 : at);
+  at = __builtin_amdgcn_readfirstlane(at);
+  if (at == kBad) return -1;
+  q0 = ld_const(cu + at);
+  q1 = ld_const(cu + at + 1);
+  return at;
 }
 
 // x / (1 + e^-x) by the hardware's 2^x and reciprocal, both within an fp32 step

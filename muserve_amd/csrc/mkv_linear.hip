@@ -474,9 +474,9 @@ __global__ __launch_bounds__(DELTA ? 512 : 256, 4) void linear_prep_kernel(LinAr
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t id = blockIdx.x;
   const int32_t kh = c.kh0 + blockIdx.y;
-  const int32_t b = tile_sequence(a.cu, a.n, a.tokens, id);
+  int64_t s0 = 0, s1 = 0;
+  const int32_t b = tile_sequence(a.cu, a.n, a.tokens, id, kChunk, s0, s1);
   if (b < 0) return;  // uniform; bad offsets
-  const int64_t s0 = a.cu[b], s1 = a.cu[b + 1];
   const int64_t t0 = s0 + (id - first_tile((int32_t)s0, b)) * kChunk;
   if (t0 < s0 || t0 >= s1) return;  // uniform; no such tile
   const int32_t len = (int32_t)(s1 - t0 < kChunk ? s1 - t0 : kChunk);
@@ -852,17 +852,20 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
   const int d0 = at_dim - (ident ? kDim : 0);  // the wave's value dims
   const bool first = o == 0 && part == 0 && c.kh0 == 0 && tid == 0;
   int32_t b = y;
-  if (MODE != kWhole)
-    b = tile_sequence(a.cu, a.n, a.tokens, y, c.seg);
-  else if (!offsets_ok(a.cu, a.n, a.tokens))
-    b = -1;
+  int64_t q0 = 0, q1 = 0;  // the sequence's rows
+  if (MODE != kWhole) {
+    b = tile_sequence(a.cu, a.n, a.tokens, y, c.seg, q0, q1);
+  } else {
+    q0 = ld_const(a.cu + b);
+    q1 = ld_const(a.cu + b + 1);
+    if (!offsets_ok(a.cu, a.n, a.tokens)) b = -1;
+  }
   if (MODE != kEnds && first && y == 0) *ok_word = b >= 0;
   if (b < 0) {
     if (MODE != kEnds && first && y == 0) raise_err(a.err, MKV_DEVERR_TABLE);
     return;
   }
-  const int64_t q0 = ld_const(a.cu + b), q1 = ld_const(a.cu + b + 1);  // the sequence's rows
-  int64_t s0 = q0, s1 = q1;                                            // this workgroup's
+  int64_t s0 = q0, s1 = q1;  // this workgroup's
   int64_t seg = 0;
   if (MODE != kWhole) {
     seg = y - first_tile((int32_t)q0, b, c.seg);
@@ -871,16 +874,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
   }
   if (s0 >= q1) return;  // uniform: no rows, or no such segment
   const bool last = s1 == q1;
-  const int32_t slot = ld_const(a.slots + b);
+  if (MODE == kEnds && last) return;  // uniform: not asked for
+  const int32_t slot = ld_const(a.slots + b);  // (its load runs with the images')
   const int64_t out_row = (int64_t)a.hv * (kDim * 2);
   uint8_t* outp = a.out + h * (kDim * 2) + (d0 + n) * 2;
-  if (slot < 0 || slot >= a.pool_slots) {  // uniform
-    if (!kOut) return;
-    if (first && s0 == q0) raise_err(a.err, MKV_DEVERR_STATE_SLOT);
-    for (int64_t t = s0 + d; t < s1; t += 4) *(uint16_t*)(outp + t * out_row) = 0;
-    return;
-  }
-  if (MODE == kEnds && last) return;  // uniform: not asked for
   const int32_t chunks = (int32_t)((s1 - s0 + kChunk - 1) / kChunk);
   const int64_t id0 = (q0 >> 6) + b + ((s0 - q0) >> 6);
   const uint8_t* kimg = c.keys + (id0 * c.khs + (kh - c.kh0)) * kKeyImage;
@@ -950,6 +947,13 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) load_images(0, l0, i);
   load_v(0);
+  if (slot < 0 || slot >= a.pool_slots) {  // uniform
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (loads into LDS do not outlive it)
+    if (!kOut) return;
+    if (first && s0 == q0) raise_err(a.err, MKV_DEVERR_STATE_SLOT);
+    for (int64_t t = s0 + d; t < s1; t += 4) *(uint16_t*)(outp + t * out_row) = 0;
+    return;
+  }
   f32x4 s[8];
   if (MODE == kEnds && (ident || seg > 0)) {
 #pragma unroll

@@ -309,13 +309,13 @@ constexpr int kConvRows = 16;
 template <int W>
 __global__ __launch_bounds__(kThreads) void conv_prefill_kernel(ConvPrefillArgs p) {
   const ConvArgs& a = p.c;
-  const int32_t b = tile_sequence(p.cu, a.batch, p.tokens, blockIdx.x);
+  int64_t seq0 = 0, end = 0;
+  const int32_t b = tile_sequence(p.cu, a.batch, p.tokens, blockIdx.x, 64, seq0, end);
   if (b < 0) {  // uniform
     if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0) raise_err(a.err, MKV_DEVERR_TABLE);
     return;
   }
-  const int64_t end = p.cu[b + 1], seq0 = p.cu[b];
-  const int64_t tile = (int64_t)blockIdx.x - first_tile(p.cu[b], b);
+  const int64_t tile = (int64_t)blockIdx.x - first_tile((int32_t)seq0, b);
   const int64_t t0 = seq0 + tile * 64 + (threadIdx.x >> 6) * kConvRows;
   const int64_t g = (int64_t)blockIdx.y * 64 + (threadIdx.x & 63);  // group of 8 channels
   if (t0 >= end || g * 8 >= a.channels) return;
@@ -323,11 +323,6 @@ __global__ __launch_bounds__(kThreads) void conv_prefill_kernel(ConvPrefillArgs 
   const int64_t row = (int64_t)a.channels * 2;
   const int32_t rows = (int32_t)(end - t0 < kConvRows ? end - t0 : kConvRows);
   uint8_t* outp = a.out + t0 * row + g * 16;
-  if (slot < 0 || slot >= a.pool_slots) {
-    if (g == 0 && t0 == seq0) raise_err(a.err, MKV_DEVERR_STATE_SLOT);
-    for (int32_t i = 0; i < rows; ++i) st16(outp + i * row, u32x4{0u, 0u, 0u, 0u});
-    return;
-  }
   const uint8_t* xp = a.x + t0 * p.x_stride + g * 16;
   u32x4 xv[3 + kConvRows], wv[kConvK], sv[W];
 #pragma unroll
@@ -337,6 +332,11 @@ __global__ __launch_bounds__(kThreads) void conv_prefill_kernel(ConvPrefillArgs 
   }
 #pragma unroll
   for (int j = 0; j < kConvK; ++j) wv[j] = ld16(a.w + (g * 8 * kConvK) * 2 + 16 * j);
+  if (slot < 0 || slot >= a.pool_slots) {  // (its load runs with the rows')
+    if (g == 0 && t0 == seq0) raise_err(a.err, MKV_DEVERR_STATE_SLOT);
+    for (int32_t i = 0; i < rows; ++i) st16(outp + i * row, u32x4{0u, 0u, 0u, 0u});
+    return;
+  }
   if (t0 == seq0) {
     uint8_t* st = a.pool + ((int64_t)slot * a.channels + g * 8) * (W * 2);
 #pragma unroll
