@@ -1410,7 +1410,8 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinArgs a, ChunkArgs c
   __shared__ __attribute__((aligned(16))) float state[2][kDim / 4][64];  // 4-key groups x (dim, key)
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, d = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int32_t part = blockIdx.x % (kDim / 16), o = blockIdx.x / (kDim / 16);
+  // (a head's workgroups on one XCD where heads are a multiple of 8: M once in its L2)
+  const int32_t heads = c.khs * a.group, o = blockIdx.x % heads, part = blockIdx.x / heads;
   const int32_t h = c.kh0 * a.group + o, b = blockIdx.y;
   if (!offsets_ok(a.cu, a.n, a.tokens)) return;
   const int64_t q0 = ld_const(a.cu + b), q1 = ld_const(a.cu + b + 1);
