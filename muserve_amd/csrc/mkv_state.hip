@@ -568,6 +568,8 @@ extern "C" int mkv_gdn_conv_prefill(void* conv_pool, int64_t pool_slots, int32_t
   if (rc != MKV_OK) return rc == kEmpty ? MKV_OK : rc;
   MKV_REQUIRE(batch <= kMaxSequences, MKV_E_UNSUPPORTED, "%s: more than %d sequences", fn,
               kMaxSequences);
+  // (a grid dimension has less than 2^32 threads)
+  MKV_REQUIRE(num_tokens <= (1ll << 29), MKV_E_UNSUPPORTED, "%s: too many rows", fn);
   MKV_REQUIRE(cu_seqlens && aligned4(cu_seqlens), MKV_E_INVALID, "%s: null pointer", fn);
   MKV_REQUIRE(x_stride >= (int64_t)channels * 2, MKV_E_INVALID,
               "%s: a stride is shorter than its row", fn);

@@ -307,3 +307,73 @@ def test_norm_of_many_rows(rows, dim):
     some = torch.cat([torch.arange(0, rows, 97), torch.arange(rows - 70, rows)])
     want = ref.gated_norm(x[some].cpu(), z[some].cpu(), w.cpu(), 1e-6)
     lu.close(got[some], want, (64 + dim ** 0.5) * lu.U32 * want.abs(), "rows")
+
+
+def test_slots_past_32_bits():
+    """State and conv pools of more than 4 GiB, used at their far ends."""
+    case("linear attention and conv on slots behind 4 GiB")
+    hk, hv, pool, C = 1, 2, 36000, 16
+    x = lu.inputs(50, 75, hk, hv, slots=2)
+    state = torch.empty(pool, hv, D, D, device=DEV)
+    assert state.numel() * 4 > 1 << 32
+    slots = [pool - 1, 33000]
+    gx = lu.on_gpu(x)
+    near = gx["state"].clone()
+    for longest, cu in ((70, [0, 70, 75]), (5, [0, 3, 8])):
+        state[slots] = near
+        got = prompt(gx, ints(slots), ints(cu), state, max_seqlen=longest)
+        want_state = near.clone()
+        want = prompt(gx, ints([0, 1]), ints(cu), want_state, max_seqlen=longest)
+        assert torch.equal(got[:cu[-1]], want[:cu[-1]]) and torch.equal(state[slots], want_state)
+    rows = {n: t[:2] if n in ("mixed", "g", "beta") else t for n, t in gx.items()}
+    got, want = step(rows, ints(slots), state), step(rows, ints([0, 1]), want_state)
+    assert torch.equal(got, want) and torch.equal(state[slots], want_state)
+    del state
+    conv = torch.empty((1 << 25) + 64, C, 4, dtype=torch.bfloat16, device=DEV)
+    assert conv.numel() * 2 > 1 << 32
+    far = [conv.shape[0] - 1, conv.shape[0] - 9]
+    near = torch.randn(2, C, 4, device=DEV).bfloat16()
+    conv[far] = near
+    y, w = torch.randn(70, C, device=DEV).bfloat16(), torch.randn(C, 4, device=DEV).bfloat16()
+    got = la.causal_conv_prefill(y, w, conv, ints(far), ints([0, 68, 70]))
+    want = la.causal_conv_prefill(y, w, near, ints([0, 1]), ints([0, 68, 70]))
+    la.check_errors(DEV)
+    assert torch.equal(got, want) and torch.equal(conv[far], near)
+
+
+def test_rows_past_32_bits():
+    """Rows of v, z and out behind 4 GiB: a short prompt behind a long one gives
+    what it gives alone (its walk may be cut otherwise: two roundings to bf16 of
+    2^-8 each way, states by what fp32 sums do)."""
+    case("linear attention on 300000 tokens of 64 heads")
+    T, hk, hv, last = 300000, 1, 64, 90
+    gen = torch.Generator(device=DEV).manual_seed(51)
+
+    def normal(*size):
+        return torch.randn(*size, generator=gen, device=DEV, dtype=torch.bfloat16)
+
+    q, k, v = normal(T, hk, D), normal(T, hk, D), normal(T, hv, D)
+    assert v.numel() * 2 > 1 << 32
+    g, beta = -0.1 * normal(T, hv).abs(), torch.sigmoid(normal(T, hv))
+    state = torch.zeros(2, hv, D, D, device=DEV)
+    w = 1 + 0.1 * normal(D)
+    out = la.linear_attn_prefill(q, k, v, g, beta, state, ints([0, 1]), ints([0, T - last, T]),
+                                 max_seqlen=T - last, qk_norm=True, z=v, norm_weight=w)
+    alone = torch.zeros(1, hv, D, D, device=DEV)
+    tail = [t[T - last:] for t in (q, k, v, g, beta)]
+    want = la.linear_attn_prefill(*tail, alone, ints([0]), ints([0, last]), max_seqlen=last,
+                                  qk_norm=True, z=tail[2], norm_weight=w)
+    la.check_errors(DEV)
+    assert torch.isfinite(out.float()).all()
+    for a, b, tol in ((out[T - last:], want, 2.0 ** -6), (state[1], alone[0], 1e-5)):
+        assert (a.double() - b.double()).norm() <= tol * b.double().norm()
+    normed = la.gated_rms_norm(v, v, w)
+    some = slice(T - 5, T)
+    assert torch.equal(normed[some], la.gated_rms_norm(v[some], v[some], w))
+    mixed = v.view(T, hv * D)
+    cw, conv = normal(hv * D, 4), torch.zeros(2, hv * D, 4, dtype=torch.bfloat16, device=DEV)
+    y = la.causal_conv_prefill(mixed, cw, conv, ints([0, 1]), ints([0, T - last, T]))
+    conv1 = torch.zeros(1, hv * D, 4, dtype=torch.bfloat16, device=DEV)
+    y1 = la.causal_conv_prefill(mixed[T - last:], cw, conv1, ints([0]), ints([0, last]))
+    la.check_errors(DEV)
+    assert torch.equal(y[T - last:], y1) and torch.equal(conv[1], conv1[0])
