@@ -332,7 +332,7 @@ int mkv_gdn_decode_gather(const void* state_pool, int64_t state_bytes, void* sta
  * where the sequence is shorter). A sequence without rows leaves its slot.
  * Rows of out [num_tokens, channels] outside the sequences are left as they
  * were. Requirements as mkv_gdn_conv_decode's, x_stride a multiple of 16, at
- * most 4096 sequences and 2^29 rows (MKV_E_UNSUPPORTED); out does not overlap x.
+ * most 4096 sequences and 2^27 rows (MKV_E_UNSUPPORTED); out does not overlap x.
  * Offsets below 0, falling or above num_tokens set MKV_DEVERR_TABLE, and the
  * call writes nothing; a slot outside [0, pool_slots) gives zeros and sets
  * MKV_DEVERR_STATE_SLOT.

@@ -290,13 +290,14 @@ __device__ __forceinline__ void conv_row(const ConvArgs& a, uint32_t bx, int64_t
 // branch): row t of sequence b takes its taps from the rows before it, and
 // from the slot's last inputs where those lie before the sequence; the slot is
 // left with the sequence's last W inputs. Bound by HBM: every row is read and
-// written once, 16 bytes per thread and row. A workgroup takes a tile of 64
-// rows (tile ids of mkv_device.h, grid.x) and 512 channels (grid.y); a thread
-// slides over 16 rows, all loaded before the first is used, the 3 rows before
-// them again. Only the thread that reads a slot's old inputs (the first rows
-// of a sequence) writes its new ones, so no other can see them early. 8 x 4096
-// rows of 1536 channels take 36 us, 5.6 TB/s; a sequence of 77 rows 7.1, its
-// offsets, rows and stores one after the other.
+// written once, 16 bytes per thread and row. A workgroup takes a tile of 16 rows
+// (tile ids of mkv_device.h, grid.x) and 512 channels (grid.y); a thread slides
+// over 4 rows, all loaded before the first is used, the 3 rows before them
+// again (they are in the L1 or L2). Only the thread that reads a slot's old
+// inputs (the first rows of a sequence) writes its new ones, so no other can see
+// them early. 8 x 4096 rows of 1536 channels take 36 us, 5.6 TB/s, and 77 rows
+// 4.2; 8 rows a thread 36 and 5.2, 16 rows 37 and 6.9 (a wave alone on its SIMD
+// computes them one after the other).
 // ---------------------------------------------------------------------------
 struct ConvPrefillArgs {
   ConvArgs c;            // x: [tokens, channels], stride x_stride; batch: sequences
@@ -304,19 +305,19 @@ struct ConvPrefillArgs {
   int64_t tokens;
   const int32_t* cu;     // [batch + 1]
 };
-constexpr int kConvRows = 16;
+constexpr int kConvRows = 4, kConvTile = 4 * kConvRows;
 
 template <int W>
 __global__ __launch_bounds__(kThreads) void conv_prefill_kernel(ConvPrefillArgs p) {
   const ConvArgs& a = p.c;
   int64_t seq0 = 0, end = 0;
-  const int32_t b = tile_sequence(p.cu, a.batch, p.tokens, blockIdx.x, 64, seq0, end);
+  const int32_t b = tile_sequence(p.cu, a.batch, p.tokens, blockIdx.x, kConvTile, seq0, end);
   if (b < 0) {  // uniform
     if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0) raise_err(a.err, MKV_DEVERR_TABLE);
     return;
   }
-  const int64_t tile = (int64_t)blockIdx.x - first_tile((int32_t)seq0, b);
-  const int64_t t0 = seq0 + tile * 64 + (threadIdx.x >> 6) * kConvRows;
+  const int64_t tile = (int64_t)blockIdx.x - first_tile((int32_t)seq0, b, kConvTile);
+  const int64_t t0 = seq0 + tile * kConvTile + (threadIdx.x >> 6) * kConvRows;
   const int64_t g = (int64_t)blockIdx.y * 64 + (threadIdx.x & 63);  // group of 8 channels
   if (t0 >= end || g * 8 >= a.channels) return;
   const int32_t slot = a.slots[b];
@@ -569,7 +570,7 @@ extern "C" int mkv_gdn_conv_prefill(void* conv_pool, int64_t pool_slots, int32_t
   MKV_REQUIRE(batch <= kMaxSequences, MKV_E_UNSUPPORTED, "%s: more than %d sequences", fn,
               kMaxSequences);
   // (a grid dimension has less than 2^32 threads)
-  MKV_REQUIRE(num_tokens <= (1ll << 29), MKV_E_UNSUPPORTED, "%s: too many rows", fn);
+  MKV_REQUIRE(num_tokens <= (1ll << 27), MKV_E_UNSUPPORTED, "%s: too many rows", fn);
   MKV_REQUIRE(cu_seqlens && aligned4(cu_seqlens), MKV_E_INVALID, "%s: null pointer", fn);
   MKV_REQUIRE(x_stride >= (int64_t)channels * 2, MKV_E_INVALID,
               "%s: a stride is shorter than its row", fn);
@@ -579,7 +580,7 @@ extern "C" int mkv_gdn_conv_prefill(void* conv_pool, int64_t pool_slots, int32_t
   p.x_stride = x_stride;
   p.tokens = num_tokens;
   p.cu = cu_seqlens;
-  const dim3 grid((unsigned)tile_ids(num_tokens, batch), (unsigned)groups);
+  const dim3 grid((unsigned)tile_ids(num_tokens, batch, kConvTile), (unsigned)groups);
   if (width == 3)
     hipLaunchKernelGGL(conv_prefill_kernel<3>, grid, dim3(kThreads), 0, as_stream(stream), p);
   else

@@ -142,7 +142,7 @@ def test_more_sequences_and_rows_than_a_call_takes():
     rc, msg = _rc("mkv_gdn_conv_prefill", FAKE, 4, 64, 4, FAKE, FAKE, 4097, 9, FAKE, 128, FAKE, 4,
                   FAKE, FAKE, None)
     assert rc == -3 and "more than 4096 sequences" in msg
-    rc, msg = _rc("mkv_gdn_conv_prefill", FAKE, 4, 64, 4, FAKE, FAKE, 2, (1 << 29) + 1, FAKE, 128,
+    rc, msg = _rc("mkv_gdn_conv_prefill", FAKE, 4, 64, 4, FAKE, FAKE, 2, (1 << 27) + 1, FAKE, 128,
                   FAKE, 4, FAKE, FAKE, None)
     assert rc == -3 and "too many rows" in msg
     rc, msg = _rc("mkv_gated_rms_norm", FAKE, 256, FAKE, 256, (1 << 29) + 1, 2, 64, FAKE, 0, 1e-6,
