@@ -83,6 +83,11 @@ def _apart(out: torch.Tensor, others, spans, names=("q", "k", "v", "g", "beta", 
                              "to be read")
 
 
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of t's shape (torch.empty takes twice as long)."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _planned(key: tuple, check, *args) -> tuple:
     plan = _plans.get(key)
     if plan is None:
@@ -241,7 +246,7 @@ def linear_attn_decode(
     dev, B, hk, hv, pool = plan[:5]
     slots = _ids("slots", slots, dev)
     if out is None:
-        out = torch.empty((B, hv, HEAD_DIM), dtype=torch.bfloat16, device=dev)
+        out = _like(v)
     else:
         _apart(out, (q, k, v, g, beta, z), plan[5])
     if slots.numel() != B:
@@ -298,7 +303,7 @@ def linear_attn_prefill(
     dev, tokens, hk, hv, pool = plan[:5]
     slots = _ids("slots", slots, dev)
     if out is None:
-        out = torch.empty((tokens, hv, HEAD_DIM), dtype=torch.bfloat16, device=dev)
+        out = _like(v)
     else:
         _apart(out, (q, k, v, g, beta, z), plan[5])
     cu = _ids("cu_seqlens", cu_seqlens, dev)
@@ -360,7 +365,7 @@ def causal_conv_prefill(
     dev, T, C, W, K, xs, spans = _planned(key, _check_conv, x, weight, conv_state, out)
     w = weight if weight.is_contiguous() else weight.contiguous()
     if out is None:
-        out = torch.empty((T, C), dtype=x.dtype, device=dev)
+        out = _like(x)
     else:
         _apart(out, (x,), spans, ("x",))
     slots, cu = _ids("slots", slots, dev), _ids("cu_seqlens", cu_seqlens, dev)
@@ -408,7 +413,7 @@ def gated_rms_norm(
     key = (_sig(x), _sig(z), _sig(weight), _sig(out))
     dev, T, H, D, xs, zs, wb, spans, whole = _planned(key, _check_norm, x, z, weight, out)
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        out = _like(x)
     else:
         at = out.data_ptr()
         _apart(out, (x, z), [0 if w and t.data_ptr() == at else n
