@@ -318,7 +318,8 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 typedef __attribute__((address_space(3))) u32x2 lds_u32x2;
 typedef __attribute__((address_space(3))) float lds_f32;
-typedef __attribute__((address_space(3))) uint16_t lds_u16;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 constexpr int kChunk = 64;
 // Operand images: blocks of 1 KiB, 16 bytes per lane, one v_mfma_f32_16x16x32
@@ -469,7 +470,8 @@ __global__ __launch_bounds__(DELTA ? 512 : 256, 4) void linear_prep_kernel(LinAr
   // e^(G_16 mt - G_j) for j < 16 mt: 16, 32 and 48 of them
   __shared__ __attribute__((aligned(16))) float since[kSlots][96];
   __shared__ float inv[2][kChunk];   // 1 / norms of k, q
-  __shared__ float unit[2][kChunk];  // the powers of two that bring rows of k, q near 1
+  // the powers of two that bring rows of k, q near 1
+  __shared__ __attribute__((aligned(16))) float unit[2][kChunk];
   const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, d = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t id = blockIdx.x;
@@ -549,12 +551,15 @@ __global__ __launch_bounds__(DELTA ? 512 : 256, 4) void linear_prep_kernel(LinAr
       const int f = wave * 4 + u;
       u32x4 w;
 #pragma unroll
-      for (int j = 0; j < 8; j += 2) {
-        const int t = 32 * (f & 1) + 16 * (j >> 2) + 4 * d + (j & 3);
-        const uint32_t at = sk + t * kRowB + (16 * (f >> 1) + m) * 2;
-        w[j >> 1] = f16_pack(
-            bits_f32((uint32_t) * (lds_u16*)(uintptr_t)at << 16) * unit[0][t],
-            bits_f32((uint32_t) * (lds_u16*)(uintptr_t)(at + kRowB) << 16) * unit[0][t + 1]);
+      for (int y = 0; y < 2; ++y) {
+        // 16 lanes name 4 tokens' rows of 16 keys, a lane gets one key of the 4 (transposing)
+        const int t = 32 * (f & 1) + 16 * y + 4 * d;
+        const uint32_t at = sk + (t + (m >> 2)) * kRowB + (16 * (f >> 1) + 4 * (m & 3)) * 2;
+        const u32x2 k4 = __builtin_bit_cast(
+            u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)at));
+        const f32x4 by = *(const f32x4*)&unit[0][t];
+        w[2 * y] = f16_pack(bits_f32(k4.x << 16) * by[0], bits_f32(k4.x & 0xffff0000u) * by[1]);
+        w[2 * y + 1] = f16_pack(bits_f32(k4.y << 16) * by[2], bits_f32(k4.y & 0xffff0000u) * by[3]);
       }
       st16(img + (32 + f) * kFrag, w);
     }
