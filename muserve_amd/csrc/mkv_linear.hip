@@ -455,8 +455,9 @@ __device__ __forceinline__ bool huge(u32x4 w) {  // any of 8 bf16
 // 16 x 16 blocks in LDS (row-major, 16-byte chunks XORed by row / 4) and inverts
 // by blocks: the diagonal ones by forward substitution, a lane per column, the
 // rest in fp32 matrix instructions (16x16x4). Bound by the latency of these
-// chains: 512 chunks of 8 heads take 44 us, a lone one 13; with one wave for
-// both parts of a head (2 waves per SIMD, not 4) 48 and 17.
+// chains: 512 chunks of 8 heads take 43 us, a lone one 13 (of which 6 until the
+// rows are staged, 6.5 A and T); with one wave for both parts of a head (2 waves
+// per SIMD, not 4) 48 and 17. K's rows all in registers would spill (70 us).
 constexpr int kRowB = 272;  // bytes of a staged row: 256 and a pad against bank conflicts
 constexpr int kBlocks = 10;
 constexpr int kSlots = 4;   // heads at a time
@@ -579,9 +580,7 @@ __global__ __launch_bounds__(DELTA ? 512 : 256, 4) void linear_prep_kernel(LinAr
 #pragma unroll
     for (int s = 0; s < 4; ++s) x[s] = lds_ld16(base + (16 * t + m) * kRowB + (32 * s + 8 * d) * 2);
   };
-  auto products = [&](int nt, const u32x4 (&x)[4]) __attribute__((always_inline)) {
-    u32x4 kn[4];
-    rows_of(sk, nt, kn);
+  auto products = [&](const u32x4 (&kn)[4], const u32x4 (&x)[4]) __attribute__((always_inline)) {
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int s = 0; s < 4; ++s) sum = mfma(kn[s], x[s], sum);
@@ -656,7 +655,9 @@ __global__ __launch_bounds__(DELTA ? 512 : 256, 4) void linear_prep_kernel(LinAr
         float p[8];
 #pragma unroll
         for (int nt = 0; nt <= mt; ++nt) {
-          const f32x4 qk = products(nt, qm), e = decays(mt, nt, gi, from);
+          u32x4 kn[4];
+          rows_of(sk, nt, kn);
+          const f32x4 qk = products(kn, qm), e = decays(mt, nt, gi, from);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             p[4 * (nt & 1) + r] = nt < mt || 4 * d + r <= m ? qi * e[r] * qk[r] : 0.f;
@@ -692,7 +693,9 @@ __global__ __launch_bounds__(DELTA ? 512 : 256, 4) void linear_prep_kernel(LinAr
         const float ki = inv[0][16 * mt + m] * __shfl(beta, 16 * mt + m);
 #pragma unroll
         for (int nt = 0; nt <= mt; ++nt) {
-          f32x4 av = products(nt, km);
+          u32x4 kn[4];
+          if (nt < mt) rows_of(sk, nt, kn);
+          f32x4 av = nt < mt ? products(kn, km) : products(km, km);
           const f32x4 e = decays(mt, nt, gi, from);
 #pragma unroll
           for (int r = 0; r < 4; ++r) av[r] = nt < mt || 4 * d + r < m ? ki * e[r] * av[r] : 0.f;
@@ -746,7 +749,6 @@ __global__ __launch_bounds__(DELTA ? 512 : 256, 4) void linear_prep_kernel(LinAr
           for (int s = 0; s < 4; ++s)
             res = __builtin_amdgcn_mfma_f32_16x16x4f32(-left[s], acc[s], res, 0, 0, 0);
           tb[mt * (mt + 1) / 2 + nt] = res;
-          __builtin_amdgcn_sched_barrier(0);
         }
       }
       wave_sync();
