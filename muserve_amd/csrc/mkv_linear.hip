@@ -1799,7 +1799,7 @@ void choose_walk(Prefill& p, int64_t tokens, int32_t n, int32_t longest, double 
       p.seg = 0;
     }
   }
-  for (int32_t len = 4; len < long_chunks; len += len < 16 ? 1 : len < 64 ? 2 : 8) {
+  for (int32_t len = 4; len < long_chunks; len += len < 16 ? 1 : len < 64 ? 2 : len / 8) {
     const int64_t ids = tile_ids(tokens, n, len * kChunk);
     if (ids > 65535) continue;  // (grid.y)
     const double of_long = ceil(long_chunks / len);
