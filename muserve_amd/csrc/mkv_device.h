@@ -85,7 +85,8 @@ __device__ __forceinline__ float sum_lanes(float x) {
 // more, never falling, at most `rows`. Every thread of the workgroup calls.
 __device__ __forceinline__ bool offsets_ok(const int32_t* cu, int32_t n, int64_t rows) {
   bool bad = false;
-  if (n < 64) {  // each wave by itself, without a barrier
+  if (n < 64) {  // each wave by itself, without a barrier (a short prompt's two kernels
+                 // take 20.0 us so, 20.9 by the reduction below)
     const int32_t i = threadIdx.x & 63;
     if (i <= n) {
       const int32_t x = cu[i];
