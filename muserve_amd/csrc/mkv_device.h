@@ -107,17 +107,21 @@ constexpr int32_t kMaxSequences = 4096;
 // Tiles of R rows of packed sequences without a list of them: tile c of
 // sequence b has the id cu[b] / R + b + c. Ids never meet (a sequence of m rows
 // from cu[b] has at most (cu[b] + m) / R - cu[b] / R + 1 tiles), and rows / R + n
-// ids cover all of them; ids in between belong to no tile.
+// ids cover all of them; ids before the first tile and between them belong to
+// none.
 __device__ __forceinline__ int32_t first_tile(int32_t row, int32_t b, int32_t r = 64) {
   return row / r + b;
 }
 inline int64_t tile_ids(int64_t rows, int32_t n, int32_t r = 64) { return rows / r + n; }
-// The sequence that a tile id would belong to and its rows [q0, q1), or -1 if the
-// offsets do not hold together. Every thread of the workgroup calls, once a
-// kernel: all offsets are read side by side (a binary search waits for log2 n
-// loads, one after another).
+// The sequence that a tile id belongs to, its rows [q0, q1) and the tile's first
+// row t0; kNoTile where it belongs to none, kBadOffsets if the offsets do not hold
+// together. Every thread of the workgroup calls, once a kernel: all offsets are
+// read side by side (a binary search waits for log2 n loads, one after another).
+constexpr int32_t kBadOffsets = -1, kNoTile = -2;
 __device__ __forceinline__ int32_t tile_sequence(const int32_t* cu, int32_t n, int64_t rows,
-                                                 int64_t id, int32_t r, int64_t& q0, int64_t& q1) {
+                                                 int64_t id, int32_t r, int64_t& q0, int64_t& q1,
+                                                 int64_t& t0) {
+  int32_t b;  // the last sequence whose first tile is not behind id, or the first one
   if (n < 64) {
     const int32_t i = threadIdx.x & 63;
     bool bad = false, before = false;
@@ -127,32 +131,34 @@ __device__ __forceinline__ int32_t tile_sequence(const int32_t* cu, int32_t n, i
       bad = x < 0 || x > rows || (i > 0 && cu[i - 1] > x);
       before = i < n && first_tile(x, i, r) <= id;
     }
-    if (__builtin_amdgcn_ballot_w64(bad) != 0) return -1;
+    if (__builtin_amdgcn_ballot_w64(bad) != 0) return kBadOffsets;
     const int32_t of = __builtin_popcountll(__builtin_amdgcn_ballot_w64(before));
-    const int32_t b = of > 0 ? of - 1 : 0;  // (ids before the first tile belong to none)
+    b = of > 0 ? of - 1 : 0;
     q0 = __builtin_amdgcn_readlane(x, b);
     q1 = __builtin_amdgcn_readlane(x, b + 1);
-    return b;
+  } else {
+    constexpr int32_t kBad = 0x7fffffff;
+    __shared__ int32_t last[16];
+    int32_t at = 0;
+    for (int32_t i = threadIdx.x; i <= n; i += blockDim.x) {
+      const int32_t x = cu[i];
+      if (x < 0 || x > rows || (i > 0 && cu[i - 1] > x))
+        at = kBad;
+      else if (i < n && first_tile(x, i, r) <= id)
+        at = at > i ? at : i;
+    }
+    at = over_lanes<64>(at, [](int32_t a, int32_t b) { return a > b ? a : b; });
+    if ((threadIdx.x & 63) == 0) last[threadIdx.x >> 6] = at;
+    __syncthreads();
+    for (uint32_t i = 0; i < blockDim.x / 64; ++i) at = at > last[i] ? at : last[i];
+    b = __builtin_amdgcn_readfirstlane(at);
+    if (b == kBad) return kBadOffsets;
+    q0 = ld_const(cu + b);
+    q1 = ld_const(cu + b + 1);
   }
-  constexpr int32_t kBad = 0x7fffffff;
-  __shared__ int32_t last[16];
-  int32_t at = 0;  // the last sequence whose first tile is not behind id
-  for (int32_t i = threadIdx.x; i <= n; i += blockDim.x) {
-    const int32_t x = cu[i];
-    if (x < 0 || x > rows || (i > 0 && cu[i - 1] > x))
-      at = kBad;
-    else if (i < n && first_tile(x, i, r) <= id)
-      at = at > i ? at : i;
-  }
-  at = over_lanes<64>(at, [](int32_t a, int32_t b) { return a > b ? a : b; });
-  if ((threadIdx.x & 63) == 0) last[threadIdx.x >> 6] = at;
-  __syncthreads();
-  for (uint32_t i = 0; i < blockDim.x / 64; ++i) at = at > last[i] ? at : last[i];
-  at = __builtin_amdgcn_readfirstlane(at);
-  if (at == kBad) return -1;
-  q0 = ld_const(cu + at);
-  q1 = ld_const(cu + at + 1);
-  return at;
+  // (ids before the first tile come out before q0, ids between tiles behind q1)
+  t0 = q0 + (id - first_tile((int32_t)q0, b, r)) * r;
+  return t0 >= q0 && t0 < q1 ? b : kNoTile;
 }
 
 // x / (1 + e^-x) by the hardware's 2^x and reciprocal, both within an fp32 step

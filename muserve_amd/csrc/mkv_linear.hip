@@ -477,11 +477,8 @@ __global__ __launch_bounds__(DELTA ? 512 : 256, 4) void linear_prep_kernel(LinAr
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t id = blockIdx.x;
   const int32_t kh = c.kh0 + blockIdx.y;
-  int64_t s0 = 0, s1 = 0;
-  const int32_t b = tile_sequence(a.cu, a.n, a.tokens, id, kChunk, s0, s1);
-  if (b < 0) return;  // uniform; bad offsets
-  const int64_t t0 = s0 + (id - first_tile((int32_t)s0, b)) * kChunk;
-  if (t0 < s0 || t0 >= s1) return;  // uniform; no such tile
+  int64_t s0 = 0, s1 = 0, t0 = 0;
+  if (tile_sequence(a.cu, a.n, a.tokens, id, kChunk, s0, s1, t0) < 0) return;  // uniform
   const int32_t len = (int32_t)(s1 - t0 < kChunk ? s1 - t0 : kChunk);
 
   // lane i has token i's gates; their loads run with the first rows'
@@ -859,27 +856,24 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
   const int d0 = at_dim - (ident ? kDim : 0);  // the wave's value dims
   const bool first = o == 0 && part == 0 && c.kh0 == 0 && tid == 0;
   int32_t b = y;
-  int64_t q0 = 0, q1 = 0;  // the sequence's rows
+  int64_t q0 = 0, q1 = 0, s0 = 0;  // the sequence's rows; this workgroup's first
   if (MODE != kWhole) {
-    b = tile_sequence(a.cu, a.n, a.tokens, y, c.seg, q0, q1);
+    b = tile_sequence(a.cu, a.n, a.tokens, y, c.seg, q0, q1, s0);
   } else {
-    q0 = ld_const(a.cu + b);
+    s0 = q0 = ld_const(a.cu + b);
     q1 = ld_const(a.cu + b + 1);
-    if (!offsets_ok(a.cu, a.n, a.tokens)) b = -1;
+    if (!offsets_ok(a.cu, a.n, a.tokens))
+      b = kBadOffsets;
+    else if (q0 == q1)
+      b = kNoTile;
   }
-  if (MODE != kEnds && first && y == 0) *ok_word = b >= 0;
-  if (b < 0) {
-    if (MODE != kEnds && first && y == 0) raise_err(a.err, MKV_DEVERR_TABLE);
-    return;
+  if (MODE != kEnds && first && y == 0) {
+    *ok_word = b != kBadOffsets;
+    if (b == kBadOffsets) raise_err(a.err, MKV_DEVERR_TABLE);
   }
-  int64_t s0 = q0, s1 = q1;  // this workgroup's
-  int64_t seg = 0;
-  if (MODE != kWhole) {
-    seg = y - first_tile((int32_t)q0, b, c.seg);
-    s0 = q0 + seg * c.seg;
-    s1 = s0 + c.seg < q1 ? s0 + c.seg : q1;
-  }
-  if (s0 >= q1) return;  // uniform: no rows, or no such segment
+  if (b < 0) return;  // uniform
+  const bool at_start = s0 == q0;
+  const int64_t s1 = MODE != kWhole && s0 + c.seg < q1 ? s0 + c.seg : q1;
   const bool last = s1 == q1;
   if (MODE == kEnds && last) return;  // uniform: not asked for
   const int32_t slot = ld_const(a.slots + b);  // (its load runs with the images')
@@ -957,18 +951,18 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
   if (slot < 0 || slot >= a.pool_slots) {  // uniform
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (loads into LDS do not outlive it)
     if (!kOut) return;
-    if (first && s0 == q0) raise_err(a.err, MKV_DEVERR_STATE_SLOT);
+    if (first && at_start) raise_err(a.err, MKV_DEVERR_STATE_SLOT);
     for (int64_t t = s0 + d; t < s1; t += 4) *(uint16_t*)(outp + t * out_row) = 0;
     return;
   }
   f32x4 s[8];
-  if (MODE == kEnds && (ident || seg > 0)) {
+  if (MODE == kEnds && (ident || !at_start)) {
 #pragma unroll
     for (int x = 0; x < 8; ++x)
 #pragma unroll
       for (int r = 0; r < 4; ++r) s[x][r] = ident && 16 * x + 4 * d + r == d0 + n ? 1.f : 0.f;
   } else {
-    const float* from = MODE == kRows && !(seg == 0 && last) ? c.ends + segment + row0 : st;
+    const float* from = MODE == kRows && !(at_start && last) ? c.ends + segment + row0 : st;
 #pragma unroll
     for (int x = 0; x < 8; ++x)
       s[x] = __builtin_bit_cast(f32x4, ld16((const uint8_t*)(from + 16 * x)));
@@ -1384,7 +1378,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
 #pragma unroll
     for (int r = 0; r < 4; ++r) s[x][r] *= inv_f;
   if (MODE == kEnds) {
-    if (ident && seg == 0) return;
+    if (ident && at_start) return;
     if (ident) {
       // as linear_join_kernel's operands: row block x of M^T, columns 16 y; lane
       // (m, e) has row m, columns 4 e .. +3. This lane has column n of y = d0 / 16.

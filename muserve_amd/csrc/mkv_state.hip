@@ -310,14 +310,14 @@ constexpr int kConvRows = 4, kConvTile = 4 * kConvRows;
 template <int W>
 __global__ __launch_bounds__(kThreads) void conv_prefill_kernel(ConvPrefillArgs p) {
   const ConvArgs& a = p.c;
-  int64_t seq0 = 0, end = 0;
-  const int32_t b = tile_sequence(p.cu, a.batch, p.tokens, blockIdx.x, kConvTile, seq0, end);
+  int64_t seq0 = 0, end = 0, t0 = 0;
+  const int32_t b = tile_sequence(p.cu, a.batch, p.tokens, blockIdx.x, kConvTile, seq0, end, t0);
   if (b < 0) {  // uniform
-    if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0) raise_err(a.err, MKV_DEVERR_TABLE);
+    if (b == kBadOffsets && threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0)
+      raise_err(a.err, MKV_DEVERR_TABLE);
     return;
   }
-  const int64_t tile = (int64_t)blockIdx.x - first_tile((int32_t)seq0, b, kConvTile);
-  const int64_t t0 = seq0 + tile * kConvTile + (threadIdx.x >> 6) * kConvRows;
+  t0 += (threadIdx.x >> 6) * kConvRows;
   const int64_t g = (int64_t)blockIdx.y * 64 + (threadIdx.x & 63);  // group of 8 channels
   if (t0 >= end || g * 8 >= a.channels) return;
   const int32_t slot = a.slots[b];
