@@ -407,13 +407,19 @@ __device__ __forceinline__ u32x4 cut(float (&x)[8]) {
   }
   return w;
 }
-// max(m, |x|, |y|): a NaN among them is passed over, or (any_of) is the result
+// max(m, |x|, |y|): a NaN among them is passed over, or (any_of) is the result. One
+// instruction each, in the compiler's hands: it waits for matrix results that they
+// read, and before a lane reads what another has of theirs. (As inline assembly they
+// had read matrix results one instruction behind.) The empty assembly keeps them in
+// their places, or values would wait for them in registers that there are not.
 __device__ __forceinline__ float any_of(float m, float x, float y) {
-  asm("v_maximum3_f32 %0, %0, |%1|, |%2|" : "+v"(m) : "v"(x), "v"(y));
+  m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(m, fabsf(x)), fabsf(y));
+  asm("" : "+v"(m));
   return m;
 }
 __device__ __forceinline__ float most_of(float m, float x, float y) {
-  asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(m) : "v"(x), "v"(y));
+  m = fmaxf(fmaxf(m, fabsf(x)), fabsf(y));
+  asm("" : "+v"(m));
   return m;
 }
 
