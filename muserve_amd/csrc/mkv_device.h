@@ -55,6 +55,22 @@ __device__ __forceinline__ T lane_of(T x) {
   return __builtin_bit_cast(
       T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
 }
+// op over a 16-lane row and its neighbour (ROWS 2), or over all 4 rows: of lanes
+// l, l ^ 16 (and l ^ 32, l ^ 48).
+template <int ROWS = 4, typename T, typename F>
+__device__ __forceinline__ T over_rows(T x, F op) {
+  const uint32_t v = __builtin_bit_cast(uint32_t, x);
+  const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  const uint32_t a = r[0], b = r[1];
+  x = op(__builtin_bit_cast(T, a), __builtin_bit_cast(T, b));
+  if (ROWS > 2) {
+    const uint32_t v2 = __builtin_bit_cast(uint32_t, x);
+    const auto r2 = __builtin_amdgcn_permlane32_swap(v2, v2, false, false);
+    const uint32_t a2 = r2[0], b2 = r2[1];
+    x = op(__builtin_bit_cast(T, a2), __builtin_bit_cast(T, b2));
+  }
+  return x;
+}
 // op over each LANES lanes side by side, in all of them.
 template <int LANES, typename T, typename F>
 __device__ __forceinline__ T over_lanes(T x, F op) {
@@ -62,18 +78,7 @@ __device__ __forceinline__ T over_lanes(T x, F op) {
   if (LANES > 2) x = op(x, lane_of<0x4e>(x));
   if (LANES > 4) x = op(x, lane_of<0x141>(x));
   if (LANES > 8) x = op(x, lane_of<0x140>(x));
-  if (LANES > 16) {  // (a 16-lane row and its neighbour)
-    const uint32_t v = __builtin_bit_cast(uint32_t, x);
-    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    const uint32_t a = r[0], b = r[1];
-    x = op(__builtin_bit_cast(T, a), __builtin_bit_cast(T, b));
-  }
-  if (LANES > 32) {
-    const uint32_t v = __builtin_bit_cast(uint32_t, x);
-    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    const uint32_t a = r[0], b = r[1];
-    x = op(__builtin_bit_cast(T, a), __builtin_bit_cast(T, b));
-  }
+  if (LANES > 16) x = over_rows<LANES / 16>(x, op);
   return x;
 }
 template <int LANES>

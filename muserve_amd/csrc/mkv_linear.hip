@@ -295,19 +295,27 @@ __global__ __launch_bounds__(256) void linear_scan_kernel(LinArgs a, int32_t* ok
 // state itself, the right-hand side, T, u) is two fp16 parts, 22 bits; the
 // product of two such drops the lower parts' (2^-22). What only the bf16 output
 // sees (the state under Q, P, u under P) is one part, 2^-12. Sums run in fp32
-// in the matrix cores. A wave keeps its state times a power of two f that holds
-// its largest element in [2^-2, 2^9], and the values go in times f too: fp16's
-// smallest step is then 2^-22 of the state or less. Against float64 a state is
-// 3e-7 off (1e-7 for fp32 arithmetic), an output 2.7e-4 before its rounding to
-// bf16 (1.66e-3). Three bf16 parts were as exact as fp32, but took 182 matrix
-// and 630 vector instructions a chunk where this takes 104 and 440.
+// in the matrix cores. Against float64 a state is 3e-7 off (1e-7 for fp32 arithmetic),
+// an output 2.7e-4 before its rounding to bf16 (1.66e-3). Three bf16 parts were as
+// exact as fp32, but took 182 matrix and 630 vector instructions a chunk where this
+// takes 104 and 440.
 //
-// A column of a matrix operand (one value dim) never mixes with another, but
-// the rows (tokens) of a chunk do, also through zeros. So that what is out of
-// the ordinary in one token (infinities, NaN, a value far past f's scale) reaches
-// only the tokens after it, such a chunk is walked token by token instead: inputs
-// past 2^60 in size, a chunk whose decays grow by more than e^2 (where products
-// could overflow and the recurrence not), operands past the limits below.
+// Scale: two fp16 parts end at 2^-25, so what is small beside what else an operand
+// holds is lost there. A value dim's state (a column of the operands, which never mixes
+// with another) is kept times a power of two f of its own, and its values go in times f
+// too. Before a chunk f goes by the dim's state, or by its values where these make the
+// dim's new state, as the chunk's decays leave little of the old: the step is then 2^-28
+// of them or less. What is left are the tokens of a dim in one chunk: where some stand
+// far above the rest, and later a strong decay leaves nothing of them, the rest is exact
+// to 2^-28 of the larger only. Where 4 tokens in a row hold less than 2^-13 of the
+// largest, or the state is left below 2^-10 of itself with no values to match, the chunk
+// is walked token by token.
+//
+// The rows (tokens) of a chunk mix also through zeros. So that what is out of the
+// ordinary in one token (infinities, NaN) reaches only the tokens after it, such a
+// chunk is walked token by token as well: inputs past 2^60 in size, a chunk whose
+// decays grow by more than e^2 (where products could overflow and the recurrence not),
+// operands past the limits below.
 // ---------------------------------------------------------------------------
 typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 bf16x8;
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -315,6 +323,7 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((__vector_size__(4 * sizeof(float)))) float f32x4;
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 typedef __attribute__((address_space(3))) u32x2 lds_u32x2;
 typedef __attribute__((address_space(3))) float lds_f32;
@@ -331,10 +340,10 @@ constexpr int kKeyImage = 48 * kFrag;  // of a chunk's key head: K, Q (4 row blo
 constexpr int kLower = 6;              // operands of a 64 x 64 lower triangle
 constexpr int kTParts = 2, kPParts = 1;
 // The factors of a chunk's tokens, [64] each: of K S0^T in the right-hand side,
-// of u in the state, e^G, of the output, of v; then e^G_63, whether to walk (two
-// words), and the largest factor of v.
+// of u in the state, e^G, of the output, of v; then e^G_63, the largest factor of v,
+// and whether to walk (two words).
 constexpr int kFactors = 2048, kFacX = 0, kFacU = 64, kFacG = 128, kFacO = 192, kFacV = 256;
-constexpr int kFacAll = 320, kFacWalk = 322, kFacMax = 324;
+constexpr int kFacAll = 320, kFacMax = 321, kFacWalk = 322;
 constexpr int head_image(bool delta) {
   return (delta ? kTParts * kLower * kFrag : 0) + kPParts * kLower * kFrag + kFactors;
 }
@@ -343,9 +352,23 @@ __device__ __forceinline__ constexpr int lower(int mt, int s) {  // operand of r
 }
 constexpr uint32_t kHugeBf16 = (127 + 60) << 7;  // k, q: |x| >= 2^60, infinities and NaN
 constexpr double kLeastDecay = -1e5;             // e^g is 0 far above it; -inf would make NaN sums
-constexpr float kMostPart = 0x1p15f;    // of operands of fp16 parts (fp16 ends at 2^16)
-constexpr float kMostValue = 0x1p13f;   // of right-hand sides and u, in units of the state's scale
-constexpr float kMostState = 0x1p12f, kHighState = 0x1p9f, kLowState = 0x1p-2f;
+constexpr float kMostPart = 0x1p15f;  // of operands of fp16 parts (fp16 ends at 2^16)
+constexpr float kMostRhs = 0x1p10f;   // of right-hand sides, in units of the dim's scale
+constexpr float kMostState = 0x1p14f;
+// T and P are held times these, which the factors of u in the state and of the
+// output undo (and e^G has): the fp16 step under a small element is less of a large
+// one.
+constexpr float kTScale = 0x1p4f, kPScale = 0x1p6f;
+// A dim's scale before a chunk holds the largest of its state, or of its values where
+// the chunk leaves the state below kLittle of them (or they are past kHighValue), in
+// these bounds, else it is brought to 2^kNearState or 2^kNearValue.
+constexpr float kLittle = 0x1p-5f;
+constexpr float kLowState = 0x1p3f, kHighState = 0x1p6f, kLowValue = 0x1p4f, kHighValue = 0x1p8f;
+constexpr int kNearState = 4, kNearValue = 6;
+// Too coarse is what a chunk's right-hand sides hold less than so much of the largest
+// of them in 4 tokens in a row, where the state is left below kLittle of these; and a
+// state that is left below kLeastState of itself and not below that.
+constexpr float kLeastQuad = 0x1p-13f, kLeastState = 0x1p-10f;
 
 constexpr uint32_t kXcds = 8;
 
@@ -642,19 +665,20 @@ __global__ __launch_bounds__(DELTA ? 512 : 256, 4) void linear_prep_kernel(LinAr
       const float rk = inv[0][lane] / unit[0][lane], rq = inv[1][lane] / unit[1][lane];
       const float head = exp_of(gsum), strong = DELTA ? beta * size : size;
       fac[kFacX + lane] = head * rk * strong;
-      fac[kFacU + lane] = exp_of(all - gsum) * rk / size;
-      fac[kFacG + lane] = head;
-      fac[kFacO + lane] = a.scale * rq;
-      fac[kFacV + lane] = strong;
       const float most =
           over_lanes<64>(fabsf(strong), [](float x, float y) { return fmaxf(x, y); });
+      const float by = (DELTA ? kTScale : 1.f) * kPScale;  // of P u
+      fac[kFacU + lane] = exp_of(all - gsum) * rk / (DELTA ? size * kTScale : size);
+      fac[kFacG + lane] = head * by;
+      fac[kFacO + lane] = a.scale * rq / by;
+      fac[kFacV + lane] = strong;
       uint8_t* pimg = img + (DELTA ? kTParts * kLower * kFrag : 0) + lane * 16;
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
         u32x4 qm[4];
         rows_of(sq, mt, qm);
         const double gi = run[slot][16 * mt + m];
-        const float from = exp_of(gi - run[slot][16 * mt]), qi = unit[1][16 * mt + m] / size;
+        const float from = exp_of(gi - run[slot][16 * mt]), qi = unit[1][16 * mt + m] / size * kPScale;
         float p[8];
 #pragma unroll
         for (int nt = 0; nt <= mt; ++nt) {
@@ -774,7 +798,7 @@ __global__ __launch_bounds__(DELTA ? 512 : 256, 4) void linear_prep_kernel(LinAr
             f32x4 v = {0.f, 0.f, 0.f, 0.f};
             if (nt <= mt) v = lds_ldf4(block4(mt * (mt + 1) / 2 + nt, m, d));
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[4 * y + r] = v[r];
+            for (int r = 0; r < 4; ++r) x[4 * y + r] = kTScale * v[r];
           }
 #pragma unroll
           for (int part = 0; part < kTParts; ++part) {
@@ -782,7 +806,7 @@ __global__ __launch_bounds__(DELTA ? 512 : 256, 4) void linear_prep_kernel(LinAr
             st16(img + lane * 16 + (part * kLower + lower(mt, s)) * kFrag, w);
           }
         }
-      const bool out_of_range = __builtin_amdgcn_ballot_w64(!(largest < kMostPart)) != 0;
+      const bool out_of_range = __builtin_amdgcn_ballot_w64(!(largest < kMostPart / kTScale)) != 0;
       if (lane == 0) ((int32_t*)fac)[kFacWalk + 1] = out_of_range;
     }
   }
@@ -975,35 +999,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
   }
   float whole = 1.f;  // kEnds without the delta rule: the segment's decay
 
-  // The state times f. Its scale is what came before a chunk, so that a value
-  // far above it is seen as such: after every chunk the state's largest element
-  // if that has left its range, for a first chunk on zeros its first token's.
+  // The state times f, of each value dim its own (a lane has one, 4 lanes share it).
   float f = 1.f, inv_f = 1.f;
-  auto over_wave = [&](float x) __attribute__((always_inline)) {
-    return over_lanes<64>(x, [](float y, float z) { return fmaxf(y, z); });
-  };
-  auto lane_most = [&]() __attribute__((always_inline)) {
-    float x = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x = most_of(most_of(x, s[i][0], s[i][1]), s[i][2], s[i][3]);
-    return x;
-  };
-  bool large = false;  // the state does not fit fp16 (infinities)
-  auto rescale = [&](float most) __attribute__((always_inline)) {  // the wave's largest |s|
-    if (most > 0x1p-100f && most < 0x1p100f) {
-      const float to = bits_f32(0x7f000000u - (f32_bits(most) & 0x7f800000u));  // most: [1, 2)
-      const float g = f * to;
-      if (g > 0x1p-100f && g < 0x1p100f) {
-        f = g;
-        inv_f = 1.f / g;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) s[i][r] *= to;
-        most *= to;
-      }
-    }
-    large = !(most < kMostState);
+  auto over_dim = [&](float x) __attribute__((always_inline)) {
+    return over_rows(x, [](float y, float z) { return fmaxf(y, z); });
   };
 
   uint32_t ob[8];  // O in bf16, as v
@@ -1027,21 +1026,6 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
     auto value = [&](int i) __attribute__((always_inline)) {
       return bits_f32(i & 1 ? v[i >> 1] & 0xffff0000u : v[i >> 1] << 16);
     };
-    if (ci == 0) {
-      float most = over_wave(lane_most());
-      if (most == 0.f && !ident) {
-        float x = fabsf(value(0));
-        if (d != 0) x = 0.f;
-        most = over_wave(x);
-        if (most == 0.f) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) x = fmaxf(x, fabsf(value(i)));
-          most = over_wave(x);
-        }
-        most *= *(lds_f32*)(uintptr_t)(l0 + kLow + kFac + kFacMax * 4);
-      }
-      rescale(most);
-    }
     const bool more = ci + 1 < chunks;
     // lane bases of the buffer's two parts: operands lie at constants from them
     uint32_t low = l0 + lane * 16, high = l0 + kLow + lane * 16;
@@ -1084,10 +1068,52 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
         for (int p = 0; p < 2; ++p)
           tq[to][2 * i + p] = later(kT + (p * kLower + lower(mt0 + i, ks)) * kFrag);
     };
-    if (kAhead && (DELTA || kOut)) {
-      read_kq(0);
-      cut_state(0);
+    const float decay = *(lds_f32*)(uintptr_t)(l0 + kLow + kFac + kFacAll * 4);
+    const float strong = *(lds_f32*)(uintptr_t)(l0 + kLow + kFac + kFacMax * 4);
+    if (kAhead && (DELTA || kOut)) read_kq(0);
+    // The dim's scale: by its state's largest element, or by its values' where these
+    // are to make its new state or would not fit.
+    float coarse = 0.f;  // right-hand sides below it are too coarse (0: none)
+    bool large = false;  // a dim of the wave does not fit fp16
+    {
+      float held = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        held = most_of(most_of(held, s[i][0], s[i][1]), s[i][2], s[i][3]);
+      u16x2 most = {0, 0};  // (bf16 without its sign is ordered as an integer)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, v[i] & 0x7fff7fffu));
+      held = over_dim(held);
+      float dim = over_dim(bits_f32((uint32_t)max(most.x, most.y) << 16)) * (strong * f);
+      const bool fresh = held * decay < kLittle * dim;
+      const bool by_value = fresh || !(dim < kHighValue);
+      const float x = by_value ? dim : held;
+      const bool out = !(x < (by_value ? kHighValue : kHighState)) ||
+                       (x < (by_value ? kLowValue : kLowState) && x > 0.f);
+      if (__builtin_amdgcn_ballot_w64(out) != 0) {
+        float to = bits_f32(0x7f000000u + ((by_value ? kNearValue : kNearState) << 23) -
+                            (f32_bits(x) & 0x7f800000u));
+        if (!out || !(x > 0x1p-110f && x < 0x1p120f && f * to > 0x1p-100f && f * to < 0x1p100f))
+          to = 1.f;
+        f *= to;
+        inv_f = 1.f / f;
+        held *= to;
+        dim *= to;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[i][r] *= to;
+      }
+      large = __builtin_amdgcn_ballot_w64(!(held < kMostState)) != 0;
+      // (M's rows are taken of what was before the segment: what a chunk's largest leave
+      // in them, 2^-28 of it, is of no matter)
+      if (!ident && fresh)
+        coarse = dim < kLowValue ? 3e38f : kLeastQuad * (dim + 4.f * held);
+      else if (!ident && decay < kLeastState)
+        coarse = 3e38f;
     }
+    if (kAhead && (DELTA || kOut)) cut_state(0);
     if (more) load_v(ci + 1);
     if (kAhead) __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_setprio(1);
@@ -1135,13 +1161,22 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
     __builtin_amdgcn_s_setprio(0);
     const u32x2 walks = *(lds_u32x2*)(uintptr_t)(l0 + kLow + kFac + kFacWalk * 4);
     const uint32_t walk = __builtin_amdgcn_readfirstlane(walks.x | walks.y);
-    const float decay = *(lds_f32*)(uintptr_t)(l0 + kLow + kFac + kFacAll * 4);
     if (MODE == kEnds && !DELTA) whole *= decay;
     const uint32_t lnow = l0;
     l0 = l1;
     l1 = lnow;
     f32x4 u[4], rhs[4];
-    bool big;  // operands past their limits, infinities and NaN
+    bool big = false;  // operands past their limits, infinities and NaN
+    auto check = [&](const f32x4 (&x)[4]) __attribute__((always_inline)) {
+      float most = 0.f;
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {  // 4 tokens in a row
+        const float quad = any_of(any_of(0.f, x[mt][0], x[mt][1]), x[mt][2], x[mt][3]);
+        big |= quad < coarse && quad > 0.f && 16 * mt + 4 * d + 4 <= len;
+        most = any_of(most, quad, quad);
+      }
+      big |= !(most < kMostRhs);
+    };
     u32x4 pf[4], tf[8];  // operands of P and of K^T
     auto read_p = [&](int ks) __attribute__((always_inline)) {
       if (!kOut) return;
@@ -1163,25 +1198,19 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
         read_t(1, 2, 0);
         __builtin_amdgcn_sched_barrier(0);
       }
-      float most = 0.f;
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt) {
+      for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           rhs[mt][r] = fmaf(value(4 * mt + r), bf[mt][r] * f, -cf[mt][r] * xa[mt][r]);
-        most = any_of(any_of(most, rhs[mt][0], rhs[mt][1]), rhs[mt][2], rhs[mt][3]);
-      }
-      big = !(most < kMostValue);
+      check(rhs);
     } else {
       const float bf = *(lds_f32*)(uintptr_t)(lnow + kLow + kFac + kFacV * 4) * f;
-      float most = 0.f;
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt) {
+      for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) u[mt][r] = value(4 * mt + r) * bf;
-        most = any_of(any_of(most, u[mt][0], u[mt][1]), u[mt][2], u[mt][3]);
-      }
-      big = !(most < kMostValue);
+      check(u);
     }
     u32x4 r0[2], r1[2];
     if (DELTA) {
@@ -1298,7 +1327,6 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
           for (int r = 0; r < 4; ++r) s[i][r] = fmaf(u * rk, kx[i][r], e * s[i][r]);
       }
       stored = true;
-      rescale(over_wave(lane_most()));
       continue;
     }
     // S = e^G S0 + (e^(G_63 - G) u) k^T; O = e^G Y + P U
@@ -1373,10 +1401,6 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
         ob[i] = pack_bf16(ya[mt][j] * (of[mt][j] * inv_f), ya[mt][j + 1] * (of[mt][j + 1] * inv_f));
       }
     }
-    const float most = lane_most();
-    if (__builtin_amdgcn_ballot_w64(!(most < kHighState)) != 0 ||
-        __builtin_amdgcn_ballot_w64(most >= kLowState) == 0)
-      rescale(over_wave(most));
   }
   if (kOut && !stored) store_o(chunks - 1);
 #pragma unroll
