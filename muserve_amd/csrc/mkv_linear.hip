@@ -291,14 +291,13 @@ __global__ __launch_bounds__(256) void linear_scan_kernel(LinArgs a, int32_t* ok
 // Precision: the matrix instructions of a chunk take fp16. Rows of k and q are
 // brought near 1 by a power of two, which the factors of their tokens undo: a
 // bf16 row is exact in fp16 then, but for elements below 2^-17 of its largest,
-// rounded to 2^-25 of that. An fp32 operand that the state depends on (the
-// state itself, the right-hand side, T, u) is two fp16 parts, 22 bits; the
-// product of two such drops the lower parts' (2^-22). What only the bf16 output
-// sees (the state under Q, P, u under P) is one part, 2^-12. Sums run in fp32
-// in the matrix cores. Against float64 a state is 3e-7 off (1e-7 for fp32 arithmetic),
-// an output 2.7e-4 before its rounding to bf16 (1.66e-3). Three bf16 parts were as
-// exact as fp32, but took 182 matrix and 630 vector instructions a chunk where this
-// takes 104 and 440.
+// rounded to 2^-25 of that. An fp32 operand (the state, the right-hand side, T, u, P)
+// is two fp16 parts, 22 bits; the product of two such drops the lower parts' (2^-22).
+// Sums run in fp32 in the matrix cores. So a state and an output before its rounding
+// to bf16 are within a few 2^-22 of what they are sums of. (With one part of the
+// state, P and u in the outputs these were 2^-12 of their terms off, which shows where
+// terms cancel; 28 matrix instructions of 132 a chunk, 3 to 6 % of a call.) Three bf16
+// parts were as exact as fp32, but take 182 matrix and 630 vector instructions a chunk.
 //
 // Scale: two fp16 parts end at 2^-25, so what is small beside what else an operand
 // holds is lost there. A value dim's state (a column of the operands, which never mixes
@@ -338,7 +337,7 @@ constexpr int kChunk = 64;
 constexpr int kFrag = 1024;
 constexpr int kKeyImage = 48 * kFrag;  // of a chunk's key head: K, Q (4 row blocks x 4), K^T (8 x 2)
 constexpr int kLower = 6;              // operands of a 64 x 64 lower triangle
-constexpr int kTParts = 2, kPParts = 1;
+constexpr int kTParts = 2, kPParts = 2;
 // The factors of a chunk's tokens, [64] each: of K S0^T in the right-hand side,
 // of u in the state, e^G, of the output, of v; then e^G_63, the largest factor of v,
 // and whether to walk (two words).
@@ -693,7 +692,9 @@ __global__ __launch_bounds__(DELTA ? 512 : 256, 4) void linear_prep_kernel(LinAr
           if ((nt & 1) || nt == mt) {
 #pragma unroll
             for (int r = 0; r < 8; r += 2) largest = most_of(largest, p[r], p[r + 1]);
-            st16(pimg + lower(mt, nt >> 1) * kFrag, upper(p));
+            const u32x4 high = cut(p);
+            st16(pimg + lower(mt, nt >> 1) * kFrag, high);
+            st16(pimg + (kLower + lower(mt, nt >> 1)) * kFrag, upper(p));
           }
           __builtin_amdgcn_sched_barrier(0);  // (registers: one block's reads at a time)
         }
@@ -1052,12 +1053,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
       float x[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = s[2 * ks + (j >> 2)][j & 3];
-      if (DELTA) {
-        sp[ks % kSets][0] = cut(x);
-        sp[ks % kSets][1] = upper(x);
-      } else {
-        sp[ks % kSets][0] = upper(x);
-      }
+      sp[ks % kSets][0] = cut(x);
+      sp[ks % kSets][1] = upper(x);
     };
     f32x4 cf[4], bf[4], ef[4];
     u32x4 tq[2][4];  // T's parts of two row blocks: (0, 1; step 0), (2, 3; 0), (2, 3; 1)
@@ -1138,18 +1135,18 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
       }
       if (DELTA || kOut) {
 #pragma unroll
-        for (int p = DELTA ? 1 : 0; p >= 0; --p) {
+        for (int p = 1; p >= 0; --p) {
           if (DELTA)
 #pragma unroll
             for (int mt = 0; mt < 4; ++mt) xa[mt] = mfma16(kf[ks % kSets][mt], sp[ks % kSets][p], xa[mt]);
-          if (kOut && p == 0)
+          if (kOut)
 #pragma unroll
             for (int mt = 0; mt < 4; ++mt) ya[mt] = mfma16(qf[ks % kSets][mt], sp[ks % kSets][p], ya[mt]);
         }
         if (kAhead && ks < 3) {
           __builtin_amdgcn_sched_group_barrier(kSchedDsRead, (DELTA ? 4 : 0) + (kOut ? 4 : 0), 0);
 #pragma unroll
-          for (int i = 0; i < (DELTA ? 8 : 0) + (kOut ? 4 : 0); ++i) {
+          for (int i = 0; i < (DELTA ? 8 : 0) + (kOut ? 8 : 0); ++i) {
             __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
             __builtin_amdgcn_sched_group_barrier(kSchedValu, 2, 0);
           }
@@ -1177,11 +1174,13 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
       }
       big |= !(most < kMostRhs);
     };
-    u32x4 pf[4], tf[8];  // operands of P and of K^T
+    u32x4 pf[kPParts][4], tf[8];  // operands of P and of K^T
     auto read_p = [&](int ks) __attribute__((always_inline)) {
       if (!kOut) return;
 #pragma unroll
-      for (int mt = 2 * ks; mt < 4; ++mt) pf[mt] = later(kP + lower(mt, ks) * kFrag);
+      for (int p = 0; p < kPParts; ++p)
+#pragma unroll
+        for (int mt = 2 * ks; mt < 4; ++mt) pf[p][mt] = later(kP + (p * kLower + lower(mt, ks)) * kFrag);
     };
     auto read_kt = [&](int ks, int from, int to) __attribute__((always_inline)) {
 #pragma unroll
@@ -1356,7 +1355,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
       // the state's products while the vector unit rounds u and scales Y for the output's
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = u[2 * ks + (j >> 2)][j & 3];
-      const u32x4 uh = upper(x);
+      const u32x4 uh = cut(x), ul = upper(x);
       if (kOut && ks == 0) {
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt)
@@ -1385,7 +1384,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
       if (kAhead && ks == 0) read_kt(1, 0, 8);
       if (kOut) {
 #pragma unroll
-        for (int mt = 2 * ks; mt < 4; ++mt) ya[mt] = mfma16(pf[mt], uh, ya[mt]);
+        for (int p = 2; p >= 0; --p)  // lower x upper, upper x lower, upper x upper
+#pragma unroll
+          for (int mt = 2 * ks; mt < 4; ++mt)
+            ya[mt] = mfma16(pf[p == 2][mt], p == 1 ? ul : uh, ya[mt]);
         if (ks == 0) {
           read_p(1);
 #pragma unroll

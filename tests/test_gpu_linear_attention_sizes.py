@@ -46,9 +46,10 @@ def want_by_dim(x, rows, state, scale=D ** -0.5):
 
 def check(x, T, **more):
     gx = lu.on_gpu(x)
-    prompt(gx, ints([0]), ints([0, T]), gx["state"], **more)
+    out = prompt(gx, ints([0]), ints([0, T]), gx["state"], **more)
     torch.cuda.synchronize()
-    _, state, s_tol, _ = want_by_dim(x, slice(0, T), x["state"][0])
+    want, state, s_tol, o_tol = want_by_dim(x, slice(0, T), x["state"][0])
+    lu.close(out, want, o_tol, "outputs")
     err = (gx["state"][0].double().cpu() - state).norm(dim=-1)
     bound = s_tol + 2.0 ** -140
     assert (err <= bound).all(), f"states: {float((err / bound).max()):.3g} times the bound"
@@ -126,3 +127,43 @@ def test_strong_decays_at_every_token(g, delta):
     x = lu.inputs(92, 700, 2, 4, raw=False, delta=delta)
     x["g"] = g * (0.5 + torch.rand(700, 4, generator=torch.Generator().manual_seed(3)))
     check(x, 700)
+
+
+@pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("of", ["state", "values"])
+def test_outputs_that_cancel(of, delta):
+    """Queries of two elements whose products cancel to 2^-8 or less: an output's error
+    is one of its terms, and these are not rounded to fewer bits than fp32 has."""
+    case(f"linear attention, outputs that cancel, of the {of}, delta {delta}")
+    T, hk, hv = 9, 2, 4
+    x = lu.inputs(80, T, hk, hv, raw=False, delta=delta, qk_norm=False)
+    gen = torch.Generator().manual_seed(81)
+    q, k, v = lu.split(x["mixed"], hk, hv)
+    x["g"] = x["g"][:, :1].expand(T, hv).contiguous()
+    q.zero_()
+    if of == "state":  # rows w_n a: the queries' keys are 0, 1, the others' from 64 on
+        x["g"].zero_()
+        k[..., :64] = 0
+        a, w = torch.rand(D, generator=gen) + 1, torch.randn(hv, D, generator=gen)
+        x["state"][0] = w[:, :, None] * a
+        c = torch.rand(T, hk, generator=gen) + 0.5
+        q[..., 0], q[..., 1] = c * a[1], -c * a[0]
+    else:  # two writes that differ in sign, to keys 0 and 1, and decays between
+        x["state"].zero_()
+        k.zero_()
+        k[0, :, 0] = k[1, :, 1] = 1
+        v[1] = -v[0]
+        v[2:] = 0
+        if delta:
+            x["beta"].fill_(1.0)
+        decay = x["g"][1, 0].exp()
+        c = torch.rand(T, hk, generator=gen) + 0.5
+        q[2:, :, 0], q[2:, :, 1] = c[2:], c[2:] * decay
+    check(x, T, max_seqlen=T)
+
+
+@pytest.mark.parametrize("how", [dict(), dict(raw=False, qk_norm=False), dict(delta=False)], ids=str)
+@pytest.mark.parametrize("T", [9, 30, 64, 150])
+def test_outputs_by_value_dim(T, how):
+    case(f"linear attention, bounds by value dim, {T} tokens, {how}")
+    check(lu.inputs(82 + T, T, 2, 4, **how), T)
