@@ -387,9 +387,8 @@ int mkv_linear_attn_decode(void* state, int64_t pool_slots, int32_t num_k_heads,
  * from where the last one ended) and leaves its final state there. A sequence
  * without rows leaves its slot; rows of out outside the sequences are left as
  * they were. max_seqlen is a hint of the longest sequence (0: not known) that
- * chooses between forms of the computation; any value is right. With z the
- * output is rounded to bf16 before the norm as well (rows of a slot outside the
- * pool are zeros before it). Arguments and requirements otherwise as above,
+ * chooses between forms of the computation; any value is right. Rows of a slot
+ * outside the pool are zeros, with z too. Arguments and requirements otherwise as above,
  * batch <= 4096, num_tokens < 2^31, num_tokens * num_v_heads <= 2^30, rows of v
  * at most 16 MiB apart (MKV_E_UNSUPPORTED).
  * Every value dim is as exact as its own size asks for (a state to 2^-21 or so of

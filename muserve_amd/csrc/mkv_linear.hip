@@ -143,6 +143,30 @@ __device__ __forceinline__ float weight_at(const uint8_t* w, int32_t bf16, int64
   return bf16 ? bf16_at(w + 2 * i) : *(const float*)(w + 4 * i);
 }
 
+// o / sqrt(mean(o^2) + eps) w silu(z) of a head whose 128 dims a workgroup of 4 waves
+// has, dims r0 + 32 i in the 8 lanes l of a row; part: a float for each wave.
+template <int ROWS>
+__device__ __forceinline__ void norm_over_dims(const LinArgs& a, int64_t token, int32_t h, int r0,
+                                               int l, float* part, float (&o)[ROWS]) {
+  static_assert(ROWS * 32 == kDim && kThreads == 256, "a head");
+  float q = 0.f;
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) q = fmaf(o[i], o[i], q);
+  q = sum_lanes<64>(l == 0 ? q : 0.f);  // (8 lanes have the same rows)
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = q;
+  __syncthreads();
+  q = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) q += part[i];
+  const float r = 1.f / sqrtf(q * (1.f / kDim) + a.eps);
+  const uint8_t* zp = a.z + token * a.z_stride + h * (kDim * 2);
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int d = r0 + 32 * i;
+    o[i] = o[i] * r * weight_at(a.w, a.w_bf16, d) * silu_bf16(bf16_at(zp + 2 * d));
+  }
+}
+
 // One workgroup per (value head, request): the head's 64 KiB state is read
 // once, updated in registers and written back. Bound by HBM: 128 KiB per
 // (request, head) against 0.8 KiB of everything else; 256 requests of 8 heads
@@ -187,25 +211,8 @@ __global__ __launch_bounds__(kThreads) void linear_decode_kernel(LinArgs a) {
       for (int j = 0; j < 4; ++j) x[j] = f32_bits(m.s[i][4 * c + j]);
       st_stream((uint8_t*)st, (uint32_t)((r0 + kGroups * i) * kDim + 32 * c + 4 * l) * 4, x);
     }
-  if (a.z) {  // uniform: o / sqrt(mean(o^2) + eps) w silu(z)
-    __shared__ float part[kThreads / 64];
-    float q = 0.f;
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) q = fmaf(o[i], o[i], q);
-    q = sum_lanes<64>(l == 0 ? q : 0.f);  // (8 lanes have the same rows)
-    if ((tid & 63) == 0) part[tid >> 6] = q;
-    __syncthreads();
-    q = 0.f;
-#pragma unroll
-    for (int i = 0; i < kThreads / 64; ++i) q += part[i];
-    const float r = 1.f / sqrtf(q * (1.f / kDim) + a.eps);
-    const uint8_t* zp = a.z + b * a.z_stride + h * (kDim * 2);
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      const int d = r0 + kGroups * i;
-      o[i] = o[i] * r * weight_at(a.w, a.w_bf16, d) * silu_bf16(bf16_at(zp + 2 * d));
-    }
-  }
+  __shared__ float part[kThreads / 64];
+  if (a.z) norm_over_dims<kRows>(a, b, h, r0, l, part, o);  // uniform
   if (l == 0) {
 #pragma unroll
     for (int i = 0; i < kRows; ++i)
@@ -217,17 +224,17 @@ __global__ __launch_bounds__(kThreads) void linear_decode_kernel(LinArgs a) {
 // Prompts
 // ---------------------------------------------------------------------------
 
-// One workgroup per 64 value dims of a (head, sequence), token after token:
-// bound by the chain from one to the next, 1.8 us each while few workgroups run.
-__global__ __launch_bounds__(256) void linear_scan_kernel(LinArgs a, int32_t* ok_word) {
-  constexpr int kRows = 2;
+// One workgroup per 64 value dims of a (head, sequence), or per 128 with the output
+// norm, which needs them all, token after token: bound by the chain from one to the
+// next, 1.8 us each while few workgroups run.
+template <bool NORM>
+__global__ __launch_bounds__(256) void linear_scan_kernel(LinArgs a) {
+  constexpr int kRows = NORM ? 4 : 2, kParts = 4 / kRows;
   const int tid = threadIdx.x, l = tid & 7, r0 = tid >> 3;
-  const int32_t h = blockIdx.x >> 1, kh = h / a.group, d0 = (blockIdx.x & 1) * 64;
+  const int32_t h = blockIdx.x / kParts, kh = h / a.group, d0 = blockIdx.x % kParts * 64;
   const int32_t b = blockIdx.y;
   const bool first = blockIdx.x == 0 && tid == 0;
-  const bool ok = offsets_ok(a.cu, a.n, a.tokens);
-  if (first && b == 0) *ok_word = ok;
-  if (!ok) {
+  if (!offsets_ok(a.cu, a.n, a.tokens)) {
     if (first && b == 0) raise_err(a.err, MKV_DEVERR_TABLE);
     return;
   }
@@ -236,8 +243,9 @@ __global__ __launch_bounds__(256) void linear_scan_kernel(LinArgs a, int32_t* ok
   const int32_t slot = a.slots[b];
   if (slot < 0 || slot >= a.pool_slots) {  // uniform
     if (first) raise_err(a.err, MKV_DEVERR_STATE_SLOT);
-    for (int64_t t = t0 + (tid >> 5); t < t1; t += 8)
-      *(uint32_t*)(a.out + (t * a.hv + h) * (kDim * 2) + d0 * 2 + 4 * (tid & 31)) = 0u;
+    constexpr int kWords = kRows * 16;  // of a token's dims
+    for (int64_t t = t0 + tid / kWords; t < t1; t += 256 / kWords)
+      *(uint32_t*)(a.out + (t * a.hv + h) * (kDim * 2) + d0 * 2 + 4 * (tid % kWords)) = 0u;
     return;
   }
   float* st = a.state + ((int64_t)slot * a.hv + h) * kStateHead + (int64_t)d0 * kDim;
@@ -250,6 +258,7 @@ __global__ __launch_bounds__(256) void linear_scan_kernel(LinArgs a, int32_t* ok
 #pragma unroll
       for (int j = 0; j < 4; ++j) m.s[i][4 * c + j] = bits_f32(x[j]);
     }
+  __shared__ float part[2][4];
   for (int64_t t = t0; t < t1; ++t) {
     float g, beta, v[kRows], o[kRows];
     m.keys(a, t, kh, l);
@@ -259,6 +268,8 @@ __global__ __launch_bounds__(256) void linear_scan_kernel(LinArgs a, int32_t* ok
     for (int i = 0; i < kRows; ++i) v[i] = bf16_at(vp + 2 * (r0 + 32 * i));
     m.norms(a);
     m.step(a, g, beta, v, o);
+    if constexpr (NORM)  // (the last token's sums may still be read)
+      norm_over_dims<kRows>(a, t, h, r0, l, part[(t - t0) & 1], o);
     if (l == 0) {
 #pragma unroll
       for (int i = 0; i < kRows; ++i)
@@ -368,6 +379,8 @@ constexpr int kNearState = 4, kNearValue = 6;
 // of them in 4 tokens in a row, where the state is left below kLittle of these; and a
 // state that is left below kLeastState of itself and not below that.
 constexpr float kLeastQuad = 0x1p-13f, kLeastState = 0x1p-10f;
+
+constexpr int64_t kMostStride = 1 << 24;  // 64 rows through a buffer descriptor
 
 constexpr uint32_t kXcds = 8;
 
@@ -852,10 +865,10 @@ enum { kWhole = 0, kEnds = 1, kRows = 2 };
 // (8 x 4096 tokens, 8 heads, on 128 CUs: 199 us) for 578 vector, 104 matrix and
 // 88 LDS instructions of a wave alone on its SIMD; with 8 waves 3.8, with 16 (no
 // outputs, 128 value dims and 128 rows of M) 5.8.
-template <int WAVES, bool DELTA, int MODE>
-__global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(LinArgs a, ChunkArgs c,
-                                                                             int32_t* ok_word) {
+template <int WAVES, bool DELTA, int MODE, bool NORM = false>
+__global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(LinArgs a, ChunkArgs c) {
   constexpr bool kOut = MODE != kEnds;
+  static_assert(!NORM || (WAVES == 8 && kOut), "the norm is taken over a head's dims");
   // With 4 waves per SIMD these hide each other's waits in 128 registers; with
   // fewer, operands are read a step ahead.
   constexpr bool kAhead = WAVES < 16;
@@ -898,10 +911,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
     else if (q0 == q1)
       b = kNoTile;
   }
-  if (MODE != kEnds && first && y == 0) {
-    *ok_word = b != kBadOffsets;
-    if (b == kBadOffsets) raise_err(a.err, MKV_DEVERR_TABLE);
-  }
+  if (MODE != kEnds && first && y == 0 && b == kBadOffsets) raise_err(a.err, MKV_DEVERR_TABLE);
   if (b < 0) return;  // uniform
   const bool at_start = s0 == q0;
   const int64_t s1 = MODE != kWhole && s0 + c.seg < q1 ? s0 + c.seg : q1;
@@ -1014,6 +1024,78 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
       __builtin_amdgcn_raw_buffer_store_b32(swap_pair(ob[i]), rows, oat,
                                             (16 * (i >> 1) + 2 * (i & 1)) * os, 0);
   };
+  // The output norm. Each wave leaves its dims' sums of squares of a chunk's tokens in
+  // LDS; behind the next chunk's barrier they are added up, and the outputs, still in
+  // registers, are normed and stored.
+  __shared__ __attribute__((aligned(16))) float sums[NORM ? 2 : 1][NORM ? kChunk : 1][8];
+  __shared__ __attribute__((aligned(16))) float rms[NORM ? WAVES : 1][kChunk];
+  f32x4 held_o[4];   // outputs of the chunk before: tokens 16 x + 4 d + r
+  uint32_t held_z[8];  // their z, as v
+  const float weight = NORM ? weight_at(a.w, a.w_bf16, d0 + n) : 0.f;
+  auto load_z = [&](int32_t ci) __attribute__((always_inline)) {
+    if (a.z_stride <= kMostStride) {  // uniform
+      const int32_t zs = (int32_t)a.z_stride;
+      const uint32_t zat = (uint32_t)((4 * d + odd) * zs + (d0 + n - odd) * 2);
+      const __amdgpu_buffer_rsrc_t rows = rows_of(a.z, a.z_stride, ci);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        held_z[i] =
+            __builtin_amdgcn_raw_buffer_load_b32(rows, zat, (16 * (i >> 1) + 2 * (i & 1)) * zs, 0);
+    } else {
+      const int64_t t0 = s0 + (int64_t)ci * kChunk + 4 * d + odd;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int64_t t = t0 + 16 * (i >> 1) + 2 * (i & 1);
+        held_z[i] = 0u;
+        if (t < s1)
+          held_z[i] = *(const uint32_t*)(a.z + t * a.z_stride + (h * kDim + d0 + n - odd) * 2);
+      }
+    }
+  };
+  auto leave_sums = [&](int32_t ci) __attribute__((always_inline)) {
+    // sums over the 16 dims of a row of lanes; lane (n, d) comes to have token 16 (n / 4)
+    // + 4 d + n % 4: half the tokens are given away for each of the first two bits of n
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = held_o[i >> 2][i & 3] * held_o[i >> 2][i & 3];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float keep = n & 1 ? x[2 * i + 1] : x[2 * i], give = n & 1 ? x[2 * i] : x[2 * i + 1];
+      x[i] = keep + lane_of<0xb1>(give);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float keep = n & 2 ? x[2 * i + 1] : x[2 * i], give = n & 2 ? x[2 * i] : x[2 * i + 1];
+      x[i] = keep + lane_of<0x4e>(give);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] += lane_of<0x128>(x[i]);  // rotations of a row by 8 and 4 lanes
+      x[i] += lane_of<0x124>(x[i]);
+    }
+    const float y01 = n & 4 ? x[1] : x[0], y23 = n & 4 ? x[3] : x[2];
+    sums[ci & 1][16 * (n >> 2) + 4 * d + (n & 3)][wave] = n & 8 ? y23 : y01;
+  };
+  auto store_normed = [&](int32_t ci) __attribute__((always_inline)) {
+    const f32x4 lo = *(const f32x4*)&sums[ci & 1][lane][0], hi = *(const f32x4*)&sums[ci & 1][lane][4];
+    const float q = ((lo[0] + lo[1]) + (lo[2] + lo[3])) + ((hi[0] + hi[1]) + (hi[2] + hi[3]));
+    rms[wave][lane] = 1.f / sqrtf(q * (1.f / kDim) + a.eps);
+    wave_sync();
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      const f32x4 by = *(const f32x4*)&rms[wave][16 * mt + 4 * d];
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const uint32_t z = swap_pair(held_z[2 * mt + y]);
+        ob[2 * mt + y] =
+            pack_bf16(held_o[mt][2 * y] * by[2 * y] * weight * silu_bf16(bits_f32(z << 16)),
+                      held_o[mt][2 * y + 1] * by[2 * y + 1] * weight *
+                          silu_bf16(bits_f32(z & 0xffff0000u)));
+      }
+    }
+    wave_sync();  // (rms is read)
+    store_o(ci);
+  };
   bool stored = true;
   for (int32_t ci = 0; ci < chunks; ++ci) {
     const int64_t t0 = s0 + (int64_t)ci * kChunk;
@@ -1027,6 +1109,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
     auto value = [&](int i) __attribute__((always_inline)) {
       return bits_f32(i & 1 ? v[i >> 1] & 0xffff0000u : v[i >> 1] << 16);
     };
+    if (NORM && ci > 0) store_normed(ci - 1);
     const bool more = ci + 1 < chunks;
     // lane bases of the buffer's two parts: operands lie at constants from them
     uint32_t low = l0 + lane * 16, high = l0 + kLow + lane * 16;
@@ -1175,12 +1258,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
       big |= !(most < kMostRhs);
     };
     u32x4 pf[kPParts][4], tf[8];  // operands of P and of K^T
-    auto read_p = [&](int ks) __attribute__((always_inline)) {
+    auto read_p = [&](int p, int ks) __attribute__((always_inline)) {
       if (!kOut) return;
 #pragma unroll
-      for (int p = 0; p < kPParts; ++p)
-#pragma unroll
-        for (int mt = 2 * ks; mt < 4; ++mt) pf[p][mt] = later(kP + (p * kLower + lower(mt, ks)) * kFrag);
+      for (int mt = 2 * ks; mt < 4; ++mt) pf[p][mt] = later(kP + (p * kLower + lower(mt, ks)) * kFrag);
     };
     auto read_kt = [&](int ks, int from, int to) __attribute__((always_inline)) {
 #pragma unroll
@@ -1254,10 +1335,11 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
     }
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) ef[mt] = lds_ldf4(fac + (kFacU + 16 * mt) * 4);
-    read_p(0);
+    read_p(1, 0);
     if (kAhead) __builtin_amdgcn_sched_barrier(0);
-    if (kOut && !stored) store_o(ci - 1);
+    if (kOut && !NORM && !stored) store_o(ci - 1);
     stored = false;
+    if (NORM) load_z(ci);
     if (DELTA) {
 #pragma unroll
       for (int p = 2; p >= 0; --p)
@@ -1318,13 +1400,20 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
         const float u = DELTA ? beta * (vt - e * rk * over_keys(x)) : vt;
         if (kOut) {
           const float out = a.scale * inv_f * (e * rq * over_keys(y) + u * (over_keys(kq) * rk * rq));
-          if (d == 0) *(uint16_t*)(outp + token * out_row) = f32_to_bf16_rne(out);
+          if (NORM) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (16 * (i >> 2) + 4 * d + (i & 3) == t) held_o[i >> 2][i & 3] = out;
+          } else if (d == 0) {
+            *(uint16_t*)(outp + token * out_row) = f32_to_bf16_rne(out);
+          }
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i)
 #pragma unroll
           for (int r = 0; r < 4; ++r) s[i][r] = fmaf(u * rk, kx[i][r], e * s[i][r]);
       }
+      if (NORM) leave_sums(ci);
       stored = true;
       continue;
     }
@@ -1381,6 +1470,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
       }
       __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_setprio(0);
+      read_p(0, ks);
       if (kAhead && ks == 0) read_kt(1, 0, 8);
       if (kOut) {
 #pragma unroll
@@ -1389,14 +1479,20 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
           for (int mt = 2 * ks; mt < 4; ++mt)
             ya[mt] = mfma16(pf[p == 2][mt], p == 1 ? ul : uh, ya[mt]);
         if (ks == 0) {
-          read_p(1);
+          read_p(1, 1);
 #pragma unroll
           for (int mt = 0; mt < 4; ++mt) of[mt] = lds_ldf4(fac + (kFacO + 16 * mt) * 4);
         }
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    if (kOut) {
+    if (NORM) {
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) held_o[mt][r] = ya[mt][r] * (of[mt][r] * inv_f);
+      leave_sums(ci);
+    } else if (kOut) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int mt = i >> 1, j = 2 * (i & 1);
@@ -1404,7 +1500,12 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
       }
     }
   }
-  if (kOut && !stored) store_o(chunks - 1);
+  if (NORM) {
+    arrive_all();
+    store_normed(chunks - 1);
+  } else if (kOut && !stored) {
+    store_o(chunks - 1);
+  }
 #pragma unroll
   for (int x = 0; x < 8; ++x)
 #pragma unroll
@@ -1538,9 +1639,6 @@ struct NormArgs {
   float eps;
   uint8_t* out;  // [tokens, heads, dim]
   int64_t rows;  // tokens * heads
-  const int32_t* cu;  // with n: only the tokens of cu[0] .. cu[n] - 1, if *ok
-  int32_t n;
-  const int32_t* ok;
 };
 
 // 8 weights as floats
@@ -1568,17 +1666,11 @@ __global__ __launch_bounds__(kThreads) void gated_norm_kernel(NormArgs a) {
     const int d = (s * LANES + lane) * 8;
     if (d < a.dim) load_weights<BF16>(a.w, d, w[s]);
   }
-  uint32_t first = 0, end = 0xffffffffu;
-  if (a.cu) {  // rows outside the sequences stay as they are
-    if (!*a.ok) return;
-    first = (uint32_t)a.cu[0];
-    end = (uint32_t)a.cu[a.n];
-  }
   const int64_t wg = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
   const int64_t row = wg * (kThreads / LANES) + threadIdx.x / LANES;
   const uint32_t at = row < a.rows ? (uint32_t)row : 0;
   const uint32_t token = heads == 1 ? at : at / heads, head = at - token * heads;
-  const bool there = row < a.rows && token >= first && token < end;
+  const bool there = row < a.rows;
   const int64_t off = (int64_t)head * a.dim * 2;
   const uint8_t* xp = a.x + token * a.x_stride + off;
   const uint8_t* zp = a.z + token * a.z_stride + off;
@@ -1759,7 +1851,7 @@ extern "C" int mkv_linear_attn_decode(
 namespace mkv {
 namespace {
 
-constexpr int64_t kHeadBytes = 1024;  // the workspace's first bytes: the offsets' verdict
+constexpr int64_t kLeastBytes = 16;  // of a workspace, so that no call goes without one
 // Images of one launch at most: more key heads are run in turn in the same
 // space, which leaves CUs idle (64 heads, 32768 tokens, 1 GiB of images: 1034 us
 // at once, 1411 in two launches, 1544 in three).
@@ -1805,7 +1897,8 @@ float pass_time(const float (&cost)[2], double wgs, double chunks, int cus) {
 // 1024 half heads 186, whole ones 145, segments of 8 chunks 227; 1 x 1024 whole
 // 70, segments of 4 chunks 64; 6 of 80 to 3000 whole 160, segments of 6 to 8
 // chunks 106 to 118.)
-void choose_walk(Prefill& p, int64_t tokens, int32_t n, int32_t longest, double heads, bool delta) {
+void choose_walk(Prefill& p, int64_t tokens, int32_t n, int32_t longest, double heads, bool delta,
+                 bool norm) {
   const ChunkCosts& c = delta ? kDeltaCosts : kDecayCosts;
   const int cus = device_cus();
   const double most = longest > 0 && longest < tokens ? longest : tokens;
@@ -1813,7 +1906,7 @@ void choose_walk(Prefill& p, int64_t tokens, int32_t n, int32_t longest, double 
   const double long_chunks = ceil(most / kChunk), rest_chunks = ceil(rest / kChunk);
   const double work = long_chunks + (n - 1) * rest_chunks;  // chunks of one head
   float best = 3e38f;
-  for (int32_t waves = 4; waves <= 8; waves += 4) {
+  for (int32_t waves = norm ? 8 : 4; waves <= 8; waves += 4) {
     const float (&cost)[2] = waves == 4 ? c.rows4 : c.rows8;
     const double parts = 8.0 / waves, wgs = heads * parts * n;
     // (rounds of sequences of different lengths fill up: at least the longest one)
@@ -1836,7 +1929,7 @@ void choose_walk(Prefill& p, int64_t tokens, int32_t n, int32_t longest, double 
     const float join = kPassStart + (float)of_long * c.join;
     const float by8 = pass_time(c.ends8, heads * starts * (delta ? 2 : 1), len, cus);
     const float by16 = pass_time(c.ends16, heads * starts, len, cus);
-    for (int32_t waves = 4; waves <= 8; waves += 4) {
+    for (int32_t waves = norm ? 8 : 4; waves <= 8; waves += 4) {
       const float t = join + (delta && by16 < by8 ? by16 : by8) +
                       pass_time(waves == 4 ? c.rows4 : c.rows8, heads * (8 / waves) * segs, len, cus);
       if (t < best) {
@@ -1850,9 +1943,9 @@ void choose_walk(Prefill& p, int64_t tokens, int32_t n, int32_t longest, double 
 }
 
 Prefill plan_prefill(int64_t tokens, int32_t n, int32_t longest, int32_t hk, int32_t hv,
-                     bool delta) {
+                     bool delta, bool norm) {
   Prefill p{};
-  p.total = kHeadBytes;
+  p.total = kLeastBytes;
   p.chunked = tokens > 0 && n > 0 && (longest == 0 || longest > kScanTokens);
   if (!p.chunked) return p;
   p.ids = tile_ids(tokens, n);
@@ -1861,13 +1954,13 @@ Prefill plan_prefill(int64_t tokens, int32_t n, int32_t longest, int32_t hk, int
                     : kImageBytes / images > hk ? hk
                                                 : kImageBytes / images);
   const int64_t heads = (int64_t)p.khs * (hv / hk);
-  choose_walk(p, tokens, n, longest, (double)heads, delta);
+  choose_walk(p, tokens, n, longest, (double)heads, delta, norm);
   if (p.seg) p.segs = tile_ids(tokens, n, p.seg);
   p.key_bytes = p.ids * p.khs * kKeyImage;
   p.head_bytes = p.ids * heads * head_image(delta);
   p.end_bytes = p.segs * heads * kStateHead * 4;
   p.step_bytes = delta ? p.end_bytes : p.segs * heads * 4;
-  p.total = kHeadBytes + p.key_bytes + p.head_bytes + p.end_bytes + p.step_bytes;
+  p.total = p.key_bytes + p.head_bytes + p.end_bytes + p.step_bytes;
   return p;
 }
 
@@ -1879,12 +1972,11 @@ dim3 walk_grid(const LinArgs& a, const ChunkArgs& c) {
 template <bool DELTA>
 void run_chunks(const LinArgs& a, const Prefill& p, uint8_t* ws, hipStream_t s) {
   ChunkArgs c{};
-  c.keys = ws + kHeadBytes;
+  c.keys = ws;
   c.heads = c.keys + p.key_bytes;
   c.ends = (float*)(c.heads + p.head_bytes);
   c.steps = (float*)((uint8_t*)c.ends + p.end_bytes);
   c.seg = p.seg;
-  int32_t* ok = (int32_t*)ws;
   for (int32_t kh0 = 0; kh0 < a.hk; kh0 += p.khs) {
     c.kh0 = kh0;
     c.khs = a.hk - kh0 < p.khs ? a.hk - kh0 : p.khs;
@@ -1896,24 +1988,28 @@ void run_chunks(const LinArgs& a, const Prefill& p, uint8_t* ws, hipStream_t s) 
       c.parts = DELTA && p.end_waves == 8 ? 2 : 1;  // (with the delta rule M's 128 rows too)
       if (p.end_waves == 16)
         hipLaunchKernelGGL((linear_chunk_kernel<DELTA ? 16 : 8, DELTA, kEnds>), walk_grid(a, c),
-                           dim3(DELTA ? 1024 : 512), 0, s, a, c, ok);
+                           dim3(DELTA ? 1024 : 512), 0, s, a, c);
       else
         hipLaunchKernelGGL((linear_chunk_kernel<8, DELTA, kEnds>), walk_grid(a, c), dim3(512), 0, s,
-                           a, c, ok);
+                           a, c);
       hipLaunchKernelGGL(linear_join_kernel<DELTA>, dim3(heads * (kDim / 16), n), dim3(256), 0, s,
                          a, c);
     }
     c.parts = 8 / p.waves;
     c.rows = p.seg ? (int32_t)p.segs : a.n;
     const dim3 grid = walk_grid(a, c), block(64 * p.waves);
-    if (p.seg && p.waves == 8)
-      hipLaunchKernelGGL((linear_chunk_kernel<8, DELTA, kRows>), grid, block, 0, s, a, c, ok);
+    if (p.seg && p.waves == 8 && a.z)
+      hipLaunchKernelGGL((linear_chunk_kernel<8, DELTA, kRows, true>), grid, block, 0, s, a, c);
+    else if (p.seg && p.waves == 8)
+      hipLaunchKernelGGL((linear_chunk_kernel<8, DELTA, kRows>), grid, block, 0, s, a, c);
     else if (p.seg)
-      hipLaunchKernelGGL((linear_chunk_kernel<4, DELTA, kRows>), grid, block, 0, s, a, c, ok);
+      hipLaunchKernelGGL((linear_chunk_kernel<4, DELTA, kRows>), grid, block, 0, s, a, c);
+    else if (p.waves == 8 && a.z)
+      hipLaunchKernelGGL((linear_chunk_kernel<8, DELTA, kWhole, true>), grid, block, 0, s, a, c);
     else if (p.waves == 8)
-      hipLaunchKernelGGL((linear_chunk_kernel<8, DELTA, kWhole>), grid, block, 0, s, a, c, ok);
+      hipLaunchKernelGGL((linear_chunk_kernel<8, DELTA, kWhole>), grid, block, 0, s, a, c);
     else
-      hipLaunchKernelGGL((linear_chunk_kernel<4, DELTA, kWhole>), grid, block, 0, s, a, c, ok);
+      hipLaunchKernelGGL((linear_chunk_kernel<4, DELTA, kWhole>), grid, block, 0, s, a, c);
   }
 }
 
@@ -1926,7 +2022,14 @@ extern "C" int64_t mkv_linear_attn_prefill_workspace_bytes(int64_t num_tokens, i
   if (num_tokens < 0 || num_tokens >= (1ll << 31) || batch < 0 || max_seqlen < 0 ||
       num_k_heads <= 0 || num_v_heads <= 0 || num_v_heads % num_k_heads != 0)
     return -1;
-  return plan_prefill(num_tokens, batch, max_seqlen, num_k_heads, num_v_heads, delta != 0).total;
+  // (with and without the output norm: its walk may have other segments)
+  int64_t most = 0;
+  for (const bool norm : {false, true}) {
+    const int64_t bytes =
+        plan_prefill(num_tokens, batch, max_seqlen, num_k_heads, num_v_heads, delta != 0, norm).total;
+    most = bytes > most ? bytes : most;
+  }
+  return most;
 }
 
 extern "C" int mkv_linear_attn_prefill(
@@ -1950,10 +2053,11 @@ extern "C" int mkv_linear_attn_prefill(
   MKV_REQUIRE(batch <= kMaxSequences, MKV_E_UNSUPPORTED, "%s: more than %d sequences", fn,
               kMaxSequences);
   MKV_REQUIRE(num_tokens <= kNormMaxRows / num_v_heads, MKV_E_UNSUPPORTED, "%s: too many rows", fn);
-  MKV_REQUIRE(v_stride <= (1 << 24), MKV_E_UNSUPPORTED, "%s: rows of v more than 16 MiB apart", fn);
+  MKV_REQUIRE(v_stride <= kMostStride, MKV_E_UNSUPPORTED, "%s: rows of v more than 16 MiB apart", fn);
   if (batch == 0 || num_tokens == 0) return MKV_OK;
   const Prefill p =
-      plan_prefill(num_tokens, batch, max_seqlen, num_k_heads, num_v_heads, beta != nullptr);
+      plan_prefill(num_tokens, batch, max_seqlen, num_k_heads, num_v_heads, beta != nullptr,
+                   z != nullptr);
   MKV_REQUIRE(cu_seqlens && workspace && aligned4(cu_seqlens), MKV_E_INVALID, "%s: null pointer",
               fn);
   MKV_REQUIRE(aligned16(workspace) && workspace_bytes >= p.total, MKV_E_INVALID,
@@ -1961,19 +2065,15 @@ extern "C" int mkv_linear_attn_prefill(
               (long long)p.total);
   a.cu = cu_seqlens;
   const hipStream_t s = as_stream(stream);
-  int32_t* ok = (int32_t*)workspace;
-  if (!p.chunked)
-    hipLaunchKernelGGL(linear_scan_kernel, dim3((unsigned)num_v_heads * 2, (unsigned)batch),
-                       dim3(256), 0, s, a, ok);
+  const dim3 scan((unsigned)num_v_heads * (a.z ? 1 : 2), (unsigned)batch);
+  if (!p.chunked && a.z)
+    hipLaunchKernelGGL(linear_scan_kernel<true>, scan, dim3(256), 0, s, a);
+  else if (!p.chunked)
+    hipLaunchKernelGGL(linear_scan_kernel<false>, scan, dim3(256), 0, s, a);
   else if (a.beta)
     run_chunks<true>(a, p, (uint8_t*)workspace, s);
   else
     run_chunks<false>(a, p, (uint8_t*)workspace, s);
-  const int launched = check_launch(fn);
-  if (launched != MKV_OK || !a.z) return launched;
-  NormArgs m{a.out, a.z, a.w, (int64_t)a.hv * kDim * 2, a.z_stride, a.hv, kDim, a.w_bf16, a.eps,
-             a.out, num_tokens * a.hv, a.cu, a.n, ok};
-  run_norm(m, s);
   return check_launch(fn);
 }
 
@@ -1996,7 +2096,7 @@ extern "C" int mkv_gated_rms_norm(const void* x, int64_t x_stride, const void* z
               MKV_E_ALIGN, "%s: rows must be 16-byte aligned, the weight to its type", fn);
   MKV_REQUIRE(tokens <= kNormMaxRows / heads, MKV_E_UNSUPPORTED, "%s: too many rows", fn);
   NormArgs a{(const uint8_t*)x, (const uint8_t*)z, (const uint8_t*)weight, x_stride, z_stride,
-             heads, dim, weight_bf16, eps, (uint8_t*)out, tokens * heads, nullptr, 0, nullptr};
+             heads, dim, weight_bf16, eps, (uint8_t*)out, tokens * heads};
   run_norm(a, as_stream(stream));
   return check_launch(fn);
 }

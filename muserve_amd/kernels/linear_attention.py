@@ -296,9 +296,8 @@ def linear_attn_prefill(
     goes on where the last one ended) and leaves its final state there. Rows of
     ``out`` outside the sequences are left as they were. ``max_seqlen`` (the
     longest sequence, if the caller knows it) helps to choose the form of the
-    computation. With ``z`` the output is rounded to bf16 before the norm too.
-    Offsets that do not hold together are a device fault, and the call then
-    writes nothing."""
+    computation. Offsets that do not hold together are a device fault, and the
+    call then writes nothing."""
     plan = _common(q, k, v, g, beta, state, slots, a_log, dt_bias, z, norm_weight, out)
     dev, tokens, hk, hv, pool = plan[:5]
     slots = _ids("slots", slots, dev)
