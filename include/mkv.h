@@ -398,7 +398,10 @@ int mkv_linear_attn_decode(void* state, int64_t pool_slots, int32_t num_k_heads,
  * Offsets below 0, falling or above num_tokens set MKV_DEVERR_TABLE, and the
  * call writes neither rows nor states. The workspace must be 16-byte aligned
  * and hold mkv_linear_attn_prefill_workspace_bytes (-1: bad sizes) for the
- * same arguments, delta: beta is given.
+ * same arguments, delta: beta is given. That is 48 KiB for each 64 tokens and key
+ * head and 26 (14 without beta) for each value head, up to 2 GiB or, if more,
+ * what one value head takes; beyond that heads are run in turn. Sequences that are
+ * cut into segments add 128 KiB a segment and value head (64 without beta).
  */
 int mkv_linear_attn_prefill(void* state, int64_t pool_slots, int32_t num_k_heads,
                             int32_t num_v_heads, int32_t head_dim, const int32_t* slots,

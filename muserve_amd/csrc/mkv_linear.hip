@@ -1852,9 +1852,10 @@ namespace mkv {
 namespace {
 
 constexpr int64_t kLeastBytes = 16;  // of a workspace, so that no call goes without one
-// Images of one launch at most: more key heads are run in turn in the same
-// space, which leaves CUs idle (64 heads, 32768 tokens, 1 GiB of images: 1034 us
-// at once, 1411 in two launches, 1544 in three).
+// Images of one launch at most: more key heads, or value heads of one, are run in turn
+// in the same space, which leaves CUs idle (64 heads, 32768 tokens, 1 GiB of images:
+// 1034 us at once, 1411 in two launches, 1544 in three). One value head at least: 74 KiB
+// for 64 tokens.
 constexpr int64_t kImageBytes = 2048ll << 20;
 // Up to so many tokens per sequence are walked one by one (8 heads; token by
 // token, in chunks: 1 sequence of 8 tokens 15 us, 20; 32 of 8 23, 29; 64 of 8
@@ -1869,6 +1870,7 @@ struct Prefill {
   int32_t end_waves;  // of a workgroup that computes segments' ends
   int64_t segs;   // segment ids
   int32_t khs;    // key heads of a launch
+  int32_t vhs;    // value heads of each: all, or some of a single one's
   int64_t key_bytes, head_bytes, end_bytes, step_bytes, total;
 };
 
@@ -1949,11 +1951,11 @@ Prefill plan_prefill(int64_t tokens, int32_t n, int32_t longest, int32_t hk, int
   p.chunked = tokens > 0 && n > 0 && (longest == 0 || longest > kScanTokens);
   if (!p.chunked) return p;
   p.ids = tile_ids(tokens, n);
-  const int64_t images = p.ids * (kKeyImage + (int64_t)(hv / hk) * head_image(delta));
-  p.khs = (int32_t)(kImageBytes / images < 1    ? 1
-                    : kImageBytes / images > hk ? hk
-                                                : kImageBytes / images);
-  const int64_t heads = (int64_t)p.khs * (hv / hk);
+  const int64_t group = hv / hk, head = p.ids * head_image(delta), key = p.ids * kKeyImage;
+  const auto within = [](int64_t x, int64_t most) { return x < 1 ? 1 : x < most ? x : most; };
+  p.khs = (int32_t)within(kImageBytes / (key + group * head), hk);
+  p.vhs = (int32_t)(p.khs > 1 ? group : within((kImageBytes - key) / head, group));
+  const int64_t heads = (int64_t)p.khs * p.vhs;
   choose_walk(p, tokens, n, longest, (double)heads, delta, norm);
   if (p.seg) p.segs = tile_ids(tokens, n, p.seg);
   p.key_bytes = p.ids * p.khs * kKeyImage;
@@ -1969,8 +1971,26 @@ dim3 walk_grid(const LinArgs& a, const ChunkArgs& c) {
   return dim3((unsigned)((pairs + kXcds - 1) / kXcds * kXcds * a.group * c.parts));
 }
 
+// The call on some value heads of one key head.
+LinArgs some_heads(const LinArgs& all, int32_t kh, int32_t first, int32_t count) {
+  LinArgs a = all;
+  const int64_t h = (int64_t)kh * all.group + first, gate = all.gates_bf16 ? 2 : 4;
+  a.hk = 1;
+  a.group = count;  // (hv stays: the strides of states and outputs)
+  a.q += kh * (kDim * 2);
+  a.k += kh * (kDim * 2);
+  a.v += h * (kDim * 2);
+  a.g += h * gate;
+  if (a.beta) a.beta += h * gate;
+  if (a.a_log) a.a_log += h, a.dt_bias += h;
+  if (a.z) a.z += h * (kDim * 2);
+  a.out += h * (kDim * 2);
+  a.state += h * kStateHead;
+  return a;
+}
+
 template <bool DELTA>
-void run_chunks(const LinArgs& a, const Prefill& p, uint8_t* ws, hipStream_t s) {
+void run_heads(const LinArgs& a, const Prefill& p, uint8_t* ws, hipStream_t s) {
   ChunkArgs c{};
   c.keys = ws;
   c.heads = c.keys + p.key_bytes;
@@ -2011,6 +2031,14 @@ void run_chunks(const LinArgs& a, const Prefill& p, uint8_t* ws, hipStream_t s) 
     else
       hipLaunchKernelGGL((linear_chunk_kernel<4, DELTA, kWhole>), grid, block, 0, s, a, c);
   }
+}
+
+template <bool DELTA>
+void run_chunks(const LinArgs& a, const Prefill& p, uint8_t* ws, hipStream_t s) {
+  if (p.vhs == a.group) return run_heads<DELTA>(a, p, ws, s);
+  for (int32_t kh = 0; kh < a.hk; ++kh)
+    for (int32_t o = 0; o < a.group; o += p.vhs)
+      run_heads<DELTA>(some_heads(a, kh, o, a.group - o < p.vhs ? a.group - o : p.vhs), p, ws, s);
 }
 
 }  // namespace

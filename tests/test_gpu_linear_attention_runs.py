@@ -377,3 +377,40 @@ def test_rows_past_32_bits():
     y1 = la.causal_conv_prefill(mixed[T - last:], cw, conv1, ints([0]), ints([0, last]))
     la.check_errors(DEV)
     assert torch.equal(y[T - last:], y1) and torch.equal(conv[1], conv1[0])
+
+
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("delta", [True, False])
+def test_heads_of_one_key_head_in_turn(delta, norm):
+    """More images than a launch holds, all of one key head: its value heads in turn,
+    with a few of them alone as the reference (bounds as for key heads in turn)."""
+    case(f"linear attention, 2/192 heads x 70000 tokens in several launches, delta {delta}")
+    T, hk, hv = 70000, 2, 192
+    gen = torch.Generator(device=DEV).manual_seed(61)
+
+    def normal(*size):
+        return torch.randn(*size, generator=gen, device=DEV).bfloat16()
+
+    q, k, v = normal(T, hk, D), normal(T, hk, D), normal(T, hv, D)
+    x = {"g": normal(T, hv), "beta": normal(T, hv) if delta else None,
+         "z": normal(T, hv, D) if norm else None}
+    a_log, dt = torch.rand(hv, generator=gen, device=DEV), torch.randn(hv, generator=gen, device=DEV)
+    w = 1 + 0.1 * torch.randn(D, generator=gen, device=DEV) if norm else None
+    state = torch.randn(3, hv, D, D, generator=gen, device=DEV)
+    kept, cu, at = state.clone(), ints([5, 40000, T - 3]), ints([2, 0])
+    out = torch.full((T, hv, D), 7.0, device=DEV).bfloat16()
+    la.linear_attn_prefill(q, k, v, x["g"], x["beta"], state, at, cu, qk_norm=True, a_log=a_log,
+                           dt_bias=dt, z=x["z"], norm_weight=w, out=out)
+    for h in (0, 29, 95, 96, 191):
+        st, kh, one = kept[:, h:h + 1].contiguous(), h // 96, slice(h, h + 1)
+        some = {n: None if t is None else t[:, one].contiguous() for n, t in x.items()}
+        want = la.linear_attn_prefill(q[:, kh:kh + 1].contiguous(), k[:, kh:kh + 1].contiguous(),
+                                      v[:, one].contiguous(), some["g"], some["beta"], st, at, cu,
+                                      qk_norm=True, a_log=a_log[one], dt_bias=dt[one], z=some["z"],
+                                      norm_weight=w)
+        rows = slice(5, T - 3)
+        for got, ref_, tol in ((out[rows, one], want[rows], 2.0 ** -7), (state[:, one], st, 1e-5)):
+            ref_ = ref_.double()
+            assert (got.double() - ref_).norm() <= tol * ref_.norm(), h
+    la.check_errors(DEV)
+    assert (out[:5] == 7).all() and (out[T - 3:] == 7).all() and torch.equal(state[1], kept[1])

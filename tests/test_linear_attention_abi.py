@@ -148,3 +148,13 @@ def test_more_sequences_and_rows_than_a_call_takes():
     rc, msg = _rc("mkv_gated_rms_norm", FAKE, 256, FAKE, 256, (1 << 29) + 1, 2, 64, FAKE, 0, 1e-6,
                   FAKE, None)
     assert rc == -3 and "too many rows" in msg
+
+
+def test_workspace_of_many_heads_on_one_key_head():
+    """Value heads of one key head run in turn where their images would take more than
+    2 GiB; what is joined of segments comes on top."""
+    size = _lib.load().mkv_linear_attn_prefill_workspace_bytes
+    for tokens in (300000, 1000000):
+        for delta in (0, 1):
+            assert 1 << 30 < size(tokens, 2, tokens, 1, 64, delta) < 3 << 30
+    assert size(32768, 8, 4096, 2, 8, 1) < 1 << 29
