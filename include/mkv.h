@@ -389,8 +389,8 @@ int mkv_linear_attn_decode(void* state, int64_t pool_slots, int32_t num_k_heads,
  * they were. max_seqlen is a hint of the longest sequence (0: not known) that
  * chooses between forms of the computation; any value is right. Rows of a slot
  * outside the pool are zeros, with z too. Arguments and requirements otherwise as above,
- * batch <= 4096, num_tokens < 2^31, num_tokens * num_v_heads <= 2^30, rows of v
- * at most 16 MiB apart (MKV_E_UNSUPPORTED).
+ * batch <= 4096, num_tokens < 2^31, num_tokens * num_v_heads <= 2^30, num_tokens / 64
+ * + batch < 2^23, rows of v at most 16 MiB apart (MKV_E_UNSUPPORTED).
  * Every value dim is as exact as its own size asks for (a state to 2^-21 or so of
  * what the dim holds). Within 64 rows of a sequence, where a dim's values stand
  * above others of it by up to 2^13 and decays then leave nothing of them, the

@@ -1862,6 +1862,9 @@ constexpr int64_t kImageBytes = 2048ll << 20;
 // 37, 44; of 12 51, 44; 256 of 4 77, 121; of 8 123, 121).
 constexpr int32_t kScanTokens = 8;
 
+constexpr double kMostThreads = 4294967296.;  // of a grid dimension, less than this
+constexpr int32_t kPrepThreads = 512;
+
 struct Prefill {
   bool chunked;
   int64_t ids;    // tiles
@@ -1922,7 +1925,7 @@ void choose_walk(Prefill& p, int64_t tokens, int32_t n, int32_t longest, double 
   }
   for (int32_t len = 4; len < long_chunks; len += len < 16 ? 1 : len < 64 ? 2 : len / 8) {
     const int64_t ids = tile_ids(tokens, n, len * kChunk);
-    if (ids > 65535) continue;  // (grid.y)
+    if (heads * 2 * 512 * (ids + kXcds) >= kMostThreads) continue;
     const double of_long = ceil(long_chunks / len);
     // (others of different lengths end inside a segment, half of one on average)
     const double of_rest = rest_chunks == long_chunks ? of_long : rest_chunks / len + .5;
@@ -2002,7 +2005,7 @@ void run_heads(const LinArgs& a, const Prefill& p, uint8_t* ws, hipStream_t s) {
     c.khs = a.hk - kh0 < p.khs ? a.hk - kh0 : p.khs;
     const unsigned heads = (unsigned)(c.khs * a.group), n = (unsigned)a.n;
     hipLaunchKernelGGL(linear_prep_kernel<DELTA>, dim3((unsigned)p.ids, (unsigned)c.khs),
-                       dim3(DELTA ? 512 : 256), 0, s, a, c);
+                       dim3(DELTA ? kPrepThreads : kPrepThreads / 2), 0, s, a, c);
     if (p.seg) {
       c.rows = (int32_t)p.segs;
       c.parts = DELTA && p.end_waves == 8 ? 2 : 1;  // (with the delta rule M's 128 rows too)
@@ -2086,6 +2089,9 @@ extern "C" int mkv_linear_attn_prefill(
   const Prefill p =
       plan_prefill(num_tokens, batch, max_seqlen, num_k_heads, num_v_heads, beta != nullptr,
                    z != nullptr);
+  // (the walk's grids stay within theirs: whole sequences have at most 2^31 threads)
+  MKV_REQUIRE((double)p.ids * kPrepThreads < kMostThreads, MKV_E_UNSUPPORTED, "%s: too many rows",
+              fn);
   MKV_REQUIRE(cu_seqlens && workspace && aligned4(cu_seqlens), MKV_E_INVALID, "%s: null pointer",
               fn);
   MKV_REQUIRE(aligned16(workspace) && workspace_bytes >= p.total, MKV_E_INVALID,

@@ -158,3 +158,13 @@ def test_workspace_of_many_heads_on_one_key_head():
         for delta in (0, 1):
             assert 1 << 30 < size(tokens, 2, tokens, 1, 64, delta) < 3 << 30
     assert size(32768, 8, 4096, 2, 8, 1) < 1 << 29
+
+
+def test_rows_of_one_head_that_a_launch_does_not_take():
+    """2^29 rows of one head are 2^23 chunks of 512 threads: as many as a grid dimension
+    has; a little less passes (the next check speaks)."""
+    one = dict(hk=1, hv=1, qs=256, ks=256, vs=256, gs=4, bs=4, longest=0, wsb=8)
+    rc, msg = prefill(tokens=1 << 29, **one)
+    assert rc == -3 and "too many rows" in msg
+    rc, msg = prefill(tokens=(1 << 29) - 512, batch=7, **one)
+    assert rc == -1 and "workspace" in msg
