@@ -3,6 +3,7 @@ and the slots of empty ones stay as they are (bounds in tests/linear_util.py).""
 import pytest
 import torch
 
+from muserve_amd import _lib
 from muserve_amd.kernels import linear_attention as la
 from muserve_amd.state_pool import StatePool
 from oracle import linear as ref
@@ -140,3 +141,63 @@ def test_prompts_of_a_step_behind_its_decode_rows():
     assert ((a - b).abs() <= 2.0 ** -7 * b.norm(dim=-1, keepdim=True)).all()
     err = (pools[0].state - pools[1].state).double().flatten(-2).norm(dim=-1)
     assert (err <= 1e-5 * pools[1].state.double().flatten(-2).norm(dim=-1)).all()
+
+
+@pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("longest", [8, 70, 3000])
+def test_bad_slots_and_offsets_in_every_form(longest, delta):
+    """Token by token, in chunks and in segments (and 70 sequences of each)."""
+    case(f"linear attention, bad slots and offsets, up to {longest} tokens, delta {delta}")
+    for n in (2, 70):
+        lens = [longest, 5] + [3] * (n - 2)
+        total = sum(lens) + 6
+        x = lu.on_gpu(lu.inputs(140, total, 1, 2, slots=n, delta=delta))
+        cu = [1]
+        for m in lens:
+            cu.append(cu[-1] + m)
+        kept = torch.randn(total, 2, D, device=DEV).bfloat16()
+        for bad in (-1, n, 2 ** 31 - 1):
+            state, out = x["state"].clone(), kept.clone()
+            prompt(x, ints([bad, *range(1, n)]), ints(cu), state, out=out, max_seqlen=longest)
+            with pytest.raises(_lib.MkvDeviceError, match="state-pool slot"):
+                la.check_errors(DEV)
+            assert not out[1:1 + longest].any() and out[1 + longest:cu[-1]].any()
+            assert torch.equal(out[:1], kept[:1]) and torch.equal(out[cu[-1]:], kept[cu[-1]:])
+            assert torch.equal(state[0], x["state"][0]) and not torch.equal(state[1], x["state"][1])
+        for at, value in ((0, -1), (1, cu[2] + 1), (n, total + 1), (n // 2, 2 ** 31 - 1)):
+            state, out, wrong = x["state"].clone(), kept.clone(), list(cu)
+            wrong[at] = value
+            prompt(x, ints(range(n)), ints(wrong), state, out=out, max_seqlen=longest)
+            with pytest.raises(_lib.MkvDeviceError, match="inconsistent offsets"):
+                la.check_errors(DEV)
+            assert torch.equal(out, kept) and torch.equal(state, x["state"])
+
+
+@pytest.mark.parametrize("call", ["linear_attn_decode", "linear_attn_prefill", "conv_prefill"])
+def test_repeated_slots_through_the_calls(call):
+    """Each in-place call reports a repeated slot where the pool checks (what the slots
+    hold then is not said)."""
+    case(f"StatePool.{call} with a repeated slot under the duplicate check")
+    hk, hv, C = 2, 8, 64
+    pool = StatePool(num_layers=1, num_slots=4, conv_shape=(C, 4), device=DEV)
+    pool.check_unique = True
+    x = lu.on_gpu(lu.inputs(2, 4, hk, hv))
+    rows = torch.randn(4, C, device=DEV).bfloat16()
+    w = torch.randn(C, 4, device=DEV).bfloat16()
+
+    def run(slots):
+        at = ints(slots)
+        if call == "conv_prefill":
+            pool.conv_prefill(0, at, rows, w, ints([0, 3, 4]))
+        elif call == "linear_attn_prefill":
+            pool.linear_attn_prefill(0, at, *lu.split(x["mixed"], hk, hv), x["g"], x["beta"],
+                                     ints([0, 3, 4]))
+        else:
+            pool.linear_attn_decode(0, at, *lu.split(x["mixed"][:2], hk, hv), x["g"][:2],
+                                    x["beta"][:2])
+        pool.check_errors()
+
+    run([1, 3])
+    with pytest.raises(_lib.MkvDeviceError, match="more than once"):
+        run([2, 2])
+    run([2, 0])
