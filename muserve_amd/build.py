@@ -43,7 +43,8 @@ HIP_FLAGS = [
 
 # mkv_linear: results of matrix instructions in ordinary registers (its loops do
 # vector arithmetic on all of them; through the accumulator file each value
-# costs two moves).
+# costs two moves). An option of the compiler's insides: one that does not know it
+# builds without, as right and slower.
 EXTRA_FLAGS = {"mkv_linear": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
@@ -66,6 +67,18 @@ def _run(cmd: list[str]) -> None:
         sys.stderr.write("\n".join(noise) + "\n")
 
 
+def compile_source(cc: str, source: Path, obj: Path, extra: list[str]) -> None:
+    """One source with ``extra`` flags, or without where the compiler knows none of them."""
+    cmd = [cc, *HIP_FLAGS, "-c", str(source), "-o", str(obj)]
+    try:
+        _run([*cmd, *extra])
+    except RuntimeError as e:
+        if not extra or "Unknown command line argument" not in str(e):
+            raise
+        sys.stderr.write(f"{source.name}: built without {' '.join(extra)}\n")
+        _run(cmd)
+
+
 def build(verbose: bool = False, jobs: int | None = None) -> Path:
     """Compile all HIP sources and link the library; returns its path."""
     cc = hipcc()
@@ -74,14 +87,13 @@ def build(verbose: bool = False, jobs: int | None = None) -> Path:
     if not sources:
         raise RuntimeError(f"no HIP sources under {CSRC}")
     objs = [BUILD / (s.stem + ".o") for s in sources]
-    cmds = [[cc, *HIP_FLAGS, *EXTRA_FLAGS.get(s.stem, []), "-c", str(s), "-o", str(o)]
-            for s, o in zip(sources, objs)]
-    jobs = jobs or min(len(cmds), os.cpu_count() or 4, 8)
+    jobs = jobs or min(len(sources), os.cpu_count() or 4, 8)
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
-        for cmd, fut in [(c, ex.submit(_run, c)) for c in cmds]:
-            if verbose:
-                print(" ".join(cmd))
+        for source, fut in [(s, ex.submit(compile_source, cc, s, o, EXTRA_FLAGS.get(s.stem, [])))
+                            for s, o in zip(sources, objs)]:
             fut.result()
+            if verbose:
+                print(f"compiled {source.name}")
     tmp = LIB_PATH.with_suffix(".so.tmp")
     _run([cc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(tmp), *map(str, objs)])
     os.replace(tmp, LIB_PATH)
