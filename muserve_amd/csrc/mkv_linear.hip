@@ -1878,30 +1878,32 @@ struct Prefill {
 };
 
 // What a pass takes (us on MI355X, fitted to 12 shapes of 1 to 32 sequences of
-// 300 to 32768 tokens under all choices, 5 % off on average): so many a chunk
-// where up to half the CUs have a workgroup, and where all have; a join so many
-// a segment.
+// 300 to 32768 tokens under all choices, 4 % off on average): so many a chunk
+// where up to half the CUs have a workgroup, and where all have (normed8: by 8 waves
+// with the output norm); a join so many a segment.
 struct ChunkCosts {
-  float rows4[2], rows8[2], ends8[2], ends16[2], join;
+  float rows4[2], rows8[2], normed8[2], ends8[2], ends16[2], join;
 };
-constexpr ChunkCosts kDeltaCosts = {{2.7f, 3.2f}, {3.4f, 4.9f}, {2.4f, 3.0f}, {3.8f, 5.5f}, 1.6f};
-constexpr ChunkCosts kDecayCosts = {{1.9f, 2.1f}, {2.4f, 2.8f}, {1.4f, 2.5f}, {1.4f, 2.5f}, 0.4f};
-constexpr float kPassStart = 7.f;  // a pass's launch, its first loads and its last stores
+constexpr ChunkCosts kDeltaCosts = {{3.2f, 3.6f}, {3.9f, 5.2f}, {5.1f, 6.7f},
+                                    {2.6f, 3.2f}, {4.2f, 5.7f}, 1.6f};
+constexpr ChunkCosts kDecayCosts = {{2.5f, 2.6f}, {3.0f, 3.3f}, {4.2f, 4.6f},
+                                    {1.6f, 2.5f}, {1.6f, 2.5f}, 0.35f};
+constexpr float kPassStart = 5.5f;  // a pass's launch, its first loads and its last stores
 
 // A pass of `wgs` workgroups of at most `chunks` chunks each, one per CU at a time.
-float pass_time(const float (&cost)[2], double wgs, double chunks, int cus) {
+float pass_time(const float (&cost)[2], double wgs, double chunks, int cus, double uneven = 1.) {
   const double half = cus / 2.0, load = wgs <= half ? 0. : wgs >= cus ? 1. : (wgs - half) / half;
-  const double rounds = wgs <= cus ? 1. : ceil(wgs / cus);
+  const double rounds = wgs * uneven <= cus ? 1. : ceil(wgs * uneven / cus);
   return (float)(kPassStart + rounds * chunks * (cost[0] + load * (cost[1] - cost[0])));
 }
 
 // Whole sequences or segments of them, and workgroups of half a head or of one,
 // by those costs. The batch is taken as its longest sequence and others alike.
-// (us, prep and all, 8 heads: 1 x 32768 tokens whole 1507, segments of 8 chunks
-// 345, of 16 269, of 32 288; 8 x 4096 whole 242, segments of 16 chunks 232; 32 x
-// 1024 half heads 186, whole ones 145, segments of 8 chunks 227; 1 x 1024 whole
-// 70, segments of 4 chunks 64; 6 of 80 to 3000 whole 160, segments of 6 to 8
-// chunks 106 to 118.)
+// (us, prep and all, 8 heads: 1 x 32768 tokens whole 1797, segments of 8 chunks
+// 350, of 16 286, of 32 330; 8 x 4096 whole 275, segments of 16 chunks 242, with the
+// norm 399 and 260; 32 x 1024 half heads 194, whole ones 151, segments of 8 chunks
+// 249; 1 x 1024 whole 78, segments of 4 chunks 61; 6 of 80 to 3000 whole 182,
+// segments of 6 chunks 106.)
 void choose_walk(Prefill& p, int64_t tokens, int32_t n, int32_t longest, double heads, bool delta,
                  bool norm) {
   const ChunkCosts& c = delta ? kDeltaCosts : kDecayCosts;
@@ -1912,7 +1914,7 @@ void choose_walk(Prefill& p, int64_t tokens, int32_t n, int32_t longest, double 
   const double work = long_chunks + (n - 1) * rest_chunks;  // chunks of one head
   float best = 3e38f;
   for (int32_t waves = norm ? 8 : 4; waves <= 8; waves += 4) {
-    const float (&cost)[2] = waves == 4 ? c.rows4 : c.rows8;
+    const float (&cost)[2] = norm ? c.normed8 : waves == 4 ? c.rows4 : c.rows8;
     const double parts = 8.0 / waves, wgs = heads * parts * n;
     // (rounds of sequences of different lengths fill up: at least the longest one)
     const double each = wgs <= cus ? long_chunks : fmax(long_chunks, work * heads * parts / cus);
@@ -1931,12 +1933,18 @@ void choose_walk(Prefill& p, int64_t tokens, int32_t n, int32_t longest, double 
     const double of_rest = rest_chunks == long_chunks ? of_long : rest_chunks / len + .5;
     const double segs = of_long + (n - 1) * of_rest;
     const double starts = segs - n;  // segments whose end is asked for
+    // (Ids of no segment, between those of sequences that end inside one, leave the XCDs
+    // uneven loads, the more so the more of them there are: almost as many workgroups as
+    // CUs take two rounds then. 9 x 1500 tokens in segments of 8 chunks, 216 workgroups,
+    // 235 us for 158 whole; 16 x 2000 in ones of 16, 256 workgroups, 242 for 198.)
+    const double uneven = n == 1 || fmod(most, len * kChunk) == 0 ? 1. : n <= 8 ? 1.1 : 1.35;
     const float join = kPassStart + (float)of_long * c.join;
-    const float by8 = pass_time(c.ends8, heads * starts * (delta ? 2 : 1), len, cus);
-    const float by16 = pass_time(c.ends16, heads * starts, len, cus);
+    const float by8 = pass_time(c.ends8, heads * starts * (delta ? 2 : 1), len, cus, uneven);
+    const float by16 = pass_time(c.ends16, heads * starts, len, cus, uneven);
     for (int32_t waves = norm ? 8 : 4; waves <= 8; waves += 4) {
+      const float (&cost)[2] = norm ? c.normed8 : waves == 4 ? c.rows4 : c.rows8;
       const float t = join + (delta && by16 < by8 ? by16 : by8) +
-                      pass_time(waves == 4 ? c.rows4 : c.rows8, heads * (8 / waves) * segs, len, cus);
+                      pass_time(cost, heads * (8 / waves) * segs, len, cus, uneven);
       if (t < best) {
         best = t;
         p.waves = waves;
