@@ -351,9 +351,9 @@ constexpr int kLower = 6;              // operands of a 64 x 64 lower triangle
 constexpr int kTParts = 2, kPParts = 2;
 // The factors of a chunk's tokens, [64] each: of K S0^T in the right-hand side,
 // of u in the state, e^G, of the output, of v; then e^G_63, the largest factor of v,
-// and whether to walk (two words).
+// whether to walk (two words), and log2 of e^G.
 constexpr int kFactors = 2048, kFacX = 0, kFacU = 64, kFacG = 128, kFacO = 192, kFacV = 256;
-constexpr int kFacAll = 320, kFacMax = 321, kFacWalk = 322;
+constexpr int kFacAll = 320, kFacMax = 321, kFacWalk = 322, kFacLog = 384;
 constexpr int head_image(bool delta) {
   return (delta ? kTParts * kLower * kFrag : 0) + kPParts * kLower * kFrag + kFactors;
 }
@@ -375,10 +375,13 @@ constexpr float kTScale = 0x1p4f, kPScale = 0x1p6f;
 constexpr float kLittle = 0x1p-5f;
 constexpr float kLowState = 0x1p3f, kHighState = 0x1p6f, kLowValue = 0x1p4f, kHighValue = 0x1p8f;
 constexpr int kNearState = 4, kNearValue = 6;
-// Too coarse is what a chunk's right-hand sides hold less than so much of the largest
-// of them in 4 tokens in a row, where the state is left below kLittle of these; and a
-// state that is left below kLeastState of itself and not below that.
-constexpr float kLeastQuad = 0x1p-13f, kLeastState = 0x1p-10f;
+// Too coarse is what the values of 4 tokens in a row do to a dim in such a chunk, if it
+// is less than kLeastQuad of its largest right-hand side and nothing larger of what was
+// before is left by then, or there are kManyQuads of them (the few others stand out);
+// and all it does, where the state is left below kLeastState of itself, and the values
+// are below kLeastValue of it.
+constexpr float kLeastQuad = 0x1p-13f, kLeastState = 0x1p-10f, kLeastValue = 0x1p-9f;
+constexpr int kManyQuads = 4;
 
 constexpr int64_t kMostStride = 1 << 24;  // 64 rows through a buffer descriptor
 
@@ -684,6 +687,7 @@ __global__ __launch_bounds__(DELTA ? 512 : 256, 4) void linear_prep_kernel(LinAr
       fac[kFacG + lane] = head * by;
       fac[kFacO + lane] = a.scale * rq / by;
       fac[kFacV + lane] = strong;
+      fac[kFacLog + lane] = (float)(gsum * 1.4426950408889634074);
       uint8_t* pimg = img + (DELTA ? kTParts * kLower * kFrag : 0) + lane * 16;
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
@@ -1153,19 +1157,25 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
     if (kAhead && (DELTA || kOut)) read_kq(0);
     // The dim's scale: by its state's largest element, or by its values' where these
     // are to make its new state or would not fit.
-    float coarse = 0.f;  // right-hand sides below it are too coarse (0: none)
+    float coarse = 0.f;  // u below it is too coarse (0: none)
+    float state_size = 0.f;
+    uint32_t least = 0;  // values (as bf16 bits) whose u may be below that
+    auto value_quad = [&](int mt) __attribute__((always_inline)) {  // of 4 tokens in a row
+      // (bf16 without its sign is ordered as an integer)
+      const u16x2 x = __builtin_elementwise_max(__builtin_bit_cast(u16x2, v[2 * mt] & 0x7fff7fffu),
+                                                __builtin_bit_cast(u16x2, v[2 * mt + 1] & 0x7fff7fffu));
+      return (uint32_t)max(x.x, x.y);
+    };
     bool large = false;  // a dim of the wave does not fit fp16
+    bool small = false;  // there are such values
     {
       float held = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         held = most_of(most_of(held, s[i][0], s[i][1]), s[i][2], s[i][3]);
-      u16x2 most = {0, 0};  // (bf16 without its sign is ordered as an integer)
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, v[i] & 0x7fff7fffu));
+      const uint32_t most = max(max(value_quad(0), value_quad(1)), max(value_quad(2), value_quad(3)));
       held = over_dim(held);
-      float dim = over_dim(bits_f32((uint32_t)max(most.x, most.y) << 16)) * (strong * f);
+      float dim = over_dim(bits_f32(most << 16)) * (strong * f);
       const bool fresh = held * decay < kLittle * dim;
       const bool by_value = fresh || !(dim < kHighValue);
       const float x = by_value ? dim : held;
@@ -1189,9 +1199,13 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
       // (M's rows are taken of what was before the segment: what a chunk's largest leave
       // in them, 2^-28 of it, is of no matter)
       if (!ident && fresh)
-        coarse = dim < kLowValue ? 3e38f : kLeastQuad * (dim + 4.f * held);
-      else if (!ident && decay < kLeastState)
+        coarse = dim < kLowValue ? 3e38f : kLeastQuad * (DELTA ? dim + 4.f * held : dim);
+      else if (!ident && decay < kLeastState && dim < kLeastValue * held && dim > 0.f)
         coarse = 3e38f;
+      if (coarse > 0.f) least = f32_bits(coarse * __builtin_amdgcn_rcpf(strong * f)) >> 16;
+      state_size = held;
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) small |= value_quad(mt) < least && value_quad(mt) != 0;
     }
     if (kAhead && (DELTA || kOut)) cut_state(0);
     if (more) load_v(ci + 1);
@@ -1250,12 +1264,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
     auto check = [&](const f32x4 (&x)[4]) __attribute__((always_inline)) {
       float most = 0.f;
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt) {  // 4 tokens in a row
-        const float quad = any_of(any_of(0.f, x[mt][0], x[mt][1]), x[mt][2], x[mt][3]);
-        big |= quad < coarse && quad > 0.f && 16 * mt + 4 * d + 4 <= len;
-        most = any_of(most, quad, quad);
-      }
-      big |= !(most < kMostRhs);
+      for (int mt = 0; mt < 4; ++mt) most = any_of(any_of(most, x[mt][0], x[mt][1]), x[mt][2], x[mt][3]);
+      big = !(most < kMostRhs);
     };
     u32x4 pf[kPParts][4], tf[8];  // operands of P and of K^T
     auto read_p = [&](int p, int ks) __attribute__((always_inline)) {
@@ -1359,7 +1369,42 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
       }
       big |= !(most < kMostPart);
     }
-    if (__builtin_expect(walk != 0 || large || __builtin_amdgcn_ballot_w64(big) != 0, 0)) {
+    bool by_token = walk != 0 || large || __builtin_amdgcn_ballot_w64(big) != 0;
+    if (__builtin_expect(!by_token && __builtin_amdgcn_ballot_w64(small) != 0, 0)) {
+      // log2 of what is left at a token of all before it, and of the state: of the largest
+      // of log2 |u_j| - log2 e^G_j, and then times e^G of the token
+      const float scale = DELTA ? kTScale : 1.f;
+      const float limit = __builtin_amdgcn_logf(coarse * scale);
+      float before = __builtin_amdgcn_logf(state_size * scale);
+      int32_t quads = 0;
+      bool lost = false;
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        const f32x4 gl = lds_ldf4(fac + (kFacLog + 16 * mt) * 4);
+        float own = -3e38f, quad = -3e38f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float x = __builtin_amdgcn_logf(fabsf(u[mt][r]));
+          quad = fmaxf(quad, x);
+          own = fmaxf(own, x - gl[r]);
+        }
+        float left = before;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float other = __shfl(own, n + 16 * k);
+          left = k < d ? fmaxf(left, other) : left;
+          before = fmaxf(before, other);
+        }
+        if (value_quad(mt) < least && value_quad(mt) != 0 && 16 * mt + 4 * d + 4 <= len) {
+          ++quads;
+          lost |= fmaxf(quad, left + gl[0]) < limit;
+        }
+      }
+      quads = over_rows(quads, [](int32_t y, int32_t z) { return y + z; });
+      lost |= quads >= kManyQuads;
+      by_token = __builtin_amdgcn_ballot_w64(lost) != 0;
+    }
+    if (__builtin_expect(by_token, 0)) {
       // token by token: sums over keys in the lane's registers and the 4 lanes of its value dim
       auto over_keys = [&](float x) __attribute__((always_inline)) {
         x += __shfl_xor(x, 16);
