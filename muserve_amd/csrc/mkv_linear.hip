@@ -67,13 +67,15 @@ __device__ __forceinline__ void load_gates(const LinArgs& a, int64_t token, int3
 }
 
 // 4 consecutive bf16
-__device__ __forceinline__ void load4(const uint8_t* p, float (&x)[4]) {
-  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-  const u32x2 w = *(const u32x2*)p;
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void unpack4(u32x2 w, float (&x)[4]) {
   x[0] = bits_f32(w.x << 16);
   x[1] = bits_f32(w.x & 0xffff0000u);
   x[2] = bits_f32(w.y << 16);
   x[3] = bits_f32(w.y & 0xffff0000u);
+}
+__device__ __forceinline__ void load4(const uint8_t* p, float (&x)[4]) {
+  unpack4(*(const u32x2*)p, x);
 }
 
 // The recurrence over a few tokens with a head's state in registers: a row of
@@ -332,7 +334,6 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((__vector_size__(4 * sizeof(float)))) float f32x4;
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 typedef __attribute__((address_space(3))) u32x2 lds_u32x2;
@@ -1405,44 +1406,59 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
       by_token = __builtin_amdgcn_ballot_w64(lost) != 0;
     }
     if (__builtin_expect(by_token, 0)) {
-      // token by token: sums over keys in the lane's registers and the 4 lanes of its value dim
+      // token by token: sums over keys in the lane's registers and the 4 lanes of its value
+      // dim. Lane i has token i's gates, and the next token's rows load beside this one's
+      // sums: 0.7 us a token, 1.3 with all of it in line.
       auto over_keys = [&](float x) __attribute__((always_inline)) {
-        x += __shfl_xor(x, 16);
-        x += __shfl_xor(x, 32);
-        return x;
+        return over_rows(x, [](float y, float z) { return y + z; });
       };
-#pragma unroll 1
-      for (int32_t t = 0; t < len; ++t) {
+      float g = 0.f, beta = 0.f;
+      if (lane < len) load_gates(a, t0 + lane, h, g, beta);
+      const uint32_t decays = f32_bits(expf(g)), betas = f32_bits(beta);
+      u32x2 kw[8], qw[8];
+      float vw = 0.f;
+      auto fetch = [&](int32_t t) __attribute__((always_inline)) {
         const int64_t token = t0 + t;
         const uint8_t* kp = a.k + token * a.k_stride + kh * (kDim * 2) + d * 8;
         const uint8_t* qp = a.q + token * a.q_stride + kh * (kDim * 2) + d * 8;
-        float kx[8][4], kk = 0.f, qq = 0.f, kq = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          float qx[4];
-          load4(kp + 32 * i, kx[i]);
-          if (kOut) load4(qp + 32 * i, qx);
+          kw[i] = *(const u32x2*)(kp + 32 * i);
+          if (kOut) qw[i] = *(const u32x2*)(qp + 32 * i);
+        }
+        if (!ident) vw = bf16_at(a.v + token * a.v_stride + (h * kDim + d0 + n) * 2);
+      };
+      fetch(0);
+#pragma unroll 1
+      for (int32_t t = 0; t < len; ++t) {
+        float kx[8][4], qx[8][4], kk = 0.f, qq = 0.f, kq = 0.f, x = 0.f, y = 0.f;
+        const float vt = f * vw;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          unpack4(kw[i], kx[i]);
+          if (kOut) unpack4(qw[i], qx[i]);
+        }
+        if (t + 1 < len) fetch(t + 1);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             kk = fmaf(kx[i][r], kx[i][r], kk);
             x = fmaf(s[i][r], kx[i][r], x);
             if (kOut) {
-              qq = fmaf(qx[r], qx[r], qq);
-              kq = fmaf(kx[i][r], qx[r], kq);
-              y = fmaf(s[i][r], qx[r], y);
+              qq = fmaf(qx[i][r], qx[i][r], qq);
+              kq = fmaf(kx[i][r], qx[i][r], kq);
+              y = fmaf(s[i][r], qx[i][r], y);
             }
           }
-        }
-        float rk = 1.f, rq = 1.f, g, beta;
+        float rk = 1.f, rq = 1.f;
         if (a.qk_norm) {
           rk = 1.f / sqrtf(over_keys(kk) + kL2Eps);
           if (kOut) rq = 1.f / sqrtf(over_keys(qq) + kL2Eps);
         }
-        load_gates(a, token, h, g, beta);
-        const float e = expf(g);
-        const float vt =
-            ident ? 0.f : f * bf16_at(a.v + token * a.v_stride + (h * kDim + d0 + n) * 2);
-        const float u = DELTA ? beta * (vt - e * rk * over_keys(x)) : vt;
+        const float e = bits_f32(__builtin_amdgcn_readlane(decays, t));
+        const float b = bits_f32(__builtin_amdgcn_readlane(betas, t));
+        const float u = DELTA ? b * (vt - e * rk * over_keys(x)) : vt;
         if (kOut) {
           const float out = a.scale * inv_f * (e * rq * over_keys(y) + u * (over_keys(kq) * rk * rq));
           if (NORM) {
@@ -1450,7 +1466,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
             for (int i = 0; i < 16; ++i)
               if (16 * (i >> 2) + 4 * d + (i & 3) == t) held_o[i >> 2][i & 3] = out;
           } else if (d == 0) {
-            *(uint16_t*)(outp + token * out_row) = f32_to_bf16_rne(out);
+            *(uint16_t*)(outp + (t0 + t) * out_row) = f32_to_bf16_rne(out);
           }
         }
 #pragma unroll
