@@ -392,9 +392,9 @@ int mkv_linear_attn_decode(void* state, int64_t pool_slots, int32_t num_k_heads,
  * batch <= 4096, num_tokens < 2^31, num_tokens * num_v_heads <= 2^30, num_tokens / 64
  * + batch < 2^23, rows of v at most 16 MiB apart (MKV_E_UNSUPPORTED).
  * Every value dim is as exact as its own size asks for (a state to 2^-21 or so of
- * what the dim holds). Within 64 rows of a sequence, where a dim's values stand
- * above others of it by up to 2^13 and decays then leave nothing of them, the
- * others are exact to 2^-28 of the larger.
+ * what the dim holds). Where decays leave nothing of a dim's larger values within 64
+ * rows of a sequence, what stays is exact to 2^-28 of these; where that is too little
+ * (values below 2^-13 of them, in 4 rows in a row) as in fp32.
  * Offsets below 0, falling or above num_tokens set MKV_DEVERR_TABLE, and the
  * call writes neither rows nor states. The workspace must be 16-byte aligned
  * and hold mkv_linear_attn_prefill_workspace_bytes (-1: bad sizes) for the

@@ -307,7 +307,8 @@ __global__ __launch_bounds__(256) void linear_scan_kernel(LinArgs a) {
 // rounded to 2^-25 of that. An fp32 operand (the state, the right-hand side, T, u, P)
 // is two fp16 parts, 22 bits; the product of two such drops the lower parts' (2^-22).
 // Sums run in fp32 in the matrix cores. So a state and an output before its rounding
-// to bf16 are within a few 2^-22 of what they are sums of. (With one part of the
+// to bf16 are within a few 2^-22 of what they are sums of (600 tokens: states 1.4e-7
+// from float64 in the norm, 1.0e-7 token by token; outputs 1.66e-3 both). (With one part of the
 // state, P and u in the outputs these were 2^-12 of their terms off, which shows where
 // terms cancel; 28 matrix instructions of 132 a chunk, 3 to 6 % of a call.) Three bf16
 // parts were as exact as fp32, but take 182 matrix and 630 vector instructions a chunk.
@@ -317,11 +318,12 @@ __global__ __launch_bounds__(256) void linear_scan_kernel(LinArgs a) {
 // with another) is kept times a power of two f of its own, and its values go in times f
 // too. Before a chunk f goes by the dim's state, or by its values where these make the
 // dim's new state, as the chunk's decays leave little of the old: the step is then 2^-28
-// of them or less. What is left are the tokens of a dim in one chunk: where some stand
-// far above the rest, and later a strong decay leaves nothing of them, the rest is exact
-// to 2^-28 of the larger only. Where 4 tokens in a row hold less than 2^-13 of the
-// largest, or the state is left below 2^-10 of itself with no values to match, the chunk
-// is walked token by token.
+// of them or less. What is left are the tokens of a dim in one chunk. Where some stand
+// far above the rest, and decays leave nothing of them, the rest is exact to 2^-28 of
+// the larger only; where that is too little (values of 4 tokens in a row below 2^-13 of
+// it), the chunk is walked token by token. (One f for a wave's 16 dims left a dim of
+// 2^-20 of the largest without a digit, and f by the state alone the values behind a
+// forgotten state of 2^20 of them. f by dim and chunk costs 2 to 6 % of a call.)
 //
 // The rows (tokens) of a chunk mix also through zeros. So that what is out of the
 // ordinary in one token (infinities, NaN) reaches only the tokens after it, such a
@@ -500,7 +502,7 @@ __device__ __forceinline__ bool huge(u32x4 w) {  // any of 8 bf16
 // 16 x 16 blocks in LDS (row-major, 16-byte chunks XORed by row / 4) and inverts
 // by blocks: the diagonal ones by forward substitution, a lane per column, the
 // rest in fp32 matrix instructions (16x16x4). Bound by the latency of these
-// chains: 512 chunks of 8 heads take 43 us, a lone one 13 (of which 6 until the
+// chains: 512 chunks of 8 heads take 45 us, a lone one 13 (of which 6 until the
 // rows are staged, 6.5 A and T); with one wave for both parts of a head (2 waves
 // per SIMD, not 4) 48 and 17. K's rows all in registers would spill (70 us).
 constexpr int kRowB = 272;  // bytes of a staged row: 256 and a pad against bank conflicts
@@ -866,10 +868,11 @@ enum { kWhole = 0, kEnds = 1, kRows = 2 };
 // 16x16x32 (lane (n, d): value dim n, keys 16 x + 4 d + r), which are also the B
 // operands of K S0^T and Q S0^T. The images of a chunk go straight into LDS,
 // shared by the waves, while the chunk before it is computed: two buffers, one
-// barrier a chunk. Bound by instruction issue: with 4 waves a chunk takes 3.05 us
-// (8 x 4096 tokens, 8 heads, on 128 CUs: 199 us) for 578 vector, 104 matrix and
-// 88 LDS instructions of a wave alone on its SIMD; with 8 waves 3.8, with 16 (no
-// outputs, 128 value dims and 128 rows of M) 5.8.
+// barrier a chunk. Bound by instruction issue: with 4 waves a chunk takes 3.6 us
+// (8 x 4096 tokens, 8 heads, whole on 128 CUs: 230 us), a wave alone on its SIMD; with
+// 8 waves 5.6 (32768 tokens in segments of 16 chunks: 95 us) for 682 vector, 132 matrix
+// and 95 LDS instructions a wave, with the output norm 7.1 and 972 vector, with 16
+// waves (no outputs, 128 value dims and 128 rows of M) 6.2.
 template <int WAVES, bool DELTA, int MODE, bool NORM = false>
 __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(LinArgs a, ChunkArgs c) {
   constexpr bool kOut = MODE != kEnds;
@@ -1378,7 +1381,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
       const float limit = __builtin_amdgcn_logf(coarse * scale);
       float before = __builtin_amdgcn_logf(state_size * scale);
       int32_t quads = 0;
-      bool lost = false;
+      bool lost = false, last = false;  // (of a sequence's last 1 to 3 tokens)
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
         const f32x4 gl = lds_ldf4(fac + (kFacLog + 16 * mt) * 4);
@@ -1396,14 +1399,21 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
           left = k < d ? fmaxf(left, other) : left;
           before = fmaxf(before, other);
         }
-        if (value_quad(mt) < least && value_quad(mt) != 0 && 16 * mt + 4 * d + 4 <= len) {
-          ++quads;
-          lost |= fmaxf(quad, left + gl[0]) < limit;
+        if (value_quad(mt) < least && value_quad(mt) != 0) {
+          const bool gone = fmaxf(quad, left + gl[0]) < limit;
+          if (16 * mt + 4 * d + 4 <= len) {
+            ++quads;
+            lost |= gone;
+          } else {
+            last |= gone;
+          }
         }
       }
       quads = over_rows(quads, [](int32_t y, int32_t z) { return y + z; });
       lost |= quads >= kManyQuads;
-      by_token = __builtin_amdgcn_ballot_w64(lost) != 0;
+      // (few tokens are small by chance; not in half of the dims)
+      by_token = __builtin_amdgcn_ballot_w64(lost) != 0 ||
+                 __builtin_popcountll(__builtin_amdgcn_ballot_w64(last)) >= 8;
     }
     if (__builtin_expect(by_token, 0)) {
       // token by token: sums over keys in the lane's registers and the 4 lanes of its value
@@ -1914,13 +1924,13 @@ namespace {
 
 constexpr int64_t kLeastBytes = 16;  // of a workspace, so that no call goes without one
 // Images of one launch at most: more key heads, or value heads of one, are run in turn
-// in the same space, which leaves CUs idle (64 heads, 32768 tokens, 1 GiB of images:
-// 1034 us at once, 1411 in two launches, 1544 in three). One value head at least: 74 KiB
-// for 64 tokens.
+// in the same space, which leaves CUs idle (16/64 heads, 32768 tokens, 1.2 GiB of
+// images: 1723 us at once; in launches of 13 and 3 key heads 2813, of 6, 6 and 4 2010).
+// One value head at least: 74 KiB for 64 tokens.
 constexpr int64_t kImageBytes = 2048ll << 20;
 // Up to so many tokens per sequence are walked one by one (8 heads; token by
-// token, in chunks: 1 sequence of 8 tokens 15 us, 20; 32 of 8 23, 29; 64 of 8
-// 37, 44; of 12 51, 44; 256 of 4 77, 121; of 8 123, 121).
+// token, in chunks: 1 sequence of 8 tokens 15 us, 15; 32 of 8 23, 29; 64 of 8
+// 37, 45; of 12 51, 44; 256 of 4 73, 121; of 8 113, 122; with the norm 2 to 12 more).
 constexpr int32_t kScanTokens = 8;
 
 constexpr double kMostThreads = 4294967296.;  // of a grid dimension, less than this

@@ -167,3 +167,19 @@ def test_outputs_that_cancel(of, delta):
 def test_outputs_by_value_dim(T, how):
     case(f"linear attention, bounds by value dim, {T} tokens, {how}")
     check(lu.inputs(82 + T, T, 2, 4, **how), T)
+
+
+@pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("T", [17, 30, 66, 131])
+def test_small_values_at_the_end(T, delta):
+    """The last one to three tokens of 2^-20 of the others, behind a decay that leaves
+    nothing of those."""
+    case(f"linear attention, small values at the end of {T} tokens, delta {delta}")
+    x = lu.inputs(93, T, 2, 4, raw=False, delta=delta)
+    last = T - T % 4
+    assert 0 < T - last < 4
+    _, _, v = lu.split(x["mixed"], 2, 4)
+    v[last:] *= 2.0 ** -20
+    x["g"][last] = -45.0
+    x["state"] *= 0.1
+    check(x, T)
