@@ -1381,7 +1381,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
       const float limit = __builtin_amdgcn_logf(coarse * scale);
       float before = __builtin_amdgcn_logf(state_size * scale);
       int32_t quads = 0;
-      bool lost = false, last = false;  // (of a sequence's last 1 to 3 tokens)
+      bool lost = false, lost_end = false;  // (the latter of a sequence's last 1 to 3 tokens)
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
         const f32x4 gl = lds_ldf4(fac + (kFacLog + 16 * mt) * 4);
@@ -1405,7 +1405,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
             ++quads;
             lost |= gone;
           } else {
-            last |= gone;
+            lost_end |= gone;
           }
         }
       }
@@ -1413,7 +1413,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_chunk_kernel(Lin
       lost |= quads >= kManyQuads;
       // (few tokens are small by chance; not in half of the dims)
       by_token = __builtin_amdgcn_ballot_w64(lost) != 0 ||
-                 __builtin_popcountll(__builtin_amdgcn_ballot_w64(last)) >= 8;
+                 __builtin_popcountll(__builtin_amdgcn_ballot_w64(lost_end)) >= 8;
     }
     if (__builtin_expect(by_token, 0)) {
       // token by token: sums over keys in the lane's registers and the 4 lanes of its value
