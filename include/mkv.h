@@ -18,6 +18,9 @@
  *               — the reference layout of muserve/kv_cache.py:4-10,45-49; a
  *               (layer, K|V) plane is an array of `num_pages*16` token rows.
  *   fp8 scales  [layers, 2, num_pages, 16, heads] float32, one per (token, head).
+ *   4-bit pool  [layers, 2, num_pages, 16, heads, 136] bytes: a (token, head) row is
+ *               128 bytes of e2m1 codes (dim 2i in a byte's low half, 2i + 1 in its
+ *               high half), then 8 e8m0 scales, one for every 32 dims.
  *   block table [batch, table_width] int32 page ids, seq_lens [batch] int32.
  *
  * The names follow the reference's domain: a "page" is one 16-token block of
@@ -239,6 +242,85 @@ int mkv_gather_dequant_fp8(const void* k_pool, const void* v_pool,
                            void* k_out, void* v_out, int64_t out_layer_stride,
                            int32_t num_layers, int32_t num_heads,
                            int32_t head_dim, int32_t* err, void* stream);
+
+/* ---- 4-bit quantize-on-append / dequant-gather --------------------------- */
+
+/*
+ * Append with quantisation to 4 bits: every 32 dims of a (token, head) row of bf16
+ * values x share a power of two
+ *   e    = the least integer with max |x_i| <= 7 * 2^e, kept in [-120, 125]
+ *   code = e2m1_rne(x_i * 2^-e), magnitudes above 6 as 6 (values 0, 0.5, 1, 1.5, 2,
+ *          3, 4, 6 and their negatives; ties to the even code)
+ * with the scale byte e + 127 behind the row's codes. A value is code * 2^e. A block
+ * with an infinity or a NaN has the scale byte 255 and codes 0, and reads back as
+ * NaN; a scale byte of 0 (a row never written) with codes 0 reads as zeros.
+ * head_dim must be 256; the source strides and the pool's address are as
+ * mkv_append_fp8's. No reference counterpart (the reference has no 4-bit cache).
+ */
+int mkv_append_fp4(void* k_pool, void* v_pool, int64_t pool_layer_stride, int64_t num_slots,
+                   const void* k_src, const void* v_src, int64_t src_layer_stride,
+                   int64_t src_token_stride, const int64_t* slot_mapping, int64_t num_tokens,
+                   int32_t num_layers, int32_t num_heads, int32_t head_dim, int32_t* err,
+                   void* stream);
+
+/*
+ * Dequant-gather of a 4-bit pool: as mkv_gather_dequant_fp8, for any number of heads.
+ * Every finite value of the pool is a bf16 value, so nothing is rounded.
+ */
+int mkv_gather_dequant_fp4(const void* k_pool, const void* v_pool, int64_t pool_layer_stride,
+                           int64_t num_pages, const int32_t* block_tables, int64_t table_stride,
+                           int32_t table_width, const int32_t* seq_lens, const int32_t* starts,
+                           int32_t batch, int64_t out_len, const int64_t* out_offsets, void* k_out,
+                           void* v_out, int64_t out_layer_stride, int32_t num_layers,
+                           int32_t num_heads, int32_t head_dim, int32_t* err, void* stream);
+
+/* ---- q / k norm and rotation ------------------------------------------------ */
+
+/*
+ * The RMS norm of each query and key head and the rotation by its position, in one
+ * pass: what the attention layer does with its projections before the pool
+ * (muserve/model/qwen35_layer_v2.py:458-469). For a row x of head_dim values
+ *   y = x / sqrt(mean(x^2) + eps) * w            (w + 1 with zero_centered; y = x
+ *                                                  where the weight is null)
+ * and of its first rotary_dim dims, with the angle a_i = position * inv_freq[i] and
+ * c = rope_scale * cos a_i, s = rope_scale * sin a_i,
+ *   (y_i, y_{i + rotary_dim/2}) -> (y_i c - y_{i+rotary_dim/2} s,
+ *                                   y_{i+rotary_dim/2} c + y_i s)
+ * (interleaved: the same of y_{2i}, y_{2i+1}). Norm, rotation and products are fp32,
+ * the angle fp64; one rounding to the output's type.
+ *
+ * q and k are [num_tokens, heads, head_dim] in bf16 (fp16 with `fp16`) at any token
+ * and head strides (bytes, multiples of 16), q_out and k_out contiguous; an output may
+ * be its input where that is contiguous. head_dim is 64, 128 or 256, rotary_dim a
+ * multiple of 16 up to it. positions are int64, inv_freq [rotary_dim / 2] fp32 or
+ * (freq_fp64) fp64. weight_type: 0 no weights, 1 bf16, 2 fp16, 3 fp32.
+ */
+int mkv_qk_norm_rope(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                     int64_t k_token_stride, int64_t k_head_stride, int64_t num_tokens,
+                     int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t fp16,
+                     const int64_t* positions, const void* inv_freq, int32_t freq_fp64,
+                     int32_t rotary_dim, int32_t interleaved, float rope_scale,
+                     const void* q_weight, const void* k_weight, int32_t weight_type,
+                     int32_t zero_centered, float eps, void* q_out, void* k_out, void* stream);
+
+/*
+ * The same, with K and V going to the pool's rows at slot_mapping (as an append: -1
+ * skips a token's K and V, its queries are still written; slots unique) in place of a
+ * k_out. pool_type 1: rows of the inputs' type; 2: fp8 codes with scale planes, as
+ * mkv_append_fp8 writes them; 3: 4-bit rows, as mkv_append_fp4's (both of bf16 heads of
+ * 256, quantised from the rotated row rounded to bf16). The planes are one layer's.
+ */
+int mkv_append_rope(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                    int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                    int64_t v_token_stride, int64_t v_head_stride, int64_t num_tokens,
+                    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t fp16,
+                    const int64_t* positions, const void* inv_freq, int32_t freq_fp64,
+                    int32_t rotary_dim, int32_t interleaved, float rope_scale,
+                    const void* q_weight, const void* k_weight, int32_t weight_type,
+                    int32_t zero_centered, float eps, void* q_out, int32_t pool_type,
+                    void* k_pool, void* v_pool, float* k_scale, float* v_scale,
+                    int64_t num_slots, const int64_t* slot_mapping, int32_t* err, void* stream);
+
 
 /* ---- page copies (copy-on-write) ---------------------------------------- */
 
@@ -735,6 +817,26 @@ int mkv_decode_attention_fp8(const void* q, const void* k_codes, const void* v_c
                              int32_t max_seq_len, float softmax_scale, void* out,
                              void* workspace, int64_t workspace_bytes, int32_t* err,
                              void* stream);
+
+/*
+ * The same over a 4-bit pool (mkv_append_fp4's rows), dequantised in registers: a
+ * cached value is code * 2^e, exactly. q and out are bf16; 1 to 8 query heads per KV
+ * head, head_dim 256, batch x num_kv_heads at most 4096. Softmax in fp32; a weight
+ * enters the product with V with 16 significant bits. The workspace (16-byte aligned)
+ * is mkv_decode_attention_fp4_workspace_bytes (-1 for an unsupported shape); error bits
+ * as mkv_decode_attention_bf16. Page ids below shared_pages are read through the
+ * caches.
+ */
+int mkv_decode_attention_fp4(const void* q, const void* k_cache, const void* v_cache,
+                             int64_t num_pages, int64_t shared_pages, int32_t num_kv_heads,
+                             int32_t num_q_heads, int32_t head_dim, const int32_t* page_table,
+                             int64_t table_stride, int32_t table_width, const int32_t* seq_lens,
+                             int32_t batch, int32_t max_seq_len, float softmax_scale, void* out,
+                             void* workspace, int64_t workspace_bytes, int32_t* err,
+                             void* stream);
+int64_t mkv_decode_attention_fp4_workspace_bytes(int32_t batch, int32_t num_kv_heads,
+                                                 int32_t num_q_heads);
+
 
 /*
  * Decode attention over contiguous per-sequence caches instead of the pool:

@@ -63,6 +63,14 @@ SIGNATURES: dict[str, list] = {
                        _I32, _I32, _P, _P],
     "mkv_gather_dequant_fp8": [_P, _P, _P, _P, _I64, _I64, _I64, _P, _I64, _I32, _P, _P, _I32,
                                _I64, _P, _P, _P, _I64, _I32, _I32, _I32, _P, _P],
+    "mkv_append_fp4": [_P, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _I64, _I32, _I32, _I32, _P, _P],
+    "mkv_gather_dequant_fp4": [_P, _P, _I64, _I64, _P, _I64, _I32, _P, _P, _I32, _I64, _P, _P, _P,
+                               _I64, _I32, _I32, _I32, _P, _P],
+    "mkv_qk_norm_rope": [_P, _I64, _I64, _P, _I64, _I64, _I64, _I32, _I32, _I32, _I32, _P, _P,
+                         _I32, _I32, _I32, _F32, _P, _P, _I32, _I32, _F32, _P, _P, _P],
+    "mkv_append_rope": [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I32, _I32, _I32,
+                        _I32, _P, _P, _I32, _I32, _I32, _F32, _P, _P, _I32, _I32, _F32, _P, _I32,
+                        _P, _P, _P, _P, _I64, _P, _P, _P],
     "mkv_copy_blocks": [_P, _I64, _I32, _I64, _I64, _P, _P, _I32, _P, _P],
     "mkv_state_gather": [_P, _I64, _P, _P, _I64, _P, _I64, _P, _I32, _P, _P],
     "mkv_state_scatter": [_P, _I64, _P, _P, _I64, _P, _I64, _P, _I32, _P, _P],
@@ -111,6 +119,9 @@ SIGNATURES: dict[str, list] = {
                                  _I32, _I32, _F32, _P, _P, _I64, _P, _P],
     "mkv_decode_attention_fp8": [_P, _P, _P, _P, _P, _I64, _I64, _I32, _I32, _I32, _P, _I64, _I32,
                                  _P, _I32, _I32, _F32, _P, _P, _I64, _P, _P],
+    "mkv_decode_attention_fp4": [_P, _P, _P, _I64, _I64, _I32, _I32, _I32, _P, _I64, _I32, _P,
+                                 _I32, _I32, _F32, _P, _P, _I64, _P, _P],
+    "mkv_decode_attention_fp4_workspace_bytes": [_I32, _I32, _I32],
     "mkv_decode_attention_contig": [_P, _P, _P, _I32, _I32, _I32, _I32, _I64, _P, _I32, _I32, _F32,
                                     _P, _P, _I64, _P, _P],
     "mkv_probe_read_pages": [_P, _P, _I32, _I64, _P, _I64, _I32, _I32, _P, _P],
@@ -119,7 +130,8 @@ SIGNATURES: dict[str, list] = {
 }
 _INT64_RESULT = {"mkv_bm_state_bytes", "mkv_decode_attention_workspace_bytes",
                  "mkv_prefill_attention_workspace_bytes", "mkv_prefill_attention_plan_bytes",
-                 "mkv_linear_attn_prefill_workspace_bytes"}
+                 "mkv_linear_attn_prefill_workspace_bytes",
+                 "mkv_decode_attention_fp4_workspace_bytes"}
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
@@ -176,6 +188,16 @@ def call(name: str, *args) -> None:
     if rc != 0:
         msg = lib.mkv_last_error().decode(errors="replace")
         raise MkvError(f"{name} failed ({rc}): {msg}")
+
+
+def call_on(dev: torch.device, name: str, *args) -> None:
+    """``call`` on the current stream of ``dev`` (its last argument), also where
+    another device is the current one."""
+    if torch.cuda.current_device() == dev.index:
+        call(name, *args, stream_of(dev))
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args, stream_of(dev))
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -18,7 +18,7 @@
 // round to nearest even, non-saturating), v_cvt_pk_f32_fp8 and
 // v_cvt_pk_bf16_f32, each equal to torch's CPU conversion on every input
 // (mkv_check_conversions re-checks them, and the divide, on the device).
-#include "mkv_device.h"
+#include "mkv_quant.h"
 
 namespace mkv {
 namespace {
@@ -26,8 +26,6 @@ namespace {
 constexpr int kHeadDim = 256;
 constexpr int kLanesPerRow = 16;                         // lanes per quantisation row
 constexpr int kRowsPerWg = kThreads / kLanesPerRow;      // 16 rows per workgroup
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 // Two fp8 codes (bytes 0-1 or 2-3 of word) times scale, as a packed bf16 pair.
 #define dequant2(word, high, scale)                                                       \
@@ -51,54 +49,6 @@ struct AppendFp8Args {
   uint32_t num_heads;
   int32_t* err;
 };
-
-__device__ __forceinline__ float bf16_lo(uint32_t w) { return bits_f32(w << 16); }
-__device__ __forceinline__ float bf16_hi(uint32_t w) { return bits_f32(w & 0xffff0000u); }
-
-// torch.clamp(x, -448, 448): NaN passes through unchanged.
-__device__ __forceinline__ float clamp448(float x) {
-  return x < -448.0f ? -448.0f : (x > 448.0f ? 448.0f : x);
-}
-
-// Quantises one 256-value row held as 16 values per lane of a 16-lane group
-// and returns the lane's 16 codes, plus the row's scale.
-__device__ __forceinline__ u32x4 quantise_row(const u32x4 r0, const u32x4 r1, float& scale_out) {
-  const uint32_t w[8] = {r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w};
-  float x[16];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    x[2 * i] = bf16_lo(w[i]);
-    x[2 * i + 1] = bf16_hi(w[i]);
-  }
-  // absmax over the row. On |x| bit patterns integer max is float max, and
-  // any NaN (above +inf as an integer) wins, as torch's amax propagates NaN.
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const uint32_t ab = f32_bits(x[i]) & 0x7fffffffu;
-    m = ab > m ? ab : m;
-  }
-#pragma unroll
-  for (int off = kLanesPerRow / 2; off >= 1; off >>= 1) {
-    const uint32_t o = (uint32_t)__shfl_xor((int)m, off, kLanesPerRow);
-    m = o > m ? o : m;
-  }
-  const float amax = bits_f32(m);
-  const float clamped = amax < 1e-12f ? 1e-12f : amax;  // .clamp(min=1e-12); NaN stays
-  const float scale = clamped / 448.0f;
-  const float recip = 1.0f / scale;
-  float q[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) q[i] = clamp448(div_by_recip(x[i], scale, recip));
-  uint32_t c[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i], q[4 * i + 1], 0, false);
-    c[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i + 2], q[4 * i + 3], lo, true);
-  }
-  scale_out = scale;
-  return u32x4{c[0], c[1], c[2], c[3]};
-}
 
 // One 16-lane group per (token, head) row of one (layer, K|V): grid.x covers
 // the rows, grid.y is layer * 2 + K|V. The source loads do not depend on the
@@ -133,10 +83,12 @@ __global__ __launch_bounds__(kThreads) void append_fp8_kernel(AppendFp8Args a) {
     if (slot != -1 && lane == 0 && h == 0 && !is_v) raise_err(a.err, MKV_DEVERR_SLOT);
     return;
   }
-  float scale;
-  const u32x4 codes = quantise_row(r0, r1, scale);
+  const uint32_t w[8] = {r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w};
+  uint32_t c[4];
+  const float scale = quantise_fp8<kLanesPerRow, 16>(w, c);
   uint8_t* pool = (is_v ? a.v_pool : a.k_pool) + (int64_t)l * a.pool_layer_stride;
-  st_nt(pool + slot * ((int64_t)nh * kHeadDim) + (int64_t)h * kHeadDim + lane * 16, codes);
+  st_nt(pool + slot * ((int64_t)nh * kHeadDim) + (int64_t)h * kHeadDim + lane * 16,
+        u32x4{c[0], c[1], c[2], c[3]});
   if (lane == 0) {
     float* sp = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(is_v ? a.v_scale : a.k_scale) +
                                          (int64_t)l * a.scale_layer_stride);
@@ -164,7 +116,6 @@ __global__ __launch_bounds__(kDequantThreads) void gather_dequant_kernel(GatherA
   constexpr int OUT_ROW = 2 * IN_ROW;                // bf16 bytes per output row
   constexpr int ROWS = kDequantTileCodes / IN_ROW;   // rows per tile
   constexpr int WAVE_CODES = kDequantTileCodes / (kDequantThreads / 64);
-  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
   GatherTile<ROWS> t;
   t.init(a);
   if (t.row0 >= t.nvalid) return;  // padding tile: gather_pad_kernel's

@@ -356,6 +356,76 @@ def attn_decode_fp8(
                    cache_seqlens, page_table, softmax_scale, max_seqlen, out, shared_pages)
 
 
+FP4_ROW = 136  # bytes of a 4-bit row: 128 of codes, 8 scales
+
+
+@functools.lru_cache(maxsize=1024)
+def _fp4_bytes(batch: int, num_kv_heads: int, num_q_heads: int, dev: torch.device) -> int:
+    return _lib.load().mkv_decode_attention_fp4_workspace_bytes(batch, num_kv_heads, num_q_heads)
+
+
+def attn_decode_fp4(
+    q: torch.Tensor,                    # [B, 1, NUM_Q_HEADS, HEAD_DIM] bf16
+    k_cache: torch.Tensor,              # [num_pages, PAGE_SIZE, NUM_KV_HEADS, 136] uint8
+    v_cache: torch.Tensor,              # [num_pages, PAGE_SIZE, NUM_KV_HEADS, 136] uint8
+    cache_seqlens: torch.Tensor,        # [B] int32
+    page_table: torch.Tensor,           # [B, max_pages] int32
+    softmax_scale: float | None = None,
+    *,
+    max_seqlen: int | None = None,
+    out: torch.Tensor | None = None,
+    shared_pages: int = 0,
+) -> torch.Tensor:                      # [B, 1, NUM_Q_HEADS, HEAD_DIM] bf16
+    """``attn_decode`` over a 4-bit pool (``cache.get_kv_by_layer(l)`` of a
+    ``PagedKVCache`` with ``dtype=torch.float4_e2m1fn_x2``), dequantised in
+    registers: a cached value is ``code * 2**e``, exactly. 1 to 8 query heads
+    per KV head; the other arguments are ``attn_decode``'s."""
+    if page_table is None:
+        raise ValueError("attn_decode_fp4 reads the paged pool: page_table is required")
+    dev = _lib.require_gpu(q, k_cache, v_cache, cache_seqlens, page_table)
+    if k_cache.dtype != torch.uint8 or v_cache.dtype != torch.uint8:
+        raise TypeError("attn_decode_fp4 takes uint8 caches of 4-bit rows")
+    if q.dtype != torch.bfloat16:
+        raise TypeError("attn_decode_fp4 takes a bf16 query")
+    if q.dim() != 4 or k_cache.dim() != 4:
+        raise ValueError("q must be [B, 1, heads, 256], the caches [num_pages, 16, kv_heads, 136]")
+    B, one, Hq, D = q.shape
+    P, page, Hkv, row = k_cache.shape
+    if (one != 1 or page != 16 or D != HEAD_DIM or row != FP4_ROW
+            or v_cache.shape != k_cache.shape or P == 0 or Hkv == 0):
+        raise ValueError(f"unsupported shapes q {tuple(q.shape)}, cache {tuple(k_cache.shape)}")
+    if cache_seqlens.dtype != torch.int32 or page_table.dtype != torch.int32:
+        raise TypeError("cache_seqlens and page_table must be int32")
+    if cache_seqlens.shape != (B,) or page_table.dim() != 2 or page_table.shape[0] < B:
+        raise ValueError("cache_seqlens / page_table rows do not match q")
+    width = page_table.shape[1]
+    if not (q.is_contiguous() and k_cache.is_contiguous() and v_cache.is_contiguous()
+            and cache_seqlens.is_contiguous() and (width <= 1 or page_table.stride(1) == 1)):
+        raise ValueError("q, caches, cache_seqlens and page_table rows must be contiguous")
+    if shared_pages < 0:
+        raise ValueError("shared_pages must be >= 0")
+    if max_seqlen is None:
+        max_seqlen = width * 16
+    elif max_seqlen < 0:
+        raise ValueError("bad attention shape")
+    if out is None:
+        out = torch.empty_like(q)
+    elif (out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous()
+          or out.device != dev):
+        raise ValueError("out must be a contiguous tensor shaped like q")
+    scale = D ** -0.5 if softmax_scale is None else float(softmax_scale)
+    nbytes = _fp4_bytes(B, Hkv, Hq, dev)
+    if nbytes < 0:
+        raise ValueError(f"unsupported shapes q {tuple(q.shape)}, cache {tuple(k_cache.shape)} "
+                         "(1 to 8 query heads per KV head, batch x KV heads up to 4096)")
+    ws = _scratch(nbytes, dev)
+    _lib.call_on(dev, "mkv_decode_attention_fp4", q.data_ptr(), k_cache.data_ptr(),
+                 v_cache.data_ptr(), P, shared_pages, Hkv, Hq, D, page_table.data_ptr(),
+                 max(page_table.stride(0), width), width, cache_seqlens.data_ptr(), B, max_seqlen,
+                 scale, out.data_ptr(), ws.data_ptr(), nbytes, _errword(dev).ptr())
+    return out
+
+
 def _decode_contig(q, k_cache, v_cache, cache_seqlens, softmax_scale, max_seqlen, out):
     dev = _lib.require_gpu(q, k_cache, v_cache, cache_seqlens)
     B, one, Hq, D = q.shape

@@ -15,6 +15,12 @@ attribute names, allocation order and error types. New, additive APIs:
 * ``PagedKVCache.copy_pages`` — page copies for copy-on-write;
 * fp8 e4m3fn pools (``dtype=torch.float8_e4m3fn``): ``append``/``write_kv``
   quantise bf16 input per (token, head) and ``gather`` dequantises to bf16;
+* 4-bit pools (``dtype=torch.float4_e2m1fn_x2``): the same with e2m1 codes and a
+  power of two for every 32 dims. ``cache`` is then uint8
+  ``[num_layers, 2, num_pages, 16, kv_heads, 136]``: a (token, head) row of 256
+  dims is 128 bytes of codes, then its 8 scales;
+* ``PagedKVCache.append_rope`` — the q / k norm, the rotation and the append of
+  K and V in one launch (``kernels.rope``);
 * ``BlockTables`` — device-resident block tables and lengths for a batch of
   ``SequenceKVState`` with a one-launch decode step.
 """
@@ -25,13 +31,18 @@ import torch
 
 from muserve_amd import _lib
 from muserve_amd.config import HEAD_DIM, KV_DTYPE, KV_PAGE_SIZE, NUM_KV_HEADS, NUM_LAYERS, TP_SIZE
+from muserve_amd.kernels import rope
 
 _DTYPE_MAP = {
     "float16": torch.float16,
     "bfloat16": torch.bfloat16,
     "float8_e4m3fn": torch.float8_e4m3fn,
+    "float4_e2m1fn_x2": torch.float4_e2m1fn_x2,
 }
 _FP8 = torch.float8_e4m3fn
+_FP4 = torch.float4_e2m1fn_x2
+_FP4_DIM = 256
+_FP4_ROW = _FP4_DIM // 2 + _FP4_DIM // 32  # bytes of a (token, head): codes, scales
 _SIXTEEN_BIT = (torch.float16, torch.bfloat16)
 
 
@@ -63,8 +74,10 @@ class PagedKVCache:
         rank = get_tp_rank()
         device = torch.device(device) if device is not None else torch.device(f"cuda:{rank}")
         dtype = dtype if dtype is not None else _DTYPE_MAP[KV_DTYPE]
-        if dtype not in (*_SIXTEEN_BIT, _FP8):
+        if dtype not in (*_SIXTEEN_BIT, _FP8, _FP4):
             raise ValueError(f"unsupported KV dtype {dtype}")
+        if dtype == _FP4 and head_dim != _FP4_DIM:
+            raise ValueError(f"a 4-bit pool holds heads of {_FP4_DIM} dims, not {head_dim}")
         # KV heads split across TP ranks, at least one per rank (muserve/kv_cache.py:34)
         kv_heads_per_rank = kv_heads if kv_heads is not None else max(1, NUM_KV_HEADS // TP_SIZE)
 
@@ -81,7 +94,12 @@ class PagedKVCache:
         self.dtype = dtype
 
         self.cache = torch.zeros(num_layers, 2, num_gpu_pages, KV_PAGE_SIZE, kv_heads_per_rank,
-                                 head_dim, dtype=dtype, device=device)
+                                 *((_FP4_ROW,) if dtype == _FP4 else (head_dim,)),
+                                 dtype=torch.uint8 if dtype == _FP4 else dtype, device=device)
+        # bytes of a token's row of one plane
+        self._row_bytes = kv_heads_per_rank * self.cache.shape[-1] * self.cache.element_size()
+        # what K and V are outside the pool
+        self._value_dtype = torch.bfloat16 if dtype in (_FP8, _FP4) else dtype
         # fp8 pools carry one fp32 scale per (token, head): [L, 2, P, 16, H]
         self.scales = (torch.zeros(num_layers, 2, num_gpu_pages, KV_PAGE_SIZE, kv_heads_per_rank,
                                    dtype=torch.float32, device=device)
@@ -106,11 +124,12 @@ class PagedKVCache:
     def _estimate_pages(device, kv_heads_per_rank: int, dtype: torch.dtype,
                         num_layers: int = NUM_LAYERS, head_dim: int = HEAD_DIM) -> int:
         """Pages that fit in 90 % of free HBM (muserve/kv_cache.py:60-73), with
-        the element size taken from the dtype and fp8 scales counted."""
+        the element size taken from the dtype and the scales counted."""
         free_bytes = torch.cuda.mem_get_info(device)[0]
         available = free_bytes - int(free_bytes * 0.10)
         elem = torch.empty((), dtype=dtype).element_size()
-        per_token_head = head_dim * elem + (4 if dtype == _FP8 else 0)
+        per_token_head = (_FP4_ROW if dtype == _FP4
+                          else head_dim * elem + (4 if dtype == _FP8 else 0))
         page_bytes = num_layers * 2 * KV_PAGE_SIZE * kv_heads_per_rank * per_token_head
         return int(max(1024, available // page_bytes))
 
@@ -168,7 +187,7 @@ class PagedKVCache:
         return self.kv_heads * self.head_dim
 
     def _plane_layer_stride(self) -> int:
-        return 2 * self.num_slots * self.row_elems * self.cache.element_size()
+        return 2 * self.num_slots * self._row_bytes
 
     def _scale_layer_stride(self) -> int:
         return 2 * self.num_slots * self.kv_heads * 4
@@ -212,8 +231,8 @@ class PagedKVCache:
         offset; -1 skips a token); k/v [T, H, D] for ``layer``, or
         [L, T, H, D] for layers 0..L-1 when ``layer`` is None. Slots must be
         unique (with ``check_unique`` set, a repeat is reported as
-        MkvDeviceError at the next ``check_errors``). For an fp8 pool k/v are
-        bf16 and are quantised on the way in."""
+        MkvDeviceError at the next ``check_errors``). For an fp8 or a 4-bit
+        pool k/v are bf16 and are quantised on the way in."""
         dev = self._gpu()
         if slot_mapping.dtype != torch.int64 or slot_mapping.device != dev:
             slot_mapping = slot_mapping.to(device=dev, dtype=torch.int64)
@@ -225,17 +244,14 @@ class PagedKVCache:
             if not (0 < L <= self.num_layers):
                 raise ValueError(f"k holds {L} layers, pool has {self.num_layers}")
         else:
-            L, first = 1, int(layer)
-            if not (-self.num_layers <= first < self.num_layers):
-                raise IndexError(f"layer {layer} out of range for {self.num_layers} layers")
-            first %= self.num_layers
+            L, first = 1, self._layer(layer)
         rows = (T, self.kv_heads, self.head_dim)
         want = (L, *rows) if layer is None else rows
         if k.shape != want or v.shape != want:
             raise ValueError(f"k/v must be {want}, got {tuple(k.shape)} / {tuple(v.shape)}")
         # conversions are no-ops in a decode step, whose host time is a dozen
         # such calls: they are made only where something differs
-        in_dtype = torch.bfloat16 if self.dtype == _FP8 else self.dtype
+        in_dtype = self._value_dtype
         if k.dtype != in_dtype or k.device != dev or not k.is_contiguous():
             k = k.to(device=dev, dtype=in_dtype).contiguous()
         if v.dtype != in_dtype or v.device != dev or not v.is_contiguous():
@@ -244,29 +260,90 @@ class PagedKVCache:
         if T == 0:
             return
         if self.check_unique:
-            if self._unique is None:
-                self._unique = _lib.UniqueCheck(dev, self.num_slots)
-            self._unique.run(slot_mapping, self._errors)
-        # the layer's planes by address (views of them are two indexings each)
-        esz = self.cache.element_size()
-        plane = self.num_slots * self.row_elems * esz
-        kp = self.cache.data_ptr() + 2 * first * plane
-        vp = kp + plane
+            self._check_slots(slot_mapping)
+        kp, vp = self._planes(first)
         src_layer = T * self.row_elems * 2
         src_tok = self.row_elems * 2
         stream = _lib.stream_of(dev)
         if self.dtype == _FP8:
-            splane = self.num_slots * self.kv_heads * 4
-            ks = self.scales.data_ptr() + 2 * first * splane
-            _lib.call("mkv_append_fp8", kp, vp, ks, ks + splane,
+            _lib.call("mkv_append_fp8", kp, vp, *self._scale_planes(first),
                       self._plane_layer_stride(), self._scale_layer_stride(), self.num_slots,
                       k.data_ptr(), v.data_ptr(), src_layer, src_tok, slot_mapping.data_ptr(), T,
                       L, self.kv_heads, self.head_dim, self._errors.ptr(), stream)
+        elif self.dtype == _FP4:
+            _lib.call_on(self.cache.device, "mkv_append_fp4", kp, vp, self._plane_layer_stride(),
+                         self.num_slots, k.data_ptr(), v.data_ptr(), src_layer, src_tok,
+                         slot_mapping.data_ptr(), T, L, self.kv_heads, self.head_dim,
+                         self._errors.ptr())
         else:
             _lib.call("mkv_append_bf16", kp, vp, self._plane_layer_stride(),
                       self.num_slots, k.data_ptr(), v.data_ptr(), src_layer, src_tok,
-                      slot_mapping.data_ptr(), T, L, self.row_elems * esz, self._errors.ptr(),
+                      slot_mapping.data_ptr(), T, L, self._row_bytes, self._errors.ptr(),
                       stream)
+
+    def append_rope(self, slot_mapping: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
+                    v: torch.Tensor, layer: int, positions: torch.Tensor,
+                    inv_freq: torch.Tensor, q_weight: torch.Tensor | None = None,
+                    k_weight: torch.Tensor | None = None, eps: float = 1e-6, *,
+                    rope_scale: float = 1.0, zero_centered: bool = False,
+                    interleaved: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+        """What an attention layer does between its projections and the attention
+        (muserve/model/qwen35_layer_v2.py:458-469 and the append), in one launch:
+        the norm of q's and k's heads and their rotation
+        (``kernels.rope.qk_norm_rope``, whose arguments these are), K and V [T, H,
+        head_dim] into ``layer``'s rows at ``slot_mapping``. Returns the rotated
+        queries [T, Hq, head_dim].
+
+        q, k and v may be strided views of a projection's output, in the pool's
+        16-bit type, or bf16 for an fp8 or a 4-bit pool (which quantise the rotated
+        row rounded to bf16: the pool holds what ``append`` of it would). Slot -1
+        skips a token's K and V, not its queries; slots must be unique."""
+        dev = self._gpu()
+        if slot_mapping.dtype != torch.int64 or slot_mapping.device != dev:
+            slot_mapping = slot_mapping.to(device=dev, dtype=torch.int64)
+        slot_mapping = slot_mapping.contiguous()
+        first = self._layer(layer)
+        if q.dtype != self._value_dtype:
+            raise TypeError(f"q, k and v must be {self._value_dtype} for a pool of {self.dtype}, "
+                            f"not {q.dtype}")
+        if k.dim() != 3 or k.shape[1:] != (self.kv_heads, self.head_dim) \
+                or slot_mapping.numel() != k.shape[0]:
+            raise ValueError(f"k/v must be [{slot_mapping.numel()}, {self.kv_heads}, "
+                             f"{self.head_dim}], got {tuple(k.shape)}")
+        if self.dtype == _FP8 and self.head_dim != 256:
+            raise ValueError("append_rope into an fp8 pool takes heads of 256 dims")
+        _lib.require_gpu(q, k, v, positions, inv_freq, slot_mapping, self.cache)
+        if self.check_unique and k.shape[0]:
+            self._check_slots(slot_mapping)
+        kind = rope.POOL_FP8 if self.dtype == _FP8 else \
+            rope.POOL_FP4 if self.dtype == _FP4 else rope.POOL_16
+        pool = (kind, *self._planes(first), *self._scale_planes(first), self.num_slots)
+        return rope.append_rope(q, k, v, positions, inv_freq, q_weight, k_weight, eps, rope_scale,
+                                zero_centered, interleaved, out, slot_mapping, pool, self._errors)
+
+    def _check_slots(self, slot_mapping: torch.Tensor) -> None:
+        if self._unique is None:
+            self._unique = _lib.UniqueCheck(self.device, self.num_slots)
+        self._unique.run(slot_mapping, self._errors)
+
+    def _layer(self, layer: int) -> int:
+        first = int(layer)
+        if not (-self.num_layers <= first < self.num_layers):
+            raise IndexError(f"layer {layer} out of range for {self.num_layers} layers")
+        return first % self.num_layers
+
+    def _planes(self, layer: int) -> tuple[int, int]:
+        """The layer's K and V plane by address (views of them are two indexings each)."""
+        plane = self.num_slots * self._row_bytes
+        kp = self.cache.data_ptr() + 2 * layer * plane
+        return kp, kp + plane
+
+    def _scale_planes(self, layer: int) -> tuple[int | None, int | None]:
+        if self.scales is None:
+            return None, None
+        plane = self.num_slots * self.kv_heads * 4
+        ks = self.scales.data_ptr() + 2 * layer * plane
+        return ks, ks + plane
 
     def get_kv_by_layer(self, layer_idx: int):
         """(k_cache, v_cache) views [num_pages, 16, kv_heads, head_dim]
@@ -292,7 +369,7 @@ class PagedKVCache:
         ``cu_out[b+1]``, or past the buffer's end, is cut there and flagged
         as MkvDeviceError at the next ``check_errors``). With ``layer`` None the
         first ``num_layers`` layers are gathered into [L, ...] outputs in one
-        launch. fp8 pools are dequantised to bf16. ``out`` reuses buffers.
+        launch. fp8 and 4-bit pools are dequantised to bf16. ``out`` reuses buffers.
         """
         dev = self._gpu()
         B = block_tables.shape[0]
@@ -308,7 +385,7 @@ class PagedKVCache:
             raise TypeError("block_tables and seq_lens must be int32")
         if block_tables.stride(1) != 1:
             raise ValueError("block_tables rows must be contiguous")
-        out_dtype = torch.bfloat16 if self.dtype == _FP8 else self.dtype
+        out_dtype = self._value_dtype
         rows = (B * out_len) if cu_out is None else None
         if cu_out is not None and cu_out.numel() != B + 1:
             raise ValueError("cu_out must hold B+1 offsets")
@@ -350,12 +427,19 @@ class PagedKVCache:
                       seq_lens.data_ptr(), _lib.ptr(starts), B, out_len, _lib.ptr(offs),
                       k_out.data_ptr(), v_out.data_ptr(), out_layer_stride, L, self.kv_heads,
                       self.head_dim, self._errors.ptr(), stream)
+        elif self.dtype == _FP4:
+            _lib.call_on(self.cache.device, "mkv_gather_dequant_fp4", kp.data_ptr(), vp.data_ptr(),
+                         self._plane_layer_stride(), self.num_pages, block_tables.data_ptr(),
+                         block_tables.stride(0), block_tables.shape[1], seq_lens.data_ptr(),
+                         _lib.ptr(starts), B, out_len, _lib.ptr(offs), k_out.data_ptr(),
+                         v_out.data_ptr(), out_layer_stride, L, self.kv_heads, self.head_dim,
+                         self._errors.ptr())
         else:
             _lib.call("mkv_gather_bf16", kp.data_ptr(), vp.data_ptr(), self._plane_layer_stride(),
                       self.num_pages, block_tables.data_ptr(), block_tables.stride(0),
                       block_tables.shape[1], seq_lens.data_ptr(), _lib.ptr(starts), B, out_len,
                       _lib.ptr(offs), k_out.data_ptr(), v_out.data_ptr(), out_layer_stride, L,
-                      self.row_elems * self.cache.element_size(), self._errors.ptr(), stream)
+                      self._row_bytes, self._errors.ptr(), stream)
         return k_out, v_out
 
     def copy_pages(self, src_pages, dst_pages) -> None:
@@ -376,7 +460,7 @@ class PagedKVCache:
         if n == 0:
             return
         stream = _lib.stream_of(dev)
-        page_bytes = KV_PAGE_SIZE * self.row_elems * self.cache.element_size()
+        page_bytes = KV_PAGE_SIZE * self._row_bytes
         _lib.call("mkv_copy_blocks", self.cache.data_ptr(), self.num_pages * page_bytes,
                   2 * self.num_layers, self.num_pages, page_bytes, src.data_ptr(), dst.data_ptr(),
                   n, self._errors.ptr(), stream)
