@@ -78,10 +78,9 @@ __device__ __forceinline__ uint32_t fp4_scale_byte(uint32_t m) {
   return (uint32_t)(b < 7 ? 7 : (b > 252 ? 252 : b));
 }
 
-// The float a scale byte stands for, as the conversions take it; NaN for kFp4Nan.
-__device__ __forceinline__ float fp4_scale(uint32_t byte) {
-  return byte == kFp4Nan ? bits_f32(0x7fc00000u) : bits_f32(byte << 23);
-}
+// A scale byte as the conversions take it: they go by the exponent bits alone, and
+// give NaN for all of them set.
+__device__ __forceinline__ float fp4_scale(uint32_t byte) { return bits_f32(byte << 23); }
 
 // Quantises N bf16 values a lane; 32 / N neighbouring lanes hold a block. The lane's N
 // codes, and its block's scale byte in each of those lanes. x / 2^e is exact and the
@@ -98,7 +97,7 @@ __device__ __forceinline__ uint32_t quantise_fp4(const uint32_t (&w)[N / 2], uin
   }
   m = over_lanes<kFp4Block / N>(m, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
   const uint32_t byte = fp4_scale_byte(m);
-  const float scale = bits_f32(byte << 23);
+  const float scale = fp4_scale(byte);
 #pragma unroll
   for (int i = 0; i < N / 8; ++i) {
     uint32_t c = 0;
