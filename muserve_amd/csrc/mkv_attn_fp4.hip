@@ -5,10 +5,19 @@
 // of its block table: softmax(q k^T * scale) v for each of the G query heads
 // that share a KV head. A cached token and head is 2 x 136 bytes for 1024 * G
 // flop, so HBM bounds the launch.
-//   * Work split: the (sequence, KV head) pairs' tiles of 32 tokens (two pages)
-//     form one flat list, pair after pair. Each wave of the resident grid takes
-//     an equal contiguous span of it; pieces of pairs that spans cut leave
-//     (max, sum, unnormalised output) and a second kernel joins them.
+//   * Work split: the sequences' tiles of 32 tokens (two pages) form one flat
+//     list, with one place more for each sequence, about what its start and end
+//     cost. Each wave of the resident grid takes a contiguous span of it, for
+//     one KV head; a span's KV heads are neighbouring workgroups of one XCD,
+//     which read the same lines of the rows at about the same time. Pieces of
+//     sequences that spans cut leave (max, sum, unnormalised output) for a
+//     second kernel to join; where a workgroup's four spans lie in one sequence
+//     they leave one piece. (Spans by workgroup, its waves taking the tiles in
+//     turn: a barrier for each sequence, 87 us instead of 81 at batch 256.)
+//   * Loads: page by page straight into a wave's LDS (global_load_lds, 16
+//     bytes a lane where rows are contiguous, else 4), two tiles in flight,
+//     the page ids a tile ahead of them. (Into registers in the operands' own
+//     order a K row is a line for every lane, and the launch reached 5 TB/s.)
 //   * Scores on the matrix cores (16x16x32 bf16): A = the 16 K rows of a page,
 //     codes converted to bf16 with their scale (exact), B = the query heads in
 //     columns n and n + 8. A column's lanes hold 8 tokens each; the maximum is
@@ -21,6 +30,9 @@
 //     product is free, so V is read in theirs.
 #include <math.h>
 
+#include <atomic>
+
+#include "mkv_dma.h"
 #include "mkv_quant.h"
 
 namespace mkv {
@@ -35,10 +47,12 @@ constexpr int kQRow = kHeadDim * 2;
 constexpr int kThreads4 = 256;
 constexpr int kWaves = kThreads4 / 64;
 constexpr int kTile = 32;            // tokens of a tile: two pages
+constexpr int kPage = 16 * kFp4Row;  // bytes of a page of one head
+constexpr int kTileLds = 4 * kPage;  // a tile in LDS: K's two pages, then V's
 constexpr int kMaxGroup = 8;         // query heads per KV head
 constexpr int kMaxPairs = 4096;      // batch x KV heads
+constexpr int kXcds = 8;             // MI355X: workgroups go round robin over 8 XCDs
 constexpr int kWgsPerCu = 2;
-constexpr int kJointTiles = 8;       // tiles a pair, on average, from which spans are workgroups'
 constexpr int kWidePairs = 128;      // pairs below which the merge takes 16 waves
 constexpr float kRaise = 8.f;        // log2 by which a score may pass the running maximum
 
@@ -49,12 +63,12 @@ struct Args {
   const int32_t* table;  // [B, tstride]
   const int32_t* lens;   // [B]
   uint8_t* out;          // [B, Hkv * G, 256] bf16
-  int64_t* hdr;          // workspace: [0] tiles of a span
-  int32_t* pre;          // [pairs + 1] each pair's first flat tile
-  float* ml;             // [waves, 2, G, 2] (max, sum) of cut pairs' pieces, log2 units
-  float* part;           // [waves, 2, G, 256] their unnormalised outputs
+  int64_t* hdr;          // workspace: [0] places of a span
+  int32_t* pre;          // [B + 1] each sequence's first place
+  float* ml;             // [spans, Hkv, 2, G, 2] (max, sum) of cut pieces, log2 units
+  float* part;           // [spans, Hkv, 2, G, 256] their unnormalised outputs
   int64_t num_pages, tstride, shared_below;
-  int32_t twidth, hkv, group, max_len, pairs;
+  int32_t twidth, hkv, group, max_len, batch;
   float scale_log2;
   int32_t* err;
 };
@@ -65,40 +79,42 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
                                                  __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
+template <typename T>
+__device__ __forceinline__ T lds_get(uint32_t at) {
+  return *reinterpret_cast<const __attribute__((address_space(3))) T*>(at);
+}
+// The places of a sequence in the flat list.
+__device__ __forceinline__ int32_t places_of(int32_t len) {
+  return len > 0 ? (len + kTile - 1) / kTile + 1 : 0;
+}
 // Eight codes of a word times the scale, as eight bf16.
 __device__ __forceinline__ u32x4 dequant8(uint32_t w, float s) {
   return u32x4{mkv_fp4_pair(w, 0, s), mkv_fp4_pair(w, 1, s), mkv_fp4_pair(w, 2, s),
                mkv_fp4_pair(w, 3, s)};
 }
 
-// A tile's cached rows, as a lane holds them: of each page the dims 32 g .. and 128 +
-// 32 g .. of K token c, and the dims 16 c .. of V tokens 4 g + j. One load of V scales
-// serves the page: lane c's word is of token 4 g + c % 4, the half c / 8 of its blocks.
-struct Tile {
-  u32x4 k[2][2];
-  u32x2 ks[2];
-  u32x2 v[2][4];
-  uint32_t vs[2];
-};
-
-__global__ __launch_bounds__(kThreads4, 2) void attn_fp4_span_kernel(Args a) {
-  extern __shared__ __attribute__((aligned(16))) float piece_l[];  // [waves][G][256], then (m, l)
+// ONE: one KV head, a page's rows are contiguous.
+template <bool ONE>
+__global__ __launch_bounds__(kThreads4, kWgsPerCu) void attn_fp4_span_kernel(Args a) {
+  // two tiles for each wave (in the end its piece [G][256]), the pieces' (m, l) [waves][G][2]
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   __shared__ int32_t wave_tot[kWaves];
-  __shared__ int32_t start_l[kWaves][2];  // (pair, its first tile) that a span starts in
+  __shared__ int32_t start_l[kWaves][2];  // (sequence, its first tile) that a span starts in
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int32_t hkv = ONE ? 1 : a.hkv;
   const int64_t cap = (int64_t)a.twidth * 16 < a.max_len ? (int64_t)a.twidth * 16 : a.max_len;
-  // a pair's cached tokens, cut to the table and the launch's bound
-  auto length_of = [&](int pr) __attribute__((always_inline)) {
-    const int64_t len = ld_const(a.lens + pr / a.hkv);
+  // a sequence's cached tokens, cut to the table and the launch's bound
+  auto length_of = [&](int b) __attribute__((always_inline)) {
+    const int64_t len = ld_const(a.lens + b);
     return (int32_t)(len < 0 ? 0 : (len > cap ? cap : len));
   };
-  // exclusive prefix of the tile counts of 256 pairs from `base` on, behind `before`;
-  // the round's total goes to `round`
+  // exclusive prefix of the places of 256 sequences from `base` on (a place for each
+  // tile and one more), behind `before`; the round's total goes to `round`
   auto scan = [&](int base, int32_t before, int32_t& cnt, int32_t& round)
       __attribute__((always_inline)) {
-    const int pr = base + tid;
-    cnt = pr < a.pairs ? (length_of(pr) + kTile - 1) / kTile : 0;
+    const int b = base + tid;
+    cnt = b < a.batch ? places_of(length_of(b)) : 0;
     int32_t incl = cnt;
 #pragma unroll
     for (int dd = 1; dd < 64; dd <<= 1) {
@@ -118,212 +134,294 @@ __global__ __launch_bounds__(kThreads4, 2) void attn_fp4_span_kernel(Args a) {
     return at;
   };
   int32_t T = 0, cnt, round, at = 0;
-  for (int base = 0; base < a.pairs; base += kThreads4) {
+  for (int base = 0; base < a.batch; base += kThreads4) {
     at = scan(base, T, cnt, round);
     T += round;
   }
-  if (T == 0) {
-    if (blockIdx.x == 0) {
-      for (int p = tid; p <= a.pairs; p += kThreads4) a.pre[p] = 0;
-      for (int p = tid; p < a.pairs; p += kThreads4)
-        if (ld_const(a.lens + p / a.hkv) < 0) raise_err(a.err, MKV_DEVERR_TABLE);
-    }
-    return;
-  }
-  // Spans: by workgroup, its waves taking the tiles in turn and joining their pieces in
-  // LDS, where a pair has enough tiles to keep them busy; else by wave.
-  const bool joint = T >= kJointTiles * a.pairs;
-  const int32_t step = joint ? kWaves : 1;
-  const int32_t units = (int32_t)gridDim.x * (joint ? 1 : kWaves);
-  int32_t S = (T + units - 1) / units;
-  S = S < step ? step : S;
-  const int32_t unit = joint ? (int32_t)blockIdx.x : (int32_t)blockIdx.x * kWaves + wave;
-  // the pairs that this workgroup's spans start in (and, by workgroup 0, all prefixes for
-  // the merge kernel); a round's prefix is still held where there is one round
+  // Workgroups of one XCD (those with the same number modulo 8) take neighbouring spans.
+  const int32_t xcd = blockIdx.x % kXcds, all = gridDim.x;
+  const int32_t unit = xcd * (all / kXcds) + (xcd < all % kXcds ? xcd : all % kXcds) +
+                       (int32_t)blockIdx.x / kXcds;
+  const int32_t head = unit % hkv;
+  const int32_t total = T;
+  T = T > 0 ? T - 1 : 0;  // (nothing starts at the place behind the last sequence)
+  const int32_t spans = all / hkv * kWaves;
+  const int32_t S = T > spans ? (T + spans - 1) / spans : 1;
+  const int32_t first = unit / hkv * kWaves;
+  const int32_t span = first + wave;
+  // The sequences that this workgroup's spans start in (and, by workgroup 0, the prefixes
+  // for the merge kernel); a round's prefix is still held where there is one round.
   {
-    const int32_t first = joint ? (int32_t)blockIdx.x : (int32_t)blockIdx.x * kWaves;
     int32_t before = 0;
-    for (int base = 0; base < a.pairs; base += kThreads4) {
-      if (a.pairs > kThreads4) {
+    for (int base = 0; base < a.batch; base += kThreads4) {
+      if (a.batch > kThreads4) {
         at = scan(base, before, cnt, round);
         before += round;
       }
-      const int pr = base + tid;
-      if (pr < a.pairs) {
+      const int b = base + tid;
+      if (b < a.batch) {
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
           const int64_t s = (int64_t)(first + w) * S;
-          if ((w == 0 || !joint) && s >= at && s < at + cnt) {
-            start_l[w][0] = pr;
+          if (s >= at && s < at + cnt) {
+            start_l[w][0] = b;
             start_l[w][1] = at;
           }
         }
         if (blockIdx.x == 0) {
-          a.pre[pr] = at;
-          const int64_t len = ld_const(a.lens + pr / a.hkv);
-          if ((len > cap || len < 0) && pr % a.hkv == 0) raise_err(a.err, MKV_DEVERR_TABLE);
+          a.pre[b] = at;
+          const int64_t len = ld_const(a.lens + b);
+          if (len > cap || len < 0) raise_err(a.err, MKV_DEVERR_TABLE);
         }
       }
     }
     if (blockIdx.x == 0 && tid == 0) {
-      a.pre[a.pairs] = T;
+      a.pre[a.batch] = total;
       a.hdr[0] = S;
     }
     __syncthreads();
   }
-  const int64_t s64 = (int64_t)unit * S;
-  if (s64 >= T) return;  // (joint: the whole workgroup)
+  const int64_t s64 = (int64_t)span * S;
+  if (s64 >= T) return;  // (no barrier follows, but for workgroups with four spans)
   const int32_t s0 = (int32_t)s64, s1 = s64 + S < T ? (int32_t)s64 + S : T;
-  const int32_t w0 = joint ? wave : 0;  // the wave takes the span's tiles w0, w0 + step, ..
 
+  // Of the two waves on a SIMD the arbiter favours the older one: with it alone the first
+  // workgroup of a CU ends a third before the second. They take turns, tile by tile.
+  const uint32_t wslot = __builtin_amdgcn_s_getreg((3 << 11) | 4) & 1u;
   const int c = lane & 15, g = lane >> 4;  // row / column and quad of a matrix operand
-  const int head = c & 7;
   const uint32_t low_mask = c < 8 ? 0u : 0xffff0000u;  // what the lane takes off a weight
-  const int64_t row_bytes = (int64_t)a.hkv * kFp4Row;
-  const int64_t page_bytes = 16 * row_bytes;
-  const uint32_t koff = (uint32_t)(c * row_bytes);
-  const uint32_t voff = (uint32_t)(4 * g * row_bytes), vstep = (uint32_t)row_bytes;
-  const uint32_t vsoff = (uint32_t)((4 * g + (c & 3)) * row_bytes) + kFp4Codes + 4 * (c >> 3);
-  const uint32_t vshift = 8 * ((c >> 1) & 3), kshift = 8 * g;
-
-  // a pair as the walk over the span has it
-  struct Pair {
-    int32_t p, pre0, pre1, len;
-  };
-  auto next_pair = [&](Pair& x) __attribute__((always_inline)) {  // the next one with tiles
-    do {
-      ++x.p;
-      x.len = __builtin_amdgcn_readfirstlane(length_of(x.p));
-      x.pre0 = x.pre1;
-      x.pre1 += (x.len + kTile - 1) / kTile;
-    } while (x.pre1 == x.pre0);
-  };
-  Pair ahead;  // of the tile whose page ids are read next
-  {
-    const int w = joint ? 0 : wave;
-    ahead.p = __builtin_amdgcn_readfirstlane(start_l[w][0]);
-    ahead.pre0 = __builtin_amdgcn_readfirstlane(start_l[w][1]);
-    ahead.len = __builtin_amdgcn_readfirstlane(length_of(ahead.p));
-    ahead.pre1 = ahead.pre0 + (ahead.len + kTile - 1) / kTile;
-  }
-  Pair cur = ahead;
-  // A tile's rows are loaded while the one before it is computed, and its page ids a tile
-  // earlier still: the rows' loads wait for them.
-  struct Pages {
-    int32_t id[2], left[2], hk;  // left: the page's tokens and those behind it
-  };
-  int32_t fa = s0 + w0;
-  auto read_ids = [&](Pages& x) __attribute__((always_inline)) {  // of tile fa
-    if (fa >= s1) {  // behind the span: a page that is in the caches, no token of it
-      x.id[0] = x.id[1] = x.left[0] = x.left[1] = x.hk = 0;
-      return;
-    }
-    while (fa >= ahead.pre1) next_pair(ahead);
-    const int b = ahead.p / a.hkv;
-    const int32_t tok0 = (fa - ahead.pre0) * kTile;
-    const int32_t* ids = a.table + (int64_t)b * a.tstride + tok0 / 16;
-    x.hk = ahead.p - b * a.hkv;
-    x.left[0] = ahead.len - tok0;
-    x.left[1] = x.left[0] - 16;
-    x.id[0] = ld_const(ids);
-    x.id[1] = ld_const(ids + (x.left[1] > 0 ? 1 : 0));
-    fa += step;
-  };
-  auto load = [&](Tile& t, const Pages& x, int32_t (&valid)[2]) __attribute__((always_inline)) {
+  const int32_t row_bytes = hkv * kFp4Row;
+  const uint32_t num_pages = a.num_pages < INT32_MAX ? (uint32_t)a.num_pages : INT32_MAX;
+  float* ml_l = reinterpret_cast<float*>(lds + 2 * kWaves * kTileLds);
+  const uint32_t tile_l = lds_addr(lds + wave * 2 * kTileLds);
+  const uint32_t get_k = c * kFp4Row + 16 * g;  // dims 32 g .. and 128 + 32 g ..
+  const uint32_t get_ks = c * kFp4Row + kFp4Codes + g;
+  const uint32_t get_v = 2 * kPage + 4 * g * kFp4Row + 8 * c;  // dims 16 c ..
+  const uint32_t get_vs = 2 * kPage + 4 * g * kFp4Row + kFp4Codes + c / 2;
+  // a page's rows of one head among hkv: word i is row i / 34, word i % 34 of it
+  constexpr int kWords = ONE ? 1 : (kPage / 4 + 63) / 64;
+  uint32_t word_off[kWords];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      int32_t left = x.left[i] < 0 ? 0 : (x.left[i] > 16 ? 16 : x.left[i]);
-      int32_t id = x.id[i];
-      if (id < 0 || id >= a.num_pages) {  // no token of a page id outside the pool
+  for (int j = 0; j < kWords; ++j) {
+    const int i = 64 * j + lane;
+    word_off[j] = ONE ? 16 * lane : (i / (kFp4Row / 4)) * row_bytes + (i % (kFp4Row / 4)) * 4;
+  }
+
+  // a sequence as the walk over the span has it: its tiles' places are pre0 .. pre1
+  struct Seq {
+    int32_t b, pre0, pre1, len;
+  };
+  auto next_seq = [&](Seq x) __attribute__((always_inline)) {  // the next one with tiles
+    do {
+      ++x.b;
+      x.len = __builtin_amdgcn_readfirstlane(length_of(x.b));
+    } while (x.len == 0);
+    x.pre0 = x.pre1 + 1;
+    x.pre1 = x.pre0 + (x.len + kTile - 1) / kTile;
+    return x;
+  };
+  Seq ahead;  // of the tile whose page ids are read next
+  ahead.b = __builtin_amdgcn_readfirstlane(start_l[wave][0]);
+  ahead.pre0 = __builtin_amdgcn_readfirstlane(start_l[wave][1]);
+  ahead.len = __builtin_amdgcn_readfirstlane(length_of(ahead.b));
+  ahead.pre1 = ahead.pre0 + (ahead.len + kTile - 1) / kTile;
+  int32_t fa = s0;  // and its place
+  if (fa == ahead.pre1) {  // the span starts at the place behind a sequence
+    if (++fa == s1) return;
+    ahead = next_seq(ahead);
+  }
+  Seq cur = ahead;
+
+  // The pages of a tile. Their ids are read a tile ahead of the rows' loads, which wait for
+  // them; a tile's K and V are loaded once the tile two before it has been read.
+  struct Pages {
+    int32_t id0, id1, left;  // left: the tile's tokens and those behind it, 0: no tile
+  };
+  auto read_ids = [&]() __attribute__((always_inline)) {
+    Pages x = {0, 0, 0};
+    if (fa == ahead.pre1 && ++fa < s1) ahead = next_seq(ahead);
+    if (fa < s1) {
+      const int32_t tok0 = (fa - ahead.pre0) * kTile;
+      const int32_t* ids = a.table + (int64_t)ahead.b * a.tstride + tok0 / 16;
+      x.left = ahead.len - tok0;
+      x.id0 = ld_const(ids);
+      x.id1 = ld_const(ids + (x.left > 16 ? 1 : 0));
+      ++fa;
+    }
+    return x;
+  };
+  struct Where {
+    int64_t base0, base1;    // of the pages' rows in both planes
+    int32_t valid0, valid1;  // tokens of the two pages
+    int32_t hot;             // bit i: page i is read through the caches
+    bool there;              // there is such a tile
+  };
+  auto locate = [&](Pages x) __attribute__((always_inline)) {
+    Where w;
+    w.hot = 0;
+    w.there = x.left > 0;
+    auto page = [&](int i, int32_t id, int32_t left, int64_t& base, int32_t& valid)
+        __attribute__((always_inline)) {
+      valid = left < 0 ? 0 : (left > 16 ? 16 : left);
+      if ((uint32_t)id >= num_pages) {  // no token of a page id outside the pool
         if (lane == 0 && left > 0) raise_err(a.err, MKV_DEVERR_PAGE);
         id = 0;
-        left = 0;
+        valid = 0;
       }
-      valid[i] = left;
-      const int64_t base = id * page_bytes + x.hk * kFp4Row;
-      const uint8_t* kp = a.k + base;
-      const uint8_t* vp = a.v + base;
-      t.k[i][0] = *reinterpret_cast<const u32x4a8*>(kp + (koff + 16 * g));
-      t.k[i][1] = *reinterpret_cast<const u32x4a8*>(kp + (koff + 16 * g + 64));
-      t.ks[i] = *reinterpret_cast<const u32x2*>(kp + (koff + kFp4Codes));
+      w.hot |= id < a.shared_below ? 1 << i : 0;
+      base = (int64_t)id * (16 * row_bytes) + head * kFp4Row;
+    };
+    page(0, x.id0, x.left, w.base0, w.valid0);
+    page(1, x.id1, x.left - 16, w.base1, w.valid1);
+    return w;
+  };
+  constexpr int kPageLoads = ONE ? 3 : kWords;  // instructions of a page's rows
+  auto load_page = [&](const uint8_t* src, uint32_t dst, bool hot) __attribute__((always_inline)) {
+    lds_reads_done();
+    if constexpr (ONE) {
+      if (hot) {
+        dma16_cached(src, word_off[0], dst);
+        dma16_cached(src + 1024, word_off[0], dst + 1024);
+        if (lane < 8) dma16_cached(src + 2048, word_off[0], dst + 2048);
+      } else {
+        dma16(src, word_off[0], dst);
+        dma16(src + 1024, word_off[0], dst + 1024);
+        if (lane < 8) dma16(src + 2048, word_off[0], dst + 2048);
+      }
+    } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        t.v[i][j] = *reinterpret_cast<const u32x2*>(vp + (voff + j * vstep + 8 * c));
-      t.vs[i] = *reinterpret_cast<const uint32_t*>(vp + vsoff);
+      for (int j = 0; j < kWords - 1; ++j) dma4_at_cached(src, word_off[j], dst + 256 * j);
+      if (lane < 32) dma4_at_cached(src, word_off[kWords - 1], dst + 256 * (kWords - 1));
     }
+  };
+  auto load_k = [&](Where w, uint32_t slot) __attribute__((always_inline)) {
+    load_page(a.k + w.base0, slot, w.hot & 1);
+    load_page(a.k + w.base1, slot + kPage, w.hot & 2);
+  };
+  auto load_v = [&](Where w, uint32_t slot) __attribute__((always_inline)) {
+    load_page(a.v + w.base0, slot + 2 * kPage, w.hot & 1);
+    load_page(a.v + w.base1, slot + 3 * kPage, w.hot & 2);
   };
 
   u32x4 qb[8];
   f32x4 acc[16];
   float m_run, l_run;
-  auto compute = [&](const Tile& t, const int32_t (&valid)[2]) __attribute__((always_inline)) {
-    // scores: lane (c, g) gets tokens 4 g + j of each page, for head c & 7
-    float sv[8], mx = -INFINITY;
+  int32_t f = fa;          // the place of the tile that is computed next
+  uint32_t slot = tile_l;  // and where it lies
+  const uint32_t both = 2 * tile_l + kTileLds;
+  Where now = locate(read_ids());
+  load_k(now, slot);
+  load_v(now, slot);
+  Where next = locate(read_ids());
+  if (next.there) {
+    load_k(next, both - slot);
+    load_v(next, both - slot);
+  }
+  Pages pages = read_ids();
+  auto load_q = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      f32x4 sc = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < 8; ++s) {  // the dims of K's operand: 32 g + 8 s, 128 + 32 g + 8 (s - 4)
+      // (columns behind the last head repeat it: their results are not used)
+      const int h = (c & 7) < a.group ? (c & 7) : a.group - 1;
+      const int dim = 32 * g + 8 * (s & 3) + 128 * (s >> 2);
+      qb[s] = ld16(a.q + (((int64_t)cur.b * hkv + head) * a.group + h) * kQRow + 2 * dim);
+    }
+  };
+  load_q();
+  for (;;) {  // the span's sequences
+    const int32_t end = cur.pre1 < s1 ? cur.pre1 : s1;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float scale = fp4_scale((t.ks[i][h] >> kshift) & 255u);
+    for (int j = 0; j < 16; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m_run = -INFINITY;
+    l_run = 0.f;
+    while (f < end) {
+      __builtin_amdgcn_s_setprio(0);
+      if (((uint32_t)(f + wslot) & 1u) != 0) __builtin_amdgcn_s_setprio(1);
+      const bool has1 = next.there;
+      // the tile's K has come once what was asked for behind it is all that is in flight
+      if (has1) vm_wait_n<6 * kPageLoads>(); else vm_wait_n<2 * kPageLoads>();
+      u32x4 k[2][2];
+      float ks[2][2];
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
-          sc = mfma(dequant8(t.k[i][h][s], scale), qb[4 * h + s], sc);
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          k[i][h] = lds_get<u32x4a8>(slot + i * kPage + get_k + 64 * h);
+          ks[i][h] = fp4_scale(lds_get<uint8_t>(slot + i * kPage + get_ks + 4 * h));
+        }
+      const Where after = locate(pages);
+      const bool has2 = after.there;
+      if (has2) load_k(after, slot);
+      pages = read_ids();
+      // scores: lane (c, g) gets tokens 4 g + j of each page, for head c & 7
+      float sv[8];
+      {
+        f32x4 sc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            sc[i] = mfma(dequant8(k[i][s >> 2][s & 3], ks[i][s >> 2]), qb[s], sc[i]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sv[j] = sc[j >> 2][j & 3] * a.scale_log2;
       }
+      const bool part = now.valid0 < 16 || now.valid1 < 16;
+      if (part) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        sv[4 * i + j] = 4 * g + j < valid[i] ? sc[j] * a.scale_log2 : -INFINITY;
-        mx = fmaxf(mx, sv[4 * i + j]);
+        for (int j = 0; j < 8; ++j)
+          sv[j] = 4 * g + (j & 3) < (j < 4 ? now.valid0 : now.valid1) ? sv[j] : -INFINITY;
       }
-    }
-    if (__builtin_amdgcn_ballot_w64(mx > m_run + kRaise) != 0) {
-      const float top = over_rows<4>(mx, [](float x, float y) { return fmaxf(x, y); });
-      const float m_new = fmaxf(m_run, top);
-      const float alpha = m_run == -INFINITY ? 0.f : exp2_fast(m_run - m_new);
-      m_run = m_new;
-      l_run *= alpha;
-      // output rows 4 g + i belong to head (4 g + i) & 7
-      float al[4];
+      const float mx = fmaxf(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])),
+                             fmaxf(fmaxf(sv[4], sv[5]), fmaxf(sv[6], sv[7])));
+      if (__builtin_amdgcn_ballot_w64(mx > m_run + kRaise) != 0) {
+        const float top = over_rows<4>(mx, [](float x, float y) { return fmaxf(x, y); });
+        const float m_new = fmaxf(m_run, top);
+        const float alpha = m_run == -INFINITY ? 0.f : exp2_fast(m_run - m_new);
+        m_run = m_new;
+        l_run *= alpha;
+        // output rows 4 g + i belong to head (4 g + i) & 7
+        float al[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) al[i] = __shfl(alpha, (4 * g + i) & 7);
+        for (int i = 0; i < 4; ++i) al[i] = __shfl(alpha, (4 * g + i) & 7);
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
+        for (int j = 0; j < 16; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[j][i] *= al[i];
-    }
-    const float m_ref = m_run == -INFINITY ? 0.f : m_run;
-    u32x4 pa;
-#pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      const float p0 = exp2_fast(sv[j] - m_ref), p1 = exp2_fast(sv[j + 1] - m_ref);
-      l_run += p0 + p1;
-      // upper 8 bits of the weight in rows below 8, what is left of it in the others
-      const uint32_t x0 = f32_bits(p0 - bits_f32(f32_bits(p0) & low_mask));
-      const uint32_t x1 = f32_bits(p1 - bits_f32(f32_bits(p1) & low_mask));
-      pa[j / 2] = __builtin_amdgcn_perm(x1, x0, 0x07060302u);
-    }
-    u32x2 v[8];
-    float vsc[8];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint32_t w[4] = {lane_of<0x00>(t.vs[i]), lane_of<0x55>(t.vs[i]), lane_of<0xaa>(t.vs[i]),
-                             lane_of<0xff>(t.vs[i])};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[4 * i + j] = t.v[i][j];
-        vsc[4 * i + j] = fp4_scale((w[j] >> vshift) & 255u);
+          for (int i = 0; i < 4; ++i) acc[j][i] *= al[i];
       }
-    }
-    if (valid[0] < 16 || valid[1] < 16) {  // rows that hold anything: zeros
+      const float m_ref = m_run == -INFINITY ? 0.f : m_run;
+      u32x4 pa;
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        const float p0 = exp2_fast(sv[j] - m_ref), p1 = exp2_fast(sv[j + 1] - m_ref);
+        l_run += p0 + p1;
+        // upper 8 bits of the weight in rows below 8, what is left of it in the others
+        const uint32_t x0 = f32_bits(p0 - bits_f32(f32_bits(p0) & low_mask));
+        const uint32_t x1 = f32_bits(p1 - bits_f32(f32_bits(p1) & low_mask));
+        pa[j / 2] = __builtin_amdgcn_perm(x1, x0, 0x07060302u);
+      }
+      if (has2) vm_wait_n<6 * kPageLoads>();
+      else if (has1) vm_wait_n<4 * kPageLoads>();
+      else vm_wait_n<0>();
+      u32x2 v[8];
+      float vsc[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const bool ok = 4 * g + (j & 3) < valid[j >> 2];
-        v[j] = ok ? v[j] : u32x2{0u, 0u};
-        vsc[j] = ok ? vsc[j] : 1.f;
+        const uint32_t row = (j >> 2) * kPage + (j & 3) * kFp4Row;
+        v[j] = lds_get<u32x2>(slot + get_v + row);
+        vsc[j] = fp4_scale(lds_get<uint8_t>(slot + get_vs + row));
       }
-    }
+      if (has2) load_v(after, slot);
+      if (part) {  // rows that hold anything: zeros
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      // dims 8 w + 2 e and + 1 of the lane's 16, of its 8 tokens: pairs of dims to pairs of tokens
+        for (int j = 0; j < 8; ++j) {
+          const bool ok = 4 * g + (j & 3) < (j < 4 ? now.valid0 : now.valid1);
+          v[j] = ok ? v[j] : u32x2{0u, 0u};
+          vsc[j] = ok ? vsc[j] : 1.f;
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        // dims 8 w + 2 e and + 1 of the lane's 16, of its 8 tokens: pairs of dims to pairs of tokens
 #define MKV_PV(e)                                                                              \
   {                                                                                            \
     u32x4 lo, hi;                                                                              \
@@ -336,122 +434,87 @@ __global__ __launch_bounds__(kThreads4, 2) void attn_fp4_span_kernel(Args a) {
     acc[8 * w + 2 * e] = mfma(pa, lo, acc[8 * w + 2 * e]);                                     \
     acc[8 * w + 2 * e + 1] = mfma(pa, hi, acc[8 * w + 2 * e + 1]);                             \
   }
-      MKV_PV(0) MKV_PV(1) MKV_PV(2) MKV_PV(3)
+        MKV_PV(0) MKV_PV(1) MKV_PV(2) MKV_PV(3)
 #undef MKV_PV
+      }
+      now = next;
+      next = after;
+      slot = both - slot;
+      ++f;
     }
-  };
-
-  Tile t;
-  Pages pages;
-  int32_t valid[2];
-  int32_t f = s0 + w0;  // the wave's next tile
-  read_ids(pages);
-  load(t, pages, valid);
-  read_ids(pages);
-  for (;;) {            // the span's pairs
-    const int32_t end = cur.pre1 < s1 ? cur.pre1 : s1;
-#pragma unroll
-    for (int s = 0; s < 8; ++s) {  // the dims of K's operand: 32 g + 8 s, 128 + 32 g + 8 (s - 4)
-      const int dim = 32 * g + 8 * (s & 3) + 128 * (s >> 2);
-      qb[s] = head < a.group
-                  ? ld16(a.q + ((int64_t)cur.p * a.group + head) * kQRow + 2 * dim)
-                  : u32x4{0u, 0u, 0u, 0u};
+    const Seq done = cur;
+    const bool last = cur.pre1 + 1 >= s1;
+    if (!last) {  // the next sequence's query rows come while this one's piece goes
+      cur = next_seq(cur);
+      f = cur.pre0;
+      load_q();
     }
-#pragma unroll
-    for (int j = 0; j < 16; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    m_run = -INFINITY;
-    l_run = 0.f;
-    while (f < end) {
-      Tile next;
-      int32_t next_valid[2];
-      load(next, pages, next_valid);
-      read_ids(pages);
-      compute(t, valid);
-      t = next;
-      valid[0] = next_valid[0];
-      valid[1] = next_valid[1];
-      f += step;
-    }
-    // the pair's piece in this span: the quads' sums, and the weights' two parts
+    // the sequence's piece in this span: the quads' sums, and the weights' two parts
     const float l = over_rows<4>(l_run, [](float x, float y) { return x + y; });
 #pragma unroll
     for (int j = 0; j < 16; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[j][i] += __shfl_xor(acc[j][i], 32);
-    const bool whole = cur.pre0 >= s0 && cur.pre1 <= s1;
-    // (cut pairs: the span's first goes to slot 0, its last to slot 1)
-    const int64_t slot = ((int64_t)unit * 2 + (cur.pre0 <= s0 ? 0 : 1)) * a.group;
-    uint8_t* out = a.out + (int64_t)cur.p * a.group * kQRow;
-    if (!joint) {
+    const bool whole = done.pre0 >= s0 && done.pre1 <= s1;
+    // (cut sequences: the span's first goes to slot 0, its last to slot 1)
+    const int64_t piece =
+        (((int64_t)span * hkv + head) * 2 + (done.pre0 <= s0 ? 0 : 1)) * a.group;
+    uint8_t* out = a.out + ((int64_t)done.b * hkv + head) * a.group * kQRow;
+    // the workgroup's spans lie in one sequence: one piece, its first span's
+    const bool joint = done.pre0 <= first * S && done.pre1 >= (first + kWaves) * (int64_t)S;
+    if (joint && lane < a.group) {
+      ml_l[(wave * a.group + lane) * 2] = m_run;
+      ml_l[(wave * a.group + lane) * 2 + 1] = l;
+    }
+    float* piece_l = reinterpret_cast<float*>(lds + wave * 2 * kTileLds);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int h = 4 * g + i;
-        const float L = __shfl(l, h & 7), M = __shfl(m_run, h & 7);
-        if (h >= a.group) continue;  // (rows 8 and up are the other part)
-        if (whole) {
-          const float inv = 1.f / L;
-          uint32_t o[8];
+    for (int i = 0; i < 4; ++i) {
+      const int h = 4 * g + i;
+      const float L = __shfl(l, h & 7), M = __shfl(m_run, h & 7);
+      if (h >= a.group) continue;  // (rows 8 and up are the other part)
+      if (whole) {
+        const float inv = 1.f / L;
+        uint32_t o[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            o[j] = L == 0.f ? 0u : pack_bf16(acc[2 * j][i] * inv, acc[2 * j + 1][i] * inv);
-          st16(out + h * kQRow + c * 32, u32x4{o[0], o[1], o[2], o[3]});
-          st16(out + h * kQRow + c * 32 + 16, u32x4{o[4], o[5], o[6], o[7]});
-        } else {
-          float* dst = a.part + (slot + h) * kHeadDim + c * 16;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<f32x4*>(dst + 4 * j) = f32x4{acc[4 * j][i], acc[4 * j + 1][i],
-                                                           acc[4 * j + 2][i], acc[4 * j + 3][i]};
-          if (c == 0) {
-            a.ml[(slot + h) * 2] = M;
-            a.ml[(slot + h) * 2 + 1] = L;
-          }
-        }
-      }
-    } else {
-      float* ml = piece_l + kWaves * a.group * kHeadDim;  // [waves][G][2]
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int h = 4 * g + i;
-        if (h >= a.group) continue;
-        float* dst = piece_l + (wave * a.group + h) * kHeadDim + c * 16;
+        for (int j = 0; j < 8; ++j)
+          o[j] = L == 0.f ? 0u : pack_bf16(acc[2 * j][i] * inv, acc[2 * j + 1][i] * inv);
+        st16(out + h * kQRow + c * 32, u32x4{o[0], o[1], o[2], o[3]});
+        st16(out + h * kQRow + c * 32 + 16, u32x4{o[4], o[5], o[6], o[7]});
+      } else {
+        float* dst = joint ? piece_l + h * kHeadDim + c * 16 : a.part + (piece + h) * kHeadDim + c * 16;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           *reinterpret_cast<f32x4*>(dst + 4 * j) = f32x4{acc[4 * j][i], acc[4 * j + 1][i],
                                                          acc[4 * j + 2][i], acc[4 * j + 3][i]};
+        if (!joint && c == 0) {
+          a.ml[(piece + h) * 2] = M;
+          a.ml[(piece + h) * 2 + 1] = L;
+        }
       }
-      if (lane < a.group) {
-        ml[(wave * a.group + lane) * 2] = m_run;
-        ml[(wave * a.group + lane) * 2 + 1] = l;
-      }
+    }
+    if (joint) {
       __syncthreads();
+      const int64_t at = ((int64_t)first * hkv + head) * 2 * a.group;
       for (int h = 0; h < a.group; ++h) {  // a thread per dim
         float M = -INFINITY, O = 0.f, L = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) M = fmaxf(M, ml[(w * a.group + h) * 2]);
+        for (int w = 0; w < kWaves; ++w) M = fmaxf(M, ml_l[(w * a.group + h) * 2]);
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-          const float m = ml[(w * a.group + h) * 2];
+          const float m = ml_l[(w * a.group + h) * 2];
           // (a wave without a score: 1, so that a NaN of its sums stays)
           const float e = m == -INFINITY ? 1.f : exp2_fast(m - M);
-          O += e * piece_l[(w * a.group + h) * kHeadDim + tid];
-          L += e * ml[(w * a.group + h) * 2 + 1];
+          O += e * reinterpret_cast<const float*>(lds + w * 2 * kTileLds)[h * kHeadDim + tid];
+          L += e * ml_l[(w * a.group + h) * 2 + 1];
         }
-        if (whole) {
-          reinterpret_cast<uint16_t*>(out + h * kQRow)[tid] =
-              f32_to_bf16_rne(L == 0.f ? 0.f : O / L);
-        } else {
-          a.part[(slot + h) * kHeadDim + tid] = O;
-          if (tid == 0) {
-            a.ml[(slot + h) * 2] = M;
-            a.ml[(slot + h) * 2 + 1] = L;
-          }
+        a.part[(at + h) * kHeadDim + tid] = O;
+        if (tid == 0) {
+          a.ml[(at + h) * 2] = M;
+          a.ml[(at + h) * 2 + 1] = L;
         }
       }
-      __syncthreads();  // the pieces are read before the next pair's
     }
-    if (end == s1) return;
-    next_pair(cur);
+    if (last) return;
   }
 }
 
@@ -465,23 +528,34 @@ __global__ __launch_bounds__(64 * WAVES) void attn_fp4_merge_kernel(Args a) {
   __shared__ __attribute__((aligned(16))) float wave_o[WAVES][kHeadDim];
   __shared__ float wave_ml[WAVES][2];
   const int pr = blockIdx.x / a.group, h = blockIdx.x % a.group;
+  const int b = pr / a.hkv, head = pr - b * a.hkv;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t span = ld_const(a.hdr);  // (loaded beside the pair's bounds)
-  const int32_t p0 = ld_const(a.pre + pr), p1 = ld_const(a.pre + pr + 1);
+  const int64_t span = ld_const(a.hdr);  // (loaded beside the sequence's bounds)
+  const int32_t p0 = ld_const(a.pre + b);
+  int32_t p1 = ld_const(a.pre + b + 1);
   asm volatile("" ::"s"(span));
   uint16_t* out = reinterpret_cast<uint16_t*>(a.out + ((int64_t)pr * a.group + h) * kQRow);
   if (p1 <= p0) {
     if (tid < kHeadDim) out[tid] = 0;
     return;
   }
+  --p1;  // without the place behind its tiles
   const uint32_t S = (uint32_t)span;
   const uint32_t u0 = (uint32_t)p0 / S, u1 = (uint32_t)(p1 - 1) / S;
   if (u0 == u1) return;  // written with its span
-  const int n = (int)(u1 - u0 + 1);
+  // spans u0 .. u1; those of the workgroups that lie in the sequence, g0 .. g1, as one each
+  const uint32_t g0 = ((uint32_t)p0 + kWaves * S - 1) / (kWaves * S);
+  const uint32_t g1 = (uint32_t)p1 / (kWaves * S);
+  const int lead = g1 > g0 ? (int)(kWaves * g0 - u0) : (int)(u1 - u0 + 1);
+  const int mid = g1 > g0 ? (int)(g1 - g0) : 0;
+  const int n = lead + mid + (mid > 0 ? (int)(u1 + 1 - kWaves * g1) : 0);
   auto at_of = [&](int i) __attribute__((always_inline)) {
-    const int slot = i == 0 && (uint32_t)p0 != u0 * S ? 1 : 0;
-    return ((int64_t)(u0 + i) * 2 + slot) * a.group + h;
+    const uint32_t u = i < lead ? u0 + i
+                                : (i < lead + mid ? kWaves * (g0 + i - lead)
+                                                  : kWaves * g1 + (i - lead - mid));
+    const int slot = u == u0 && (uint32_t)p0 != u0 * S ? 1 : 0;
+    return (((int64_t)u * a.hkv + head) * 2 + slot) * a.group + h;
   };
   float m_run = -INFINITY, l_run = 0.f;
   f32x4 o_run = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -535,17 +609,44 @@ __global__ __launch_bounds__(64 * WAVES) void attn_fp4_merge_kernel(Args a) {
   out[tid] = f32_to_bf16_rne(L == 0.f ? 0.f : O / L);
 }
 
+// Workgroups of the span kernel: the resident ones, as many for each KV head.
+int64_t span_grid(int32_t hkv) {
+  const int64_t fit = (int64_t)device_cus() * kWgsPerCu / hkv;
+  return (fit < 1 ? 1 : fit) * hkv;
+}
+
 struct WsLayout {
   int64_t pre, ml, part, total;
 };
-WsLayout ws_layout(int64_t pairs, int64_t group) {
-  const int64_t waves = (int64_t)device_cus() * kWgsPerCu * kWaves;
+WsLayout ws_layout(int64_t batch, int32_t hkv, int64_t group) {
+  const int64_t pieces = span_grid(hkv) * kWaves * 2 * group;
   WsLayout w;
   w.pre = 256;
-  w.ml = w.pre + ((pairs + 1) * 4 + 255) / 256 * 256;
-  w.part = w.ml + waves * 2 * group * 2 * 4;
-  w.total = w.part + waves * 2 * group * kHeadDim * 4;
+  w.ml = w.pre + ((batch + 1) * 4 + 255) / 256 * 256;
+  w.part = w.ml + (pieces * 2 * 4 + 255) / 256 * 256;
+  w.total = w.part + pieces * kHeadDim * 4;
   return w;
+}
+
+// Launches the span kernel, once its LDS has been asked for on this device.
+template <bool ONE>
+int launch_spans(const Args& a, hipStream_t st, const char* fn) {
+  constexpr size_t most = kWaves * (2 * kTileLds + kMaxGroup * 2 * 4);
+  static std::atomic<uint64_t> asked[16];  // a bit a device
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) dev = 0;
+  const uint64_t bit = 1ull << (dev & 63);
+  std::atomic<uint64_t>& word = asked[(dev >> 6) & 15];
+  if (!(word.load(std::memory_order_relaxed) & bit)) {
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(attn_fp4_span_kernel<ONE>),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, most) != hipSuccess)
+      return set_error(MKV_E_LAUNCH, "%s: %zu bytes of LDS refused", fn, most);
+    word.fetch_or(bit, std::memory_order_relaxed);
+  }
+  const size_t lds = kWaves * (2 * kTileLds + (size_t)a.group * 2 * 4);
+  hipLaunchKernelGGL(attn_fp4_span_kernel<ONE>, dim3((unsigned)span_grid(a.hkv)), dim3(kThreads4),
+                     lds, st, a);
+  return MKV_OK;
 }
 
 bool shape_ok(int32_t batch, int32_t hkv, int32_t hq) {
@@ -561,7 +662,7 @@ using namespace mkv;
 extern "C" int64_t mkv_decode_attention_fp4_workspace_bytes(int32_t batch, int32_t num_kv_heads,
                                                             int32_t num_q_heads) {
   if (!shape_ok(batch, num_kv_heads, num_q_heads)) return -1;
-  return ws_layout((int64_t)batch * num_kv_heads, num_q_heads / num_kv_heads).total;
+  return ws_layout(batch, num_kv_heads, num_q_heads / num_kv_heads).total;
 }
 
 extern "C" int mkv_decode_attention_fp4(const void* q, const void* k_cache, const void* v_cache,
@@ -597,7 +698,7 @@ extern "C" int mkv_decode_attention_fp4(const void* q, const void* k_cache, cons
   MKV_REQUIRE((int64_t)batch * num_kv_heads * (((int64_t)max_seq_len + 15) / 16) < (1ll << 31),
               MKV_E_UNSUPPORTED, "%s: batch x KV heads x pages above 2^31", fn);
   const int32_t pairs = batch * num_kv_heads;
-  const WsLayout L = ws_layout(pairs, group);
+  const WsLayout L = ws_layout(batch, num_kv_heads, group);
   MKV_REQUIRE(workspace && workspace_bytes >= L.total && aligned16(workspace), MKV_E_INVALID,
               "%s: workspace of %lld bytes (16-byte aligned) required", fn, (long long)L.total);
   Args a;
@@ -619,13 +720,12 @@ extern "C" int mkv_decode_attention_fp4(const void* q, const void* k_cache, cons
   a.hkv = num_kv_heads;
   a.group = group;
   a.max_len = max_seq_len;
-  a.pairs = pairs;
+  a.batch = batch;
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
   a.err = err;
   const hipStream_t st = as_stream(stream);
-  const size_t lds = (size_t)kWaves * group * (kHeadDim + 2) * 4;
-  hipLaunchKernelGGL(attn_fp4_span_kernel, dim3((unsigned)(device_cus() * kWgsPerCu)),
-                     dim3(kThreads4), lds, st, a);
+  const int rc = num_kv_heads == 1 ? launch_spans<true>(a, st, fn) : launch_spans<false>(a, st, fn);
+  if (rc != MKV_OK) return rc;
   if (pairs < kWidePairs)
     hipLaunchKernelGGL(attn_fp4_merge_kernel<16>, dim3((unsigned)(pairs * group)), dim3(16 * 64), 0,
                        st, a);
