@@ -15,8 +15,7 @@
 //     they leave one piece. (Spans by workgroup, its waves taking the tiles in
 //     turn: a barrier for each sequence, 87 us instead of 81 at batch 256.)
 //   * Loads: page by page straight into a wave's LDS (global_load_lds, 16
-//     bytes a lane where rows are contiguous, else 4), two tiles in flight,
-//     the page ids a tile ahead of them. (Into registers in the operands' own
+//     bytes a lane), two tiles in flight, the page ids a tile ahead of them. (Into registers in the operands' own
 //     order a K row is a line for every lane, and the launch reached 5 TB/s.)
 //   * Scores on the matrix cores (16x16x32 bf16): A = the 16 K rows of a page,
 //     codes converted to bf16 with their scale (exact), B = the query heads in
@@ -47,8 +46,13 @@ constexpr int kQRow = kHeadDim * 2;
 constexpr int kThreads4 = 256;
 constexpr int kWaves = kThreads4 / 64;
 constexpr int kTile = 32;            // tokens of a tile: two pages
-constexpr int kPage = 16 * kFp4Row;  // bytes of a page of one head
-constexpr int kTileLds = 4 * kPage;  // a tile in LDS: K's two pages, then V's
+// A row in LDS: the nine aligned 16-byte chunks that it lies in (a row starts at a
+// multiple of 8, at byte 0 or 8 of its first chunk; an odd row's last chunk ends with it, an
+// even row has one behind it). Eight rows lie on different banks.
+constexpr int kRowLds = 144;
+constexpr int kPage = 16 * kRowLds;  // bytes of a page of one head there
+constexpr int kTileLds = 4 * kPage;  // a tile: K's two pages, then V's
+constexpr int kPageLoads = (kPage + 1023) / 1024;  // instructions of a page
 constexpr int kMaxGroup = 8;         // query heads per KV head
 constexpr int kMaxPairs = 4096;      // batch x KV heads
 constexpr int kXcds = 8;             // MI355X: workgroups go round robin over 8 XCDs
@@ -63,7 +67,7 @@ struct Args {
   const int32_t* table;  // [B, tstride]
   const int32_t* lens;   // [B]
   uint8_t* out;          // [B, Hkv * G, 256] bf16
-  int64_t* hdr;          // workspace: [0] places of a span
+  int32_t* hdr;          // workspace: the spans' sizes
   int32_t* pre;          // [B + 1] each sequence's first place
   float* ml;             // [spans, Hkv, 2, G, 2] (max, sum) of cut pieces, log2 units
   float* part;           // [spans, Hkv, 2, G, 256] their unnormalised outputs
@@ -71,6 +75,23 @@ struct Args {
   int32_t twidth, hkv, group, max_len, batch;
   float scale_log2;
   int32_t* err;
+};
+
+// The spans of the flat list: `least` places each, the first `more` one more.
+struct Spans {
+  int32_t least, more;
+  __device__ __forceinline__ int32_t start(int32_t u) const {
+    return u * least + (u < more ? u : more);
+  }
+  __device__ __forceinline__ int32_t of(int32_t place) const {  // of a place of the list
+    const int32_t head = more * (least + 1);
+    return place < head ? place / (least + 1) : more + (place - head) / least;
+  }
+  // whether the workgroup with span `first` has all its spans, and in the places p0 .. p1
+  __device__ __forceinline__ bool whole(int32_t first, int32_t p0, int32_t p1) const {
+    const int32_t s = start(first), e = start(first + kWaves);
+    return e - s >= kWaves && s >= p0 && e <= p1;
+  }
 };
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -93,8 +114,6 @@ __device__ __forceinline__ u32x4 dequant8(uint32_t w, float s) {
                mkv_fp4_pair(w, 3, s)};
 }
 
-// ONE: one KV head, a page's rows are contiguous.
-template <bool ONE>
 __global__ __launch_bounds__(kThreads4, kWgsPerCu) void attn_fp4_span_kernel(Args a) {
   // two tiles for each wave (in the end its piece [G][256]), the pieces' (m, l) [waves][G][2]
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -102,7 +121,7 @@ __global__ __launch_bounds__(kThreads4, kWgsPerCu) void attn_fp4_span_kernel(Arg
   __shared__ int32_t start_l[kWaves][2];  // (sequence, its first tile) that a span starts in
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int32_t hkv = ONE ? 1 : a.hkv;
+  const int32_t hkv = a.hkv;
   const int64_t cap = (int64_t)a.twidth * 16 < a.max_len ? (int64_t)a.twidth * 16 : a.max_len;
   // a sequence's cached tokens, cut to the table and the launch's bound
   auto length_of = [&](int b) __attribute__((always_inline)) {
@@ -146,7 +165,7 @@ __global__ __launch_bounds__(kThreads4, kWgsPerCu) void attn_fp4_span_kernel(Arg
   const int32_t total = T;
   T = T > 0 ? T - 1 : 0;  // (nothing starts at the place behind the last sequence)
   const int32_t spans = all / hkv * kWaves;
-  const int32_t S = T > spans ? (T + spans - 1) / spans : 1;
+  const Spans cut = {T / spans, T % spans};
   const int32_t first = unit / hkv * kWaves;
   const int32_t span = first + wave;
   // The sequences that this workgroup's spans start in (and, by workgroup 0, the prefixes
@@ -162,7 +181,7 @@ __global__ __launch_bounds__(kThreads4, kWgsPerCu) void attn_fp4_span_kernel(Arg
       if (b < a.batch) {
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-          const int64_t s = (int64_t)(first + w) * S;
+          const int32_t s = cut.start(first + w);
           if (s >= at && s < at + cnt) {
             start_l[w][0] = b;
             start_l[w][1] = at;
@@ -177,13 +196,13 @@ __global__ __launch_bounds__(kThreads4, kWgsPerCu) void attn_fp4_span_kernel(Arg
     }
     if (blockIdx.x == 0 && tid == 0) {
       a.pre[a.batch] = total;
-      a.hdr[0] = S;
+      a.hdr[0] = cut.least;
+      a.hdr[1] = cut.more;
     }
     __syncthreads();
   }
-  const int64_t s64 = (int64_t)span * S;
-  if (s64 >= T) return;  // (no barrier follows, but for workgroups with four spans)
-  const int32_t s0 = (int32_t)s64, s1 = s64 + S < T ? (int32_t)s64 + S : T;
+  const int32_t s0 = cut.start(span), s1 = cut.start(span + 1);
+  if (s0 >= s1) return;  // (no barrier follows, but for workgroups with four spans)
 
   // Of the two waves on a SIMD the arbiter favours the older one: with it alone the first
   // workgroup of a CU ends a third before the second. They take turns, tile by tile.
@@ -191,20 +210,22 @@ __global__ __launch_bounds__(kThreads4, kWgsPerCu) void attn_fp4_span_kernel(Arg
   const int c = lane & 15, g = lane >> 4;  // row / column and quad of a matrix operand
   const uint32_t low_mask = c < 8 ? 0u : 0xffff0000u;  // what the lane takes off a weight
   const int32_t row_bytes = hkv * kFp4Row;
+  // page ids read through the caches: shared ones, and all where KV heads share lines
+  const int64_t hot_below = hkv > 1 ? a.num_pages : a.shared_below;
   const uint32_t num_pages = a.num_pages < INT32_MAX ? (uint32_t)a.num_pages : INT32_MAX;
   float* ml_l = reinterpret_cast<float*>(lds + 2 * kWaves * kTileLds);
   const uint32_t tile_l = lds_addr(lds + wave * 2 * kTileLds);
-  const uint32_t get_k = c * kFp4Row + 16 * g;  // dims 32 g .. and 128 + 32 g ..
-  const uint32_t get_ks = c * kFp4Row + kFp4Codes + g;
-  const uint32_t get_v = 2 * kPage + 4 * g * kFp4Row + 8 * c;  // dims 16 c ..
-  const uint32_t get_vs = 2 * kPage + 4 * g * kFp4Row + kFp4Codes + c / 2;
-  // a page's rows of one head among hkv: word i is row i / 34, word i % 34 of it
-  constexpr int kWords = ONE ? 1 : (kPage / 4 + 63) / 64;
-  uint32_t word_off[kWords];
+  const uint32_t odd_k = ((c * hkv + head) & 1) * 8;  // where a row starts in its first chunk
+  const uint32_t odd_v[2] = {(head & 1) * 8u, ((hkv + head) & 1) * 8u};  // of rows 4 g + j, j even, odd
+  const uint32_t get_k = c * kRowLds + odd_k + 16 * g;  // dims 32 g .. and 128 + 32 g ..
+  const uint32_t get_ks = c * kRowLds + odd_k + kFp4Codes + g;
+  const uint32_t get_v = 2 * kPage + 4 * g * kRowLds + 8 * c;  // dims 16 c ..
+  const uint32_t get_vs = 2 * kPage + 4 * g * kRowLds + kFp4Codes + c / 2;
+  uint32_t chunk_off[kPageLoads];  // of a page's rows of this head, chunk 64 j + lane
 #pragma unroll
-  for (int j = 0; j < kWords; ++j) {
-    const int i = 64 * j + lane;
-    word_off[j] = ONE ? 16 * lane : (i / (kFp4Row / 4)) * row_bytes + (i % (kFp4Row / 4)) * 4;
+  for (int j = 0; j < kPageLoads; ++j) {
+    const int i = 64 * j + lane, r = i / (kRowLds / 16);
+    chunk_off[j] = ((r * row_bytes + head * kFp4Row) & ~15) + 16 * (i % (kRowLds / 16));
   }
 
   // a sequence as the walk over the span has it: its tiles' places are pre0 .. pre1
@@ -268,30 +289,25 @@ __global__ __launch_bounds__(kThreads4, kWgsPerCu) void attn_fp4_span_kernel(Arg
         id = 0;
         valid = 0;
       }
-      w.hot |= id < a.shared_below ? 1 << i : 0;
-      base = (int64_t)id * (16 * row_bytes) + head * kFp4Row;
+      w.hot |= id < hot_below ? 1 << i : 0;
+      base = (int64_t)id * (16 * row_bytes);
     };
     page(0, x.id0, x.left, w.base0, w.valid0);
     page(1, x.id1, x.left - 16, w.base1, w.valid1);
     return w;
   };
-  constexpr int kPageLoads = ONE ? 3 : kWords;  // instructions of a page's rows
+  // a page's rows to LDS, kPageLoads instructions
   auto load_page = [&](const uint8_t* src, uint32_t dst, bool hot) __attribute__((always_inline)) {
     lds_reads_done();
-    if constexpr (ONE) {
-      if (hot) {
-        dma16_cached(src, word_off[0], dst);
-        dma16_cached(src + 1024, word_off[0], dst + 1024);
-        if (lane < 8) dma16_cached(src + 2048, word_off[0], dst + 2048);
-      } else {
-        dma16(src, word_off[0], dst);
-        dma16(src + 1024, word_off[0], dst + 1024);
-        if (lane < 8) dma16(src + 2048, word_off[0], dst + 2048);
-      }
+    constexpr int kRest = (kPage % 1024) / 16;  // chunks of the last instruction
+    if (hot) {
+      dma16_cached(src, chunk_off[0], dst);
+      dma16_cached(src, chunk_off[1], dst + 1024);
+      if (lane < kRest) dma16_cached(src, chunk_off[2], dst + 2048);
     } else {
-#pragma unroll
-      for (int j = 0; j < kWords - 1; ++j) dma4_at_cached(src, word_off[j], dst + 256 * j);
-      if (lane < 32) dma4_at_cached(src, word_off[kWords - 1], dst + 256 * (kWords - 1));
+      dma16(src, chunk_off[0], dst);
+      dma16(src, chunk_off[1], dst + 1024);
+      if (lane < kRest) dma16(src, chunk_off[2], dst + 2048);
     }
   };
   auto load_k = [&](Where w, uint32_t slot) __attribute__((always_inline)) {
@@ -406,7 +422,7 @@ __global__ __launch_bounds__(kThreads4, kWgsPerCu) void attn_fp4_span_kernel(Arg
       float vsc[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const uint32_t row = (j >> 2) * kPage + (j & 3) * kFp4Row;
+        const uint32_t row = (j >> 2) * kPage + (j & 3) * kRowLds + odd_v[j & 1];
         v[j] = lds_get<u32x2>(slot + get_v + row);
         vsc[j] = fp4_scale(lds_get<uint8_t>(slot + get_vs + row));
       }
@@ -449,66 +465,78 @@ __global__ __launch_bounds__(kThreads4, kWgsPerCu) void attn_fp4_span_kernel(Arg
       f = cur.pre0;
       load_q();
     }
-    // the sequence's piece in this span: the quads' sums, and the weights' two parts
+    // The sequence's piece in this span: the quads' sums, and those of the weights' two
+    // parts, which the wave's halves hold. A swap of the halves of two tiles leaves both sums
+    // in half the registers: lanes below 32 have the dims 16 c .. + 7, the others 16 c + 8 ..,
+    // of the heads 4 (g % 2) + i.
     const float l = over_rows<4>(l_run, [](float x, float y) { return x + y; });
+    float o[8][4];
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
+    for (int j = 0; j < 8; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[j][i] += __shfl_xor(acc[j][i], 32);
+      for (int i = 0; i < 4; ++i) {
+        const auto r = __builtin_amdgcn_permlane32_swap(f32_bits(acc[j][i]), f32_bits(acc[j + 8][i]),
+                                                        false, false);
+        o[j][i] = bits_f32(r[0]) + bits_f32(r[1]);
+      }
+    const int h0 = 4 * (g & 1), d0 = 16 * c + 8 * (g >> 1);
     const bool whole = done.pre0 >= s0 && done.pre1 <= s1;
     // (cut sequences: the span's first goes to slot 0, its last to slot 1)
     const int64_t piece =
         (((int64_t)span * hkv + head) * 2 + (done.pre0 <= s0 ? 0 : 1)) * a.group;
     uint8_t* out = a.out + ((int64_t)done.b * hkv + head) * a.group * kQRow;
     // the workgroup's spans lie in one sequence: one piece, its first span's
-    const bool joint = done.pre0 <= first * S && done.pre1 >= (first + kWaves) * (int64_t)S;
-    if (joint && lane < a.group) {
-      ml_l[(wave * a.group + lane) * 2] = m_run;
-      ml_l[(wave * a.group + lane) * 2 + 1] = l;
-    }
+    const bool joint = cut.whole(first, done.pre0, done.pre1);
     float* piece_l = reinterpret_cast<float*>(lds + wave * 2 * kTileLds);
+    if (lane < a.group) {
+      float* ml = joint ? ml_l + (wave * a.group + lane) * 2 : a.ml + (piece + lane) * 2;
+      if (!whole) {
+        ml[0] = m_run;
+        ml[1] = l;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int h = 4 * g + i;
-      const float L = __shfl(l, h & 7), M = __shfl(m_run, h & 7);
-      if (h >= a.group) continue;  // (rows 8 and up are the other part)
+      const int h = h0 + i;
+      const float L = __shfl(l, h);
+      if (h >= a.group) continue;
       if (whole) {
         const float inv = 1.f / L;
-        uint32_t o[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          o[j] = L == 0.f ? 0u : pack_bf16(acc[2 * j][i] * inv, acc[2 * j + 1][i] * inv);
-        st16(out + h * kQRow + c * 32, u32x4{o[0], o[1], o[2], o[3]});
-        st16(out + h * kQRow + c * 32 + 16, u32x4{o[4], o[5], o[6], o[7]});
-      } else {
-        float* dst = joint ? piece_l + h * kHeadDim + c * 16 : a.part + (piece + h) * kHeadDim + c * 16;
+        uint32_t w[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          *reinterpret_cast<f32x4*>(dst + 4 * j) = f32x4{acc[4 * j][i], acc[4 * j + 1][i],
-                                                         acc[4 * j + 2][i], acc[4 * j + 3][i]};
-        if (!joint && c == 0) {
-          a.ml[(piece + h) * 2] = M;
-          a.ml[(piece + h) * 2 + 1] = L;
-        }
+          w[j] = L == 0.f ? 0u : pack_bf16(o[2 * j][i] * inv, o[2 * j + 1][i] * inv);
+        st16(out + h * kQRow + 2 * d0, u32x4{w[0], w[1], w[2], w[3]});
+      } else {
+        float* dst = (joint ? piece_l + h * kHeadDim : a.part + (piece + h) * kHeadDim) + d0;
+        *reinterpret_cast<f32x4*>(dst) = f32x4{o[0][i], o[1][i], o[2][i], o[3][i]};
+        *reinterpret_cast<f32x4*>(dst + 4) = f32x4{o[4][i], o[5][i], o[6][i], o[7][i]};
       }
     }
     if (joint) {
       __syncthreads();
       const int64_t at = ((int64_t)first * hkv + head) * 2 * a.group;
-      for (int h = 0; h < a.group; ++h) {  // a thread per dim
-        float M = -INFINITY, O = 0.f, L = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) M = fmaxf(M, ml_l[(w * a.group + h) * 2]);
+      for (int h = wave; h < a.group; h += kWaves) {  // a head a wave, four dims a lane
+        float m[kWaves], ls[kWaves], M = -INFINITY, L = 0.f;
+        f32x4 x[kWaves], O = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-          const float m = ml_l[(w * a.group + h) * 2];
-          // (a wave without a score: 1, so that a NaN of its sums stays)
-          const float e = m == -INFINITY ? 1.f : exp2_fast(m - M);
-          O += e * reinterpret_cast<const float*>(lds + w * 2 * kTileLds)[h * kHeadDim + tid];
-          L += e * ml_l[(w * a.group + h) * 2 + 1];
+          m[w] = ml_l[(w * a.group + h) * 2];
+          ls[w] = ml_l[(w * a.group + h) * 2 + 1];
+          x[w] = reinterpret_cast<const f32x4*>(lds + w * 2 * kTileLds)[h * (kHeadDim / 4) + lane];
         }
-        a.part[(at + h) * kHeadDim + tid] = O;
-        if (tid == 0) {
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) M = fmaxf(M, m[w]);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+          // (a wave without a score: 1, so that a NaN of its sums stays)
+          const float e = m[w] == -INFINITY ? 1.f : exp2_fast(m[w] - M);
+#pragma unroll
+          for (int d = 0; d < 4; ++d) O[d] += e * x[w][d];
+          L += e * ls[w];
+        }
+        *reinterpret_cast<f32x4*>(a.part + (at + h) * kHeadDim + 4 * lane) = O;
+        if (lane == 0) {
           a.ml[(at + h) * 2] = M;
           a.ml[(at + h) * 2 + 1] = L;
         }
@@ -531,30 +559,30 @@ __global__ __launch_bounds__(64 * WAVES) void attn_fp4_merge_kernel(Args a) {
   const int b = pr / a.hkv, head = pr - b * a.hkv;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t span = ld_const(a.hdr);  // (loaded beside the sequence's bounds)
+  const Spans cut = {ld_const(a.hdr), ld_const(a.hdr + 1)};  // (with the sequence's bounds)
   const int32_t p0 = ld_const(a.pre + b);
   int32_t p1 = ld_const(a.pre + b + 1);
-  asm volatile("" ::"s"(span));
+  asm volatile("" ::"s"(cut.least), "s"(cut.more));
   uint16_t* out = reinterpret_cast<uint16_t*>(a.out + ((int64_t)pr * a.group + h) * kQRow);
   if (p1 <= p0) {
     if (tid < kHeadDim) out[tid] = 0;
     return;
   }
   --p1;  // without the place behind its tiles
-  const uint32_t S = (uint32_t)span;
-  const uint32_t u0 = (uint32_t)p0 / S, u1 = (uint32_t)(p1 - 1) / S;
+  const int32_t u0 = cut.of(p0), u1 = cut.of(p1 - 1);
   if (u0 == u1) return;  // written with its span
-  // spans u0 .. u1; those of the workgroups that lie in the sequence, g0 .. g1, as one each
-  const uint32_t g0 = ((uint32_t)p0 + kWaves * S - 1) / (kWaves * S);
-  const uint32_t g1 = (uint32_t)p1 / (kWaves * S);
-  const int lead = g1 > g0 ? (int)(kWaves * g0 - u0) : (int)(u1 - u0 + 1);
-  const int mid = g1 > g0 ? (int)(g1 - g0) : 0;
-  const int n = lead + mid + (mid > 0 ? (int)(u1 + 1 - kWaves * g1) : 0);
+  // spans u0 .. u1; those of the workgroups g0 .. g1 that lie in the sequence as one each
+  int32_t g0 = u0 / kWaves, g1 = u1 / kWaves + 1;
+  g0 += cut.start(g0 * kWaves) < p0 ? 1 : 0;
+  g1 -= cut.whole(kWaves * (g1 - 1), p0, p1) ? 0 : 1;
+  const int mid = g1 > g0 ? g1 - g0 : 0;
+  const int lead = mid > 0 ? kWaves * g0 - u0 : u1 - u0 + 1;
+  const int n = lead + mid + (mid > 0 ? u1 + 1 - kWaves * g1 : 0);
   auto at_of = [&](int i) __attribute__((always_inline)) {
-    const uint32_t u = i < lead ? u0 + i
-                                : (i < lead + mid ? kWaves * (g0 + i - lead)
-                                                  : kWaves * g1 + (i - lead - mid));
-    const int slot = u == u0 && (uint32_t)p0 != u0 * S ? 1 : 0;
+    const int32_t u = i < lead ? u0 + i
+                               : (i < lead + mid ? kWaves * (g0 + i - lead)
+                                                 : kWaves * g1 + (i - lead - mid));
+    const int slot = u == u0 && p0 != cut.start(u0) ? 1 : 0;
     return (((int64_t)u * a.hkv + head) * 2 + slot) * a.group + h;
   };
   float m_run = -INFINITY, l_run = 0.f;
@@ -629,7 +657,6 @@ WsLayout ws_layout(int64_t batch, int32_t hkv, int64_t group) {
 }
 
 // Launches the span kernel, once its LDS has been asked for on this device.
-template <bool ONE>
 int launch_spans(const Args& a, hipStream_t st, const char* fn) {
   constexpr size_t most = kWaves * (2 * kTileLds + kMaxGroup * 2 * 4);
   static std::atomic<uint64_t> asked[16];  // a bit a device
@@ -638,13 +665,13 @@ int launch_spans(const Args& a, hipStream_t st, const char* fn) {
   const uint64_t bit = 1ull << (dev & 63);
   std::atomic<uint64_t>& word = asked[(dev >> 6) & 15];
   if (!(word.load(std::memory_order_relaxed) & bit)) {
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(attn_fp4_span_kernel<ONE>),
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(attn_fp4_span_kernel),
                             hipFuncAttributeMaxDynamicSharedMemorySize, most) != hipSuccess)
       return set_error(MKV_E_LAUNCH, "%s: %zu bytes of LDS refused", fn, most);
     word.fetch_or(bit, std::memory_order_relaxed);
   }
   const size_t lds = kWaves * (2 * kTileLds + (size_t)a.group * 2 * 4);
-  hipLaunchKernelGGL(attn_fp4_span_kernel<ONE>, dim3((unsigned)span_grid(a.hkv)), dim3(kThreads4),
+  hipLaunchKernelGGL(attn_fp4_span_kernel, dim3((unsigned)span_grid(a.hkv)), dim3(kThreads4),
                      lds, st, a);
   return MKV_OK;
 }
@@ -709,7 +736,7 @@ extern "C" int mkv_decode_attention_fp4(const void* q, const void* k_cache, cons
   a.lens = seq_lens;
   a.out = static_cast<uint8_t*>(out);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  a.hdr = reinterpret_cast<int64_t*>(ws);
+  a.hdr = reinterpret_cast<int32_t*>(ws);
   a.pre = reinterpret_cast<int32_t*>(ws + L.pre);
   a.ml = reinterpret_cast<float*>(ws + L.ml);
   a.part = reinterpret_cast<float*>(ws + L.part);
@@ -724,7 +751,7 @@ extern "C" int mkv_decode_attention_fp4(const void* q, const void* k_cache, cons
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
   a.err = err;
   const hipStream_t st = as_stream(stream);
-  const int rc = num_kv_heads == 1 ? launch_spans<true>(a, st, fn) : launch_spans<false>(a, st, fn);
+  const int rc = launch_spans(a, st, fn);
   if (rc != MKV_OK) return rc;
   if (pairs < kWidePairs)
     hipLaunchKernelGGL(attn_fp4_merge_kernel<16>, dim3((unsigned)(pairs * group)), dim3(16 * 64), 0,
