@@ -358,30 +358,14 @@ def attn_decode_fp8(
 
 FP4_ROW = 136  # bytes of a 4-bit row: 128 of codes, 8 scales
 
+# What attn_decode_fp4's arguments come to, by their types, shapes, strides and
+# devices alone (checking them anew takes 6 us of a call's 14).
+_fp4_plans: dict[tuple, tuple] = {}
+_FP4_PLANS = 4096
 
-@functools.lru_cache(maxsize=1024)
-def _fp4_bytes(batch: int, num_kv_heads: int, num_q_heads: int, dev: torch.device) -> int:
-    return _lib.load().mkv_decode_attention_fp4_workspace_bytes(batch, num_kv_heads, num_q_heads)
 
-
-def attn_decode_fp4(
-    q: torch.Tensor,                    # [B, 1, NUM_Q_HEADS, HEAD_DIM] bf16
-    k_cache: torch.Tensor,              # [num_pages, PAGE_SIZE, NUM_KV_HEADS, 136] uint8
-    v_cache: torch.Tensor,              # [num_pages, PAGE_SIZE, NUM_KV_HEADS, 136] uint8
-    cache_seqlens: torch.Tensor,        # [B] int32
-    page_table: torch.Tensor,           # [B, max_pages] int32
-    softmax_scale: float | None = None,
-    *,
-    max_seqlen: int | None = None,
-    out: torch.Tensor | None = None,
-    shared_pages: int = 0,
-) -> torch.Tensor:                      # [B, 1, NUM_Q_HEADS, HEAD_DIM] bf16
-    """``attn_decode`` over a 4-bit pool (``cache.get_kv_by_layer(l)`` of a
-    ``PagedKVCache`` with ``dtype=torch.float4_e2m1fn_x2``), dequantised in
-    registers: a cached value is ``code * 2**e``, exactly. 1 to 8 query heads
-    per KV head; the other arguments are ``attn_decode``'s."""
-    if page_table is None:
-        raise ValueError("attn_decode_fp4 reads the paged pool: page_table is required")
+def _fp4_check(q, k_cache, v_cache, cache_seqlens, page_table):
+    """(device, the sizes of the call by ctypes, workspace bytes, keys the table holds)."""
     dev = _lib.require_gpu(q, k_cache, v_cache, cache_seqlens, page_table)
     if k_cache.dtype != torch.uint8 or v_cache.dtype != torch.uint8:
         raise TypeError("attn_decode_fp4 takes uint8 caches of 4-bit rows")
@@ -402,10 +386,53 @@ def attn_decode_fp4(
     if not (q.is_contiguous() and k_cache.is_contiguous() and v_cache.is_contiguous()
             and cache_seqlens.is_contiguous() and (width <= 1 or page_table.stride(1) == 1)):
         raise ValueError("q, caches, cache_seqlens and page_table rows must be contiguous")
+    stride = page_table.stride(0) if B > 1 else width
+    if stride < width:
+        raise ValueError("page_table rows must not overlap")
+    nbytes = _lib.load().mkv_decode_attention_fp4_workspace_bytes(B, Hkv, Hq)
+    if nbytes < 0:
+        raise ValueError(f"unsupported shapes q {tuple(q.shape)}, cache {tuple(k_cache.shape)} "
+                         "(1 to 8 query heads per KV head, batch x KV heads up to 4096)")
+    name = "mkv_decode_attention_fp4"
+    return (dev, _lib.constants(name, 3, P)[0], _lib.constants(name, 5, Hkv, Hq, D),
+            _lib.constants(name, 9, stride, width), _lib.constants(name, 12, B)[0], nbytes,
+            width * 16)
+
+
+def attn_decode_fp4(
+    q: torch.Tensor,                    # [B, 1, NUM_Q_HEADS, HEAD_DIM] bf16
+    k_cache: torch.Tensor,              # [num_pages, PAGE_SIZE, NUM_KV_HEADS, 136] uint8
+    v_cache: torch.Tensor,              # [num_pages, PAGE_SIZE, NUM_KV_HEADS, 136] uint8
+    cache_seqlens: torch.Tensor,        # [B] int32
+    page_table: torch.Tensor,           # [B, max_pages] int32
+    softmax_scale: float | None = None,
+    *,
+    max_seqlen: int | None = None,
+    out: torch.Tensor | None = None,
+    shared_pages: int = 0,
+) -> torch.Tensor:                      # [B, 1, NUM_Q_HEADS, HEAD_DIM] bf16
+    """``attn_decode`` over a 4-bit pool (``cache.get_kv_by_layer(l)`` of a
+    ``PagedKVCache`` with ``dtype=torch.float4_e2m1fn_x2``), dequantised in
+    registers: a cached value is ``code * 2**e``, exactly. 1 to 8 query heads
+    per KV head; the other arguments are ``attn_decode``'s."""
+    if page_table is None:
+        raise ValueError("attn_decode_fp4 reads the paged pool: page_table is required")
+    key = (q.dtype, q.shape, q.is_contiguous(), q.get_device(), k_cache.dtype, k_cache.shape,
+           k_cache.is_contiguous(), k_cache.get_device(), v_cache.dtype, v_cache.shape,
+           v_cache.is_contiguous(), v_cache.get_device(), cache_seqlens.dtype,
+           cache_seqlens.shape, cache_seqlens.is_contiguous(), cache_seqlens.get_device(),
+           page_table.dtype, page_table.shape, page_table.stride(), page_table.get_device())
+    plan = _fp4_plans.get(key)
+    if plan is None:
+        plan = _fp4_check(q, k_cache, v_cache, cache_seqlens, page_table)
+        if len(_fp4_plans) >= _FP4_PLANS:
+            _fp4_plans.clear()
+        _fp4_plans[key] = plan
+    dev, pages, heads, table, batch, nbytes, held = plan
     if shared_pages < 0:
         raise ValueError("shared_pages must be >= 0")
     if max_seqlen is None:
-        max_seqlen = width * 16
+        max_seqlen = held
     elif max_seqlen < 0:
         raise ValueError("bad attention shape")
     if out is None:
@@ -413,16 +440,12 @@ def attn_decode_fp4(
     elif (out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous()
           or out.device != dev):
         raise ValueError("out must be a contiguous tensor shaped like q")
-    scale = D ** -0.5 if softmax_scale is None else float(softmax_scale)
-    nbytes = _fp4_bytes(B, Hkv, Hq, dev)
-    if nbytes < 0:
-        raise ValueError(f"unsupported shapes q {tuple(q.shape)}, cache {tuple(k_cache.shape)} "
-                         "(1 to 8 query heads per KV head, batch x KV heads up to 4096)")
     ws = _scratch(nbytes, dev)
     _lib.call_on(dev, "mkv_decode_attention_fp4", q.data_ptr(), k_cache.data_ptr(),
-                 v_cache.data_ptr(), P, shared_pages, Hkv, Hq, D, page_table.data_ptr(),
-                 max(page_table.stride(0), width), width, cache_seqlens.data_ptr(), B, max_seqlen,
-                 scale, out.data_ptr(), ws.data_ptr(), nbytes, _errword(dev).ptr())
+                 v_cache.data_ptr(), pages, shared_pages, *heads, page_table.data_ptr(), *table,
+                 cache_seqlens.data_ptr(), batch, max_seqlen,
+                 HEAD_DIM ** -0.5 if softmax_scale is None else float(softmax_scale),
+                 out.data_ptr(), ws.data_ptr(), nbytes, _errword(dev).word.data_ptr())
     return out
 
 

@@ -23,10 +23,6 @@ _plans: dict[tuple, tuple] = {}
 _PLANS = 4096
 
 
-def _sig(t: torch.Tensor | None):
-    return None if t is None else (t.dtype, t.shape, t.stride(), t.get_device())
-
-
 def _heads(name: str, t: torch.Tensor, tokens: int, dim: int, dtype: torch.dtype):
     """(heads, bytes between tokens, bytes between heads) of t [tokens, heads, dim]."""
     if t.dtype != dtype:
@@ -74,14 +70,26 @@ def _check(q, k, v, positions, inv_freq, q_weight, k_weight, interleaved):
         if kind and kind != _WEIGHT_KINDS[w.dtype]:
             raise TypeError("q_weight and k_weight must be of one type")
         kind = _WEIGHT_KINDS[w.dtype]
-    return (dev, positions.dtype == torch.int64, (q_token, q_head), (k_token, k_head), strides,
-            (tokens, hq, hk, dim, 1 if q.dtype == torch.float16 else 0),
-            (1 if inv_freq.dtype == torch.float64 else 0, rot, 1 if interleaved else 0), kind)
+    name, at = ("mkv_qk_norm_rope", 6) if v is None else ("mkv_append_rope", 9)
+    direct = positions.dtype == torch.int64 and positions.is_contiguous()
+    return (dev, direct, _lib.constants(name, 1, q_token, q_head),
+            _lib.constants(name, 4, k_token, k_head), _lib.constants(name, 7, *strides),
+            _lib.constants(name, at, tokens, hq, hk, dim, 1 if q.dtype == torch.float16 else 0),
+            _lib.constants(name, at + 7, 1 if inv_freq.dtype == torch.float64 else 0, rot,
+                           1 if interleaved else 0), kind)
 
 
 def _plan(q, k, v, positions, inv_freq, q_weight, k_weight, interleaved):
-    key = (_sig(q), _sig(k), _sig(v), _sig(positions), _sig(inv_freq), _sig(q_weight),
-           _sig(k_weight), interleaved)
+    # (attributes in a row: a helper for each tensor costs half as much again)
+    key = (q.dtype, q.shape, q.stride(), q.get_device(), k.dtype, k.shape, k.stride(),
+           k.get_device(), positions.dtype, positions.shape, positions.is_contiguous(),
+           positions.get_device(), inv_freq.dtype, inv_freq.shape, inv_freq.is_contiguous(),
+           inv_freq.get_device(), interleaved,
+           None if q_weight is None else (q_weight.dtype, q_weight.shape,
+                                          q_weight.is_contiguous(), q_weight.get_device()),
+           None if k_weight is None else (k_weight.dtype, k_weight.shape,
+                                          k_weight.is_contiguous(), k_weight.get_device()),
+           None if v is None else (v.dtype, v.shape, v.stride(), v.get_device()))
     plan = _plans.get(key)
     if plan is None:
         plan = _check(q, k, v, positions, inv_freq, q_weight, k_weight, interleaved)
@@ -143,21 +151,20 @@ def qk_norm_rope(
     elements); the outputs are contiguous, and ``out`` may be the inputs
     themselves where those are."""
     plan = _plan(q, k, None, positions, inv_freq, q_weight, k_weight, interleaved)
-    dev, long, q_strides, k_strides, _, sizes, freq, kind = plan
+    dev, direct, q_strides, k_strides, _, sizes, freq, kind = plan
     if out is None:
         q_out, k_out = _like(q), _like(k)
     else:
         q_out, k_out = out
         _given("out[0]", q_out, q, (k, positions, inv_freq, q_weight, k_weight))
         _given("out[1]", k_out, k, (q, q_out, positions, inv_freq, q_weight, k_weight))
-    if not long:
-        positions = positions.long()
-    elif not positions.is_contiguous():
-        positions = positions.contiguous()
+    if not direct:
+        positions = positions.long().contiguous()
     _lib.call_on(dev, "mkv_qk_norm_rope", q.data_ptr(), *q_strides, k.data_ptr(), *k_strides,
                  *sizes, positions.data_ptr(), inv_freq.data_ptr(), *freq, rope_scale,
-                 _lib.ptr(q_weight), _lib.ptr(k_weight), kind, 1 if zero_centered else 0, eps,
-                 q_out.data_ptr(), k_out.data_ptr())
+                 None if q_weight is None else q_weight.data_ptr(),
+                 None if k_weight is None else k_weight.data_ptr(), kind, 1 if zero_centered else 0,
+                 eps, q_out.data_ptr(), k_out.data_ptr())
     return q_out, k_out
 
 
@@ -169,18 +176,17 @@ def append_rope(q, k, v, positions, inv_freq, q_weight, k_weight, eps, rope_scal
     """``PagedKVCache.append_rope`` once the pool is known: ``pool`` is (type,
     K plane, V plane, K scales, V scales, slots) by address."""
     plan = _plan(q, k, v, positions, inv_freq, q_weight, k_weight, interleaved)
-    dev, long, q_strides, k_strides, v_strides, sizes, freq, kind = plan
+    dev, direct, q_strides, k_strides, v_strides, sizes, freq, kind = plan
     if out is None:
         out = _like(q)
     else:
         _given("out", out, q, (k, v, positions, inv_freq, q_weight, k_weight, slots))
-    if not long:
-        positions = positions.long()
-    elif not positions.is_contiguous():
-        positions = positions.contiguous()
+    if not direct:
+        positions = positions.long().contiguous()
     _lib.call_on(dev, "mkv_append_rope", q.data_ptr(), *q_strides, k.data_ptr(), *k_strides,
                  v.data_ptr(), *v_strides, *sizes, positions.data_ptr(), inv_freq.data_ptr(), *freq,
-                 rope_scale, _lib.ptr(q_weight), _lib.ptr(k_weight), kind,
+                 rope_scale, None if q_weight is None else q_weight.data_ptr(),
+                 None if k_weight is None else k_weight.data_ptr(), kind,
                  1 if zero_centered else 0, eps, out.data_ptr(), *pool, slots.data_ptr(),
-                 errors.ptr())
+                 errors.word.data_ptr())
     return out

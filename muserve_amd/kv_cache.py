@@ -100,6 +100,8 @@ class PagedKVCache:
         self._row_bytes = kv_heads_per_rank * self.cache.shape[-1] * self.cache.element_size()
         # what K and V are outside the pool
         self._value_dtype = torch.bfloat16 if dtype in (_FP8, _FP4) else dtype
+        self._rope_pool = (rope.POOL_FP8 if dtype == _FP8 else
+                           rope.POOL_FP4 if dtype == _FP4 else rope.POOL_16)
         # fp8 pools carry one fp32 scale per (token, head): [L, 2, P, 16, H]
         self.scales = (torch.zeros(num_layers, 2, num_gpu_pages, KV_PAGE_SIZE, kv_heads_per_rank,
                                    dtype=torch.float32, device=device)
@@ -261,7 +263,7 @@ class PagedKVCache:
             return
         if self.check_unique:
             self._check_slots(slot_mapping)
-        kp, vp = self._planes(first)
+        kp, vp = self._planes(first)  # (views of them are two indexings each)
         src_layer = T * self.row_elems * 2
         src_tok = self.row_elems * 2
         stream = _lib.stream_of(dev)
@@ -312,12 +314,11 @@ class PagedKVCache:
                              f"{self.head_dim}], got {tuple(k.shape)}")
         if self.dtype == _FP8 and self.head_dim != 256:
             raise ValueError("append_rope into an fp8 pool takes heads of 256 dims")
-        _lib.require_gpu(q, k, v, positions, inv_freq, slot_mapping, self.cache)
+        if q.device != self.cache.device:
+            raise RuntimeError(f"q on {q.device}, the pool on {self.cache.device}")
         if self.check_unique and k.shape[0]:
             self._check_slots(slot_mapping)
-        kind = rope.POOL_FP8 if self.dtype == _FP8 else \
-            rope.POOL_FP4 if self.dtype == _FP4 else rope.POOL_16
-        pool = (kind, *self._planes(first), *self._scale_planes(first), self.num_slots)
+        pool = (self._rope_pool, *self._planes(first), *self._scale_planes(first), self.num_slots)
         return rope.append_rope(q, k, v, positions, inv_freq, q_weight, k_weight, eps, rope_scale,
                                 zero_centered, interleaved, out, slot_mapping, pool, self._errors)
 
@@ -333,7 +334,7 @@ class PagedKVCache:
         return first % self.num_layers
 
     def _planes(self, layer: int) -> tuple[int, int]:
-        """The layer's K and V plane by address (views of them are two indexings each)."""
+        """The layer's K and V plane by address."""
         plane = self.num_slots * self._row_bytes
         kp = self.cache.data_ptr() + 2 * layer * plane
         return kp, kp + plane
@@ -411,31 +412,35 @@ class PagedKVCache:
                                  or v_out.numel() != k_out.numel()):
                 raise ValueError(f"packed out buffers must hold whole rows for {L} layers")
         _lib.require_gpu(block_tables, seq_lens, k_out, v_out, self.cache)
+        # conversions are no-ops in a serving loop, and made only where something differs
         if starts is not None:
             starts = starts.to(device=dev, dtype=torch.int32).contiguous()
-        offs = None if cu_out is None else cu_out.to(device=dev, dtype=torch.int64).contiguous()
-        seq_lens = seq_lens.contiguous()
+        offs = cu_out
+        if offs is not None and (offs.dtype != torch.int64 or offs.device != dev
+                                 or not offs.is_contiguous()):
+            offs = offs.to(device=dev, dtype=torch.int64).contiguous()
+        if not seq_lens.is_contiguous():
+            seq_lens = seq_lens.contiguous()
         out_elem = 2
         out_layer_stride = (k_out.numel() // L) * out_elem
         stream = _lib.stream_of(dev)
-        kp, vp = self.cache[first, 0], self.cache[first, 1]
+        kp, vp = self._planes(first)  # (by address, as in append)
         if self.dtype == _FP8:
-            _lib.call("mkv_gather_dequant_fp8", kp.data_ptr(), vp.data_ptr(),
-                      self.scales[first, 0].data_ptr(), self.scales[first, 1].data_ptr(),
+            _lib.call("mkv_gather_dequant_fp8", kp, vp, *self._scale_planes(first),
                       self._plane_layer_stride(), self._scale_layer_stride(), self.num_pages,
                       block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1],
                       seq_lens.data_ptr(), _lib.ptr(starts), B, out_len, _lib.ptr(offs),
                       k_out.data_ptr(), v_out.data_ptr(), out_layer_stride, L, self.kv_heads,
                       self.head_dim, self._errors.ptr(), stream)
         elif self.dtype == _FP4:
-            _lib.call_on(self.cache.device, "mkv_gather_dequant_fp4", kp.data_ptr(), vp.data_ptr(),
+            _lib.call_on(self.cache.device, "mkv_gather_dequant_fp4", kp, vp,
                          self._plane_layer_stride(), self.num_pages, block_tables.data_ptr(),
                          block_tables.stride(0), block_tables.shape[1], seq_lens.data_ptr(),
                          _lib.ptr(starts), B, out_len, _lib.ptr(offs), k_out.data_ptr(),
                          v_out.data_ptr(), out_layer_stride, L, self.kv_heads, self.head_dim,
                          self._errors.ptr())
         else:
-            _lib.call("mkv_gather_bf16", kp.data_ptr(), vp.data_ptr(), self._plane_layer_stride(),
+            _lib.call("mkv_gather_bf16", kp, vp, self._plane_layer_stride(),
                       self.num_pages, block_tables.data_ptr(), block_tables.stride(0),
                       block_tables.shape[1], seq_lens.data_ptr(), _lib.ptr(starts), B, out_len,
                       _lib.ptr(offs), k_out.data_ptr(), v_out.data_ptr(), out_layer_stride, L,
