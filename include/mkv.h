@@ -823,8 +823,9 @@ int mkv_decode_attention_fp8(const void* q, const void* k_codes, const void* v_c
  * cached value is code * 2^e, exactly. q and out are bf16; 1 to 8 query heads per KV
  * head, head_dim 256, batch x num_kv_heads at most 4096. Softmax in fp32; a weight
  * enters the product with V with 16 significant bits. The workspace (16-byte aligned)
- * is mkv_decode_attention_fp4_workspace_bytes (-1 for an unsupported shape); error bits
- * as mkv_decode_attention_bf16. Page ids below shared_pages are read through the
+ * is mkv_decode_attention_fp4_workspace_bytes (-1 for an unsupported shape; 0, and none
+ * needed, for few sequences of a small max_seq_len); error bits as
+ * mkv_decode_attention_bf16. Page ids below shared_pages are read through the
  * caches.
  */
 int mkv_decode_attention_fp4(const void* q, const void* k_cache, const void* v_cache,
@@ -835,7 +836,7 @@ int mkv_decode_attention_fp4(const void* q, const void* k_cache, const void* v_c
                              void* workspace, int64_t workspace_bytes, int32_t* err,
                              void* stream);
 int64_t mkv_decode_attention_fp4_workspace_bytes(int32_t batch, int32_t num_kv_heads,
-                                                 int32_t num_q_heads);
+                                                 int32_t num_q_heads, int32_t max_seq_len);
 
 
 /*

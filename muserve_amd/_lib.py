@@ -121,7 +121,7 @@ SIGNATURES: dict[str, list] = {
                                  _P, _I32, _I32, _F32, _P, _P, _I64, _P, _P],
     "mkv_decode_attention_fp4": [_P, _P, _P, _I64, _I64, _I32, _I32, _I32, _P, _I64, _I32, _P,
                                  _I32, _I32, _F32, _P, _P, _I64, _P, _P],
-    "mkv_decode_attention_fp4_workspace_bytes": [_I32, _I32, _I32],
+    "mkv_decode_attention_fp4_workspace_bytes": [_I32, _I32, _I32, _I32],
     "mkv_decode_attention_contig": [_P, _P, _P, _I32, _I32, _I32, _I32, _I64, _P, _I32, _I32, _F32,
                                     _P, _P, _I64, _P, _P],
     "mkv_probe_read_pages": [_P, _P, _I32, _I64, _P, _I64, _I32, _I32, _P, _P],

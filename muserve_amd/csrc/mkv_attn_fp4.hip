@@ -57,6 +57,9 @@ constexpr int kMaxGroup = 8;         // query heads per KV head
 constexpr int kMaxPairs = 4096;      // batch x KV heads
 constexpr int kXcds = 8;             // MI355X: workgroups go round robin over 8 XCDs
 constexpr int kWgsPerCu = 2;
+constexpr int kPairWaves = 8;        // of a workgroup that takes a whole (sequence, KV head)
+constexpr int kPairTiles = 24;       // tiles of the longest sequence up to which they do, and
+constexpr int kPairMore = 16;        // as many more with a sequence for each CU
 constexpr int kWidePairs = 128;      // pairs below which the merge takes 16 waves
 constexpr float kRaise = 8.f;        // log2 by which a score may pass the running maximum
 
@@ -114,11 +117,13 @@ __device__ __forceinline__ u32x4 dequant8(uint32_t w, float s) {
                mkv_fp4_pair(w, 3, s)};
 }
 
-__global__ __launch_bounds__(kThreads4, kWgsPerCu) void attn_fp4_span_kernel(Args a) {
+// PAIR: a workgroup a (sequence, KV head), its waves taking the tiles in turn and joining
+// their pieces in LDS: no second kernel, no prefix over the sequences.
+template <bool PAIR>
+__global__ __launch_bounds__(PAIR ? 64 * kPairWaves : kThreads4, 2) void attn_fp4_kernel(Args a) {
+  constexpr int WAVES = PAIR ? kPairWaves : kWaves, STEP = PAIR ? WAVES : 1;
   // two tiles for each wave (in the end its piece [G][256]), the pieces' (m, l) [waves][G][2]
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  __shared__ int32_t wave_tot[kWaves];
-  __shared__ int32_t start_l[kWaves][2];  // (sequence, its first tile) that a span starts in
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int32_t hkv = a.hkv;
@@ -128,81 +133,128 @@ __global__ __launch_bounds__(kThreads4, kWgsPerCu) void attn_fp4_span_kernel(Arg
     const int64_t len = ld_const(a.lens + b);
     return (int32_t)(len < 0 ? 0 : (len > cap ? cap : len));
   };
-  // exclusive prefix of the places of 256 sequences from `base` on (a place for each
-  // tile and one more), behind `before`; the round's total goes to `round`
-  auto scan = [&](int base, int32_t before, int32_t& cnt, int32_t& round)
-      __attribute__((always_inline)) {
-    const int b = base + tid;
-    cnt = b < a.batch ? places_of(length_of(b)) : 0;
-    int32_t incl = cnt;
-#pragma unroll
-    for (int dd = 1; dd < 64; dd <<= 1) {
-      const int32_t o = __shfl_up(incl, dd);
-      if (lane >= dd) incl += o;
-    }
-    __syncthreads();  // wave_tot's earlier readers are done
-    if (lane == 63) wave_tot[wave] = incl;
-    __syncthreads();
-    int32_t at = before + incl - cnt;
-    round = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      at += w < wave ? wave_tot[w] : 0;
-      round += wave_tot[w];
-    }
-    return at;
+  // a sequence as the walk over the span has it: its tiles' places are pre0 .. pre1
+  struct Seq {
+    int32_t b, pre0, pre1, len;
   };
-  int32_t T = 0, cnt, round, at = 0;
-  for (int base = 0; base < a.batch; base += kThreads4) {
-    at = scan(base, T, cnt, round);
-    T += round;
-  }
-  // Workgroups of one XCD (those with the same number modulo 8) take neighbouring spans.
-  const int32_t xcd = blockIdx.x % kXcds, all = gridDim.x;
-  const int32_t unit = xcd * (all / kXcds) + (xcd < all % kXcds ? xcd : all % kXcds) +
-                       (int32_t)blockIdx.x / kXcds;
-  const int32_t head = unit % hkv;
-  const int32_t total = T;
-  T = T > 0 ? T - 1 : 0;  // (nothing starts at the place behind the last sequence)
-  const int32_t spans = all / hkv * kWaves;
-  const Spans cut = {T / spans, T % spans};
-  const int32_t first = unit / hkv * kWaves;
-  const int32_t span = first + wave;
-  // The sequences that this workgroup's spans start in (and, by workgroup 0, the prefixes
-  // for the merge kernel); a round's prefix is still held where there is one round.
-  {
-    int32_t before = 0;
-    for (int base = 0; base < a.batch; base += kThreads4) {
-      if (a.batch > kThreads4) {
-        at = scan(base, before, cnt, round);
-        before += round;
-      }
+  auto next_seq = [&](Seq x) __attribute__((always_inline)) {  // the next one with tiles
+    do {
+      ++x.b;
+      x.len = __builtin_amdgcn_readfirstlane(length_of(x.b));
+    } while (x.len == 0);
+    x.pre0 = x.pre1 + 1;
+    x.pre1 = x.pre0 + (x.len + kTile - 1) / kTile;
+    return x;
+  };
+  Seq cur;             // the sequence that is worked on
+  Spans cut;
+  int32_t head;        // KV head
+  int32_t first, span;  // the workgroup's first span and the wave's: the places s0 .. s1
+  int32_t s0, s1, fa;  // fa: the wave's next tile whose page ids are read
+  if constexpr (PAIR) {
+    const int32_t b = blockIdx.x / hkv;
+    head = blockIdx.x - b * hkv;
+    const int64_t given = ld_const(a.lens + b);
+    if ((given > cap || given < 0) && head == 0 && tid == 0) raise_err(a.err, MKV_DEVERR_TABLE);
+    cur.b = b;
+    cur.pre0 = s0 = 0;
+    cur.len = length_of(b);
+    cur.pre1 = s1 = (cur.len + kTile - 1) / kTile;
+    if (s1 == 0) {
+      if (tid < a.group * 32)
+        st16(a.out + ((int64_t)blockIdx.x * a.group * 32 + tid) * 16, u32x4{0u, 0u, 0u, 0u});
+      return;
+    }
+    fa = wave;
+  } else {
+    __shared__ int32_t wave_tot[kWaves];
+    __shared__ int32_t start_l[kWaves][2];  // (sequence, its first tile) that a span starts in
+    // exclusive prefix of the places of 256 sequences from `base` on (a place for each
+    // tile and one more), behind `before`; the round's total goes to `round`
+    auto scan = [&](int base, int32_t before, int32_t& cnt, int32_t& round)
+        __attribute__((always_inline)) {
       const int b = base + tid;
-      if (b < a.batch) {
+      cnt = b < a.batch ? places_of(length_of(b)) : 0;
+      int32_t incl = cnt;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-          const int32_t s = cut.start(first + w);
-          if (s >= at && s < at + cnt) {
-            start_l[w][0] = b;
-            start_l[w][1] = at;
+      for (int dd = 1; dd < 64; dd <<= 1) {
+        const int32_t o = __shfl_up(incl, dd);
+        if (lane >= dd) incl += o;
+      }
+      __syncthreads();  // wave_tot's earlier readers are done
+      if (lane == 63) wave_tot[wave] = incl;
+      __syncthreads();
+      int32_t at = before + incl - cnt;
+      round = 0;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        at += w < wave ? wave_tot[w] : 0;
+        round += wave_tot[w];
+      }
+      return at;
+    };
+    int32_t T = 0, cnt, round, at = 0;
+    for (int base = 0; base < a.batch; base += kThreads4) {
+      at = scan(base, T, cnt, round);
+      T += round;
+    }
+    // Workgroups of one XCD (those with the same number modulo 8) take neighbouring spans.
+    const int32_t xcd = blockIdx.x % kXcds, all = gridDim.x;
+    const int32_t unit = xcd * (all / kXcds) + (xcd < all % kXcds ? xcd : all % kXcds) +
+                         (int32_t)blockIdx.x / kXcds;
+    head = unit % hkv;
+    const int32_t total = T;
+    T = T > 0 ? T - 1 : 0;  // (nothing starts at the place behind the last sequence)
+    const int32_t spans = all / hkv * kWaves;
+    cut = {T / spans, T % spans};
+    first = unit / hkv * kWaves;
+    span = first + wave;
+    // The sequences that this workgroup's spans start in (and, by workgroup 0, the prefixes
+    // for the merge kernel); a round's prefix is still held where there is one round.
+    {
+      int32_t before = 0;
+      for (int base = 0; base < a.batch; base += kThreads4) {
+        if (a.batch > kThreads4) {
+          at = scan(base, before, cnt, round);
+          before += round;
+        }
+        const int b = base + tid;
+        if (b < a.batch) {
+#pragma unroll
+          for (int w = 0; w < kWaves; ++w) {
+            const int32_t s = cut.start(first + w);
+            if (s >= at && s < at + cnt) {
+              start_l[w][0] = b;
+              start_l[w][1] = at;
+            }
+          }
+          if (blockIdx.x == 0) {
+            a.pre[b] = at;
+            const int64_t len = ld_const(a.lens + b);
+            if (len > cap || len < 0) raise_err(a.err, MKV_DEVERR_TABLE);
           }
         }
-        if (blockIdx.x == 0) {
-          a.pre[b] = at;
-          const int64_t len = ld_const(a.lens + b);
-          if (len > cap || len < 0) raise_err(a.err, MKV_DEVERR_TABLE);
-        }
       }
+      if (blockIdx.x == 0 && tid == 0) {
+        a.pre[a.batch] = total;
+        a.hdr[0] = cut.least;
+        a.hdr[1] = cut.more;
+      }
+      __syncthreads();
     }
-    if (blockIdx.x == 0 && tid == 0) {
-      a.pre[a.batch] = total;
-      a.hdr[0] = cut.least;
-      a.hdr[1] = cut.more;
+    s0 = cut.start(span);
+    s1 = cut.start(span + 1);
+    if (s0 >= s1) return;  // (no barrier follows, but for workgroups with four spans)
+    cur.b = __builtin_amdgcn_readfirstlane(start_l[wave][0]);
+    cur.pre0 = __builtin_amdgcn_readfirstlane(start_l[wave][1]);
+    cur.len = __builtin_amdgcn_readfirstlane(length_of(cur.b));
+    cur.pre1 = cur.pre0 + (cur.len + kTile - 1) / kTile;
+    fa = s0;
+    if (fa == cur.pre1) {  // the span starts at the place behind a sequence
+      if (++fa == s1) return;
+      cur = next_seq(cur);
     }
-    __syncthreads();
   }
-  const int32_t s0 = cut.start(span), s1 = cut.start(span + 1);
-  if (s0 >= s1) return;  // (no barrier follows, but for workgroups with four spans)
 
   // Of the two waves on a SIMD the arbiter favours the older one: with it alone the first
   // workgroup of a CU ends a third before the second. They take turns, tile by tile.
@@ -213,7 +265,7 @@ __global__ __launch_bounds__(kThreads4, kWgsPerCu) void attn_fp4_span_kernel(Arg
   // page ids read through the caches: shared ones, and all where KV heads share lines
   const int64_t hot_below = hkv > 1 ? a.num_pages : a.shared_below;
   const uint32_t num_pages = a.num_pages < INT32_MAX ? (uint32_t)a.num_pages : INT32_MAX;
-  float* ml_l = reinterpret_cast<float*>(lds + 2 * kWaves * kTileLds);
+  float* ml_l = reinterpret_cast<float*>(lds + 2 * WAVES * kTileLds);
   const uint32_t tile_l = lds_addr(lds + wave * 2 * kTileLds);
   const uint32_t odd_k = ((c * hkv + head) & 1) * 8;  // where a row starts in its first chunk
   const uint32_t odd_v[2] = {(head & 1) * 8u, ((hkv + head) & 1) * 8u};  // of rows 4 g + j, j even, odd
@@ -228,30 +280,7 @@ __global__ __launch_bounds__(kThreads4, kWgsPerCu) void attn_fp4_span_kernel(Arg
     chunk_off[j] = ((r * row_bytes + head * kFp4Row) & ~15) + 16 * (i % (kRowLds / 16));
   }
 
-  // a sequence as the walk over the span has it: its tiles' places are pre0 .. pre1
-  struct Seq {
-    int32_t b, pre0, pre1, len;
-  };
-  auto next_seq = [&](Seq x) __attribute__((always_inline)) {  // the next one with tiles
-    do {
-      ++x.b;
-      x.len = __builtin_amdgcn_readfirstlane(length_of(x.b));
-    } while (x.len == 0);
-    x.pre0 = x.pre1 + 1;
-    x.pre1 = x.pre0 + (x.len + kTile - 1) / kTile;
-    return x;
-  };
-  Seq ahead;  // of the tile whose page ids are read next
-  ahead.b = __builtin_amdgcn_readfirstlane(start_l[wave][0]);
-  ahead.pre0 = __builtin_amdgcn_readfirstlane(start_l[wave][1]);
-  ahead.len = __builtin_amdgcn_readfirstlane(length_of(ahead.b));
-  ahead.pre1 = ahead.pre0 + (ahead.len + kTile - 1) / kTile;
-  int32_t fa = s0;  // and its place
-  if (fa == ahead.pre1) {  // the span starts at the place behind a sequence
-    if (++fa == s1) return;
-    ahead = next_seq(ahead);
-  }
-  Seq cur = ahead;
+  Seq ahead = cur;  // of the tile whose page ids are read next
 
   // The pages of a tile. Their ids are read a tile ahead of the rows' loads, which wait for
   // them; a tile's K and V are loaded once the tile two before it has been read.
@@ -260,14 +289,14 @@ __global__ __launch_bounds__(kThreads4, kWgsPerCu) void attn_fp4_span_kernel(Arg
   };
   auto read_ids = [&]() __attribute__((always_inline)) {
     Pages x = {0, 0, 0};
-    if (fa == ahead.pre1 && ++fa < s1) ahead = next_seq(ahead);
+    if (!PAIR && fa == ahead.pre1 && ++fa < s1) ahead = next_seq(ahead);
     if (fa < s1) {
       const int32_t tok0 = (fa - ahead.pre0) * kTile;
       const int32_t* ids = a.table + (int64_t)ahead.b * a.tstride + tok0 / 16;
       x.left = ahead.len - tok0;
       x.id0 = ld_const(ids);
       x.id1 = ld_const(ids + (x.left > 16 ? 1 : 0));
-      ++fa;
+      fa += STEP;
     }
     return x;
   };
@@ -326,8 +355,10 @@ __global__ __launch_bounds__(kThreads4, kWgsPerCu) void attn_fp4_span_kernel(Arg
   uint32_t slot = tile_l;  // and where it lies
   const uint32_t both = 2 * tile_l + kTileLds;
   Where now = locate(read_ids());
-  load_k(now, slot);
-  load_v(now, slot);
+  if (!PAIR || now.there) {
+    load_k(now, slot);
+    load_v(now, slot);
+  }
   Where next = locate(read_ids());
   if (next.there) {
     load_k(next, both - slot);
@@ -352,7 +383,7 @@ __global__ __launch_bounds__(kThreads4, kWgsPerCu) void attn_fp4_span_kernel(Arg
     l_run = 0.f;
     while (f < end) {
       __builtin_amdgcn_s_setprio(0);
-      if (((uint32_t)(f + wslot) & 1u) != 0) __builtin_amdgcn_s_setprio(1);
+      if (((uint32_t)(f / STEP + wslot) & 1u) != 0) __builtin_amdgcn_s_setprio(1);
       const bool has1 = next.there;
       // the tile's K has come once what was asked for behind it is all that is in flight
       if (has1) vm_wait_n<6 * kPageLoads>(); else vm_wait_n<2 * kPageLoads>();
@@ -456,10 +487,10 @@ __global__ __launch_bounds__(kThreads4, kWgsPerCu) void attn_fp4_span_kernel(Arg
       now = next;
       next = after;
       slot = both - slot;
-      ++f;
+      f += STEP;
     }
     const Seq done = cur;
-    const bool last = cur.pre1 + 1 >= s1;
+    const bool last = PAIR || cur.pre1 + 1 >= s1;
     if (!last) {  // the next sequence's query rows come while this one's piece goes
       cur = next_seq(cur);
       f = cur.pre0;
@@ -480,13 +511,13 @@ __global__ __launch_bounds__(kThreads4, kWgsPerCu) void attn_fp4_span_kernel(Arg
         o[j][i] = bits_f32(r[0]) + bits_f32(r[1]);
       }
     const int h0 = 4 * (g & 1), d0 = 16 * c + 8 * (g >> 1);
-    const bool whole = done.pre0 >= s0 && done.pre1 <= s1;
-    // (cut sequences: the span's first goes to slot 0, its last to slot 1)
-    const int64_t piece =
-        (((int64_t)span * hkv + head) * 2 + (done.pre0 <= s0 ? 0 : 1)) * a.group;
     uint8_t* out = a.out + ((int64_t)done.b * hkv + head) * a.group * kQRow;
     // the workgroup's spans lie in one sequence: one piece, its first span's
-    const bool joint = cut.whole(first, done.pre0, done.pre1);
+    const bool joint = PAIR || cut.whole(first, done.pre0, done.pre1);
+    const bool whole = !PAIR && done.pre0 >= s0 && done.pre1 <= s1;
+    // (cut sequences: the span's first goes to slot 0, its last to slot 1)
+    const int64_t piece =
+        PAIR ? 0 : (((int64_t)span * hkv + head) * 2 + (done.pre0 <= s0 ? 0 : 1)) * a.group;
     float* piece_l = reinterpret_cast<float*>(lds + wave * 2 * kTileLds);
     if (lane < a.group) {
       float* ml = joint ? ml_l + (wave * a.group + lane) * 2 : a.ml + (piece + lane) * 2;
@@ -515,30 +546,37 @@ __global__ __launch_bounds__(kThreads4, kWgsPerCu) void attn_fp4_span_kernel(Arg
     }
     if (joint) {
       __syncthreads();
-      const int64_t at = ((int64_t)first * hkv + head) * 2 * a.group;
-      for (int h = wave; h < a.group; h += kWaves) {  // a head a wave, four dims a lane
-        float m[kWaves], ls[kWaves], M = -INFINITY, L = 0.f;
-        f32x4 x[kWaves], O = f32x4{0.f, 0.f, 0.f, 0.f};
+      const int64_t at = PAIR ? 0 : ((int64_t)first * hkv + head) * 2 * a.group;
+      for (int h = wave; h < a.group; h += WAVES) {  // a head a wave, four dims a lane
+        float m[WAVES], ls[WAVES], M = -INFINITY, L = 0.f;
+        f32x4 x[WAVES], O = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
+        for (int w = 0; w < WAVES; ++w) {
           m[w] = ml_l[(w * a.group + h) * 2];
           ls[w] = ml_l[(w * a.group + h) * 2 + 1];
           x[w] = reinterpret_cast<const f32x4*>(lds + w * 2 * kTileLds)[h * (kHeadDim / 4) + lane];
         }
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) M = fmaxf(M, m[w]);
+        for (int w = 0; w < WAVES; ++w) M = fmaxf(M, m[w]);
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
+        for (int w = 0; w < WAVES; ++w) {
           // (a wave without a score: 1, so that a NaN of its sums stays)
           const float e = m[w] == -INFINITY ? 1.f : exp2_fast(m[w] - M);
 #pragma unroll
           for (int d = 0; d < 4; ++d) O[d] += e * x[w][d];
           L += e * ls[w];
         }
-        *reinterpret_cast<f32x4*>(a.part + (at + h) * kHeadDim + 4 * lane) = O;
-        if (lane == 0) {
-          a.ml[(at + h) * 2] = M;
-          a.ml[(at + h) * 2 + 1] = L;
+        if constexpr (PAIR) {
+          const float inv = 1.f / L;
+          *reinterpret_cast<u32x2*>(out + h * kQRow + 8 * lane) =
+              L == 0.f ? u32x2{0u, 0u}
+                       : u32x2{pack_bf16(O[0] * inv, O[1] * inv), pack_bf16(O[2] * inv, O[3] * inv)};
+        } else {
+          *reinterpret_cast<f32x4*>(a.part + (at + h) * kHeadDim + 4 * lane) = O;
+          if (lane == 0) {
+            a.ml[(at + h) * 2] = M;
+            a.ml[(at + h) * 2 + 1] = L;
+          }
         }
       }
     }
@@ -637,16 +675,28 @@ __global__ __launch_bounds__(64 * WAVES) void attn_fp4_merge_kernel(Args a) {
   out[tid] = f32_to_bf16_rne(L == 0.f ? 0.f : O / L);
 }
 
-// Workgroups of the span kernel: the resident ones, as many for each KV head.
+// Workgroups of spans: the resident ones, as many for each KV head.
 int64_t span_grid(int32_t hkv) {
   const int64_t fit = (int64_t)device_cus() * kWgsPerCu / hkv;
   return (fit < 1 ? 1 : fit) * hkv;
+}
+// Whether each (sequence, KV head) gets a workgroup: for short contexts, where that costs
+// less than the prefix and the second kernel do. Measured (us by spans and by pairs, 4
+// query heads): 1 sequence of 512 tokens 10.4, 8.7, of 1024 10.8, 12.4; 64 of 1024 15.0,
+// 14.6, of 2048 18.5, 23.3; 256 of 512 20.6, 11.6, of 1024 25.7, 17.3, lognormal up to 1024
+// 18.6, 15.0, up to 2048 23.5, 23.7; 512 of 1024 40.5, 33.8, lognormal 28.2, 27.1.
+bool by_pairs(int64_t pairs, int64_t max_len) {
+  const int64_t cus = device_cus();
+  if (pairs > 2 * cus) return false;
+  const int64_t some = pairs < cus ? pairs : cus;
+  return max_len <= (kPairTiles + kPairMore * some / cus) * kTile;
 }
 
 struct WsLayout {
   int64_t pre, ml, part, total;
 };
-WsLayout ws_layout(int64_t batch, int32_t hkv, int64_t group) {
+WsLayout ws_layout(int64_t batch, int32_t hkv, int64_t group, int64_t max_len) {
+  if (by_pairs(batch * hkv, max_len)) return WsLayout{0, 0, 0, 0};
   const int64_t pieces = span_grid(hkv) * kWaves * 2 * group;
   WsLayout w;
   w.pre = 256;
@@ -656,23 +706,24 @@ WsLayout ws_layout(int64_t batch, int32_t hkv, int64_t group) {
   return w;
 }
 
-// Launches the span kernel, once its LDS has been asked for on this device.
-int launch_spans(const Args& a, hipStream_t st, const char* fn) {
-  constexpr size_t most = kWaves * (2 * kTileLds + kMaxGroup * 2 * 4);
+// Launches `grid` workgroups, once their LDS has been asked for on this device.
+template <bool PAIR>
+int launch(const Args& a, int64_t grid, hipStream_t st, const char* fn) {
+  constexpr int WAVES = PAIR ? kPairWaves : kWaves;
+  constexpr size_t most = WAVES * (2 * kTileLds + kMaxGroup * 2 * 4);
   static std::atomic<uint64_t> asked[16];  // a bit a device
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess) dev = 0;
   const uint64_t bit = 1ull << (dev & 63);
   std::atomic<uint64_t>& word = asked[(dev >> 6) & 15];
   if (!(word.load(std::memory_order_relaxed) & bit)) {
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(attn_fp4_span_kernel),
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(attn_fp4_kernel<PAIR>),
                             hipFuncAttributeMaxDynamicSharedMemorySize, most) != hipSuccess)
       return set_error(MKV_E_LAUNCH, "%s: %zu bytes of LDS refused", fn, most);
     word.fetch_or(bit, std::memory_order_relaxed);
   }
-  const size_t lds = kWaves * (2 * kTileLds + (size_t)a.group * 2 * 4);
-  hipLaunchKernelGGL(attn_fp4_span_kernel, dim3((unsigned)span_grid(a.hkv)), dim3(kThreads4),
-                     lds, st, a);
+  const size_t lds = WAVES * (2 * kTileLds + (size_t)a.group * 2 * 4);
+  hipLaunchKernelGGL(attn_fp4_kernel<PAIR>, dim3((unsigned)grid), dim3(64 * WAVES), lds, st, a);
   return MKV_OK;
 }
 
@@ -687,9 +738,10 @@ bool shape_ok(int32_t batch, int32_t hkv, int32_t hq) {
 using namespace mkv;
 
 extern "C" int64_t mkv_decode_attention_fp4_workspace_bytes(int32_t batch, int32_t num_kv_heads,
-                                                            int32_t num_q_heads) {
-  if (!shape_ok(batch, num_kv_heads, num_q_heads)) return -1;
-  return ws_layout(batch, num_kv_heads, num_q_heads / num_kv_heads).total;
+                                                            int32_t num_q_heads,
+                                                            int32_t max_seq_len) {
+  if (!shape_ok(batch, num_kv_heads, num_q_heads) || max_seq_len < 0) return -1;
+  return ws_layout(batch, num_kv_heads, num_q_heads / num_kv_heads, max_seq_len).total;
 }
 
 extern "C" int mkv_decode_attention_fp4(const void* q, const void* k_cache, const void* v_cache,
@@ -725,8 +777,9 @@ extern "C" int mkv_decode_attention_fp4(const void* q, const void* k_cache, cons
   MKV_REQUIRE((int64_t)batch * num_kv_heads * (((int64_t)max_seq_len + 15) / 16) < (1ll << 31),
               MKV_E_UNSUPPORTED, "%s: batch x KV heads x pages above 2^31", fn);
   const int32_t pairs = batch * num_kv_heads;
-  const WsLayout L = ws_layout(batch, num_kv_heads, group);
-  MKV_REQUIRE(workspace && workspace_bytes >= L.total && aligned16(workspace), MKV_E_INVALID,
+  const WsLayout L = ws_layout(batch, num_kv_heads, group, max_seq_len);
+  MKV_REQUIRE(L.total == 0 || (workspace && workspace_bytes >= L.total && aligned16(workspace)),
+              MKV_E_INVALID,
               "%s: workspace of %lld bytes (16-byte aligned) required", fn, (long long)L.total);
   Args a;
   a.q = static_cast<const uint8_t*>(q);
@@ -751,7 +804,11 @@ extern "C" int mkv_decode_attention_fp4(const void* q, const void* k_cache, cons
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
   a.err = err;
   const hipStream_t st = as_stream(stream);
-  const int rc = launch_spans(a, st, fn);
+  if (L.total == 0) {
+    const int rc = launch<true>(a, pairs, st, fn);
+    return rc != MKV_OK ? rc : check_launch(fn);
+  }
+  const int rc = launch<false>(a, span_grid(num_kv_heads), st, fn);
   if (rc != MKV_OK) return rc;
   if (pairs < kWidePairs)
     hipLaunchKernelGGL(attn_fp4_merge_kernel<16>, dim3((unsigned)(pairs * group)), dim3(16 * 64), 0,

@@ -53,12 +53,14 @@ __global__ __launch_bounds__(kThreads) void append_fp4_kernel(AppendFp4Args a) {
   if ((lane & 1) == 0) dst[kFp4Codes + lane / 2] = (uint8_t)byte;
 }
 
-// Gather: a tile is ROWS output rows of one (layer, K|V, sequence); 32 lanes take a
-// (row, head): 8 codes and their block's scale byte in, 16 bytes out.
+// Gather: a tile is kGatherRows output rows of one (layer, K|V, sequence); 32 lanes take
+// a (row, head): 8 codes and their block's scale byte in, 16 bytes out, a tile's rows
+// loaded before the first is stored.
 constexpr int kGatherRows = 16;
 constexpr int kGatherThreads = 256;
 
 __global__ __launch_bounds__(kGatherThreads) void gather_fp4_kernel(GatherArgs a, int32_t heads) {
+  constexpr int GROUPS = kGatherThreads / 32, EACH = kGatherRows / GROUPS;
   GatherTile<kGatherRows> t;
   t.init(a);
   const int64_t row_limit = a.out_offsets ? t.nvalid : a.out_len;
@@ -68,22 +70,32 @@ __global__ __launch_bounds__(kGatherThreads) void gather_fp4_kernel(GatherArgs a
   const int lane = threadIdx.x & 31, group = threadIdx.x >> 5;
   const uint8_t* plane = (t.is_v ? a.v_pool : a.k_pool) + (int64_t)t.layer * a.pool_layer_stride;
   uint8_t* out = (t.is_v ? a.v_out : a.k_out) + (int64_t)t.layer * a.out_layer_stride;
-  for (int r = group; r < kGatherRows; r += kGatherThreads / 32) {
-    const int64_t row = t.row0 + r;
-    if (row >= row_limit) break;
+  const uint8_t* src[EACH];  // null: a row past the data, or of a bad page id
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int r = e * GROUPS + group;
     const int64_t p = t.p0 + r;
-    const int32_t page = row < t.nvalid ? t.page_of(p) : -1;
-    const uint8_t* src = plane + ((int64_t)(page < 0 ? 0 : page) * 16 + (p & 15)) * heads * kFp4Row;
-    uint8_t* dst = out + (t.out_row + r) * heads * (kHeadDim * 2);
-    for (int h = 0; h < heads; ++h) {
-      u32x4 x = u32x4{0u, 0u, 0u, 0u};  // rows past the data, and of a bad page id
-      if (page >= 0) {
-        const uint32_t c = *reinterpret_cast<const uint32_t*>(src + h * kFp4Row + lane * 4);
-        const float s = fp4_scale(src[h * kFp4Row + kFp4Codes + lane / 4]);
-        x = u32x4{mkv_fp4_pair(c, 0, s), mkv_fp4_pair(c, 1, s), mkv_fp4_pair(c, 2, s),
-                  mkv_fp4_pair(c, 3, s)};
+    const int32_t page = t.row0 + r < t.nvalid ? t.page_of(p) : -1;
+    src[e] = page < 0 ? nullptr : plane + ((int64_t)page * 16 + (p & 15)) * heads * kFp4Row;
+  }
+  for (int h = 0; h < heads; ++h) {
+    uint32_t c[EACH], b[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      c[e] = b[e] = 0;
+      if (src[e]) {
+        c[e] = *reinterpret_cast<const uint32_t*>(src[e] + h * kFp4Row + lane * 4);
+        b[e] = src[e][h * kFp4Row + kFp4Codes + lane / 4];
       }
-      st16(dst + h * (kHeadDim * 2) + lane * 16, x);
+    }
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      const int r = e * GROUPS + group;
+      const float s = fp4_scale(b[e]);
+      if (t.row0 + r < row_limit)
+        st16(out + ((t.out_row + r) * heads + h) * (kHeadDim * 2) + lane * 16,
+             u32x4{mkv_fp4_pair(c[e], 0, s), mkv_fp4_pair(c[e], 1, s), mkv_fp4_pair(c[e], 2, s),
+                   mkv_fp4_pair(c[e], 3, s)});
     }
   }
 }

@@ -90,6 +90,17 @@ __global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_kernel(RopeArgs a) 
   const int64_t tok = (int64_t)blockIdx.x * GROUPS + group;
   const bool live = tok < a.tokens;
   const int half = a.rot / 2;
+  const int h0 = blockIdx.y * a.per_wg;
+  const int h1 = h0 + a.per_wg < a.heads ? h0 + a.per_wg : a.heads;
+  // a head's row, 16 bytes a lane: the next one is asked for before one is worked on, the
+  // first before the turns are computed
+  auto row_of = [&](int h) __attribute__((always_inline)) {
+    const int which = h < a.hq ? 0 : (h < a.hq + a.hk ? 1 : 2);
+    const int hh = h - (which == 0 ? 0 : (which == 1 ? a.hq : a.hq + a.hk));
+    return ld16(a.src[which] + tok * a.token_stride[which] + hh * a.head_stride[which] + lane * 16);
+  };
+  u32x4 r = u32x4{0u, 0u, 0u, 0u};
+  if (live) r = row_of(h0);
   if (live) {  // the token's turns: (cos, sin) of each frequency
     const double pos = (double)a.positions[tok];
     for (int i = lane; i < half; i += LANES) {
@@ -127,16 +138,13 @@ __global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_kernel(RopeArgs a) 
       store = false;
     }
   }
-  const int h0 = blockIdx.y * a.per_wg;
-  const int h1 = h0 + a.per_wg < a.heads ? h0 + a.per_wg : a.heads;
   float w[8], wp[8];
   int have = -1;  // whose weights are held
   for (int h = h0; h < h1; ++h) {
     const int which = h < a.hq ? 0 : (h < a.hq + a.hk ? 1 : 2);
     const int hh = h - (which == 0 ? 0 : (which == 1 ? a.hq : a.hq + a.hk));
-    if (which > 0 && !store) continue;
-    const u32x4 r = ld16(a.src[which] + tok * a.token_stride[which] +
-                         hh * a.head_stride[which] + lane * 16);
+    u32x4 next = r;
+    if (h + 1 < h1) next = row_of(h + 1);
     u32x4 out = r;
     if (which < 2) {
       const void* wt = a.weight[which];
@@ -173,10 +181,12 @@ __global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_kernel(RopeArgs a) 
                             turned ? x[2 * i + 1] * c[2 * i + 1] + xp[2 * i + 1] * s[2 * i + 1]
                                    : x[2 * i + 1]);
     }
+    r = next;
+    if (which > 0 && !store) continue;
     if (which == 0) {
-      st16(a.q_out + (tok * a.hq + hh) * (2 * D) + lane * 16, out);
+      st_nt(a.q_out + (tok * a.hq + hh) * (2 * D) + lane * 16, out);
     } else if constexpr (POOL == kPoolNone) {
-      st16(a.k_out + (tok * a.hk + hh) * (2 * D) + lane * 16, out);
+      st_nt(a.k_out + (tok * a.hk + hh) * (2 * D) + lane * 16, out);
     } else {
       const int64_t row = slot * a.hk + hh;
       uint8_t* pool = a.pool[which - 1];

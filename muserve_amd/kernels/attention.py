@@ -364,8 +364,16 @@ _fp4_plans: dict[tuple, tuple] = {}
 _FP4_PLANS = 4096
 
 
+@functools.lru_cache(maxsize=4096)
+def _fp4_bytes(batch: int, num_kv_heads: int, num_q_heads: int, max_seqlen: int,
+               dev: torch.device) -> int:
+    with torch.cuda.device(dev):
+        return _lib.load().mkv_decode_attention_fp4_workspace_bytes(
+            batch, num_kv_heads, num_q_heads, min(max_seqlen, (1 << 31) - 1))
+
+
 def _fp4_check(q, k_cache, v_cache, cache_seqlens, page_table):
-    """(device, the sizes of the call by ctypes, workspace bytes, keys the table holds)."""
+    """(device, the sizes of the call by ctypes, keys the table holds, the shape)."""
     dev = _lib.require_gpu(q, k_cache, v_cache, cache_seqlens, page_table)
     if k_cache.dtype != torch.uint8 or v_cache.dtype != torch.uint8:
         raise TypeError("attn_decode_fp4 takes uint8 caches of 4-bit rows")
@@ -389,14 +397,13 @@ def _fp4_check(q, k_cache, v_cache, cache_seqlens, page_table):
     stride = page_table.stride(0) if B > 1 else width
     if stride < width:
         raise ValueError("page_table rows must not overlap")
-    nbytes = _lib.load().mkv_decode_attention_fp4_workspace_bytes(B, Hkv, Hq)
-    if nbytes < 0:
+    if _fp4_bytes(B, Hkv, Hq, 0, dev) < 0:
         raise ValueError(f"unsupported shapes q {tuple(q.shape)}, cache {tuple(k_cache.shape)} "
                          "(1 to 8 query heads per KV head, batch x KV heads up to 4096)")
     name = "mkv_decode_attention_fp4"
     return (dev, _lib.constants(name, 3, P)[0], _lib.constants(name, 5, Hkv, Hq, D),
-            _lib.constants(name, 9, stride, width), _lib.constants(name, 12, B)[0], nbytes,
-            width * 16)
+            _lib.constants(name, 9, stride, width), _lib.constants(name, 12, B)[0], width * 16,
+            (B, Hkv, Hq))
 
 
 def attn_decode_fp4(
@@ -428,7 +435,7 @@ def attn_decode_fp4(
         if len(_fp4_plans) >= _FP4_PLANS:
             _fp4_plans.clear()
         _fp4_plans[key] = plan
-    dev, pages, heads, table, batch, nbytes, held = plan
+    dev, pages, heads, table, batch, held, shape = plan
     if shared_pages < 0:
         raise ValueError("shared_pages must be >= 0")
     if max_seqlen is None:
@@ -440,12 +447,14 @@ def attn_decode_fp4(
     elif (out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous()
           or out.device != dev):
         raise ValueError("out must be a contiguous tensor shaped like q")
-    ws = _scratch(nbytes, dev)
+    nbytes = _fp4_bytes(*shape, max_seqlen, dev)
+    ws = _scratch(nbytes, dev) if nbytes else None
     _lib.call_on(dev, "mkv_decode_attention_fp4", q.data_ptr(), k_cache.data_ptr(),
                  v_cache.data_ptr(), pages, shared_pages, *heads, page_table.data_ptr(), *table,
                  cache_seqlens.data_ptr(), batch, max_seqlen,
                  HEAD_DIM ** -0.5 if softmax_scale is None else float(softmax_scale),
-                 out.data_ptr(), ws.data_ptr(), nbytes, _errword(dev).word.data_ptr())
+                 out.data_ptr(), ws.data_ptr() if nbytes else None, nbytes,
+                 _errword(dev).word.data_ptr())
     return out
 
 

@@ -56,7 +56,7 @@ def test_gather_refusals(change, code):
 
 def decode(**change):
     a = dict(q=FAKE, k=FAKE, v=FAKE, pages=4, shared=0, hkv=1, hq=4, dim=256, table=FAKE, tstride=4,
-             width=4, lens=FAKE, batch=1, most=64, scale=0.0625, out=FAKE, ws=FAKE, bytes=1 << 40,
+             width=4, lens=FAKE, batch=1, most=1 << 20, scale=0.0625, out=FAKE, ws=FAKE, bytes=1 << 40,
              err=FAKE, stream=None)
     a.update(change)
     return rc("mkv_decode_attention_fp4", *a.values())
@@ -76,8 +76,11 @@ def test_decode_refusals(change, code):
 def test_empty_decode_and_workspaces():
     assert decode(batch=0, q=None, ws=None)[0] == 0
     size = _lib.load().mkv_decode_attention_fp4_workspace_bytes
-    assert size(1, 1, 4) > 0 and size(4096, 1, 8) > size(1, 1, 8)
-    for bad in ((1, 1, 9), (4097, 1, 1), (1, 2, 3), (-1, 1, 1), (1, 0, 1)):
+    long = 1 << 20
+    assert size(1, 1, 4, long) > 0 and size(4096, 1, 8, long) > size(1, 1, 8, long)
+    assert size(1, 1, 4, 512) == 0 < size(4096, 1, 4, 512)
+    for bad in ((1, 1, 9, long), (4097, 1, 1, 9), (1, 2, 3, 9), (-1, 1, 1, 9), (1, 0, 1, 9),
+                (1, 1, 1, -1)):
         assert size(*bad) == -1
 
 

@@ -72,7 +72,10 @@ def test_matches_the_oracle(hq, hkv):
 
 @pytest.mark.parametrize("lens", [
     [1], [32], [33], [4096], [16 * 127 + 5], [16 * 1200 + 1, 0, 9], [40000], [20] * 126 + [4800],
-    [5] * 700, [0, 0, 0], list(range(1, 120))])
+    [5] * 700, [0, 0, 0], list(range(1, 120)),
+    # around the longest contexts that get a workgroup for each sequence
+    [768], [784], [300, 768, 0, 31], [300, 784, 0, 31], [900] + [7] * 127, [1040] + [7] * 127,
+    [20] * 512, [20] * 513])
 def test_shapes_of_batches(lens):
     case(f"4-bit decode attention: {len(lens)} sequences, longest {max(lens)}")
     args = build(3 + len(lens), lens, 4, 1)
