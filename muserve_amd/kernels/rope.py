@@ -172,15 +172,16 @@ POOL_16, POOL_FP8, POOL_FP4 = 1, 2, 3
 
 
 def append_rope(q, k, v, positions, inv_freq, q_weight, k_weight, eps, rope_scale, zero_centered,
-                interleaved, out, slots, pool, errors):
+                interleaved, out, slots, pool, errors, cache, scales):
     """``PagedKVCache.append_rope`` once the pool is known: ``pool`` is (type,
-    K plane, V plane, K scales, V scales, slots) by address."""
+    K plane, V plane, K scales, V scales, slots) by address, of the tensors
+    ``cache`` and ``scales``."""
     plan = _plan(q, k, v, positions, inv_freq, q_weight, k_weight, interleaved)
     dev, direct, q_strides, k_strides, v_strides, sizes, freq, kind = plan
     if out is None:
         out = _like(q)
     else:
-        _given("out", out, q, (k, v, positions, inv_freq, q_weight, k_weight, slots))
+        _given("out", out, q, (k, v, positions, inv_freq, q_weight, k_weight, slots, cache, scales))
     if not direct:
         positions = positions.long().contiguous()
     _lib.call_on(dev, "mkv_append_rope", q.data_ptr(), *q_strides, k.data_ptr(), *k_strides,

@@ -320,7 +320,8 @@ class PagedKVCache:
             self._check_slots(slot_mapping)
         pool = (self._rope_pool, *self._planes(first), *self._scale_planes(first), self.num_slots)
         return rope.append_rope(q, k, v, positions, inv_freq, q_weight, k_weight, eps, rope_scale,
-                                zero_centered, interleaved, out, slot_mapping, pool, self._errors)
+                                zero_centered, interleaved, out, slot_mapping, pool, self._errors,
+                                self.cache, self.scales)
 
     def _check_slots(self, slot_mapping: torch.Tensor) -> None:
         if self._unique is None:
