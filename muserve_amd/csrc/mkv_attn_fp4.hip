@@ -4,7 +4,12 @@
 // One query token per sequence attends to the first seq_lens[b] cached tokens
 // of its block table: softmax(q k^T * scale) v for each of the G query heads
 // that share a KV head. A cached token and head is 2 x 136 bytes for 1024 * G
-// flop, so HBM bounds the launch.
+// flop, so HBM bounds the launch where there is much to read, and the chain of
+// a span's first loads (1.2 us to the sequence, 2.8 to its K), its end (1.6)
+// and the second kernel (4) where there is little. Measured: 256 sequences, 4
+// query heads on a KV head, 439 MB, 76-83 us and 5 us for the second kernel; 2
+// sequences of 131072 tokens, 16 on 2, 143 MB, 35 and 6 us; 1 sequence of 2000
+// tokens, 4 on 1, 7 and 3 us.
 //   * Work split: the sequences' tiles of 32 tokens (two pages) form one flat
 //     list, with one place more for each sequence, about what its start and end
 //     cost. Each wave of the resident grid takes a contiguous span of it, for
@@ -14,9 +19,12 @@
 //     second kernel to join; where a workgroup's four spans lie in one sequence
 //     they leave one piece. (Spans by workgroup, its waves taking the tiles in
 //     turn: a barrier for each sequence, 87 us instead of 81 at batch 256.)
+//     Short contexts take a workgroup for each (sequence, KV head) instead, and
+//     no second kernel (by_pairs).
 //   * Loads: page by page straight into a wave's LDS (global_load_lds, 16
-//     bytes a lane), two tiles in flight, the page ids a tile ahead of them. (Into registers in the operands' own
-//     order a K row is a line for every lane, and the launch reached 5 TB/s.)
+//     bytes a lane), two tiles in flight, the page ids a tile ahead of them.
+//     (Into registers in the operands' own order a K row is a line for every
+//     lane: 90 us at batch 256; through registers to LDS: 97.)
 //   * Scores on the matrix cores (16x16x32 bf16): A = the 16 K rows of a page,
 //     codes converted to bf16 with their scale (exact), B = the query heads in
 //     columns n and n + 8. A column's lanes hold 8 tokens each; the maximum is
@@ -60,7 +68,7 @@ constexpr int kWgsPerCu = 2;
 constexpr int kPairWaves = 8;        // of a workgroup that takes a whole (sequence, KV head)
 constexpr int kPairTiles = 24;       // tiles of the longest sequence up to which they do, and
 constexpr int kPairMore = 16;        // as many more with a sequence for each CU
-constexpr int kWidePairs = 128;      // pairs below which the merge takes 16 waves
+constexpr int kWidePieces = 256;     // pieces of a sequence from which the merge takes 16 waves
 constexpr float kRaise = 8.f;        // log2 by which a score may pass the running maximum
 
 struct Args {
@@ -586,8 +594,11 @@ __global__ __launch_bounds__(PAIR ? 64 * kPairWaves : kThreads4, 2) void attn_fp
 
 // Joins the pieces of one (pair, query head) that spans cut, and writes the zeros of an
 // empty pair. Wave w takes the pieces w, w + WAVES, .., four dims a lane, BATCH of them
-// in flight; the waves' sums are joined in LDS. WAVES is 16 where few pairs leave the
-// CUs idle and have many pieces, else 4.
+// in flight; the waves' sums are joined in LDS. WAVES is 16 where a sequence is cut into
+// many pieces, else 4. Measured (us of both kernels with 4 waves and with 16): 1 sequence of
+// 4096 tokens (128 pieces) 10.8, 11.7, of 32768 (1024) 21.8, 17.4; 8 of 4096 (128) 13.7, 13.9,
+// of 32768 (256) 25.0, 24.0; 2 of 100000 and two KV heads (512) 34.4, 32.2; 128 of 4096 (16)
+// 33.8, 35.6.
 template <int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void attn_fp4_merge_kernel(Args a) {
   constexpr int BATCH = 8;
@@ -682,8 +693,8 @@ int64_t span_grid(int32_t hkv) {
 }
 // Whether each (sequence, KV head) gets a workgroup: for short contexts, where that costs
 // less than the prefix and the second kernel do. Measured (us by spans and by pairs, 4
-// query heads): 1 sequence of 512 tokens 10.4, 8.7, of 1024 10.8, 12.4; 64 of 1024 15.0,
-// 14.6, of 2048 18.5, 23.3; 256 of 512 20.6, 11.6, of 1024 25.7, 17.3, lognormal up to 1024
+// query heads): 1 sequence of 512 tokens 9.9, 8.8, of 1024 10.2, 12.6; 64 of 1024 14.3,
+// 14.6, of 2048 18.5, 23.3; 256 of 512 20.2, 11.1, of 1024 25.7, 16.7, lognormal up to 1024
 // 18.6, 15.0, up to 2048 23.5, 23.7; 512 of 1024 40.5, 33.8, lognormal 28.2, 27.1.
 bool by_pairs(int64_t pairs, int64_t max_len) {
   const int64_t cus = device_cus();
@@ -810,7 +821,10 @@ extern "C" int mkv_decode_attention_fp4(const void* q, const void* k_cache, cons
   }
   const int rc = launch<false>(a, span_grid(num_kv_heads), st, fn);
   if (rc != MKV_OK) return rc;
-  if (pairs < kWidePairs)
+  // pieces of a sequence, at most about one for each of its tiles and of its spans
+  const int64_t tiles = ((int64_t)max_seq_len + kTile - 1) / kTile;
+  const int64_t spans = span_grid(num_kv_heads) / num_kv_heads * kWaves / batch;
+  if (tiles >= kWidePieces && spans >= kWidePieces)
     hipLaunchKernelGGL(attn_fp4_merge_kernel<16>, dim3((unsigned)(pairs * group)), dim3(16 * 64), 0,
                        st, a);
   else
