@@ -173,3 +173,83 @@ def test_unaligned_rows_are_refused():
     with pytest.raises(RuntimeError, match="misaligned"):
         qk_norm_rope(even, even.clone(), pos, freq, out=(odd, torch.empty_like(even)))
     torch.cuda.synchronize()
+
+
+def random_rows(rng, *shape):
+    rows = rng.integers(0, 256, (*shape, fp4.ROW), dtype=np.uint8)
+    rows[..., 128:] = rng.integers(122, 130, (*shape, 8))
+    return rows
+
+
+@pytest.mark.parametrize("lens,hq,hkv", [
+    ([40, 3], 520, 520),                     # more KV heads than the grid has places for
+    ([30000, 17000], 4, 2), ([20001], 6, 3), ([9000, 0, 8191], 10, 2),
+    ([8160], 4, 1), ([8192], 4, 1),          # around the joining kernel's width
+    ([9] * 2047 + [70], 2, 2),               # the most pairs of a call
+    ([2000, 1, 700] * 60, 8, 1)])
+def test_shapes_of_heads(lens, hq, hkv):
+    case(f"4-bit decode attention: {len(lens)} sequences, longest {max(lens)}, {hq} heads on {hkv}")
+    rng = np.random.default_rng(hq + len(lens))
+    pages = [-(-n // 16) for n in lens]
+    P = sum(pages) + 2
+    perm = rng.permutation(P)
+    table = np.zeros((len(lens), max(pages)), dtype=np.int32)
+    at = 0
+    for b, n in enumerate(pages):
+        table[b, :n] = perm[at:at + n]
+        at += n
+    k, v = random_rows(rng, P, 16, hkv), random_rows(rng, P, 16, hkv)
+    q = (0.2 * torch.randn(len(lens), 1, hq, 256,
+                           generator=torch.Generator().manual_seed(hq))).bfloat16()
+    out = A.attn_decode_fp4(q.to(DEV), *(torch.from_numpy(x).to(DEV) for x in (k, v)),
+                            torch.tensor(lens, dtype=torch.int32, device=DEV),
+                            torch.from_numpy(table).to(DEV))
+    A.check_errors(DEV)
+    want, mass, smax = att.decode_attention(q[:, 0].double().numpy(), fp4.values(k), fp4.values(v),
+                                            np.asarray(lens), table, 1 / 16, stats=True)
+    tol = 2.0 ** -8 * np.abs(want) + (2.0 ** -14 + 2.0 ** -16 * (1 + smax[..., None])) * mass
+    assert (np.abs(out[:, 0].double().cpu().numpy() - want) <= tol).all()
+
+
+def test_rows_behind_4_gib():
+    """Queries whose rows are 3 GiB apart, pages behind 4 GiB of a plane."""
+    case("append_rope: rows and pages behind 4 GiB")
+    g = torch.Generator(device=DEV).manual_seed(8)
+    step = 3 << 29
+    flat = torch.empty(2 * step + 512, dtype=torch.bfloat16, device=DEV)
+    q = flat.as_strided((3, 2, 256), (step, 256, 1))
+    q.copy_(torch.randn(3, 2, 256, device=DEV, generator=g))
+    kv = torch.randn(2, 3, 1, 256, device=DEV, generator=g).bfloat16()
+    freq, pos = FREQ.float().to(DEV), torch.tensor([0, 5, 99], device=DEV)
+    want_q, want_k = qk_norm_rope(q.contiguous(), kv[0], pos, freq)
+    assert torch.equal(qk_norm_rope(q, kv[0], pos, freq)[0], want_q)
+    pages = (4 << 30) // (16 * 512) + 40
+    pool = PagedKVCache(pages, num_layers=1, kv_heads=1, dtype=torch.bfloat16, device=DEV,
+                        verbose=False)
+    slots = torch.tensor([1, (pages - 20) * 16 + 7, pages * 16 - 1], device=DEV)
+    assert torch.equal(pool.append_rope(slots, q, kv[0], kv[1], 0, pos, freq), want_q)
+    pool.check_errors()
+    rows = pool.cache.view(2, pages * 16, 1, 256)
+    assert torch.equal(rows[0][slots], want_k) and torch.equal(rows[1][slots], kv[1])
+
+
+@pytest.mark.parametrize("dim,tokens", [(64, 40000), (128, 33333)])
+def test_many_tokens(dim, tokens):
+    case(f"norm + rotation of {tokens} tokens, heads of {dim}")
+    g = torch.Generator(device=DEV).manual_seed(dim)
+    q, k = (torch.randn(tokens, h, dim, device=DEV, generator=g).half() for h in (3, 1))
+    freq = (1e4 ** (-torch.arange(0, dim, 2).double() / dim)).to(DEV)
+    pos = torch.arange(tokens, device=DEV)
+    w = torch.rand(dim, device=DEV, generator=g)
+    got = qk_norm_rope(q, k, pos, freq, w, w)
+    angle = pos[:, None].double() * freq
+    c, s = angle.cos()[:, None], angle.sin()[:, None]
+    for x, out in zip((q, k), got):
+        y = x.double()
+        y = y / (y.square().mean(-1, keepdim=True) + 1e-6).sqrt() * w.double()
+        a, b = y.chunk(2, -1)
+        want = torch.cat([a * c - b * s, b * c + a * s], -1)
+        # a rounding to fp16 and a few of fp32, of the rotated pair's size
+        size = torch.cat([a.abs() + b.abs()] * 2, -1)
+        assert ((out.double() - want).abs() <= 2.0 ** -11 * want.abs() + 2.0 ** -20 * size
+                + 2.0 ** -25).all()
