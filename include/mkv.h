@@ -822,7 +822,8 @@ int mkv_decode_attention_fp8(const void* q, const void* k_codes, const void* v_c
  * The same over a 4-bit pool (mkv_append_fp4's rows), dequantised in registers: a
  * cached value is code * 2^e, exactly. q and out are bf16; 1 to 8 query heads per KV
  * head, head_dim 256, batch x num_kv_heads at most 4096. Softmax in fp32; a weight
- * enters the product with V with 16 significant bits. The workspace (16-byte aligned)
+ * enters the product with V as two bf16 values, both rounded to nearest (within 2^-18 of
+ * itself, to either side). The workspace (16-byte aligned)
  * is mkv_decode_attention_fp4_workspace_bytes (-1 for an unsupported shape; 0, and none
  * needed, for few sequences of a small max_seq_len); error bits as
  * mkv_decode_attention_bf16. Page ids below shared_pages are read through the

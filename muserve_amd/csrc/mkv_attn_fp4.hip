@@ -31,10 +31,11 @@
 //     lazy (raised when a score passes it by 2^8), so most tiles need no
 //     reduction over lanes, and each lane sums its own tokens' weights.
 //   * P V on the matrix cores: A = the weights in two bf16 parts (the rows n
-//     hold the upper 8 bits, the rows n + 8 the next 8: 16 bits of weight for
-//     the price of rows that would be empty), B = V, 16 dims a lane. The score
-//     tile's lanes already hold the A operand: the tokens' order inside the
-//     product is free, so V is read in theirs.
+//     hold the weight rounded, the rows n + 8 what that left, rounded: within
+//     2^-18 of the weight, to either side, for the price of rows that would be
+//     empty), B = V, 16 dims a lane. The score tile's lanes already hold the A
+//     operand: the tokens' order inside the product is free, so V is read in
+//     theirs.
 #include <math.h>
 
 #include <atomic>
@@ -268,7 +269,7 @@ __global__ __launch_bounds__(PAIR ? 64 * kPairWaves : kThreads4, 2) void attn_fp
   // workgroup of a CU ends a third before the second. They take turns, tile by tile.
   const uint32_t wslot = __builtin_amdgcn_s_getreg((3 << 11) | 4) & 1u;
   const int c = lane & 15, g = lane >> 4;  // row / column and quad of a matrix operand
-  const uint32_t low_mask = c < 8 ? 0u : 0xffff0000u;  // what the lane takes off a weight
+  const uint32_t rest_mask = c < 8 ? 0u : ~0u;  // the lane takes a weight's first part off
   const int32_t row_bytes = hkv * kFp4Row;
   // page ids read through the caches: shared ones, and all where KV heads share lines
   const int64_t hot_below = hkv > 1 ? a.num_pages : a.shared_below;
@@ -449,10 +450,9 @@ __global__ __launch_bounds__(PAIR ? 64 * kPairWaves : kThreads4, 2) void attn_fp
       for (int j = 0; j < 8; j += 2) {
         const float p0 = exp2_fast(sv[j] - m_ref), p1 = exp2_fast(sv[j + 1] - m_ref);
         l_run += p0 + p1;
-        // upper 8 bits of the weight in rows below 8, what is left of it in the others
-        const uint32_t x0 = f32_bits(p0 - bits_f32(f32_bits(p0) & low_mask));
-        const uint32_t x1 = f32_bits(p1 - bits_f32(f32_bits(p1) & low_mask));
-        pa[j / 2] = __builtin_amdgcn_perm(x1, x0, 0x07060302u);
+        // the weight's bf16 in rows below 8, in the others that of what it left (exact)
+        const uint32_t near = pack_bf16(p0, p1) & rest_mask;
+        pa[j / 2] = pack_bf16(p0 - bits_f32(near << 16), p1 - bits_f32(near & 0xffff0000u));
       }
       if (has2) vm_wait_n<6 * kPageLoads>();
       else if (has1) vm_wait_n<4 * kPageLoads>();

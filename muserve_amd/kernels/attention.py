@@ -428,7 +428,9 @@ def attn_decode_fp4(
     """``attn_decode`` over a 4-bit pool (``cache.get_kv_by_layer(l)`` of a
     ``PagedKVCache`` with ``dtype=torch.float4_e2m1fn_x2``), dequantised in
     registers: a cached value is ``code * 2**e``, exactly. 1 to 8 query heads
-    per KV head; the other arguments are ``attn_decode``'s."""
+    per KV head; the other arguments are ``attn_decode``'s. Scores, softmax and
+    sums are fp32; a probability enters the product with V as two bf16 values,
+    both rounded (within 2^-18 of it), and the output is rounded once."""
     if page_table is None:
         raise ValueError("attn_decode_fp4 reads the paged pool: page_table is required")
     key = (q.dtype, q.shape, q.is_contiguous(), q.get_device(), k_cache.dtype, k_cache.shape,
