@@ -113,9 +113,11 @@ def _given(name: str, out: torch.Tensor, own: torch.Tensor, others) -> None:
     if out.shape != own.shape or out.dtype != own.dtype or out.device != own.device \
             or not out.is_contiguous():
         raise ValueError(f"{name} must be a contiguous tensor of its input's shape and type")
+    if out.data_ptr() != own.data_ptr() or not own.is_contiguous():
+        others = (own, *others)  # (also where another input is the same tensor as its own)
     lo, hi = _span(out)
-    for t in (own, *others):
-        if t is None or (t is own and t.data_ptr() == out.data_ptr() and own.is_contiguous()):
+    for t in others:
+        if t is None:
             continue
         a, b = _span(t)
         if a < hi and lo < b:
