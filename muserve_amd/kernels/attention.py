@@ -72,6 +72,13 @@ def _decode_scratch(B: int, Hkv: int, Hq: int, max_seqlen: int, dev: torch.devic
     return _scratch(_decode_bytes(B, Hkv, Hq, dev), dev)
 
 
+def _held(width: int) -> int:
+    """Keys that a page table of ``width`` pages a row holds, the most that any
+    ``max_seqlen`` bounds (a larger one, cut to the library's 32 bits, would mean
+    another)."""
+    return min(width * 16, (1 << 31) - 1)
+
+
 def attn_prefill(
     q: torch.Tensor,            # [total_tokens, NUM_Q_HEADS, HEAD_DIM] bf16
     k: torch.Tensor,            # [total_tokens, NUM_KV_HEADS, HEAD_DIM] bf16
@@ -306,8 +313,8 @@ def attn_decode(
 ) -> torch.Tensor:                      # [B, 1, NUM_Q_HEADS, HEAD_DIM] bf16 / fp16
     """bf16 or fp16 caches (fp16 is the reference's default pool dtype,
     muserve/config.py:37), with q and the output in the caches' dtype.
-    ``max_seqlen`` bounds ``cache_seqlens`` (default: what the page table
-    holds). ``out`` may be given to write in place.
+    ``max_seqlen`` bounds ``cache_seqlens`` (default, and at most: what the page
+    table holds). ``out`` may be given to write in place.
 
     ``shared_pages``: page ids below it may be read by several sequences of
     the batch (prompt pages shared through prefix reuse, e.g. a
@@ -376,7 +383,7 @@ def _fp4_bytes(batch: int, num_kv_heads: int, num_q_heads: int, max_seqlen: int,
                dev: torch.device) -> int:
     with torch.cuda.device(dev):
         return _lib.load().mkv_decode_attention_fp4_workspace_bytes(
-            batch, num_kv_heads, num_q_heads, min(max_seqlen, (1 << 31) - 1))
+            batch, num_kv_heads, num_q_heads, max_seqlen)
 
 
 def _fp4_check(q, k_cache, v_cache, cache_seqlens, page_table):
@@ -409,7 +416,7 @@ def _fp4_check(q, k_cache, v_cache, cache_seqlens, page_table):
                          "(1 to 8 query heads per KV head, batch x KV heads up to 4096)")
     name = "mkv_decode_attention_fp4"
     return (dev, _lib.constants(name, 3, P)[0], _lib.constants(name, 5, Hkv, Hq, D),
-            _lib.constants(name, 9, stride, width), _lib.constants(name, 12, B)[0], width * 16,
+            _lib.constants(name, 9, stride, width), _lib.constants(name, 12, B)[0], _held(width),
             (B, Hkv, Hq))
 
 
@@ -451,6 +458,8 @@ def attn_decode_fp4(
         max_seqlen = held
     elif max_seqlen < 0:
         raise ValueError("bad attention shape")
+    else:
+        max_seqlen = min(int(max_seqlen), held)
     if out is None:
         out = torch.empty_like(q)
     elif (out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous()
@@ -521,8 +530,7 @@ def _decode(fn, q, k_cache, v_cache, k_scales, v_scales, cache_seqlens, page_tab
             and cache_seqlens.is_contiguous() and page_table.stride(1) == 1):
         raise ValueError("q, caches, cache_seqlens and page_table rows must be contiguous")
     width = page_table.shape[1]
-    if max_seqlen is None:
-        max_seqlen = width * 16
+    max_seqlen = _held(width) if max_seqlen is None else min(int(max_seqlen), _held(width))
     if out is None:
         out = torch.empty_like(q)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from muserve_amd import _lib
-from muserve_amd.kernels import rope
+from muserve_amd.kernels import attention, rope
 from muserve_amd.kv_cache import PagedKVCache
 
 CPU = torch.device("cpu")
@@ -14,7 +14,8 @@ CPU = torch.device("cpu")
 def calls(monkeypatch):
     """The launches that would have been made: (entry point, arguments)."""
     made = []
-    monkeypatch.setattr(rope, "_plans", {})  # (what is kept here is of no device)
+    for module, kept in ((rope, "_plans"), (attention, "_fp4_plans"), (attention, "_errors")):
+        monkeypatch.setattr(module, kept, {})  # (what is kept here is of no device)
     monkeypatch.setattr(_lib, "require_gpu", lambda *tensors: CPU)
     monkeypatch.setattr(_lib, "call_on", lambda dev, name, *args: made.append((name, args)))
     monkeypatch.setattr(_lib, "call", lambda name, *args: made.append((name, args)))
@@ -49,3 +50,31 @@ def test_an_output_in_place_of_a_tensor_that_is_given_twice(calls):
     rope.qk_norm_rope(x, y, pos, freq, out=(x, y))
     cache.append_rope(slots, x, y, y, 0, pos, freq, out=x)
     assert [name for name, _ in calls] == ["mkv_qk_norm_rope"] * 2 + ["mkv_append_rope"]
+
+
+BOUNDS = [(None, 64), (40, 40), (64, 64), (65, 64), (1 << 25, 64), (1 << 31, 64), (1 << 32, 64),
+          ((1 << 32) + 5, 64), (1 << 70, 64)]
+
+
+@pytest.mark.parametrize("given,meant", BOUNDS)
+def test_a_bound_on_the_lengths_ends_with_the_table(calls, monkeypatch, given, meant):
+    """max_seqlen above what the table holds bounds nothing, also where it passes 32 bits."""
+    asked = []
+    monkeypatch.setattr(attention, "_fp4_bytes",
+                        lambda b, hkv, hq, most, dev: asked.append(most) or 0)
+    q = torch.zeros(2, 1, 4, 256, dtype=torch.bfloat16)
+    lens, table = torch.zeros(2, dtype=torch.int32), torch.zeros(2, 4, dtype=torch.int32)
+    rows = [torch.zeros(3, 16, 1, 136, dtype=torch.uint8) for _ in range(2)]
+    attention.attn_decode_fp4(q, *rows, lens, table, max_seqlen=given)
+    rows = [torch.zeros(3, 16, 1, 256, dtype=torch.bfloat16) for _ in range(2)]
+    attention.attn_decode(q, *rows, lens, table, max_seqlen=given)
+    attention.attn_decode(q.half(), *(x.half() for x in rows), lens, table, max_seqlen=given)
+    rows, scales = [x.to(torch.float8_e4m3fn) for x in rows], [torch.ones(3, 16, 1)] * 2
+    attention.attn_decode_fp8(q, *rows, *scales, lens, table, max_seqlen=given)
+    at = {"mkv_decode_attention_fp4": 13, "mkv_decode_attention_bf16": 13,
+          "mkv_decode_attention_f16": 13, "mkv_decode_attention_fp8": 15}
+    assert [name for name, _ in calls] == ["mkv_decode_attention_fp4", "mkv_decode_attention_bf16",
+                                           "mkv_decode_attention_f16", "mkv_decode_attention_fp8"]
+    for name, args in calls:
+        assert args[at[name]] == meant, name
+    assert asked[-1] == meant

@@ -80,3 +80,33 @@ def test_probabilities_are_not_cut(way):
     err = np.abs(got - want)
     tol = 2.0 ** -8 * np.abs(want) + (2.0 ** -18 + 2.0 ** -21) * mass
     assert (err <= tol).all(), f"{(err > tol).sum()} of {err.size} off, worst {(err / tol).max()}"
+
+
+def filled(seed, lens, hq, hkv, way, spread=1.0):
+    """Queries, the two planes' rows of quantised normal values, page tables."""
+    rng, g = np.random.default_rng(seed), torch.Generator().manual_seed(seed)
+    table, pages = tables(rng, lens, way)
+    k, v = (fp4.quantize_rows(torch.randn(pages, 16, hkv, 256, generator=g).bfloat16().double().numpy())
+            for _ in range(2))
+    q = (spread * torch.randn(len(lens), 1, hq, 256, generator=g)).bfloat16()
+    return q, k, v, np.asarray(lens), table
+
+
+@pytest.mark.parametrize("most", [1 << 25, (1 << 31) - 1, 1 << 31, 1 << 32, (1 << 32) + 5, 1 << 70])
+@pytest.mark.parametrize("way", WAYS)
+def test_bounds_that_pass_32_bits(way, most):
+    """No bound at all, as without one."""
+    case(f"decode attention, max_seqlen {most}, {way}")
+    args = filled(22, [70, 1, 33], 4, 1, way)
+    takes(way, 3, 4, 1, args[-1].shape[1])
+    want = attend(*args)
+    got = attend(*args, max_seqlen=most)
+    A.check_errors(DEV)
+    assert np.array_equal(got, want) and want.any(-1).all()
+    q, k, v, lens, table = args
+    dev = [x.to(DEV) for x in (q, *(torch.from_numpy(fp4.values(x)).bfloat16() for x in (k, v)),
+                               torch.from_numpy(lens.astype(np.int32)), torch.from_numpy(table))]
+    want = A.attn_decode(*dev)
+    got = A.attn_decode(*dev, max_seqlen=most)
+    A.check_errors(DEV)
+    assert torch.equal(got, want) and want.any(-1).all()
