@@ -37,10 +37,11 @@ _DTYPE_MAP = {
     "float16": torch.float16,
     "bfloat16": torch.bfloat16,
     "float8_e4m3fn": torch.float8_e4m3fn,
-    "float4_e2m1fn_x2": torch.float4_e2m1fn_x2,
 }
 _FP8 = torch.float8_e4m3fn
-_FP4 = torch.float4_e2m1fn_x2
+_FP4 = getattr(torch, "float4_e2m1fn_x2", None)  # (a torch without it has no 4-bit pools)
+if _FP4 is not None:
+    _DTYPE_MAP["float4_e2m1fn_x2"] = _FP4
 _FP4_DIM = 256
 _FP4_ROW = _FP4_DIM // 2 + _FP4_DIM // 32  # bytes of a (token, head): codes, scales
 _SIXTEEN_BIT = (torch.float16, torch.bfloat16)

@@ -1,12 +1,17 @@
 """Arguments of the attention layer's operators that are settled before a launch: what reaches
 the library, and what does not. The launches themselves are replaced, so no GPU is needed."""
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
 from muserve_amd import _lib
 from muserve_amd.kernels import attention, rope
-from muserve_amd.kv_cache import PagedKVCache
+from muserve_amd.kv_cache import _DTYPE_MAP, PagedKVCache
 
+ROOT = Path(__file__).resolve().parent.parent
 CPU = torch.device("cpu")
 
 
@@ -78,3 +83,26 @@ def test_a_bound_on_the_lengths_ends_with_the_table(calls, monkeypatch, given, m
     for name, args in calls:
         assert args[at[name]] == meant, name
     assert asked[-1] == meant
+
+
+def test_a_torch_without_the_4_bit_type():
+    """Everything but 4-bit pools is there without torch.float4_e2m1fn_x2."""
+    code = """
+import torch
+del torch.float4_e2m1fn_x2
+from muserve_amd import kv_cache, scheduler
+from muserve_amd.kernels import attention, rope
+for dtype in (torch.bfloat16, torch.float16, torch.float8_e4m3fn):
+    cache = kv_cache.PagedKVCache(4, num_layers=1, kv_heads=1, dtype=dtype, device="cpu",
+                                  verbose=False)
+    assert cache.dtype == dtype and cache.cache.dtype == dtype
+    assert kv_cache._DTYPE_MAP[str(dtype).removeprefix("torch.")] == dtype
+try:
+    kv_cache.PagedKVCache(4, num_layers=1, kv_heads=1, dtype=torch.uint8, device="cpu")
+    raise AssertionError("a pool of uint8")
+except ValueError:
+    pass
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True)
+    assert done.returncode == 0, done.stderr
+    assert _DTYPE_MAP["float4_e2m1fn_x2"] == torch.float4_e2m1fn_x2
