@@ -382,12 +382,16 @@ class PagedKVCache:
             out_len = block_tables.shape[1] * KV_PAGE_SIZE
         if layer is None:
             L, first = (num_layers or self.num_layers), 0
+            if not (0 < L <= self.num_layers):
+                raise ValueError(f"{num_layers} layers asked for, the pool has {self.num_layers}")
         else:
-            L, first = 1, int(layer) % self.num_layers
+            L, first = 1, self._layer(layer)
         if block_tables.dtype != torch.int32 or seq_lens.dtype != torch.int32:
             raise TypeError("block_tables and seq_lens must be int32")
         if block_tables.stride(1) != 1:
             raise ValueError("block_tables rows must be contiguous")
+        if seq_lens.numel() < B or (starts is not None and starts.numel() < B):
+            raise ValueError(f"seq_lens and starts must hold an entry for each of {B} tables")
         out_dtype = self._value_dtype
         rows = (B * out_len) if cu_out is None else None
         if cu_out is not None and cu_out.numel() != B + 1:

@@ -106,3 +106,27 @@ except ValueError:
     done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True)
     assert done.returncode == 0, done.stderr
     assert _DTYPE_MAP["float4_e2m1fn_x2"] == torch.float4_e2m1fn_x2
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn, torch.float4_e2m1fn_x2])
+def test_a_gather_reads_inside_the_pool_and_its_arguments(calls, dtype):
+    cache = pool(dtype, layers=3, heads=2)
+    table, lens = torch.zeros(2, 1, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    for layer in (3, -4, 7):
+        with pytest.raises(IndexError):
+            cache.gather(layer, table, lens)
+    for layers in (4, -1):
+        with pytest.raises(ValueError, match="layers"):
+            cache.gather(None, table, lens, num_layers=layers)
+    with pytest.raises(ValueError, match="entry"):
+        cache.gather(0, table, lens[:1])
+    with pytest.raises(ValueError, match="entry"):
+        cache.gather(0, table, lens, starts=lens[:1])
+    assert not calls
+    k, _ = cache.gather(-1, table, lens, starts=lens)
+    assert k.shape == (2, 16, 2, 256)
+    assert cache.gather(None, table, lens)[0].shape == (3, 2, 16, 2, 256)
+    assert cache.gather(None, table, torch.zeros(5, dtype=torch.int32), num_layers=2)[1].shape[0] == 2
+    assert len(calls) == 3
+    plane = 2 * 4 * 16 * cache._row_bytes
+    assert [args[0] - cache.cache.data_ptr() for _, args in calls] == [2 * plane, 0, 0]
