@@ -526,6 +526,8 @@ def _decode(fn, q, k_cache, v_cache, k_scales, v_scales, cache_seqlens, page_tab
                         " query")
     if cache_seqlens.dtype != torch.int32 or page_table.dtype != torch.int32:
         raise TypeError("cache_seqlens and page_table must be int32")
+    if cache_seqlens.numel() < B or page_table.shape[0] < B:
+        raise ValueError("cache_seqlens / page_table rows do not match q")
     if not (q.is_contiguous() and k_cache.is_contiguous() and v_cache.is_contiguous()
             and cache_seqlens.is_contiguous() and page_table.stride(1) == 1):
         raise ValueError("q, caches, cache_seqlens and page_table rows must be contiguous")

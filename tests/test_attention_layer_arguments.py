@@ -130,3 +130,21 @@ def test_a_gather_reads_inside_the_pool_and_its_arguments(calls, dtype):
     assert len(calls) == 3
     plane = 2 * 4 * 16 * cache._row_bytes
     assert [args[0] - cache.cache.data_ptr() for _, args in calls] == [2 * plane, 0, 0]
+
+
+def test_every_query_has_a_length_and_a_table(calls):
+    """Over each kind of pool: fewer lengths or rows of the page table than queries are refused."""
+    q = torch.zeros(3, 1, 4, 256, dtype=torch.bfloat16)
+    lens, table = torch.zeros(3, dtype=torch.int32), torch.zeros(3, 4, dtype=torch.int32)
+    wide = torch.zeros(2, 16, 1, 256, dtype=torch.bfloat16)
+    codes, scale = wide.to(torch.float8_e4m3fn), torch.ones(2, 16, 1)
+    rows = torch.zeros(2, 16, 1, 136, dtype=torch.uint8)
+    for fn, x, caches in ((attention.attn_decode, q, (wide, wide)),
+                          (attention.attn_decode, q.half(), (wide.half(), wide.half())),
+                          (attention.attn_decode_fp8, q, (codes, codes, scale, scale)),
+                          (attention.attn_decode_fp4, q, (rows, rows))):
+        with pytest.raises(ValueError, match="do not match"):
+            fn(x, *caches, lens[:2], table)
+        with pytest.raises(ValueError, match="do not match"):
+            fn(x, *caches, lens, table[:2])
+    assert not calls
