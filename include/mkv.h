@@ -254,8 +254,8 @@ int mkv_gather_dequant_fp8(const void* k_pool, const void* v_pool,
  * with the scale byte e + 127 behind the row's codes. A value is code * 2^e. A block
  * with an infinity or a NaN has the scale byte 255 and codes 0, and reads back as
  * NaN; a scale byte of 0 (a row never written) with codes 0 reads as zeros.
- * head_dim must be 256; the source strides and the pool's address are as
- * mkv_append_fp8's. No reference counterpart (the reference has no 4-bit cache).
+ * head_dim must be 256, tokens x heads at most 2^28 - 16; the source strides and the pool's
+ * address are as mkv_append_fp8's. No reference counterpart (the reference has no 4-bit cache).
  */
 int mkv_append_fp4(void* k_pool, void* v_pool, int64_t pool_layer_stride, int64_t num_slots,
                    const void* k_src, const void* v_src, int64_t src_layer_stride,
@@ -264,7 +264,8 @@ int mkv_append_fp4(void* k_pool, void* v_pool, int64_t pool_layer_stride, int64_
                    void* stream);
 
 /*
- * Dequant-gather of a 4-bit pool: as mkv_gather_dequant_fp8, for any number of heads.
+ * Dequant-gather of a 4-bit pool: as mkv_gather_dequant_fp8, for 1 to 1024 heads and
+ * an out_len up to 2^28 - 16.
  * Every finite value of the pool is a bf16 value, so nothing is rounded.
  */
 int mkv_gather_dequant_fp4(const void* k_pool, const void* v_pool, int64_t pool_layer_stride,
@@ -292,7 +293,8 @@ int mkv_gather_dequant_fp4(const void* k_pool, const void* v_pool, int64_t pool_
  * q and k are [num_tokens, heads, head_dim] in bf16 (fp16 with `fp16`) at any token
  * and head strides (bytes, multiples of 16), q_out and k_out contiguous; an output may
  * be its input where that is contiguous. head_dim is 64, 128 or 256, rotary_dim a
- * multiple of 16 up to it. positions are int64, inv_freq [rotary_dim / 2] fp32 or
+ * multiple of 16 up to it, num_tokens x head_dim at most
+ * 2^35 - 2^11. positions are int64, inv_freq [rotary_dim / 2] fp32 or
  * (freq_fp64) fp64. weight_type: 0 no weights, 1 bf16, 2 fp16, 3 fp32.
  */
 int mkv_qk_norm_rope(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,

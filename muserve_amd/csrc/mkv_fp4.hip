@@ -132,12 +132,13 @@ extern "C" int mkv_append_fp4(void* k_pool, void* v_pool, int64_t pool_layer_str
   MKV_REQUIRE((uint64_t)num_tokens < (1ull << 31), MKV_E_UNSUPPORTED,
               "mkv_append_fp4: too many rows for one call");
   const uint64_t rows = (uint64_t)num_tokens * (uint64_t)num_heads;
-  MKV_REQUIRE(rows < (1ull << 31) && num_layers <= 32767, MKV_E_UNSUPPORTED,
-              "mkv_append_fp4: too many rows for one call");
+  const int64_t wgs = (int64_t)((rows + kRowsPerWg - 1) / kRowsPerWg);
+  MKV_REQUIRE(rows < (1ull << 31) && grid_fits(wgs, kThreads) && num_layers <= 32767,
+              MKV_E_UNSUPPORTED, "mkv_append_fp4: too many rows for one call");
   AppendFp4Args a{(uint8_t*)k_pool, (uint8_t*)v_pool, pool_layer_stride, num_slots,
                   (const uint8_t*)k_src, (const uint8_t*)v_src, src_layer_stride,
                   src_token_stride, slot_mapping, (uint32_t)rows, (uint32_t)num_heads, err};
-  dim3 grid((unsigned)((rows + kRowsPerWg - 1) / kRowsPerWg), (unsigned)(2 * num_layers));
+  dim3 grid((unsigned)wgs, (unsigned)(2 * num_layers));
   if (num_heads == 1)
     hipLaunchKernelGGL(append_fp4_kernel<1>, grid, dim3(kThreads), 0, as_stream(stream), a);
   else if (num_heads == 2)
@@ -172,7 +173,10 @@ extern "C" int mkv_gather_dequant_fp4(const void* k_pool, const void* v_pool,
                                   starts, batch, out_len, out_offsets, k_out, v_out,
                                   out_layer_stride, num_heads * kHeadDim * 2, err);
   if (rc != MKV_OK) return rc;
-  hipLaunchKernelGGL(gather_fp4_kernel, gather_grid(a, kGatherRows, num_layers),
-                     dim3(kGatherThreads), 0, as_stream(stream), a, num_heads);
+  const dim3 grid = gather_grid(a, kGatherRows, num_layers);
+  MKV_REQUIRE(grid_fits(grid.x, kGatherThreads), MKV_E_UNSUPPORTED,
+              "mkv_gather_dequant_fp4: out_len too large");
+  hipLaunchKernelGGL(gather_fp4_kernel, grid, dim3(kGatherThreads), 0, as_stream(stream), a,
+                     num_heads);
   return check_launch("mkv_gather_dequant_fp4");
 }

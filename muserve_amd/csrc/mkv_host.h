@@ -32,6 +32,11 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256;  // 4 wave64s per workgroup
 
+// Whether a launch takes so many workgroups along a grid dimension: fewer than 2^32 threads.
+inline bool grid_fits(int64_t workgroups, int64_t threads) {
+  return workgroups * threads < (1ll << 32);
+}
+
 }  // namespace mkv
 
 #define MKV_REQUIRE(cond, code, ...)              \

@@ -216,10 +216,15 @@ __global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_kernel(RopeArgs a) 
   }
 }
 
+// Workgroups for the tokens: dim / 8 lanes own a token.
+int64_t workgroups(int64_t tokens, int32_t dim) {
+  const int64_t groups = kRopeThreads / (dim / 8);
+  return (tokens + groups - 1) / groups;
+}
+
 template <int D, bool F16, bool PAIRS, int POOL>
 void launch(RopeArgs& a, hipStream_t st) {
-  constexpr int GROUPS = kRopeThreads / (D / 8);
-  const int64_t wgs = (a.tokens + GROUPS - 1) / GROUPS;
+  const int64_t wgs = workgroups(a.tokens, D);
   // a token's heads over several workgroups while the tokens alone are few: up to 4 for each
   // CU (4096 tokens of 6 heads with the append: 8.8 us, with up to 2 10.4, with up to 8 8.7)
   const int64_t want = 4ll * device_cus();
@@ -269,8 +274,9 @@ int fill(const char* fn, RopeArgs& a, const void* q, int64_t q_token, int64_t q_
               "%s: head_dim %d unsupported (64, 128, 256)", fn, dim);
   MKV_REQUIRE(rot > 0 && rot <= dim && rot % 16 == 0, MKV_E_UNSUPPORTED,
               "%s: rotary dim %d unsupported (multiples of 16 up to head_dim)", fn, rot);
-  MKV_REQUIRE(hq <= 65536 && hk <= 65536 && tokens < (1ll << 31), MKV_E_UNSUPPORTED,
-              "%s: too many rows for one call", fn);
+  MKV_REQUIRE(hq <= 65536 && hk <= 65536 && tokens < (1ll << 31) &&
+                  grid_fits(workgroups(tokens, dim), kRopeThreads),
+              MKV_E_UNSUPPORTED, "%s: too many rows for one call", fn);
   MKV_REQUIRE(weight_kind >= kNoWeight && weight_kind <= kWeightF32, MKV_E_INVALID,
               "%s: bad weight type", fn);
   if (tokens == 0 || hq + hk == 0) return MKV_OK;

@@ -13,6 +13,7 @@ from muserve_amd.kv_cache import _DTYPE_MAP, PagedKVCache
 
 ROOT = Path(__file__).resolve().parent.parent
 CPU = torch.device("cpu")
+FAKE = 1 << 20  # an aligned non-null address; argument checks fail before any use
 
 
 @pytest.fixture
@@ -148,3 +149,36 @@ def test_every_query_has_a_length_and_a_table(calls):
         with pytest.raises(ValueError, match="do not match"):
             fn(x, *caches, lens, table[:2])
     assert not calls
+
+
+def library(name, *args):
+    lib = _lib.load()
+    return getattr(lib, name)(*args), lib.mkv_last_error().decode()
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("append", [False, True])
+def test_rows_of_a_rotation_fit_a_grid(dim, append):
+    """A grid dimension has fewer than 2^32 threads; dim / 8 of them own a token."""
+    row = 2 * dim
+    pools = (1, FAKE, FAKE, None, None, 16, FAKE, FAKE) if append else (FAKE,)
+    for tokens in ((1 << 35) // dim, (1 << 31) - 1):
+        got, text = library("mkv_append_rope" if append else "mkv_qk_norm_rope", FAKE, row, row,
+                            FAKE, row, row, *((FAKE, row, row) if append else ()), tokens, 1, 1, dim,
+                            0, FAKE, FAKE, 0, 16, 0, 1.0, None, None, 0, 0, 1e-6, FAKE, *pools, None)
+        assert got == -3 and "too many rows" in text
+
+
+@pytest.mark.parametrize("tokens,heads", [(1 << 28, 1), ((1 << 28) - 15, 1), (1 << 27, 2),
+                                          (1 << 20, 256)])
+def test_rows_of_a_4_bit_append_fit_a_grid(tokens, heads):
+    got, text = library("mkv_append_fp4", FAKE, FAKE, 0, 16, FAKE, FAKE, 0, 512, FAKE, tokens, 1,
+                        heads, 256, FAKE, None)
+    assert got == -3 and "too many rows" in text
+
+
+@pytest.mark.parametrize("out_len", [1 << 28, (1 << 28) - 15, (1 << 31) - 1])
+def test_rows_of_a_4_bit_gather_fit_a_grid(out_len):
+    got, text = library("mkv_gather_dequant_fp4", FAKE, FAKE, 0, 4, FAKE, 4, 4, FAKE, None, 1, out_len,
+                        None, FAKE, FAKE, 0, 1, 1, 256, FAKE, None)
+    assert got == -3 and "out_len" in text
