@@ -372,7 +372,9 @@ class PagedKVCache:
         ``cu_out[b+1]``, or past the buffer's end, is cut there and flagged
         as MkvDeviceError at the next ``check_errors``). With ``layer`` None the
         first ``num_layers`` layers are gathered into [L, ...] outputs in one
-        launch. fp8 and 4-bit pools are dequantised to bf16. ``out`` reuses buffers.
+        launch. fp8 and 4-bit pools are dequantised to bf16. ``out`` reuses buffers;
+        packed mode without it reads ``cu_out[-1]`` back (a synchronisation, which no
+        graph capture allows).
         """
         dev = self._gpu()
         B = block_tables.shape[0]
