@@ -275,8 +275,8 @@ class UniqueCheck:
             raise TypeError("ids must be a contiguous int32 or int64 tensor")
         if ids.numel() == 0:
             return
-        call("mkv_check_unique", ids.data_ptr(), ids.element_size(), ids.numel(), self.limit,
-             self.bits.data_ptr(), self.bits.numel(), err.ptr(), stream_of(ids.device))
+        call_on(ids.device, "mkv_check_unique", ids.data_ptr(), ids.element_size(), ids.numel(),
+                self.limit, self.bits.data_ptr(), self.bits.numel(), err.ptr())
 
 
 class DeviceErrors:

@@ -284,10 +284,10 @@ def _prefill(q, k, v, page_table, cu_q, cu_k, lens_k, max_seqlen_q, softmax_scal
     cu_qp, cu_kp, lens_kp = cu_q.data_ptr(), _lib.ptr(cu_k), _lib.ptr(lens_k)
     first = 0
     while True:
-        _lib.call(fn, q.data_ptr(), k.data_ptr(), v.data_ptr(), units, Hkv, Hq, D, table, stride,
-                  width, cu_qp, cu_kp, lens_kp, min(some, batch - first), Tq, max_q, scale,
-                  1 if causal else 0, splits, *(() if planned else (split_len,)), out.data_ptr(),
-                  _lib.ptr(ws), ws_bytes, _errword(dev).ptr(), _lib.stream_of(dev))
+        _lib.call_on(dev, fn, q.data_ptr(), k.data_ptr(), v.data_ptr(), units, Hkv, Hq, D, table,
+                     stride, width, cu_qp, cu_kp, lens_kp, min(some, batch - first), Tq, max_q,
+                     scale, 1 if causal else 0, splits, *(() if planned else (split_len,)),
+                     out.data_ptr(), _lib.ptr(ws), ws_bytes, _errword(dev).ptr())
         first += some
         if first >= batch:
             return out
@@ -503,10 +503,10 @@ def _decode_contig(q, k_cache, v_cache, cache_seqlens, softmax_scale, max_seqlen
         max_seqlen = S
     scale = D ** -0.5 if softmax_scale is None else float(softmax_scale)
     ws = _decode_scratch(B, Hkv, Hq, max_seqlen, dev)
-    _lib.call("mkv_decode_attention_contig", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-              1 if k_cache.dtype == torch.float16 else 0, Hkv, Hq, D, S,
-              cache_seqlens.data_ptr(), B, int(min(max_seqlen, 1 << 24)), scale, out.data_ptr(),
-              ws.data_ptr(), ws.numel(), _errword(dev).ptr(), _lib.stream_of(dev))
+    _lib.call_on(dev, "mkv_decode_attention_contig", q.data_ptr(), k_cache.data_ptr(),
+                 v_cache.data_ptr(), 1 if k_cache.dtype == torch.float16 else 0, Hkv, Hq, D, S,
+                 cache_seqlens.data_ptr(), B, int(min(max_seqlen, 1 << 24)), scale, out.data_ptr(),
+                 ws.data_ptr(), ws.numel(), _errword(dev).ptr())
     return out
 
 
@@ -542,8 +542,8 @@ def _decode(fn, q, k_cache, v_cache, k_scales, v_scales, cache_seqlens, page_tab
     scales = () if k_scales is None else (k_scales.data_ptr(), v_scales.data_ptr())
     if shared_pages < 0:
         raise ValueError("shared_pages must be >= 0")
-    _lib.call(fn, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), *scales,
-              P, int(shared_pages), Hkv, Hq, D, page_table.data_ptr(), page_table.stride(0), width,
-              cache_seqlens.data_ptr(), B, max_seqlen, scale, out.data_ptr(),
-              ws.data_ptr(), ws.numel(), _errword(dev).ptr(), _lib.stream_of(dev))
+    _lib.call_on(dev, fn, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), *scales, P,
+                 int(shared_pages), Hkv, Hq, D, page_table.data_ptr(), page_table.stride(0), width,
+                 cache_seqlens.data_ptr(), B, max_seqlen, scale, out.data_ptr(), ws.data_ptr(),
+                 ws.numel(), _errword(dev).ptr())
     return out

@@ -259,7 +259,7 @@ class PagedKVCache:
             k = k.to(device=dev, dtype=in_dtype).contiguous()
         if v.dtype != in_dtype or v.device != dev or not v.is_contiguous():
             v = v.to(device=dev, dtype=in_dtype).contiguous()
-        _lib.require_gpu(k, v, slot_mapping, self.cache)
+        on = _lib.require_gpu(k, v, slot_mapping, self.cache)
         if T == 0:
             return
         if self.check_unique:
@@ -267,22 +267,19 @@ class PagedKVCache:
         kp, vp = self._planes(first)  # (views of them are two indexings each)
         src_layer = T * self.row_elems * 2
         src_tok = self.row_elems * 2
-        stream = _lib.stream_of(dev)
         if self.dtype == _FP8:
-            _lib.call("mkv_append_fp8", kp, vp, *self._scale_planes(first),
-                      self._plane_layer_stride(), self._scale_layer_stride(), self.num_slots,
-                      k.data_ptr(), v.data_ptr(), src_layer, src_tok, slot_mapping.data_ptr(), T,
-                      L, self.kv_heads, self.head_dim, self._errors.ptr(), stream)
+            _lib.call_on(on, "mkv_append_fp8", kp, vp, *self._scale_planes(first),
+                         self._plane_layer_stride(), self._scale_layer_stride(), self.num_slots,
+                         k.data_ptr(), v.data_ptr(), src_layer, src_tok, slot_mapping.data_ptr(), T,
+                         L, self.kv_heads, self.head_dim, self._errors.ptr())
         elif self.dtype == _FP4:
-            _lib.call_on(self.cache.device, "mkv_append_fp4", kp, vp, self._plane_layer_stride(),
-                         self.num_slots, k.data_ptr(), v.data_ptr(), src_layer, src_tok,
-                         slot_mapping.data_ptr(), T, L, self.kv_heads, self.head_dim,
-                         self._errors.ptr())
+            _lib.call_on(on, "mkv_append_fp4", kp, vp, self._plane_layer_stride(), self.num_slots,
+                         k.data_ptr(), v.data_ptr(), src_layer, src_tok, slot_mapping.data_ptr(), T,
+                         L, self.kv_heads, self.head_dim, self._errors.ptr())
         else:
-            _lib.call("mkv_append_bf16", kp, vp, self._plane_layer_stride(),
-                      self.num_slots, k.data_ptr(), v.data_ptr(), src_layer, src_tok,
-                      slot_mapping.data_ptr(), T, L, self._row_bytes, self._errors.ptr(),
-                      stream)
+            _lib.call_on(on, "mkv_append_bf16", kp, vp, self._plane_layer_stride(), self.num_slots,
+                         k.data_ptr(), v.data_ptr(), src_layer, src_tok, slot_mapping.data_ptr(), T,
+                         L, self._row_bytes, self._errors.ptr())
 
     def append_rope(self, slot_mapping: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
                     v: torch.Tensor, layer: int, positions: torch.Tensor,
@@ -419,7 +416,7 @@ class PagedKVCache:
             if rows is None and (k_out.numel() % (L * self.row_elems) != 0
                                  or v_out.numel() != k_out.numel()):
                 raise ValueError(f"packed out buffers must hold whole rows for {L} layers")
-        _lib.require_gpu(block_tables, seq_lens, k_out, v_out, self.cache)
+        on = _lib.require_gpu(block_tables, seq_lens, k_out, v_out, self.cache)
         # conversions are no-ops in a serving loop, and made only where something differs
         if starts is not None:
             starts = starts.to(device=dev, dtype=torch.int32).contiguous()
@@ -431,28 +428,26 @@ class PagedKVCache:
             seq_lens = seq_lens.contiguous()
         out_elem = 2
         out_layer_stride = (k_out.numel() // L) * out_elem
-        stream = _lib.stream_of(dev)
         kp, vp = self._planes(first)  # (by address, as in append)
         if self.dtype == _FP8:
-            _lib.call("mkv_gather_dequant_fp8", kp, vp, *self._scale_planes(first),
-                      self._plane_layer_stride(), self._scale_layer_stride(), self.num_pages,
-                      block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1],
-                      seq_lens.data_ptr(), _lib.ptr(starts), B, out_len, _lib.ptr(offs),
-                      k_out.data_ptr(), v_out.data_ptr(), out_layer_stride, L, self.kv_heads,
-                      self.head_dim, self._errors.ptr(), stream)
+            _lib.call_on(on, "mkv_gather_dequant_fp8", kp, vp, *self._scale_planes(first),
+                         self._plane_layer_stride(), self._scale_layer_stride(), self.num_pages,
+                         block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1],
+                         seq_lens.data_ptr(), _lib.ptr(starts), B, out_len, _lib.ptr(offs),
+                         k_out.data_ptr(), v_out.data_ptr(), out_layer_stride, L, self.kv_heads,
+                         self.head_dim, self._errors.ptr())
         elif self.dtype == _FP4:
-            _lib.call_on(self.cache.device, "mkv_gather_dequant_fp4", kp, vp,
-                         self._plane_layer_stride(), self.num_pages, block_tables.data_ptr(),
-                         block_tables.stride(0), block_tables.shape[1], seq_lens.data_ptr(),
-                         _lib.ptr(starts), B, out_len, _lib.ptr(offs), k_out.data_ptr(),
-                         v_out.data_ptr(), out_layer_stride, L, self.kv_heads, self.head_dim,
-                         self._errors.ptr())
+            _lib.call_on(on, "mkv_gather_dequant_fp4", kp, vp, self._plane_layer_stride(),
+                         self.num_pages, block_tables.data_ptr(), block_tables.stride(0),
+                         block_tables.shape[1], seq_lens.data_ptr(), _lib.ptr(starts), B, out_len,
+                         _lib.ptr(offs), k_out.data_ptr(), v_out.data_ptr(), out_layer_stride, L,
+                         self.kv_heads, self.head_dim, self._errors.ptr())
         else:
-            _lib.call("mkv_gather_bf16", kp, vp, self._plane_layer_stride(),
-                      self.num_pages, block_tables.data_ptr(), block_tables.stride(0),
-                      block_tables.shape[1], seq_lens.data_ptr(), _lib.ptr(starts), B, out_len,
-                      _lib.ptr(offs), k_out.data_ptr(), v_out.data_ptr(), out_layer_stride, L,
-                      self._row_bytes, self._errors.ptr(), stream)
+            _lib.call_on(on, "mkv_gather_bf16", kp, vp, self._plane_layer_stride(), self.num_pages,
+                         block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1],
+                         seq_lens.data_ptr(), _lib.ptr(starts), B, out_len, _lib.ptr(offs),
+                         k_out.data_ptr(), v_out.data_ptr(), out_layer_stride, L, self._row_bytes,
+                         self._errors.ptr())
         return k_out, v_out
 
     def copy_pages(self, src_pages, dst_pages) -> None:
@@ -472,17 +467,17 @@ class PagedKVCache:
         n = src.numel()
         if n == 0:
             return
-        stream = _lib.stream_of(dev)
+        on = self.cache.device
         page_bytes = KV_PAGE_SIZE * self._row_bytes
-        _lib.call("mkv_copy_blocks", self.cache.data_ptr(), self.num_pages * page_bytes,
-                  2 * self.num_layers, self.num_pages, page_bytes, src.data_ptr(), dst.data_ptr(),
-                  n, self._errors.ptr(), stream)
+        _lib.call_on(on, "mkv_copy_blocks", self.cache.data_ptr(), self.num_pages * page_bytes,
+                     2 * self.num_layers, self.num_pages, page_bytes, src.data_ptr(),
+                     dst.data_ptr(), n, self._errors.ptr())
         if self.scales is not None:
             sbytes = KV_PAGE_SIZE * self.kv_heads * 4
             if sbytes % 16 == 0:
-                _lib.call("mkv_copy_blocks", self.scales.data_ptr(), self.num_pages * sbytes,
-                          2 * self.num_layers, self.num_pages, sbytes, src.data_ptr(),
-                          dst.data_ptr(), n, self._errors.ptr(), stream)
+                _lib.call_on(on, "mkv_copy_blocks", self.scales.data_ptr(), self.num_pages * sbytes,
+                             2 * self.num_layers, self.num_pages, sbytes, src.data_ptr(),
+                             dst.data_ptr(), n, self._errors.ptr())
 
 
 class SequenceKVState:
@@ -623,14 +618,14 @@ class BlockTables:
         for s in self.seqs:
             s.seq_len += 1
         self._lens += 1
-        stream = _lib.stream_of(dev)
         self._new_dev.copy_(staging, non_blocking=True)
         ev = torch.cuda.Event()
         ev.record(torch.cuda.current_stream(dev))
         self._events[i] = ev
-        _lib.call("mkv_decode_slots", self.seq_lens.data_ptr(), self.tables.data_ptr(),
-                  self.tables.stride(0), self.max_pages, self._new_dev.data_ptr(), self.batch,
-                  cache.num_pages, self.slots.data_ptr(), cache._errors.ptr(), stream)
+        _lib.call_on(self.tables.device, "mkv_decode_slots", self.seq_lens.data_ptr(),
+                     self.tables.data_ptr(), self.tables.stride(0), self.max_pages,
+                     self._new_dev.data_ptr(), self.batch, cache.num_pages, self.slots.data_ptr(),
+                     cache._errors.ptr())
         return self.slots
 
     def padded_len(self) -> int:

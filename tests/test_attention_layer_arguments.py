@@ -182,3 +182,61 @@ def test_rows_of_a_4_bit_gather_fit_a_grid(out_len):
     got, text = library("mkv_gather_dequant_fp4", FAKE, FAKE, 0, 4, FAKE, 4, 4, FAKE, None, 1, out_len,
                         None, FAKE, FAKE, 0, 1, 1, 256, FAKE, None)
     assert got == -3 and "out_len" in text
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn, torch.float4_e2m1fn_x2])
+@pytest.mark.parametrize("current", [False, True])
+def test_launches_on_the_tensors_device(calls, monkeypatch, dtype, current):
+    """With another device as the current one, each launch is made with the tensors' as the
+    current one: a default stream is the current device's."""
+    on, made = [], []
+
+    class Device:
+        def __init__(self, dev):
+            self.dev = dev
+
+        def __enter__(self):
+            on.append(self.dev)
+
+        def __exit__(self, *exc):
+            on.pop()
+
+    monkeypatch.undo()
+    monkeypatch.setattr(_lib, "require_gpu", lambda *tensors: CPU)
+    monkeypatch.setattr(_lib, "_device_index", lambda: CPU.index if current else 0)
+    monkeypatch.setattr(_lib, "call", lambda name, *args: made.append((name, list(on))))
+    monkeypatch.setattr(_lib, "stream_of", lambda dev: 0)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(PagedKVCache, "_gpu", lambda self: self.device)
+    for module, kept in ((rope, "_plans"), (attention, "_fp4_plans")):
+        monkeypatch.setattr(module, kept, {})
+    monkeypatch.setattr(attention, "_errword", lambda dev: _lib.DeviceErrors(CPU))
+    monkeypatch.setattr(attention, "_prefill_cus", lambda dev: 256)
+    monkeypatch.setattr(attention, "_fp4_bytes", lambda *shape: 0)
+    monkeypatch.setattr(attention, "_decode_scratch", lambda *shape: torch.zeros(16))
+    monkeypatch.setattr(attention, "_scratch", lambda n, dev: torch.zeros(16))
+
+    cache, slots = pool(dtype), torch.arange(3)
+    x = torch.zeros(3, 1, 256, dtype=torch.bfloat16)
+    table, lens = torch.zeros(3, 1, dtype=torch.int32), torch.ones(3, dtype=torch.int32)
+    cache.append(slots, x, x, layer=0)
+    cache.append_rope(slots, x, x, x, 0, torch.arange(3), torch.ones(32))
+    cache.gather(0, table, lens)
+    cache.copy_pages([1], [2])
+    q = torch.zeros(3, 1, 4, 256, dtype=torch.bfloat16)
+    if dtype == torch.bfloat16:
+        attention.attn_decode(q, *cache.get_kv_by_layer(0), lens, table)
+        attention.attn_decode(q, *(torch.zeros(3, 8, 1, 256, dtype=dtype),) * 2, lens, None)
+        cu = torch.arange(4, dtype=torch.int32)
+        attention.attn_prefill(q[:, 0], x, x, cu, cu, 1, 1)
+        attention.attn_prefill_paged(q[:, 0], *cache.get_kv_by_layer(0), cu, lens, table, 1)
+    elif dtype == torch.float8_e4m3fn:
+        attention.attn_decode_fp8(q, *cache.get_kv_by_layer(0), cache.scales[0, 0],
+                                  cache.scales[0, 1], lens, table)
+    else:
+        attention.attn_decode_fp4(q, *cache.get_kv_by_layer(0), lens, table)
+    check = _lib.UniqueCheck(CPU, 16)
+    check.run(slots, cache._errors)
+    assert len(made) == {torch.bfloat16: 9, torch.float8_e4m3fn: 7, torch.float4_e2m1fn_x2: 6}[dtype]
+    for name, entered in made:
+        assert entered == ([] if current else [CPU]), name
