@@ -69,7 +69,7 @@ constexpr int kWgsPerCu = 2;
 constexpr int kPairWaves = 8;        // of a workgroup that takes a whole (sequence, KV head)
 constexpr int kPairTiles = 24;       // tiles of the longest sequence up to which they do, and
 constexpr int kPairMore = 16;        // as many more with a sequence for each CU
-constexpr int kWidePieces = 256;     // pieces of a sequence from which the merge takes 16 waves
+constexpr int kWideSpans = 256;      // spans of a sequence from which the merge takes 16 waves
 constexpr float kRaise = 8.f;        // log2 by which a score may pass the running maximum
 
 struct Args {
@@ -594,11 +594,12 @@ __global__ __launch_bounds__(PAIR ? 64 * kPairWaves : kThreads4, 2) void attn_fp
 
 // Joins the pieces of one (pair, query head) that spans cut, and writes the zeros of an
 // empty pair. Wave w takes the pieces w, w + WAVES, .., four dims a lane, BATCH of them
-// in flight; the waves' sums are joined in LDS. WAVES is 16 where a sequence is cut into
-// many pieces, else 4. Measured (us of both kernels with 4 waves and with 16): 1 sequence of
-// 4096 tokens (128 pieces) 10.8, 11.7, of 32768 (1024) 21.8, 17.4; 8 of 4096 (128) 13.7, 13.9,
-// of 32768 (256) 25.0, 24.0; 2 of 100000 and two KV heads (512) 34.4, 32.2; 128 of 4096 (16)
-// 33.8, 35.6.
+// in flight; the waves' sums are joined in LDS. WAVES is 16 where a sequence lies in many
+// spans, else 4. Measured (us of both kernels with 4 waves and with 16; a sequence's spans,
+// and the pieces that workgroups whose spans all lie in it leave of them): 1 sequence of 4096
+// tokens (128 spans, 32 pieces) 10.8, 11.7, of 32768 (1024, 256) 21.8, 17.4; 8 of 4096 (128,
+// 32) 13.7, 13.9, of 32768 (256, 66) 25.0, 24.0; 2 of 100000 and two KV heads (512, 128) 34.4,
+// 32.2; 128 of 4096 (16, 6 to 8) 33.8, 35.6.
 template <int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void attn_fp4_merge_kernel(Args a) {
   constexpr int BATCH = 8;
@@ -821,10 +822,10 @@ extern "C" int mkv_decode_attention_fp4(const void* q, const void* k_cache, cons
   }
   const int rc = launch<false>(a, span_grid(num_kv_heads), st, fn);
   if (rc != MKV_OK) return rc;
-  // pieces of a sequence, at most about one for each of its tiles and of its spans
+  // spans of a sequence: about its share of them, and at most one for each of its tiles
   const int64_t tiles = ((int64_t)max_seq_len + kTile - 1) / kTile;
   const int64_t spans = span_grid(num_kv_heads) / num_kv_heads * kWaves / batch;
-  if (tiles >= kWidePieces && spans >= kWidePieces)
+  if (tiles >= kWideSpans && spans >= kWideSpans)
     hipLaunchKernelGGL(attn_fp4_merge_kernel<16>, dim3((unsigned)(pairs * group)), dim3(16 * 64), 0,
                        st, a);
   else

@@ -18,9 +18,10 @@ __device__ __forceinline__ void wave_sync() {
 // The loads are issued from inline assembly, so the compiler neither inserts
 // waits for them nor reorders LDS accesses across them ("memory" clobber);
 // every wait on them is explicit below. M0 holds the LDS destination of the
-// lane-0 bytes (the hardware adds 16 or 4 bytes per lane); the compiler keeps
-// nothing in M0 across these statements in this file (no LDS DMA builtins,
-// GWS, message or movrel instructions). Before a slot is refilled, the wave's
+// lane-0 bytes (the hardware adds 16 or 4 bytes per lane). The statements do
+// not tell the compiler that they write it, so a source that includes this
+// file must use nothing else that goes through M0 (LDS DMA builtins, GWS,
+// message or movrel instructions). Before a slot is refilled, the wave's
 // earlier LDS reads of it must have returned: lgkmcnt(0) first.
 
 __device__ __forceinline__ uint32_t lds_addr(const void* p) {
