@@ -288,7 +288,8 @@ int mkv_gather_dequant_fp4(const void* k_pool, const void* v_pool, int64_t pool_
  *   (y_i, y_{i + rotary_dim/2}) -> (y_i c - y_{i+rotary_dim/2} s,
  *                                   y_{i+rotary_dim/2} c + y_i s)
  * (interleaved: the same of y_{2i}, y_{2i+1}). Norm, rotation and products are fp32,
- * the angle fp64; one rounding to the output's type.
+ * the angle fp64; one rounding to the output's type. (A row whose squares sum past fp32's
+ * range, values of 2^60 and more, comes out as zeros where it is finite.)
  *
  * q and k are [num_tokens, heads, head_dim] in bf16 (fp16 with `fp16`) at any token
  * and head strides (bytes, multiples of 16), q_out and k_out contiguous; an output may
@@ -825,7 +826,8 @@ int mkv_decode_attention_fp8(const void* q, const void* k_codes, const void* v_c
  * cached value is code * 2^e, exactly. q and out are bf16; 1 to 8 query heads per KV
  * head, head_dim 256, batch x num_kv_heads at most 4096. Softmax in fp32; a weight
  * enters the product with V as two bf16 values, both rounded to nearest (within 2^-18 of
- * itself, to either side). The workspace (16-byte aligned)
+ * itself, to either side). A head whose scores are all -inf (an infinite q, or sums past
+ * fp32) comes out as NaN, a sequence without tokens as zeros. The workspace (16-byte aligned)
  * is mkv_decode_attention_fp4_workspace_bytes (-1 for an unsupported shape; 0, and none
  * needed, for few sequences of a small max_seq_len); error bits as
  * mkv_decode_attention_bf16. Page ids below shared_pages are read through the

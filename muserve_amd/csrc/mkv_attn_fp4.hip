@@ -71,6 +71,9 @@ constexpr int kPairTiles = 24;       // tiles of the longest sequence up to whic
 constexpr int kPairMore = 16;        // as many more with a sequence for each CU
 constexpr int kWideSpans = 256;      // spans of a sequence from which the merge takes 16 waves
 constexpr float kRaise = 8.f;        // log2 by which a score may pass the running maximum
+// The maximum of a piece whose tokens' scores are all -inf: no weight beside any other
+// piece, and told from the -inf of no tokens at all.
+constexpr float kLowest = -3.402823466e38f;
 
 struct Args {
   const uint8_t* q;      // [B, Hkv * G, 256] bf16
@@ -119,6 +122,11 @@ __device__ __forceinline__ T lds_get(uint32_t at) {
 // The places of a sequence in the flat list.
 __device__ __forceinline__ int32_t places_of(int32_t len) {
   return len > 0 ? (len + kTile - 1) / kTile + 1 : 0;
+}
+// An output of the weights' sum L and the maximum M: the quotient; zeros of no tokens; NaN
+// where there were some and all their scores were -inf (M is kLowest then, not -inf).
+__device__ __forceinline__ float inverse_of(float L, float M) {
+  return L == 0.f && M == -INFINITY ? 0.f : 1.f / L;  // (0 * inf: NaN)
 }
 // Eight codes of a word times the scale, as eight bf16.
 __device__ __forceinline__ u32x4 dequant8(uint32_t w, float s) {
@@ -390,6 +398,7 @@ __global__ __launch_bounds__(PAIR ? 64 * kPairWaves : kThreads4, 2) void attn_fp
     for (int j = 0; j < 16; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
     m_run = -INFINITY;
     l_run = 0.f;
+    bool some = false;  // a token of the sequence in a page of the pool
     while (f < end) {
       __builtin_amdgcn_s_setprio(0);
       if (((uint32_t)(f / STEP + wslot) & 1u) != 0) __builtin_amdgcn_s_setprio(1);
@@ -422,6 +431,7 @@ __global__ __launch_bounds__(PAIR ? 64 * kPairWaves : kThreads4, 2) void attn_fp
         for (int j = 0; j < 8; ++j) sv[j] = sc[j >> 2][j & 3] * a.scale_log2;
       }
       const bool part = now.valid0 < 16 || now.valid1 < 16;
+      some |= now.valid0 + now.valid1 > 0;
       if (part) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -509,6 +519,7 @@ __global__ __launch_bounds__(PAIR ? 64 * kPairWaves : kThreads4, 2) void attn_fp
     // in half the registers: lanes below 32 have the dims 16 c .. + 7, the others 16 c + 8 ..,
     // of the heads 4 (g % 2) + i.
     const float l = over_rows<4>(l_run, [](float x, float y) { return x + y; });
+    const float m_end = m_run == -INFINITY && some ? kLowest : m_run;
     float o[8][4];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -530,21 +541,19 @@ __global__ __launch_bounds__(PAIR ? 64 * kPairWaves : kThreads4, 2) void attn_fp
     if (lane < a.group) {
       float* ml = joint ? ml_l + (wave * a.group + lane) * 2 : a.ml + (piece + lane) * 2;
       if (!whole) {
-        ml[0] = m_run;
+        ml[0] = m_end;
         ml[1] = l;
       }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int h = h0 + i;
-      const float L = __shfl(l, h);
+      const float inv = __shfl(inverse_of(l, m_end), h);
       if (h >= a.group) continue;
       if (whole) {
-        const float inv = 1.f / L;
         uint32_t w[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          w[j] = L == 0.f ? 0u : pack_bf16(o[2 * j][i] * inv, o[2 * j + 1][i] * inv);
+        for (int j = 0; j < 4; ++j) w[j] = pack_bf16(o[2 * j][i] * inv, o[2 * j + 1][i] * inv);
         st16(out + h * kQRow + 2 * d0, u32x4{w[0], w[1], w[2], w[3]});
       } else {
         float* dst = (joint ? piece_l + h * kHeadDim : a.part + (piece + h) * kHeadDim) + d0;
@@ -575,10 +584,9 @@ __global__ __launch_bounds__(PAIR ? 64 * kPairWaves : kThreads4, 2) void attn_fp
           L += e * ls[w];
         }
         if constexpr (PAIR) {
-          const float inv = 1.f / L;
+          const float inv = inverse_of(L, M);
           *reinterpret_cast<u32x2*>(out + h * kQRow + 8 * lane) =
-              L == 0.f ? u32x2{0u, 0u}
-                       : u32x2{pack_bf16(O[0] * inv, O[1] * inv), pack_bf16(O[2] * inv, O[3] * inv)};
+              u32x2{pack_bf16(O[0] * inv, O[1] * inv), pack_bf16(O[2] * inv, O[3] * inv)};
         } else {
           *reinterpret_cast<f32x4*>(a.part + (at + h) * kHeadDim + 4 * lane) = O;
           if (lane == 0) {
@@ -684,7 +692,7 @@ __global__ __launch_bounds__(64 * WAVES) void attn_fp4_merge_kernel(Args a) {
     O += e * wave_o[w][tid];
     L += e * wave_ml[w][1];
   }
-  out[tid] = f32_to_bf16_rne(L == 0.f ? 0.f : O / L);
+  out[tid] = f32_to_bf16_rne(L == 0.f ? O * inverse_of(L, M) : O / L);
 }
 
 // Workgroups of spans: the resident ones, as many for each KV head.

@@ -357,3 +357,51 @@ def test_pages_behind_4_gib_by_spans():
         close(got[:, 0].double().cpu().numpy(), oracle(q, k, v, lens, table))
     del big
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_scores_of_minus_infinity(shape):
+    """Where all of a head's scores are -inf the softmax is NaN, not the zeros of no tokens;
+    where some are, they have no weight. Pages outside the pool count as no tokens all the same."""
+    case(f"4-bit decode attention, {shape}, scores of -inf")
+    q, k, v, lens, table = prepared(36, shape, 4, 2)
+    big = float(torch.finfo(torch.bfloat16).max)
+    k[..., :32] &= 0x77                          # dims 0 .. 63 not below 0,
+    k[..., :2] |= 0x77                             # dims 0 .. 3 the largest value, 6 * 2^e
+    q[0, 0, 0, 0] = -torch.inf                     # heads 0, 1 of sequence 0: an infinity,
+    q[0, 0, 1, :4] = -big                          # sums that pass fp32's range
+    q[4, 0, 2, 1] = -torch.inf                     # head 2 of sequence 4, on KV head 1
+    want = oracle(q.nan_to_num(), k, v, lens, table)
+    got = attend(q, k, v, lens, table)
+    A.check_errors(DEV)
+    bad = np.zeros(got.shape, dtype=bool)
+    bad[0, :2] = bad[4, 2] = True
+    assert np.array_equal(np.isnan(got), bad)
+    close(got, want, ~bad)
+    # some tokens of sequence 0 keep finite scores: heads as without the others
+    n = int(lens[0])
+    for kept in (np.arange(n - 1, n), np.arange(0, n, 7), np.arange(n // 2, n // 2 + 33)):
+        some = k.copy()
+        kept = kept[kept < n]
+        some[table[0][kept // 16], kept % 16, :, :2] = 0
+        q[0, 0, 0] = q[0, 0, 1]
+        got = attend(q, some, v, lens, table)
+        bad[0] = False
+        assert np.array_equal(np.isnan(got), bad)
+        close(got[0, :2], tuple(x[0, :2] for x in alone(q, some, v, table, kept)))
+    gone = table.copy()
+    gone[0] = len(k)
+    got = attend(q, k, v, lens, gone)
+    with pytest.raises(_lib.MkvDeviceError, match="page id"):
+        A.check_errors(DEV)
+    assert not got[0].any()
+
+
+def alone(q, k, v, table, kept):
+    """The oracle over sequence 0's tokens ``kept``: the others' weights are exp(-inf)."""
+    page, row = table[0][kept // 16], kept % 16
+    pages = -(-len(kept) // 16)
+    packed = np.zeros((2, pages * 16, *k.shape[2:]), dtype=np.uint8)
+    packed[0, :len(kept)], packed[1, :len(kept)] = k[page, row], v[page, row]
+    packed = packed.reshape(2, pages, 16, *k.shape[2:])
+    return oracle(q[:1], packed[0], packed[1], [len(kept)], np.arange(pages)[None])
