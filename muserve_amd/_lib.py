@@ -216,6 +216,14 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+def span(t: torch.Tensor) -> tuple[int, int]:
+    """Addresses of t's first element and behind its last."""
+    at = t.data_ptr()
+    if t.numel() == 0:
+        return at, at
+    return at, at + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+
+
 def require_gpu(*tensors: torch.Tensor) -> torch.device:
     """All tensors must live on one ROCm device; returns it."""
     dev = None

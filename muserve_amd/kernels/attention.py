@@ -371,13 +371,6 @@ _fp4_plans: dict[tuple, tuple] = {}
 _FP4_PLANS = 4096
 
 
-def _span(t: torch.Tensor) -> int:
-    """Bytes from the first element of t to behind the last."""
-    if t.numel() == 0:
-        return 0
-    return (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
-
-
 @functools.lru_cache(maxsize=4096)
 def _fp4_bytes(batch: int, num_kv_heads: int, num_q_heads: int, max_seqlen: int,
                dev: torch.device) -> int:
@@ -466,10 +459,10 @@ def attn_decode_fp4(
           or out.device != dev):
         raise ValueError("out must be a contiguous tensor shaped like q")
     else:  # written while other sequences' rows are still read: q itself, or apart from it all
-        at, n = out.data_ptr(), out.numel() * 2
+        lo, hi = _lib.span(out)
         for t in (q, k_cache, v_cache, cache_seqlens, page_table):
-            lo = t.data_ptr()
-            if at < lo + _span(t) and lo < at + n and not (t is q and lo == at):
+            a, b = _lib.span(t)
+            if a < hi and lo < b and not (t is q and a == lo):
                 raise ValueError("out overlaps a tensor that is still read")
     nbytes = _fp4_bytes(*shape, max_seqlen, dev)
     ws = _scratch(nbytes, dev) if nbytes else None

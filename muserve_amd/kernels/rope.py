@@ -99,14 +99,6 @@ def _plan(q, k, v, positions, inv_freq, q_weight, k_weight, interleaved):
     return plan
 
 
-def _span(t: torch.Tensor) -> tuple[int, int]:
-    """Addresses of t's first element and behind its last."""
-    at = t.data_ptr()
-    if t.numel() == 0:
-        return at, at
-    return at, at + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
-
-
 def _given(name: str, out: torch.Tensor, own: torch.Tensor, others) -> None:
     """An output that the caller gives: contiguous, and its own input itself or apart from
     everything that other rows still read."""
@@ -115,11 +107,11 @@ def _given(name: str, out: torch.Tensor, own: torch.Tensor, others) -> None:
         raise ValueError(f"{name} must be a contiguous tensor of its input's shape and type")
     if out.data_ptr() != own.data_ptr() or not own.is_contiguous():
         others = (own, *others)  # (also where another input is the same tensor as its own)
-    lo, hi = _span(out)
+    lo, hi = _lib.span(out)
     for t in others:
         if t is None:
             continue
-        a, b = _span(t)
+        a, b = _lib.span(t)
         if a < hi and lo < b:
             raise ValueError(f"{name} overlaps a tensor that other rows still read or write")
 

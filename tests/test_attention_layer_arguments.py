@@ -240,3 +240,31 @@ def test_launches_on_the_tensors_device(calls, monkeypatch, dtype, current):
     assert len(made) == {torch.bfloat16: 9, torch.float8_e4m3fn: 7, torch.float4_e2m1fn_x2: 6}[dtype]
     for name, entered in made:
         assert entered == ([] if current else [CPU]), name
+
+
+def test_what_a_tensor_spans():
+    x = torch.zeros(4, 3, 8, dtype=torch.bfloat16)
+    at = x.data_ptr()
+    assert _lib.span(x) == (at, at + 192)
+    assert _lib.span(x[1:, ::2, 2:5]) == (at + 52, at + 3 * 48 + 2 * 16 + 10)
+    assert _lib.span(x[:0])[1] - _lib.span(x[:0])[0] == 0
+    assert _lib.span(x[0, 0, :1].expand(7)) == (at, at + 2)
+
+
+def test_decode_outputs_that_overlap(calls, monkeypatch):
+    monkeypatch.setattr(attention, "_fp4_bytes", lambda *shape: 0)
+    flat = torch.zeros(8 * 1024, dtype=torch.bfloat16)
+    q = flat[:2048].view(2, 1, 4, 256)
+    rows = torch.zeros(3, 16, 1, 136, dtype=torch.uint8)
+    lens, table = torch.zeros(2, dtype=torch.int32), torch.zeros(2, 4, dtype=torch.int32)
+    for first in (8, 1024, 2040):
+        with pytest.raises(ValueError, match="overlaps"):
+            attention.attn_decode_fp4(q, rows, rows, lens, table,
+                                      out=flat[first:first + 2048].view(2, 1, 4, 256))
+    cache = rows.view(torch.bfloat16).flatten()[8:2056].view(2, 1, 4, 256)
+    with pytest.raises(ValueError, match="overlaps"):
+        attention.attn_decode_fp4(q, rows, rows, lens, table, out=cache)
+    assert not calls
+    attention.attn_decode_fp4(q, rows, rows, lens, table, out=q)
+    attention.attn_decode_fp4(q, rows, rows, lens, table, out=flat[2048:4096].view(2, 1, 4, 256))
+    assert len(calls) == 2
